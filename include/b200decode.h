@@ -356,6 +356,87 @@ int b2d_gqa_decode_noalloc(const void* q, int64_t sq_b, int64_t sq_h,
                            float scale, int nsplit, int chunk, int dtype,
                            void* out, int64_t so_b, int64_t so_h, int out_dtype, void* stream);
 
+/* ================================================================ paged KV cache
+ * No counterpart in the reference, whose cache is one contiguous [B, KVH, S, D] tensor. Keys and values
+ * live in pages of page_size positions: k / v hold num_pages pages, element (page, head, slot, d) at
+ * page*s?_p + head*s?_h + slot*s?_s + d (strides in elements; last dim contiguous), so both
+ * [num_pages, KVH, page_size, D] and [num_pages, page_size, KVH, D] pools are described. Position p of
+ * sequence b lies in page page_table[b*ld_table + p / page_size], slot p % page_size. One page table
+ * serves every layer of a model; each layer has its own pool. dtype F16 or BF16; page_size 1..1024;
+ * k, v 16-byte aligned, strides multiples of 8 elements. A page id outside [0, num_pages) is never
+ * followed: nothing is written there, and reads give zeros.
+ * ================================================================================== */
+typedef struct {
+  void* k;
+  int64_t sk_p, sk_h, sk_s;
+  void* v;
+  int64_t sv_p, sv_h, sv_s;
+  int num_pages, page_size, KVH, D, dtype;
+} b2d_paged_kv;
+
+/* Rotary embedding of N new tokens, optionally behind an RMS norm of every query and key head, plus the
+ * append of their keys and values to the paged cache. q [N, H, D], k / v [N, KVH, D] (strides s?_n, s?_h;
+ * the projections' outputs, views of a fused one included). Token i belongs to sequence seq_ids[i]
+ * (int32), or i / (N / B) when seq_ids is NULL (N % B == 0), at position positions[i] (int64).
+ *   x' = x * rsqrt(mean(x^2) + eps) * weight   (q_weight / k_weight [D], either may be NULL: x' = x)
+ *   y  = x' * cos[pos] + rotate_half(x') * sin[pos]
+ *   q_out[i, h, :] = y(q);  K page slot = y(k);  V page slot = v.
+ * Everything between the loads and the stores is fp32 and rounded once. cos / sin: [S_max, D] tables
+ * (row stride ld_cs) in the cache's dtype or F32 (cs_dtype). q_out may alias q. A token whose sequence is
+ * outside [0, B) or whose position is outside [0, S_max) is padding: nothing of it is written; one whose
+ * page is outside the table or the pool gets its q_out only. Two tokens of a call must not share a slot.
+ * D % 16 == 0, D <= 256, H % KVH == 0; 16-byte aligned pointers (weights too), strides % 8 == 0.
+ * flags: B2D_LAUNCH_PDL. */
+int b2d_paged_rope_append(const b2d_paged_kv* kv, const void* q, int64_t sq_n, int64_t sq_h,
+                          const void* k, int64_t sk_n, int64_t sk_h, const void* v, int64_t sv_n, int64_t sv_h,
+                          const int64_t* positions, const int32_t* seq_ids,
+                          const int32_t* page_table, int64_t ld_table, int pages_per_seq, int B,
+                          const void* cos, const void* sin, int64_t ld_cs, int S_max, int cs_dtype,
+                          const void* q_weight, const void* k_weight, float eps,
+                          void* q_out, int64_t sqo_n, int64_t sqo_h, int N, int H, int flags, void* stream);
+
+/* Attention of the T newest tokens of every sequence over the paged cache (T = 1: plain decode; T > 1:
+ * drafted tokens verified at once). q [B, T, H, D] (strides sq_b, sq_t, sq_h), out likewise in out_dtype
+ * (the cache's dtype or F32). seqlens[b] (int32) counts the cached keys of sequence b, its T new tokens
+ * included: query t sees the keys before position seqlens[b] - T + 1 + t, and a query that sees none (an
+ * empty sequence) gives zeros. seqlens beyond the page table are cut to it.
+ * prefix_table / prefix_len: the positions [0, prefix_len) of EVERY sequence are those of the pages
+ * prefix_table[0 .. ceil(prefix_len / page_size)) (int32, device) -- a shared system prompt, read and
+ * multiplied once for the whole batch; page_table's entries for them are not read. prefix_len 0: none.
+ * max_len: an upper bound of seqlens known to the host (0: the page table's reach); it only guides the
+ * split over the SMs, longer sequences stay right.
+ * D 64 or 128; H / KVH in 1..16; T in 1..16; 16-byte aligned q, strides % 8 == 0.
+ * workspace: b2d_paged_attention_workspace_bytes bytes for the same sizes (it may be 0), 16-byte aligned;
+ * calls that may overlap need separate ones. No initial contents are needed. flags: B2D_LAUNCH_PDL. */
+size_t b2d_paged_attention_workspace_bytes(const b2d_paged_kv* kv, int B, int T, int H, int pages_per_seq,
+                                           int prefix_len, int max_len);
+int b2d_paged_attention(const b2d_paged_kv* kv, const void* q, int64_t sq_b, int64_t sq_t, int64_t sq_h,
+                        const int32_t* page_table, int64_t ld_table, int pages_per_seq, const int32_t* seqlens,
+                        const int32_t* prefix_table, int prefix_len, int max_len, int B, int T, int H, float scale,
+                        void* out, int64_t so_b, int64_t so_t, int64_t so_h, int out_dtype,
+                        void* workspace, size_t workspace_bytes, int flags, void* stream);
+
+/* ================================================================ verification of drafted tokens
+ * Speculative sampling (no counterpart in the reference, which decodes greedily one token at a time).
+ * draft_tokens [B, K] (int64, row stride ld_tokens) were drawn from draft_probs [B, K, V] (strides sd_b,
+ * sd_k; NULL: drafts that were not sampled, i.e. probability 1 on each drafted token); target_probs
+ * [B, K+1, V] (strides st_b, st_k) are the target model's probabilities at the drafts' positions and behind
+ * the last; uniforms [B, K+1] (fp32, row stride ld_u) random numbers in [0, 1). draft_lens[b] (int32, NULL:
+ * K) is the number of drafts of sequence b, cut to [0, K]; n below. Per sequence:
+ *   a = the number of leading drafts i < n with u_i * q_i(x_i) < p_i(x_i)  (an id outside [0, V) is refused)
+ *   w = a < n: max(p_a - q_a, 0), or p_a where that is zero everywhere;  a == n: p_n
+ *   next = the first v whose running sum of w exceeds u_K * sum(w); the last v with w > 0 where none does
+ *   tokens[b] = x_0 .. x_{a-1}, next, -1 ...  (int64 [B, K+1], row stride ld_out), accepted[b] = a (int32)
+ * The tokens so drawn are distributed as the target's own. A negative or NaN weight counts as zero; a row
+ * without any weight gives -1. Sums, products and comparisons are in 64 bits. probs_dtype F32, F16 or BF16
+ * for both; V >= 1; 0 <= K <= 31; strides of the K dimension may be anything, V is contiguous.
+ * accepted may be NULL. flags: B2D_LAUNCH_PDL. */
+int b2d_verify_drafts(const int64_t* draft_tokens, int64_t ld_tokens, const int32_t* draft_lens,
+                      const void* target_probs, int64_t st_b, int64_t st_k,
+                      const void* draft_probs, int64_t sd_b, int64_t sd_k, int probs_dtype,
+                      const float* uniforms, int64_t ld_u, int64_t* tokens, int64_t ld_out, int32_t* accepted,
+                      int B, int K, int V, int flags, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -33,6 +33,13 @@ class AllreduceEpilogue(C.Structure):
                 ("step", _p), ("site", _i32), ("sites", _i32)]
 
 
+class PagedKvDesc(C.Structure):
+    """b2d_paged_kv (include/b200decode.h)."""
+    _fields_ = [("k", _p), ("sk_p", _i64), ("sk_h", _i64), ("sk_s", _i64),
+                ("v", _p), ("sv_p", _i64), ("sv_h", _i64), ("sv_s", _i64),
+                ("num_pages", _i32), ("page_size", _i32), ("KVH", _i32), ("D", _i32), ("dtype", _i32)]
+
+
 # name -> (restype, argtypes); mirrors include/b200decode.h
 SIGNATURES = {
     "b2d_strerror": (C.c_char_p, [_i32]),
@@ -81,6 +88,15 @@ SIGNATURES = {
     "b2d_gqa_decode_noalloc": (_i32, [_p, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64,
                                       _p, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _i32, _i32,
                                       _p, _i64, _i64, _i32, _p]),
+    "b2d_paged_rope_append": (_i32, [C.POINTER(PagedKvDesc), _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64,
+                                     _p, _p, _p, _i64, _i32, _i32, _p, _p, _i64, _i32, _i32, _p, _p, _f32,
+                                     _p, _i64, _i64, _i32, _i32, _i32, _p]),
+    "b2d_paged_attention_workspace_bytes": (_sz, [C.POINTER(PagedKvDesc), _i32, _i32, _i32, _i32, _i32, _i32]),
+    "b2d_paged_attention": (_i32, [C.POINTER(PagedKvDesc), _p, _i64, _i64, _i64, _p, _i64, _i32, _p,
+                                   _p, _i32, _i32, _i32, _i32, _i32, _f32, _p, _i64, _i64, _i64, _i32,
+                                   _p, _sz, _i32, _p]),
+    "b2d_verify_drafts": (_i32, [_p, _i64, _p, _p, _i64, _i64, _p, _i64, _i64, _i32, _p, _i64, _p, _i64, _p,
+                                 _i32, _i32, _i32, _i32, _p]),
 }
 
 _lib = None
@@ -137,3 +153,30 @@ def stream_ptr(device) -> int:
 
 def ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
+
+
+def cuda_index(device) -> int:
+    """The device's index; raises for tensors that are not on a GPU."""
+    import torch
+    if device.type != "cuda":
+        raise ValueError(f"the tensors are on {device}; the kernels run on a CUDA device only")
+    return device.index if device.index is not None else torch.cuda.current_device()
+
+
+def on_device(index: int):
+    """Context that makes device ``index`` current (the library launches on the current device)."""
+    import contextlib
+
+    import torch
+    return contextlib.nullcontext() if torch.cuda.current_device() == index else torch.cuda.device(index)
+
+
+def call_on(index: int, name: str, *args) -> None:
+    """``call`` an entry point whose last argument is the stream, on device ``index`` and torch's current
+    stream there, whichever device is current."""
+    import torch
+    if torch.cuda.current_device() == index:
+        call(name, *args, torch.cuda.current_stream(index).cuda_stream)
+    else:
+        with torch.cuda.device(index):
+            call(name, *args, torch.cuda.current_stream(index).cuda_stream)

@@ -1,0 +1,208 @@
+"""CPU: refusals of the paged-cache and draft-verification calls (Python and C ABI), and their oracle."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+from b200kernels import _lib
+from b200kernels.paged import PagedKV, paged_attention, paged_rope_append
+from b200kernels.speculative import verify_drafts
+from oracle.paged_ref import verify_ref
+
+OK, ARG, SHAPE, DTYPE, ALIGN = 0, 1, 2, 3, 4
+
+
+def pool(pages=4, kvh=2, ps=16, D=64, dtype=torch.float16):
+    return PagedKV(torch.zeros(pages, kvh, ps, D, dtype=dtype), torch.zeros(pages, kvh, ps, D, dtype=dtype))
+
+
+@pytest.mark.parametrize("k,v,err", [
+    (torch.zeros(4, 2, 16, 64).half(), torch.zeros(4, 2, 16, 32).half(), ValueError),
+    (torch.zeros(4, 2, 16).half(), torch.zeros(4, 2, 16).half(), ValueError),
+    (torch.zeros(4, 2, 16, 64), torch.zeros(4, 2, 16, 64), TypeError),
+    (torch.zeros(4, 2, 16, 64).half(), torch.zeros(4, 2, 16, 64).bfloat16(), TypeError),
+    (torch.zeros(4, 2, 64, 16).half().transpose(2, 3), torch.zeros(4, 2, 16, 64).half(), ValueError),
+    (torch.zeros(4, 2, 2048, 64).half(), torch.zeros(4, 2, 2048, 64).half(), ValueError),
+    (torch.zeros(4, 0, 16, 64).half(), torch.zeros(4, 0, 16, 64).half(), ValueError),
+])
+def test_pool_refusals(k, v, err):
+    with pytest.raises(err):
+        PagedKV(k, v)
+
+
+def append_args(N=2, H=4, kvh=2, D=64, B=2):
+    return dict(q=torch.zeros(N, H, D).half(), k=torch.zeros(N, kvh, D).half(), v=torch.zeros(N, kvh, D).half(),
+                positions=torch.zeros(N, dtype=torch.int64), page_table=torch.zeros(B, 3, dtype=torch.int32),
+                cos=torch.zeros(32, D).half(), sin=torch.zeros(32, D).half())
+
+
+@pytest.mark.parametrize("change,err", [
+    (dict(q=torch.zeros(2, 4, 32).half()), ValueError),
+    (dict(q=torch.zeros(2, 3, 64).half()), ValueError),             # 3 heads over 2 KV heads
+    (dict(k=torch.zeros(3, 2, 64).half()), ValueError),
+    (dict(v=torch.zeros(2, 2, 64)), TypeError),
+    (dict(q=torch.zeros(2, 4, 64).bfloat16()), TypeError),
+    (dict(positions=torch.zeros(2, dtype=torch.int32)), ValueError),
+    (dict(positions=torch.zeros(3, dtype=torch.int64)), ValueError),
+    (dict(page_table=torch.zeros(2, 3, dtype=torch.int64)), ValueError),
+    (dict(page_table=torch.zeros(3, dtype=torch.int32)), ValueError),
+    (dict(page_table=torch.zeros(3, 3, dtype=torch.int32)), ValueError),   # 2 tokens over 3 sequences
+    (dict(seq_ids=torch.zeros(2, dtype=torch.int64)), ValueError),
+    (dict(cos=torch.zeros(32, 32).half()), ValueError),
+    (dict(cos=torch.zeros(32, 64).double(), sin=torch.zeros(32, 64).double()), TypeError),
+    (dict(q_weight=torch.zeros(32).half()), ValueError),
+    (dict(k_weight=torch.zeros(64)), ValueError),
+    (dict(q_out=torch.zeros(2, 4, 64)), ValueError),
+    (dict(q=torch.zeros(2, 64, 4).half().transpose(1, 2)), ValueError),
+    (dict(), ValueError),                                           # sound, but not on a GPU
+])
+def test_append_refusals(change, err):
+    with pytest.raises(err):
+        paged_rope_append(pool(), **{**append_args(), **change})
+
+
+def attn_args(B=2, T=1, H=4, D=64):
+    return dict(q=torch.zeros(B, T, H, D).half(), page_table=torch.zeros(B, 3, dtype=torch.int32),
+                seqlens=torch.ones(B, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("change,err", [
+    (dict(q=torch.zeros(2, 1, 4, 128).half()), ValueError),
+    (dict(q=torch.zeros(2, 1, 5, 64).half()), ValueError),
+    (dict(q=torch.zeros(3, 1, 4, 64).half()), ValueError),
+    (dict(q=torch.zeros(2, 1, 4, 64)), TypeError),
+    (dict(seqlens=torch.ones(2, dtype=torch.int64)), ValueError),
+    (dict(seqlens=torch.ones(3, dtype=torch.int32)), ValueError),
+    (dict(prefix_len=5), ValueError),
+    (dict(prefix_len=33, prefix_table=torch.zeros(2, dtype=torch.int32)), ValueError),
+    (dict(prefix_len=-1, prefix_table=torch.zeros(2, dtype=torch.int32)), ValueError),
+    (dict(out=torch.zeros(2, 1, 4, 32).half()), ValueError),
+    (dict(out=torch.zeros(2, 1, 4, 64).half(), out_dtype=torch.float32), ValueError),
+    (dict(), ValueError),                                           # sound, but not on a GPU
+])
+def test_attention_refusals(change, err):
+    with pytest.raises(err):
+        paged_attention(pool(), **{**attn_args(), **change})
+
+
+@pytest.mark.parametrize("change,err", [
+    (dict(draft_tokens=torch.zeros(2, 3, dtype=torch.int32)), ValueError),
+    (dict(draft_tokens=torch.zeros(2, 32, dtype=torch.int64)), ValueError),
+    (dict(target_probs=torch.zeros(2, 3, 10)), ValueError),
+    (dict(target_probs=torch.zeros(2, 4, 0)), ValueError),
+    (dict(target_probs=torch.zeros(2, 4, 10).double()), TypeError),
+    (dict(draft_probs=torch.zeros(2, 4, 10)), ValueError),
+    (dict(draft_probs=torch.zeros(2, 3, 10).half()), TypeError),
+    (dict(uniforms=torch.zeros(2, 3)), ValueError),
+    (dict(uniforms=torch.zeros(2, 4).double()), ValueError),
+    (dict(draft_lens=torch.zeros(2, dtype=torch.int64)), ValueError),
+    (dict(tokens=torch.zeros(2, 3, dtype=torch.int64)), ValueError),
+    (dict(accepted=torch.zeros(2, dtype=torch.int64)), ValueError),
+    (dict(target_probs=torch.zeros(2, 10, 4).transpose(1, 2)), ValueError),
+    (dict(), ValueError),                                           # sound, but not on a GPU
+])
+def test_verify_refusals(change, err):
+    args = dict(draft_tokens=torch.zeros(2, 3, dtype=torch.int64), target_probs=torch.zeros(2, 4, 10),
+                uniforms=torch.zeros(2, 4))
+    with pytest.raises(err):
+        verify_drafts(**{**args, **change})
+
+
+# ---- C ABI: arguments are checked before the device is touched
+BUF = C.create_string_buffer(4096)
+P = (C.addressof(BUF) + 255) & ~255
+
+
+def desc(**kw):
+    f = dict(k=P, sk_p=2048, sk_h=1024, sk_s=64, v=P, sv_p=2048, sv_h=1024, sv_s=64, num_pages=4, page_size=16, KVH=2,
+             D=64, dtype=0)
+    f.update(kw)
+    return C.byref(_lib.PagedKvDesc(**f))
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(dtype=2), DTYPE), (dict(page_size=0), SHAPE), (dict(page_size=1025), SHAPE), (dict(KVH=0), SHAPE),
+    (dict(k=P + 2), ALIGN), (dict(sv_s=60), ALIGN), (dict(k=None), ARG), (dict(num_pages=-1), ARG), (dict(D=-8), ARG),
+])
+def test_c_pool_checks(kw, status):
+    lib = _lib.load()
+    assert lib.b2d_paged_attention(desc(**kw), P, 256, 256, 64, P, 3, 3, P, None, 0, 0, 1, 1, 4, 1.0, P, 256, 256, 64, 0,
+                                   None, 0, 0, None) == status
+    assert lib.b2d_paged_rope_append(desc(**kw), P, 256, 64, P, 128, 64, P, 128, 64, P, None, P, 3, 3, 1, P, P, 64, 32, 0,
+                                     None, None, 1e-6, P, 256, 64, 1, 4, 0, None) == status
+
+
+def test_c_attention_checks():
+    lib = _lib.load()
+
+    def call(d=None, q=P, sq=(256, 256, 64), table=P, ld=3, per=3, lens=P, pt=None, pl=0, B=1, T=1, H=4, out=P, odt=0):
+        return lib.b2d_paged_attention(d or desc(), q, *sq, table, ld, per, lens, pt, pl, 0, B, T, H, 1.0, out, 256, 256,
+                                       64, odt, None, 0, 0, None)
+    assert call(B=0) == OK and call(T=0) == OK
+    assert call(d=desc(D=96)) == SHAPE and call(T=17) == SHAPE and call(H=34) == SHAPE and call(H=5) == SHAPE
+    assert call(odt=1) == DTYPE
+    assert call(q=None) == ARG and call(lens=None) == ARG and call(out=None) == ARG and call(table=None) == ARG
+    assert call(pl=4) == ARG and call(pl=-1) == ARG and call(B=-1) == ARG
+    assert call(q=P + 2) == ALIGN and call(sq=(256, 256, 60)) == ALIGN
+    assert call(d=desc(page_size=1024), per=1 << 21) == SHAPE
+
+
+def test_c_append_checks():
+    lib = _lib.load()
+
+    def call(d=None, q=P, ksn=128, pos=P, seq=None, B=1, cs=P, ldcs=64, cdt=0, qw=None, N=1, H=4):
+        return lib.b2d_paged_rope_append(d or desc(), q, 256, 64, P, ksn, 64, P, 128, 64, pos, seq, P, 3, 3, B, cs, P, ldcs,
+                                         32, cdt, qw, None, 1e-6, P, 256, 64, N, H, 0, None)
+    assert call(N=0) == OK
+    assert call(d=desc(D=40)) == SHAPE and call(d=desc(D=272)) == SHAPE and call(H=5) == SHAPE
+    assert call(B=0) == SHAPE and call(N=3, B=2) == SHAPE
+    assert call(cdt=1) == DTYPE and call(N=-1) == ARG and call(q=None) == ARG and call(pos=None) == ARG
+    assert call(ksn=124) == ALIGN and call(ldcs=60) == ALIGN and call(qw=P + 4) == ALIGN and call(cs=P + 8) == ALIGN
+
+
+def test_c_verify_checks():
+    lib = _lib.load()
+
+    def call(draft=P, tp=P, dt=2, u=P, out=P, ldo=5, B=1, K=4, V=10):
+        return lib.b2d_verify_drafts(draft, 4, None, tp, 50, 10, None, 0, 0, dt, u, 5, out, ldo, None, B, K, V, 0, None)
+    assert call(B=0) == OK
+    assert call(K=32, ldo=33) == SHAPE and call(V=0) == SHAPE and call(ldo=4) == SHAPE and call(dt=5) == DTYPE
+    assert call(draft=None) == ARG and call(tp=None) == ARG and call(u=None) == ARG and call(out=None) == ARG
+    assert call(B=-1) == ARG and call(draft=P + 4) == ALIGN and call(tp=P + 2) == ALIGN
+
+
+# ---- the oracle draws from the target's own distribution
+def test_oracle_draws_as_the_target():
+    """Averaging over the drafts' distribution and over a fine grid of the random numbers, the first token
+    is distributed as p[0] exactly (up to the grid's step)."""
+    rng = np.random.default_rng(0)
+    V, n = 5, 400
+    p = rng.dirichlet(np.ones(V), 2)[None]
+    q = rng.dirichlet(np.ones(V), 1)[None]
+    got = np.zeros(V)
+    grid = (np.arange(n) + 0.5) / n
+    for x in range(V):
+        for u in grid:
+            accept = u * q[0, 0, x] < p[0, 0, x]
+            if accept:
+                got[x] += q[0, 0, x] / n
+            else:   # the accepting number only decides; the drawing one spans the grid
+                us = np.stack([np.full(n, u), grid], 1)
+                tok, acc = verify_ref(np.full((n, 1), x), np.repeat(p, n, 0), us, np.repeat(q, n, 0))
+                assert not acc.any()
+                got += np.bincount(tok[:, 0], minlength=V) * q[0, 0, x] / n / n
+    # each of the grid's two averages is off by at most a step per token
+    assert np.abs(got - p[0, 0]).max() <= 2.0 * V / n
+
+
+def test_oracle_edges():
+    p = np.array([[[0.5, 0.0, 0.5], [0.0, 1.0, 0.0]]])
+    same = p[:, :1]
+    # u q = p exactly is a refusal; with p == q nothing is left over, so the draw is from p
+    tok, acc = verify_ref(np.array([[0]]), p, np.array([[1.0, 0.6]]), same)
+    assert acc[0] == 0 and tok.tolist() == [[2, -1]]
+    tok, acc = verify_ref(np.array([[2]]), p, np.array([[0.9, 0.0]]), same)
+    assert acc[0] == 1 and tok.tolist() == [[2, 1]]
+    tok, acc = verify_ref(np.array([[1]]), p, np.array([[0.0, 0.999]]))   # p = 0 is never accepted
+    assert acc[0] == 0 and tok.tolist() == [[2, -1]]
