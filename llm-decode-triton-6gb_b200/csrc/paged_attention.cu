@@ -5,15 +5,29 @@
 // o[b, t, h] = sum_{j < limit} softmax_j(scale q.k_j) v_j, limit = seqlens[b] - T + 1 + t. Key j lies in
 // prefix_table's pages for j < prefix_len and in page_table[b]'s behind.
 //
-// A CTA owns one (sequence, KV head, tile of 16 RW rows): rows are the T x G query vectors that read this KV
-// head (row = t G + g), so K and V are read once for all of them. Stages of 64 keys pass through a 3-stage
-// shared-memory ring filled by 16-byte cp.async (each thread looks the page of its key rows up, keys at or
-// past the length are zero-filled without a read, so what a page holds behind its last key never enters).
-// 16-byte chunk c of key row r sits at chunk c ^ (r & 7), so ldmatrix reads hit 8 distinct bank groups.
-// S = Q K^T and O += P V by mma.sync m16n8k16 (fp32 accumulate): warp (rw, kw) takes rows [16 rw, 16 rw + 16)
-// and keys [kw 16 RW, ...) of each stage; online softmax in the log2 domain; the key warps meet in shared
-// memory. P is rounded to the cache's dtype for the second product, as its V operand is; the sum of the
-// weights is taken before that rounding, in fp32.
+// A CTA owns one (sequence, KV head, tile of 16 RW rows, split of the keys): rows are the T x G query vectors
+// that read this KV head (row = t G + g), so K and V are read once for all of them. Stages of 64 keys pass
+// through a 3-stage shared-memory ring filled by 16-byte cp.async (the page ids of a stage are looked up one
+// stage ahead; keys at or past the length are zero-filled without a read, so what a page holds behind its
+// last key never enters). 16-byte chunk c of key row r sits at chunk c ^ (r & 7), so ldmatrix reads hit 8
+// distinct bank groups. S = Q K^T and O += P V by mma.sync m16n8k16 (fp32 accumulate): warp (rw, kw) takes
+// rows [16 rw, 16 rw + 16) and its share of each stage's keys; online softmax in the log2 domain; the key
+// warps meet in shared memory. P is rounded to the cache's dtype for the second product, as its V operand
+// is; the sum of the weights is taken before that rounding, in fp32.
+//
+// Splits: the sequence's own length on the device is divided evenly over the splits, so a ragged batch needs
+// no host knowledge of its lengths. The splits of one (sequence, KV head, row tile) form a thread-block
+// cluster of up to 8 CTAs that meet through distributed shared memory, so the common case is one launch
+// without scratch; longer work takes several clusters, which leave (unnormalised O, m, l) in the workspace
+// for a small combine kernel.
+//
+// Shared prefix: a first launch (PREFIX) takes all sequences' rows as one row axis, [0, B T G), over the
+// prefix's pages, and leaves (O, m, l) per row and split; the per-sequence kernel starts behind the prefix
+// and takes those partials in at its end. It is launched as a programmatic dependent and waits for the
+// prefix launch only there. A sequence with a query that does not see the whole prefix is computed by the
+// per-sequence kernel alone, from position 0.
+#include <type_traits>
+
 #include "paged.cuh"
 
 namespace b2d {
@@ -36,7 +50,18 @@ struct PagedAttnArgs {
   PageDiv div;
   int pages_per_seq, prefix_len, B, T, H, G, rows;   // rows = T G
   float scale_log2;
+  int shared;       // positions [0, shared) are the prefix launch's (0: there is none)
+  int cs, ncl;      // CTAs of a cluster; clusters of one (sequence, KV head, row tile)
+  int tiles;        // row tiles
+  int nparts;       // partials of the prefix launch
+  int parts;        // nparts + (ncl > 1 ? ncl : 0): partials in the workspace
+  int out_f32, after_prefix;
+  float* acc;       // [parts][B T H][D] unnormalised, row = (b T + t) H + h
+  float* ml;        // [parts][B T H][2] m (log2 domain), l
 };
+
+constexpr int kMaxParts = 32;      // of the prefix launch
+constexpr int kMaxCluster = 8;     // portable size
 
 __device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool valid) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0)
@@ -59,58 +84,118 @@ __device__ __forceinline__ float exp2_fast(float x) {
 template <int D>
 constexpr size_t ring_bytes() { return static_cast<size_t>(kStages) * 2 * kKeys * D * 2; }
 
-template <typename T, typename OT, int D, int RW>
+__device__ __forceinline__ uint32_t map_cluster(uint32_t local, int rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(local), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_cluster_f32x2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];\n" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+// any infinity or NaN among 8 values
+template <typename T>
+__device__ __forceinline__ bool nonfinite8(const uint4& u) {
+  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;   // exponent bits
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bad |= (w[i] & e) == e || (w[i] >> 16 & e) == e;
+  return bad;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_out(const PagedAttnArgs& a, int64_t off, float v) {
+  if (a.out_f32) static_cast<float*>(a.out)[off] = v;
+  else static_cast<T*>(a.out)[off] = Dt<T>::from_f32(v);
+}
+
+template <typename T, int D, int RW, bool PREFIX>
 __global__ void __launch_bounds__(kThreads, 2) paged_attention_kernel(const PagedAttnArgs a) {
   constexpr int KW = kWarps / RW;       // warps that share a row tile and split a stage's keys
   constexpr int WK = kKeys / KW;        // keys of a stage that a warp takes
+  constexpr int ROWS = 16 * RW;
   constexpr int KSTEPS = D / 16, NTILES = D / 8, CH = D / 8;
   constexpr uint32_t ROWB = D * 2, TILEB = kKeys * ROWB;
   constexpr int OPAD = D + 8;
   constexpr int LOADS = kKeys * CH / kThreads;   // key rows of a stage that a thread copies a chunk of
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float s_m[kWarps][16], s_l[kWarps][16];
+  __shared__ float2 s_ml[ROWS];         // this CTA's (m, l) per row, read by the cluster
+  __shared__ unsigned long long s_bad[2];
 
-  pdl_launch_dependents();
-  pdl_wait();
-  const int row0 = blockIdx.x * 16 * RW, kvh = blockIdx.y, b = blockIdx.z;
+  if constexpr (PREFIX) {   // the dependent launch reads the same inputs: it starts once they are complete
+    pdl_wait();
+    pdl_launch_dependents();
+  } else {
+    if (!a.after_prefix) pdl_wait();
+    pdl_launch_dependents();
+  }
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rw = warp % RW, kw = warp / RW;
   const int g = lane >> 2, tq = lane & 3, mi = lane >> 3, ri = lane & 7;
+  const int nsplit = a.cs * a.ncl;
+  const int split = static_cast<int>(blockIdx.x) % nsplit, tile = static_cast<int>(blockIdx.x) / nsplit;
+  const int rank = split % a.cs;
+  const int row0 = tile * ROWS, kvh = blockIdx.y, b = PREFIX ? 0 : blockIdx.z;
+  const int rows = PREFIX ? a.B * a.rows : a.rows;
+  const int row_end = min(rows, row0 + ROWS);
   const uint32_t sbase = smem_u32(smem);
   const T* kpool = static_cast<const T*>(a.kv.k) + kvh * a.kv.sk_h;
   const T* vpool = static_cast<const T*>(a.kv.v) + kvh * a.kv.sv_h;
-  const int32_t* table = a.table + b * a.ld_table;
+  const int32_t* table = PREFIX ? a.prefix_table : a.table + b * a.ld_table;
+  if (tid < 2) s_bad[tid] = 0;
 
-  const int64_t reach = static_cast<int64_t>(a.pages_per_seq) * a.kv.page_size;
-  int len = max(a.seqlens[b], 0);
-  if (len > reach) len = max(static_cast<int>(reach), a.prefix_len);
-  const int row_end = min(a.rows, row0 + 16 * RW);
-  // keys that any row of the tile sees; limits of this thread's two rows
-  const int t_last = (row_end - 1) / a.G;
-  const int t_end = max(0, len - a.T + 1 + t_last);
-  int lim[2];
+  // keys of the tile's rows [k_begin, k_end), this split's share [t_begin, t_end), limits of this thread's rows
+  int k_begin = 0, k_end = a.shared, lim_min = a.shared, lim[2] = {a.shared, a.shared};
+  bool shares = false;
+  if constexpr (!PREFIX) {
+    const int64_t reach = static_cast<int64_t>(a.pages_per_seq) * a.kv.page_size;
+    int len = max(a.seqlens[b], 0);
+    if (len > reach) len = max(static_cast<int>(reach), a.prefix_len);
+    shares = len - a.T + 1 >= a.shared && len > 0;
+    k_begin = shares ? a.shared : 0;
+    k_end = max(0, len - a.T + 1 + (row_end - 1) / a.G);
+    lim_min = len - a.T + 1 + row0 / a.G;   // below it no row is masked
 #pragma unroll
-  for (int h = 0; h < 2; ++h) lim[h] = len - a.T + 1 + min(row0 + 16 * rw + g + 8 * h, row_end - 1) / a.G;
-  const int lim_min = len - a.T + 1 + row0 / a.G;   // below it no row is masked
+    for (int h = 0; h < 2; ++h) lim[h] = len - a.T + 1 + min(row0 + 16 * rw + g + 8 * h, row_end - 1) / a.G;
+  }
+  const int stages = (max(0, k_end - k_begin) + kKeys - 1) / kKeys;
+  const int st0 = static_cast<int>(static_cast<int64_t>(stages) * split / nsplit);
+  const int nst = static_cast<int>(static_cast<int64_t>(stages) * (split + 1) / nsplit) - st0;
+  const int t_begin = k_begin + st0 * kKeys, t_end = min(k_end, t_begin + nst * kKeys);
 
+  int pid[LOADS];
+  auto lookup = [&](int it) {   // page ids of stage `it`'s keys; -1: not read
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int tok = t_begin + it * kKeys + (tid + i * kThreads) / CH;
+      pid[i] = -1;
+      if (tok < t_end) {
+        const int pi = a.div.page(tok);
+        pid[i] = __ldg((PREFIX || tok >= a.prefix_len ? table : a.prefix_table) + pi);
+      }
+    }
+  };
   auto issue = [&](int it) {
     const uint32_t kdst = sbase + static_cast<uint32_t>(it % kStages) * 2 * TILEB, vdst = kdst + TILEB;
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       const int ci = tid + i * kThreads, r = ci / CH, c = ci % CH;
-      const int tok = it * kKeys + r;
+      const int tok = t_begin + it * kKeys + r;
       const T* ks = kpool;
       const T* vs = vpool;
-      bool ok = tok < t_end;
+      const bool ok = pid[i] >= 0 && pid[i] < a.kv.num_pages;
       if (ok) {
-        const int pi = a.div.page(tok);
-        const int page = tok < a.prefix_len ? a.prefix_table[pi] : table[pi];
-        ok = page >= 0 && page < a.kv.num_pages;
-        if (ok) {
-          const int64_t slot = a.div.slot(tok, pi);
-          ks += page * a.kv.sk_p + slot * a.kv.sk_s + c * 8;
-          vs += page * a.kv.sv_p + slot * a.kv.sv_s + c * 8;
-        }
+        const int64_t slot = a.div.slot(tok, a.div.page(tok));
+        ks += pid[i] * a.kv.sk_p + slot * a.kv.sk_s + c * 8;
+        vs += pid[i] * a.kv.sv_p + slot * a.kv.sv_s + c * 8;
       }
       const uint32_t off = static_cast<uint32_t>(r) * ROWB + static_cast<uint32_t>((c ^ (r & 7)) * 16);
       cp_async16_zfill(kdst + off, ks, ok);
@@ -118,10 +203,12 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attention_kernel(const Page
     }
   };
 
-  const int nst = (t_end + kKeys - 1) / kKeys;
+  lookup(0);
+#pragma unroll
   for (int i = 0; i < kStages - 1; ++i) {
     if (i < nst) issue(i);
     cp_async_commit();
+    lookup(i + 1);
   }
 
   // Q fragments of this warp's 16 rows
@@ -129,9 +216,10 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attention_kernel(const Page
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int row = row0 + 16 * rw + g + 8 * h;
-    const bool live = row < a.rows;
-    const int t = row / a.G, head = kvh * a.G + row - t * a.G;
-    const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.q) + b * a.sq_b + t * a.sq_t +
+    const bool live = row < rows;
+    const int qb = PREFIX ? row / a.rows : b, qr = PREFIX ? row - qb * a.rows : row;
+    const int t = qr / a.G, head = kvh * a.G + qr - t * a.G;
+    const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.q) + qb * a.sq_b + t * a.sq_t +
                                                             static_cast<int64_t>(head) * a.sq_h);
 #pragma unroll
     for (int j = 0; j < KSTEPS; ++j) {
@@ -151,10 +239,36 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attention_kernel(const Page
     __syncthreads();
     if (it + kStages - 1 < nst) issue(it + kStages - 1);
     cp_async_commit();
-    const int key0 = it * kKeys + kw * WK;
-    if (key0 >= t_end) continue;
+    lookup(it + kStages);
+    const int stage0 = t_begin + it * kKeys;
     const uint32_t kbuf = sbase + static_cast<uint32_t>(it % kStages) * 2 * TILEB, vbuf = kbuf + TILEB;
-    const bool masked = key0 + WK > lim_min;
+
+    // Keys that some rows of the tile see and others do not (the newest T - 1): a zero weight times an
+    // infinite or NaN value would reach the rows that must not see it. Such value rows (rare) are taken out
+    // of the stage and added to the rows that do see them one by one below. At most two stages hold any.
+    unsigned long long bad = 0;
+    if (!PREFIX && a.T > 1 && min(stage0 + kKeys, t_end) > lim_min) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int ci = tid + i * kThreads, r = ci / CH, c = ci % CH;
+        if (stage0 + r < lim_min || stage0 + r >= t_end) continue;
+        const uint4 x = *reinterpret_cast<const uint4*>(smem + (vbuf - sbase) + r * ROWB + ((c ^ (r & 7)) * 16));
+        if (nonfinite8<T>(x)) atomicOr(&s_bad[it & 1], 1ull << r);
+      }
+      __syncthreads();
+      bad = s_bad[it & 1];
+      if (bad) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+          const int ci = tid + i * kThreads, r = ci / CH, c = ci % CH;
+          if (bad >> r & 1) *reinterpret_cast<uint4*>(smem + (vbuf - sbase) + r * ROWB + c * 16) = make_uint4(0, 0, 0, 0);
+        }
+        __syncthreads();
+      }
+    }
+    const int key0 = stage0 + kw * WK;
+    if (key0 >= t_end) continue;
+    const bool masked = !PREFIX ? key0 + WK > min(lim_min, t_end) : key0 + WK > t_end;
 
     float s[WK / 8][4];
     float tmax[2] = {-INFINITY, -INFINITY};
@@ -174,7 +288,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attention_kernel(const Page
       for (int c = 0; c < 4; ++c) {
         const int tok = key0 + 8 * n + 2 * tq + (c & 1);
         s[n][c] *= a.scale_log2;
-        if (masked && tok >= lim[c >> 1]) s[n][c] = -INFINITY;
+        if (masked && (tok >= lim[c >> 1] || tok >= t_end)) s[n][c] = -INFINITY;
         tmax[c >> 1] = fmaxf(tmax[c >> 1], s[n][c]);
       }
     }
@@ -216,10 +330,34 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attention_kernel(const Page
         Mma<T>::run(o[np + 1], pa[0], pa[1], pa[2], pa[3], v2, v3);
       }
     }
+    if (!PREFIX && bad) {   // the value rows taken out above, for the rows that see them
+#pragma unroll
+      for (int n = 0; n < WK / 8; ++n) {
+        for (int col = 0; col < 8; ++col) {
+          const int r = kw * WK + 8 * n + col;
+          if (!(bad >> r & 1)) continue;
+          const int src = (lane & ~3) | (col >> 1);
+          const float p0 = __shfl_sync(0xffffffffu, (col & 1) ? s[n][1] : s[n][0], src);
+          const float p1 = __shfl_sync(0xffffffffu, (col & 1) ? s[n][3] : s[n][2], src);
+          const int tok = stage0 + r, pi = a.div.page(tok);
+          const int page = (tok >= a.prefix_len ? table : a.prefix_table)[pi];
+          const T* v = vpool + page * a.kv.sv_p + a.div.slot(tok, pi) * a.kv.sv_s + 2 * tq;
+#pragma unroll
+          for (int d = 0; d < NTILES; ++d)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float x = Dt<T>::to_f32(v[8 * d + e]);
+              if (tok < lim[0]) o[d][e] += p0 * x;
+              if (tok < lim[1]) o[d][2 + e] += p1 * x;
+            }
+        }
+      }
+    }
   }
   cp_async_wait<0>();
   __syncthreads();   // the ring becomes the merge buffer
 
+  // ---- the key warps meet: s_o[row] unnormalised, s_ml[row] = (m, l)
   float* s_o = reinterpret_cast<float*>(smem);   // [kWarps][16][OPAD]
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
@@ -236,48 +374,253 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attention_kernel(const Page
       *reinterpret_cast<float2*>(dst + 8 * n) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
   }
   __syncthreads();
-
-  for (int idx = tid; idx < (row_end - row0) * D; idx += kThreads) {
-    const int row = idx / D, d = idx - row * D;
-    const int w0 = row / 16, rr = row % 16;
-    float mx = -INFINITY;
+  const int nrows = row_end - row0;
+  if (tid < nrows) {
+    const int w0 = tid / 16, rr = tid % 16;
+    float mx = -INFINITY, l = 0.f;
 #pragma unroll
     for (int k = 0; k < KW; ++k) mx = fmaxf(mx, s_m[k * RW + w0][rr]);
-    float num = 0.f, den = 0.f;
 #pragma unroll
     for (int k = 0; k < KW; ++k) {
       const int w = k * RW + w0;
       const float e = s_m[w][rr] == -INFINITY ? 0.f : exp2_fast(s_m[w][rr] - mx);
-      num += e * s_o[(w * 16 + rr) * OPAD + d];
-      den += e * s_l[w][rr];
+      l += e * s_l[w][rr];
+      s_m[w][rr] = e;   // the warp's factor
     }
-    const int t = (row0 + row) / a.G, head = kvh * a.G + row0 + row - t * a.G;
-    // a row that sees no key: zeros (den is NaN, not 0, where a visible score is)
-    static_cast<OT*>(a.out)[b * a.so_b + t * a.so_t + static_cast<int64_t>(head) * a.so_h + d] =
-        Dt<OT>::from_f32(den == 0.f ? 0.f : num / den);
+    s_ml[tid] = make_float2(mx, l);
   }
+  __syncthreads();
+  if constexpr (KW > 1) {
+    for (int idx = tid; idx < nrows * D; idx += kThreads) {
+      const int row = idx / D, d = idx - row * D, w0 = row / 16, rr = row % 16;
+      float v = 0.f;
+#pragma unroll
+      for (int k = 0; k < KW; ++k) v += s_m[k * RW + w0][rr] * s_o[((k * RW + w0) * 16 + rr) * OPAD + d];
+      s_o[row * OPAD + d] = v;   // (w0, rr) of key warp 0: this thread's own element
+    }
+  }
+  if (a.cs > 1) cluster_sync();
+  else __syncthreads();
+  if constexpr (!PREFIX) {
+    if (a.after_prefix) pdl_wait();   // the prefix launch's partials
+  }
+
+  // ---- the cluster meets (and, in the last stop, the prefix's partials): entries e < cs are the cluster's
+  // CTAs, the others workspace partials; s_w[e][row] = (m, l), then the entry's factor
+  const bool last = !PREFIX && a.ncl == 1;
+  const int np = last && shares ? a.nparts : 0, ne = a.cs + np;
+  const int64_t all_rows = static_cast<int64_t>(a.B) * a.T * a.H;
+  float2* s_w = reinterpret_cast<float2*>(smem + kWarps * 16 * OPAD * 4);
+  auto out_row = [&](int row) -> int64_t {   // (b T + t) H + h
+    const int r = row0 + row, rb = PREFIX ? r / a.rows : b, rr = PREFIX ? r - rb * a.rows : r, t = rr / a.G;
+    return (static_cast<int64_t>(rb) * a.T + t) * a.H + kvh * a.G + rr - t * a.G;
+  };
+  for (int idx = tid; idx < ne * nrows; idx += kThreads) {
+    const int e = idx / nrows, row = idx - e * nrows;
+    float2 v;
+    if (e < a.cs) v = a.cs > 1 ? ld_cluster_f32x2(map_cluster(smem_u32(&s_ml[row]), e)) : s_ml[row];
+    else v = *reinterpret_cast<const float2*>(a.ml + ((e - a.cs) * all_rows + out_row(row)) * 2);
+    s_w[e * ROWS + row] = v;
+  }
+  __syncthreads();
+  if (tid < nrows) {
+    float mx = -INFINITY, l = 0.f;
+    for (int e = 0; e < ne; ++e) mx = fmaxf(mx, s_w[e * ROWS + tid].x);
+    for (int e = 0; e < ne; ++e) {
+      const float2 v = s_w[e * ROWS + tid];
+      const float f = v.x == -INFINITY ? 0.f : exp2_fast(v.x - mx);
+      l += f * v.y;
+      s_w[e * ROWS + tid].x = f;
+    }
+    // a row that sees no key: zeros (l is NaN, not 0, where a visible score is)
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    for (int e = 0; e < ne; ++e) s_w[e * ROWS + tid].y = s_w[e * ROWS + tid].x * inv;
+    if (!last && rank == 0) {
+      const int64_t part = PREFIX ? split / a.cs : a.nparts + split / a.cs;
+      *reinterpret_cast<float2*>(a.ml + (part * all_rows + out_row(tid)) * 2) = make_float2(mx, l);
+    }
+  }
+  __syncthreads();
+  for (int idx = rank * kThreads + tid; idx < nrows * D; idx += a.cs * kThreads) {
+    const int row = idx / D, d = idx - row * D;
+    const int64_t orow = out_row(row);
+    float v = 0.f;
+    const uint32_t local = smem_u32(s_o + row * OPAD + d);
+    for (int e = 0; e < a.cs; ++e) {
+      const float x = a.cs > 1 ? ld_cluster_f32(map_cluster(local, e)) : s_o[row * OPAD + d];
+      v += (last ? s_w[e * ROWS + row].y : s_w[e * ROWS + row].x) * x;
+    }
+    if (last) {
+      for (int e = 0; e < np; ++e) v += s_w[(a.cs + e) * ROWS + row].y * a.acc[(e * all_rows + orow) * D + d];
+      const int t = (row0 + row) / a.G, head = kvh * a.G + row0 + row - t * a.G;
+      store_out<T>(a, b * a.so_b + t * a.so_t + static_cast<int64_t>(head) * a.so_h + d, v);
+    } else {
+      const int64_t part = PREFIX ? split / a.cs : a.nparts + split / a.cs;
+      a.acc[(part * all_rows + orow) * D + d] = v;
+    }
+  }
+  if (a.cs > 1) cluster_sync_relaxed();   // this CTA's shared memory stays until the others have read it
 }
 
-template <typename T, typename OT, int D, int RW>
-int launch(const PagedAttnArgs& a, bool pdl, cudaStream_t s) {
-  auto kern = paged_attention_kernel<T, OT, D, RW>;
-  constexpr size_t bytes = ring_bytes<D>();
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+// Merges the workspace's partials of a row: one warp per (b, t, h).
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) paged_combine_kernel(const PagedAttnArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t all_rows = static_cast<int64_t>(a.B) * a.T * a.H;
+  const int64_t row = blockIdx.x * static_cast<int64_t>(kWarps) + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row >= all_rows) return;
+  const int h = static_cast<int>(row % a.H);
+  const int64_t bt = row / a.H;
+  const int t = static_cast<int>(bt % a.T), b = static_cast<int>(bt / a.T);
+  int first = 0;   // a sequence that does not share the prefix takes its own partials only
+  if (a.nparts > 0) {
+    const int64_t reach = static_cast<int64_t>(a.pages_per_seq) * a.kv.page_size;
+    int len = max(a.seqlens[b], 0);
+    if (len > reach) len = max(static_cast<int>(reach), a.prefix_len);
+    first = len - a.T + 1 >= a.shared && len > 0 ? 0 : a.nparts;
+  }
+  float mx = -INFINITY;
+  for (int e = first + lane; e < a.parts; e += 32) mx = fmaxf(mx, a.ml[(e * all_rows + row) * 2]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  constexpr int PER = D / 32;
+  float v[PER] = {}, l = 0.f;
+  for (int e = first; e < a.parts; ++e) {
+    const float2 p = *reinterpret_cast<const float2*>(a.ml + (e * all_rows + row) * 2);
+    const float f = p.x == -INFINITY ? 0.f : exp2_fast(p.x - mx);
+    l += f * p.y;
+    const float* src = a.acc + (e * all_rows + row) * D + lane * PER;
+    if constexpr (PER == 4) {
+      const float4 x = *reinterpret_cast<const float4*>(src);
+      v[0] += f * x.x; v[1] += f * x.y; v[2] += f * x.z; v[3] += f * x.w;
+    } else {
+      const float2 x = *reinterpret_cast<const float2*>(src);
+      v[0] += f * x.x; v[1] += f * x.y;
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int64_t off = b * a.so_b + t * a.so_t + static_cast<int64_t>(h) * a.so_h + lane * PER;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) store_out<T>(a, off + i, v[i] * inv);
+}
+
+// ------------------------------------------------------------------ host
+template <typename... KArgs, typename... Args>
+int launch_cluster(void (*kern)(KArgs...), dim3 grid, size_t smem, int cs, bool pdl, cudaStream_t s, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (cs > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = cs;
+    attr[n].val.clusterDim.y = 1;
+    attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (pdl) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
   if (e != cudaSuccess) {
     set_cuda_error(e);
     return B2D_ERR_LAUNCH;
   }
-  const dim3 grid((a.rows + 16 * RW - 1) / (16 * RW), a.kv.KVH, a.B);
-  return launch_kernel(kern, grid, dim3(kThreads), bytes, s, pdl, a);
+  return launch_status();
 }
-template <typename T, typename OT>
-int launch_shape(const PagedAttnArgs& a, bool pdl, cudaStream_t s) {
-  const int rw = a.rows <= 16 ? 1 : a.rows <= 32 ? 2 : 4;
-  if (a.kv.D == 64)
-    return rw == 1 ? launch<T, OT, 64, 1>(a, pdl, s) : rw == 2 ? launch<T, OT, 64, 2>(a, pdl, s)
-                                                               : launch<T, OT, 64, 4>(a, pdl, s);
-  return rw == 1 ? launch<T, OT, 128, 1>(a, pdl, s) : rw == 2 ? launch<T, OT, 128, 2>(a, pdl, s)
-                                                              : launch<T, OT, 128, 4>(a, pdl, s);
+
+template <typename T, int D, int RW, bool PREFIX>
+int launch(const PagedAttnArgs& a, bool pdl, cudaStream_t s) {
+  auto kern = paged_attention_kernel<T, D, RW, PREFIX>;
+  constexpr size_t bytes = ring_bytes<D>();
+  static_assert(kWarps * 16 * (D + 8) * 4 + (kMaxParts + kMaxCluster) * 16 * RW * 8 <= bytes, "merge buffers fit the ring");
+  static bool configured[64] = {};   // per device; setting it twice is harmless
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+    if (e != cudaSuccess) {
+      set_cuda_error(e);
+      return B2D_ERR_LAUNCH;
+    }
+    if (dev >= 0 && dev < 64) configured[dev] = true;
+  }
+  const dim3 grid(a.tiles * a.cs * a.ncl, a.kv.KVH, PREFIX ? 1 : a.B);
+  return launch_cluster(kern, grid, bytes, a.cs, pdl, s, a);
+}
+template <typename T, int D, bool PREFIX>
+int launch_rows(const PagedAttnArgs& a, int rw, bool pdl, cudaStream_t s) {
+  if (rw == 1) return launch<T, D, 1, PREFIX>(a, pdl, s);
+  if (rw == 2) return launch<T, D, 2, PREFIX>(a, pdl, s);
+  return launch<T, D, 4, PREFIX>(a, pdl, s);
+}
+
+// How a call is cut: the prefix launch's splits and the per-sequence kernel's clusters.
+struct Plan {
+  int shared, rows_p, rw_p, tiles_p, cs_p, ncl_p, rw, tiles, cs, ncl, parts;
+  size_t bytes;
+};
+
+int row_warps(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+
+// Splits over the keys for `groups` independent row tiles: about two CTAs per SM in all, at least 128 keys
+// each; up to 8 form a cluster.
+void split_keys(int64_t groups, int64_t keys, int sm, int most, int* cs, int* ncl) {
+  int64_t want = 2 * sm / groups;
+  const int64_t room = (keys + 127) / 128;
+  if (want > room) want = room;
+  if (want < 1) want = 1;
+  *cs = 1;
+  while (*cs < kMaxCluster && *cs * 2 <= want) *cs *= 2;
+  int64_t n = *cs == kMaxCluster ? want / kMaxCluster : 1;
+  if (n > most) n = most;
+  *ncl = static_cast<int>(n < 1 ? 1 : n);
+}
+
+Plan make_plan(const b2d_paged_kv* kv, int B, int T, int H, int pages_per_seq, int prefix_len, int max_len, int sm) {
+  Plan p{};
+  const int64_t reach = static_cast<int64_t>(pages_per_seq) * kv->page_size;
+  const int64_t rows = static_cast<int64_t>(T) * (H / kv->KVH);
+  p.shared = B > 1 ? prefix_len : 0;   // one sequence: nothing to share
+  p.rw = row_warps(rows);
+  p.tiles = static_cast<int>((rows + 16 * p.rw - 1) / (16 * p.rw));
+  int64_t keys = max_len > 0 && max_len < reach ? max_len : reach;
+  if (keys < prefix_len) keys = prefix_len;
+  split_keys(static_cast<int64_t>(B) * kv->KVH * p.tiles, keys - p.shared, sm, kMaxParts, &p.cs, &p.ncl);
+  p.rw_p = row_warps(B * rows);
+  p.tiles_p = static_cast<int>((B * rows + 16 * p.rw_p - 1) / (16 * p.rw_p));
+  if (p.shared > 0)
+    split_keys(static_cast<int64_t>(kv->KVH) * p.tiles_p, p.shared, sm, kMaxParts, &p.cs_p, &p.ncl_p);
+  p.parts = p.ncl_p + (p.ncl > 1 ? p.ncl : 0);
+  p.bytes = static_cast<size_t>(p.parts) * B * T * H * (kv->D + 2) * 4;
+  return p;
+}
+
+template <typename T, int D>
+int run(PagedAttnArgs& a, const Plan& p, bool pdl, cudaStream_t s) {
+  int st;
+  if (p.shared > 0) {
+    PagedAttnArgs ap = a;
+    ap.tiles = p.tiles_p; ap.cs = p.cs_p; ap.ncl = p.ncl_p;
+    if ((st = launch_rows<T, D, true>(ap, p.rw_p, pdl, s)) != B2D_OK) return st;
+    a.after_prefix = 1;
+  }
+  if ((st = launch_rows<T, D, false>(a, p.rw, pdl || a.after_prefix, s)) != B2D_OK) return st;
+  if (p.ncl > 1) {
+    const int64_t rows = static_cast<int64_t>(a.B) * a.T * a.H;
+    st = launch_kernel(paged_combine_kernel<T, D>, dim3(static_cast<unsigned>((rows + kWarps - 1) / kWarps)),
+                       dim3(kThreads), 0, s, true, a);
+  }
+  return st;
 }
 
 int check_shapes(const b2d_paged_kv* kv, int B, int T, int H, int pages_per_seq, int prefix_len, int max_len) {
@@ -297,8 +640,10 @@ using namespace b2d;
 
 extern "C" size_t b2d_paged_attention_workspace_bytes(const b2d_paged_kv* kv, int B, int T, int H, int pages_per_seq,
                                                       int prefix_len, int max_len) {
-  if (check_shapes(kv, B, T, H, pages_per_seq, prefix_len, max_len) != B2D_OK) return 0;
-  return 0;
+  if (check_shapes(kv, B, T, H, pages_per_seq, prefix_len, max_len) != B2D_OK || B == 0 || T == 0 || H == 0) return 0;
+  DeviceInfo di;
+  if (device_info(&di) != B2D_OK) return 0;
+  return make_plan(kv, B, T, H, pages_per_seq, prefix_len, max_len, di.sm_count).bytes;
 }
 
 extern "C" int b2d_paged_attention(const b2d_paged_kv* kv, const void* q, int64_t sq_b, int64_t sq_t, int64_t sq_h,
@@ -319,6 +664,11 @@ extern "C" int b2d_paged_attention(const b2d_paged_kv* kv, const void* q, int64_
     return B2D_ERR_ALIGN;
   DeviceInfo di;
   if ((st = device_info(&di)) != B2D_OK) return st;
+  const Plan p = make_plan(kv, B, T, H, pages_per_seq, prefix_len, max_len, di.sm_count);
+  if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes)) return B2D_ERR_WORKSPACE;
+  if (!aligned(workspace, 16)) return B2D_ERR_ALIGN;
+  if (static_cast<int64_t>(B) * T * H >= (int64_t(1) << 31) || static_cast<int64_t>(p.tiles_p) * p.cs_p * p.ncl_p >= (int64_t(1) << 31))
+    return B2D_ERR_SHAPE;
   PagedAttnArgs a{};
   a.q = q; a.sq_b = sq_b; a.sq_t = sq_t; a.sq_h = sq_h;
   a.table = page_table; a.ld_table = ld_table; a.seqlens = seqlens; a.prefix_table = prefix_table;
@@ -327,10 +677,12 @@ extern "C" int b2d_paged_attention(const b2d_paged_kv* kv, const void* q, int64_
   a.pages_per_seq = pages_per_seq; a.prefix_len = prefix_len;
   a.B = B; a.T = T; a.H = H; a.G = H / kv->KVH; a.rows = T * a.G;
   a.scale_log2 = scale * kLog2e;
+  a.shared = p.shared; a.cs = p.cs; a.ncl = p.ncl; a.tiles = p.tiles; a.nparts = p.ncl_p; a.parts = p.parts;
+  a.out_f32 = out_dtype == B2D_F32;
+  a.acc = static_cast<float*>(workspace);
+  a.ml = a.acc ? a.acc + static_cast<int64_t>(p.parts) * B * T * H * kv->D : nullptr;
   const bool pdl = (flags & B2D_LAUNCH_PDL) != 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (kv->dtype == B2D_F16)
-    return out_dtype == B2D_F32 ? launch_shape<__half, float>(a, pdl, s) : launch_shape<__half, __half>(a, pdl, s);
-  return out_dtype == B2D_F32 ? launch_shape<__nv_bfloat16, float>(a, pdl, s)
-                              : launch_shape<__nv_bfloat16, __nv_bfloat16>(a, pdl, s);
+  if (kv->dtype == B2D_F16) return kv->D == 64 ? run<__half, 64>(a, p, pdl, s) : run<__half, 128>(a, p, pdl, s);
+  return kv->D == 64 ? run<__nv_bfloat16, 64>(a, p, pdl, s) : run<__nv_bfloat16, 128>(a, p, pdl, s);
 }
