@@ -19,7 +19,7 @@ CSRC = PKG_ROOT / "csrc"
 INCLUDE = REPO_ROOT / "include"
 LIB_PATH = PKG_ROOT / "b200kernels" / "libb200decode.so"
 SOURCES = ["capi.cu", "nf4_gemm.cu", "nf4_gemm_tma.cu", "nf4_tc5.cu", "nf4_format.cu", "gqa_decode.cu", "decode_glue.cu", "tp_allreduce.cu", "lm_head.cu",
-           "paged_append.cu", "paged_attention.cu", "verify_drafts.cu"]
+           "paged_append.cu", "paged_attention.cu", "paged_prefix.cu", "verify_drafts.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

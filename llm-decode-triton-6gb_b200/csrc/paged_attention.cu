@@ -31,7 +31,7 @@
 #include <mutex>
 #include <type_traits>
 
-#include "paged.cuh"
+#include "paged_attention.cuh"
 #include "pipeline.cuh"
 
 namespace b2d {
@@ -45,38 +45,11 @@ constexpr int kStages = 3;
 constexpr int kMaxT = 16, kMaxG = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 
-struct PagedAttnArgs {
-  const void* q; int64_t sq_b, sq_t, sq_h;
-  const int32_t* table; int64_t ld_table;
-  const int32_t* seqlens;
-  const int32_t* prefix_table;
-  void* out; int64_t so_b, so_t, so_h;
-  b2d_paged_kv kv;
-  PageDiv div;
-  int pages_per_seq, prefix_len, B, T, H, G, rows;   // rows = T G
-  float scale_log2;
-  int shared;       // positions [0, shared) are the prefix launch's (0: there is none)
-  int cs, ncl;      // CTAs of a cluster; clusters of one (sequence, KV head, row tile)
-  int tiles;        // row tiles
-  int nparts;       // partials of the prefix launch
-  int parts;        // nparts + (ncl > 1 ? ncl : 0): partials in the workspace
-  int out_f32, after_prefix;
-  int box_rows;     // key rows of a tensor copy; 0: the pages take cp.async
-  float* acc;       // [parts][B T H][D] unnormalised, row = (b T + t) H + h
-  float* ml;        // [parts][B T H][2] m (log2 domain), l
-};
-
-constexpr int kMaxParts = 32;      // of the prefix launch
 constexpr int kMaxCluster = 8;     // portable size
 
 constexpr size_t kRingBytes = static_cast<size_t>(kStages) * kStageBytes;
 template <int D>
 __host__ __device__ constexpr int stage_keys() { return kStageBytes / (2 * D * 2); }
-
-// Tensor maps of the pools: [pages][heads][slots][D], boxes of 64 elements x box_rows slots.
-struct PoolMaps {
-  CUtensorMap k, v;
-};
 
 __device__ __forceinline__ uint32_t map_cluster(uint32_t local, int rank) {
   uint32_t r;
@@ -647,7 +620,7 @@ int box_rows(const b2d_paged_kv& kv, int prefix_len) {
 
 // How a call is cut: the prefix launch's splits and the per-sequence kernel's clusters.
 struct Plan {
-  int shared, rows_p, rw_p, tiles_p, cs_p, ncl_p, rw, tiles, cs, ncl, parts;
+  int shared, tc5, rw_p, tiles_p, cs_p, ncl_p, nparts, rw, tiles, cs, ncl, parts;
   size_t bytes;
 };
 
@@ -679,9 +652,22 @@ Plan make_plan(const b2d_paged_kv* kv, int B, int T, int H, int pages_per_seq, i
   split_keys(static_cast<int64_t>(B) * kv->KVH * p.tiles, keys - p.shared, sm, kMaxParts, &p.cs, &p.ncl);
   p.rw_p = row_warps(B * rows);
   p.tiles_p = static_cast<int>((B * rows + 16 * p.rw_p - 1) / (16 * p.rw_p));
-  if (p.shared > 0)
+  p.tc5 = p.shared >= 128 && B * rows > 64 && box_rows(*kv, prefix_len) > 0;
+  if (p.tc5) {
+    // one CTA per SM, at least two tiles of 128 keys each
+    const int64_t groups = kv->KVH * ((B * rows + 255) / 256), tiles = (p.shared + 127) / 128;
+    const int per = B * rows > 128 ? 1 : 2;   // partials of a CTA
+    int64_t n = sm / groups;
+    if (n > tiles / 2) n = tiles / 2;
+    if (n > kMaxParts / per) n = kMaxParts / per;
+    p.cs_p = 1;
+    p.ncl_p = static_cast<int>(n < 1 ? 1 : n);
+    p.nparts = p.ncl_p * per;
+  } else if (p.shared > 0) {
     split_keys(static_cast<int64_t>(kv->KVH) * p.tiles_p, p.shared, sm, kMaxParts, &p.cs_p, &p.ncl_p);
-  p.parts = p.ncl_p + (p.ncl > 1 ? p.ncl : 0);
+    p.nparts = p.ncl_p;
+  }
+  p.parts = p.nparts + (p.ncl > 1 ? p.ncl : 0);
   p.bytes = static_cast<size_t>(p.parts) * B * T * H * (kv->D + 2) * 4;
   return p;
 }
@@ -696,7 +682,13 @@ int run(PagedAttnArgs& a, const Plan& p, bool pdl, cudaStream_t s) {
   if (p.shared > 0) {
     PagedAttnArgs ap = a;
     ap.tiles = p.tiles_p; ap.cs = p.cs_p; ap.ncl = p.ncl_p;
-    if ((st = launch_rows<T, D, true>(maps, ap, p.rw_p, pdl, s)) != B2D_OK) return st;
+    if (p.tc5 && a.box_rows) {
+      st = launch_prefix_tc5(maps, ap, pdl, s);
+    } else {
+      if (p.tc5) ap.ncl = p.nparts;   // tensor maps refused: as many partials from the other kernel
+      st = launch_rows<T, D, true>(maps, ap, p.rw_p, pdl, s);
+    }
+    if (st != B2D_OK) return st;
     a.after_prefix = 1;
   }
   if ((st = launch_rows<T, D, false>(maps, a, p.rw, pdl || a.after_prefix, s)) != B2D_OK) return st;
@@ -762,7 +754,7 @@ extern "C" int b2d_paged_attention(const b2d_paged_kv* kv, const void* q, int64_
   a.pages_per_seq = pages_per_seq; a.prefix_len = prefix_len;
   a.B = B; a.T = T; a.H = H; a.G = H / kv->KVH; a.rows = T * a.G;
   a.scale_log2 = scale * kLog2e;
-  a.shared = p.shared; a.cs = p.cs; a.ncl = p.ncl; a.tiles = p.tiles; a.nparts = p.ncl_p; a.parts = p.parts;
+  a.shared = p.shared; a.cs = p.cs; a.ncl = p.ncl; a.tiles = p.tiles; a.nparts = p.nparts; a.parts = p.parts;
   a.out_f32 = out_dtype == B2D_F32;
   a.box_rows = box_rows(*kv, prefix_len);
   a.acc = static_cast<float*>(workspace);
