@@ -119,9 +119,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) paged_prefix_kernel(const _
 
   const int rows = a.B * a.rows;
   const bool pair = rows > kTile;          // two row tiles; else one, whose key tiles the warpgroups share
-  const int kvh = blockIdx.y, split = blockIdx.x % a.ncl, row0 = static_cast<int>(blockIdx.x) / a.ncl * (2 * kTile);
+  const int kvh = blockIdx.y, split = blockIdx.x % a.splits, row0 = static_cast<int>(blockIdx.x) / a.splits * (2 * kTile);
   const int ktiles = (a.shared + kTile - 1) / kTile;
-  const int t0 = ktiles * split / a.ncl, n = ktiles * (split + 1) / a.ncl - t0;   // this split's key tiles
+  const int t0 = ktiles * split / a.splits, n = ktiles * (split + 1) / a.splits - t0;   // this split's key tiles
   if (tid == 0) {
     for (int i = 0; i < kRing; ++i) {
       mbar_init(full + 8 * i, 1);
@@ -394,7 +394,7 @@ int launch(const PoolMaps& maps, const PagedAttnArgs& a, bool pdl, cudaStream_t 
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
   const unsigned row_pairs = (a.B * a.rows + 2 * kTile - 1) / (2 * kTile);
-  return launch_kernel(kern, dim3(row_pairs * a.ncl, a.kv.KVH), dim3(kPrefixThreads), bytes, s, pdl, maps, a);
+  return launch_kernel(kern, dim3(row_pairs * a.splits, a.kv.KVH), dim3(kPrefixThreads), bytes, s, pdl, maps, a);
 }
 
 }  // namespace

@@ -67,5 +67,14 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 template <int ID, int THREADS>
 __device__ __forceinline__ void named_sync() { asm volatile("bar.sync %0, %1;\n" ::"n"(ID), "n"(THREADS) : "memory"); }
+// named_sync that also tells every thread whether `p` held for all of them
+template <int ID, int THREADS>
+__device__ __forceinline__ bool named_all(bool p) {
+  uint32_t r;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.and.pred q, %2, %3, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+      : "=r"(r) : "r"(p ? 1u : 0u), "n"(ID), "n"(THREADS) : "memory");
+  return r != 0;
+}
 
 }  // namespace b2d
