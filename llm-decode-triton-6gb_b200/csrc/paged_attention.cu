@@ -41,16 +41,17 @@ constexpr int kThreads = kConsumers + 32;       // and the producer warp
 constexpr int kSlotBytes = 16 * 1024;           // K or V of a stage
 constexpr int kSlots = 5;
 constexpr int kMaxT = 16, kMaxG = 16;
-constexpr int kMaxBatch = 512;                  // sequences of a launch (larger batches take several)
+constexpr int kMaxBatch = 256;                  // sequences of a launch (larger batches take several)
 constexpr int kMaxCtas = 320;
-constexpr int kOPad = 72;                       // merge-buffer row of 64 floats
+constexpr float kLazy = 8.f;                    // log2 of the largest weight before the running maximum moves
 constexpr float kLog2e = 1.4426950408889634f;
 
+constexpr int kMergeBytes = kWarps * 16 * 72 * 4;   // a warp's 16 rows of 64 floats (or 8 of 128), padded by 8
 template <int D>
 __host__ __device__ constexpr int stage_keys() { return kSlotBytes / (D * 2); }
 template <int D, int RW>
 __host__ __device__ constexpr uint32_t smem_bytes() {
-  return kSlots * kSlotBytes + 16 * RW * D * 2 /* Q */ + (RW < 4 ? kWarps * 16 * kOPad * 4 : 0) /* merge */ + 1024;
+  return kSlots * kSlotBytes + 16 * RW * D * 2 /* Q */ + (RW < 4 ? kMergeBytes : 0) + 1024;
 }
 
 // any infinity or NaN among 8 values
@@ -87,11 +88,14 @@ struct Span {
   int len, begin;
   bool shares;      // takes the shared prefix's part in
 };
-__device__ __forceinline__ Span span_of(const PagedAttnArgs& a, int b) {
+__device__ __forceinline__ int length_of(const PagedAttnArgs& a, int b) {
   const int64_t reach = static_cast<int64_t>(a.pages_per_seq) * a.kv.page_size;
+  const int len = max(a.seqlens[b], 0);
+  return len > reach ? max(static_cast<int>(reach), a.prefix_len) : len;
+}
+__device__ __forceinline__ Span span_of(const PagedAttnArgs& a, int len) {
   Span s;
-  s.len = max(a.seqlens[b], 0);
-  if (s.len > reach) s.len = max(static_cast<int>(reach), a.prefix_len);
+  s.len = len;
   s.shares = a.shared > 0 && s.len - a.T + 1 >= a.shared;
   s.begin = s.shares ? a.shared : 0;
   return s;
@@ -112,8 +116,8 @@ struct Line {
     stages_p = streams ? (a.shared + KEYS - 1) / KEYS : 0;
     base = a.kv.KVH * tiles_p * stages_p;
   }
-  static __device__ __forceinline__ int stages_of(const PagedAttnArgs& a, int b) {
-    const Span s = span_of(a, b);
+  static __device__ __forceinline__ int stages_of(const PagedAttnArgs& a, int len) {
+    const Span s = span_of(a, len);
     return a.whole ? 1 : (s.len - s.begin + KEYS - 1) / KEYS;
   }
   __device__ __forceinline__ void close(const PagedAttnArgs& a, int stages) {   // of all sequences
@@ -129,15 +133,17 @@ struct Line {
   }
 };
 
-// Exclusive running sums of the sequences' stages into s_sum[0 .. B] (all THREADS of the block take part).
+// The sequences' lengths into s_len and the exclusive running sums of their stages into s_sum[0 .. B] (all
+// THREADS of the block take part).
 template <int D, int RW, int THREADS>
-__device__ __forceinline__ void scan_stages(const PagedAttnArgs& a, int* s_sum, int* s_warp) {
+__device__ __forceinline__ void scan_stages(const PagedAttnArgs& a, int* s_sum, int* s_len, int* s_warp) {
   constexpr int W = THREADS / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int run = 0;
   for (int b0 = 0; b0 < a.B; b0 += THREADS) {
     const int b = b0 + tid;
-    const int own = b < a.B ? Line<D, RW>::stages_of(a, b) : 0;
+    const int len = b < a.B ? length_of(a, b) : 0;
+    const int own = b < a.B ? Line<D, RW>::stages_of(a, len) : 0;
     int v = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -152,7 +158,10 @@ __device__ __forceinline__ void scan_stages(const PagedAttnArgs& a, int* s_sum, 
       if (w < warp) before += s_warp[w];
       run += s_warp[w];
     }
-    if (b < a.B) s_sum[b] = before + v - own;
+    if (b < a.B) {
+      s_sum[b] = before + v - own;
+      s_len[b] = len;
+    }
     __syncthreads();
   }
   if (tid == 0) s_sum[a.B] = run;
@@ -167,8 +176,8 @@ struct Segment {
 };
 // Segment at position pos of a share that ends at `end`; its number of positions in n.
 template <int D, int RW>
-__device__ __forceinline__ Segment segment_at(const PagedAttnArgs& a, const Line<D, RW>& line, const int* s_sum, int pos,
-                                              int end, int& n) {
+__device__ __forceinline__ Segment segment_at(const PagedAttnArgs& a, const Line<D, RW>& line, const int* s_sum,
+                                              const int* s_len, int pos, int end, int& n) {
   constexpr int KEYS = stage_keys<D>(), ROWS = 16 * RW;
   Segment g;
   int u, s0, stages, tile, first = 0, last;
@@ -193,7 +202,7 @@ __device__ __forceinline__ Segment segment_at(const PagedAttnArgs& a, const Line
       else hi = mid - 1;
     }
     g.b = lo;
-    const Span s = span_of(a, lo);
+    const Span s = span_of(a, s_len[lo]);
     first = s.begin;
     last = s.len;
     shares = s.shares;
@@ -236,16 +245,15 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
   constexpr uint32_t HALFB = KEYS * 128;   // a slot's 64-element column
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ float s_m[kWarps][16], s_l[kWarps][16];
-  __shared__ uint32_t s_bad[2][KEYS / 32];
   __shared__ __align__(8) uint64_t s_bar[2 * kSlots + 2];
-  __shared__ int s_sum[kMaxBatch + 1], s_warp[kThreads / 32];
+  __shared__ int s_sum[kMaxBatch + 1], s_len[kMaxBatch], s_warp[kThreads / 32];
   __shared__ Segment s_seg;
   __shared__ int64_t s_at[ROWS];        // per row: offset in the output, or workspace entry
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint8_t* const smem = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
   const uint32_t ring = smem_u32(smem), q_s = ring + kSlots * kSlotBytes;
-  float* const s_o = reinterpret_cast<float*>(smem + kSlots * kSlotBytes + ROWS * D * 2);   // [kWarps][16][kOPad]
+  float* const s_o = reinterpret_cast<float*>(smem + kSlots * kSlotBytes + ROWS * D * 2);   // the key warps' merge buffer
   const uint32_t full = smem_u32(s_bar), empty = full + 8 * kSlots, q_full = empty + 8 * kSlots, q_empty = q_full + 8;
   if (tid == 0) {
     for (int i = 0; i < kSlots; ++i) {
@@ -263,7 +271,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
   if (!a.after_prefix) pdl_wait();   // behind the prefix launch the inputs are complete
   pdl_launch_dependents();
   Line<D, RW> line(a);
-  scan_stages<D, RW, kThreads>(a, s_sum, s_warp);   // (its barriers also publish the mbarriers)
+  scan_stages<D, RW, kThreads>(a, s_sum, s_len, s_warp);   // (its barriers also publish the mbarriers)
   line.close(a, s_sum[a.B]);
   const int first = line.share(blockIdx.x), end = line.share(blockIdx.x + 1);
 
@@ -271,18 +279,38 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
     // ---- producer
     int it = 0, seg = 0;   // stages and segments so far
     bool ok = true;
+    // lane -> (K or V, 64-element column, page of the stage): 32 lanes are enough from boxes of 8 rows on
+    const int bp = a.box_rows, boxes = bp ? KEYS / bp : 1, per = HALVES * boxes;
+    const int kv = lane / per, rest = lane - kv * per, col = rest / boxes, pg = rest - col * boxes;
+    // page of this lane's box in stage i of a segment; -1: nothing to copy
+    auto lookup = [&](const Segment& g, int i) {
+      const int tok = g.t_begin + i * KEYS + pg * bp;
+      if (kv > 1 || tok >= g.t_end) return -1;
+      return __ldg((g.b >= 0 && tok >= a.prefix_len ? a.table + g.b * a.ld_table : a.prefix_table) + a.div.page(tok));
+    };
+    Segment ahead;         // the next segment, found while this one's copies are under way,
+    int ahead_n = 0, ahead_page = -1;   // and the pages of its first stage
+    if (first < end) {
+      ahead = segment_at(a, line, s_sum, s_len, first, end, ahead_n);
+      if (bp) ahead_page = lookup(ahead, 0);
+    }
     for (int pos = first; pos < end && ok; ++seg) {
-      int n;
-      const Segment g = segment_at(a, line, s_sum, pos, end, n);
-      pos += n;
+      const Segment g = ahead;
+      int next = ahead_page;
+      pos += ahead_n;
+      if (pos < end) {
+        ahead = segment_at(a, line, s_sum, s_len, pos, end, ahead_n);
+        if (bp) ahead_page = lookup(ahead, 0);
+      }
       const int t_begin = g.t_begin, t_end = g.t_end;
       const int32_t* table = g.b < 0 ? a.prefix_table : a.table + g.b * a.ld_table;
       const int split_at = g.b < 0 ? 0 : a.prefix_len;   // positions before it lie in prefix_table's pages
       const int nst = (t_end - t_begin + KEYS - 1) / KEYS;
-      if (seg > 0) ok = __all_sync(0xffffffffu, mbar_wait(q_empty, (seg - 1) & 1));
-      if (!ok) break;
-      // Q rows of the tile, [64-element column][row][128 bytes] swizzled; rows past the end are zeros. Lane l
-      // owns the addresses of rows l and l + 32.
+      // Q rows of the tile, behind the first stage's copies: [64-element column][row][128 bytes] swizzled; rows
+      // past the end are zeros. Lane l owns the addresses of rows l and l + 32.
+      auto send_q = [&]() {
+        if (seg > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait(q_empty, (seg - 1) & 1));
+        if (!ok) return;
 #pragma unroll
       for (int r0 = 0; r0 < ROWS; r0 += 32) {
         const int mine = r0 + lane;
@@ -306,18 +334,12 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
         mbar_arrive(q_full);
       }
       mbar_arrive_cp_async(q_full);
+      };
+      if (nst == 0) send_q();
       if (a.box_rows) {
-        // lane -> (K or V, 64-element column, page of the stage): 32 lanes are enough from boxes of 8 rows on
-        const int bp = a.box_rows, boxes = KEYS / bp, per = HALVES * boxes;
-        const int kv = lane / per, rest = lane - kv * per, col = rest / boxes, pg = rest - col * boxes;
-        auto lookup = [&](int i) {
-          const int tok = t_begin + i * KEYS + pg * bp;
-          return kv < 2 && tok < t_end ? __ldg((tok >= split_at ? table : a.prefix_table) + a.div.page(tok)) : -1;
-        };
-        int next = lookup(0);
         for (int i = 0; i < nst && ok; ++i, ++it) {
           const int page = next, tok = t_begin + i * KEYS + pg * bp;
-          next = lookup(i + 1);
+          next = lookup(g, i + 1);
 #pragma unroll
           for (int x = 0; x < 2; ++x) {   // K, then V
             const int u = 2 * it + x, slot = u % kSlots;
@@ -336,6 +358,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
             __syncwarp();
             if (copy) tma_load_4d(dst, x ? &maps.v : &maps.k, 64 * col, a.div.slot(tok, a.div.page(tok)), g.kvh, page, full + 8 * slot);
           }
+          if (i == 0) send_q();
         }
       } else {
         // lane l owns the addresses of key rows l, l + 32, ...; 8 lanes copy the 128 bytes of a row's column
@@ -368,6 +391,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
             }
             mbar_arrive_cp_async(full + 8 * slot);
           }
+          if (i == 0) send_q();
         }
       }
     }
@@ -385,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
       Segment g = s_seg;
       if (!landed) {   // a wait ran out: NaN for what is left
         int n;
-        g = segment_at(a, line, s_sum, pos, end, n);
+        g = segment_at(a, line, s_sum, s_len, pos, end, n);
       }
 #pragma unroll
       for (int j = 0; j < KSTEPS; ++j) {
@@ -425,7 +449,6 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
         const int ks = (2 * it) % kSlots, vs = (2 * it + 1) % kSlots;
         const uint32_t kbuf = ring + ks * kSlotBytes, vbuf = ring + vs * kSlotBytes;
         const int stage0 = t_begin + i * KEYS;
-        bool v_landed = false, any_bad = false;
         landed = landed && mbar_wait(full + 8 * ks, (2 * it / kSlots) & 1);
 #pragma unroll
         for (int blk = 0; blk < WK / WB; ++blk) {
@@ -435,82 +458,91 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
           float s[WB / 8][4];
           float msafe[2];
           if (!idle) {
-            float tmax[2] = {-INFINITY, -INFINITY};
+            // 16 keys per ldmatrix; even and odd k-steps in sums of their own, so that short chains of
+            // dependent products alternate
+            float s2[WB / 8][4];
 #pragma unroll
-            for (int n = 0; n < WB / 8; ++n) {
-              s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-              const int r = lead + 8 * n + ri;
+            for (int n = 0; n < WB / 8; ++n)
 #pragma unroll
-              for (int j = 0; j < KSTEPS; j += 2) {
-                const int c = 2 * j + mi;
+              for (int c = 0; c < 4; ++c) s[n][c] = s2[n][c] = 0.f;
+#pragma unroll
+            for (int j = 0; j < KSTEPS; ++j)
+#pragma unroll
+              for (int n = 0; n < WB / 8; n += 2) {
+                const int r = lead + 8 * n + 8 * (mi >> 1) + ri, c = 2 * j + (mi & 1);
                 uint32_t b0, b1, b2, b3;
                 ldsm_x4(kbuf + (c >> 3) * HALFB + r * 128 + (((c & 7) ^ (r & 7)) << 4), b0, b1, b2, b3);
-                Mma<T>::run(s[n], qa[j][0], qa[j][1], qa[j][2], qa[j][3], b0, b1);
-                Mma<T>::run(s[n], qa[j + 1][0], qa[j + 1][1], qa[j + 1][2], qa[j + 1][3], b2, b3);
+                Mma<T>::run((j & 1) ? s2[n] : s[n], qa[j][0], qa[j][1], qa[j][2], qa[j][3], b0, b1);
+                Mma<T>::run((j & 1) ? s2[n + 1] : s[n + 1], qa[j][0], qa[j][1], qa[j][2], qa[j][3], b2, b3);
               }
+            float tmax[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int n = 0; n < WB / 8; ++n)
 #pragma unroll
               for (int c = 0; c < 4; ++c) {
                 const int tok = key0 + 8 * n + 2 * tq + (c & 1);
-                s[n][c] *= a.scale_log2;
+                s[n][c] = (s[n][c] + s2[n][c]) * a.scale_log2;
                 if (masked && (tok >= lim[c >> 1] || tok >= t_end)) s[n][c] = -INFINITY;
                 tmax[c >> 1] = fmaxf(tmax[c >> 1], s[n][c]);
               }
-            }
-            float alpha[2];
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
               tmax[r] = fmaxf(tmax[r], __shfl_xor_sync(0xffffffffu, tmax[r], 1));
               tmax[r] = fmaxf(tmax[r], __shfl_xor_sync(0xffffffffu, tmax[r], 2));
-              const float m_new = fmaxf(m_run[r], tmax[r]);
-              msafe[r] = m_new == -INFINITY ? 0.f : m_new;
-              alpha[r] = exp2_fast(m_run[r] - msafe[r]);
-              m_run[r] = m_new;
-              l_run[r] *= alpha[r];
+            }
+            // the running maximum moves only when a score passes it by kLazy (or is the first)
+            if (__any_sync(0xffffffffu, tmax[0] > m_run[0] + kLazy || tmax[1] > m_run[1] + kLazy)) {
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                const bool move = tmax[r] > m_run[r] + kLazy;
+                const float alpha = move ? exp2_fast(m_run[r] - tmax[r]) : 1.f;   // m_run = -inf: 0
+                if (move) m_run[r] = tmax[r];
+                l_run[r] *= alpha;
+#pragma unroll
+                for (int n = 0; n < NTILES; ++n) {
+                  o[n][2 * r] *= alpha;
+                  o[n][2 * r + 1] *= alpha;
+                }
+              }
             }
 #pragma unroll
-            for (int n = 0; n < NTILES; ++n) {
-              o[n][0] *= alpha[0]; o[n][1] *= alpha[0];
-              o[n][2] *= alpha[1]; o[n][3] *= alpha[1];
-            }
+            for (int r = 0; r < 2; ++r) msafe[r] = m_run[r] == -INFINITY ? 0.f : m_run[r];
           }
           if (blk == WK / WB - 1) {   // the warp is done with K
             __syncwarp();
             if (lane == 0) mbar_arrive(empty + 8 * ks);
           }
-          if (!v_landed) {
-            v_landed = true;
-            landed = landed && mbar_wait(full + 8 * vs, ((2 * it + 1) / kSlots) & 1);
-            // The stage at the end: value rows past it become zeros. And keys that some rows of the tile see
-            // and others do not (the newest T - 1): a zero weight times an infinite or NaN value would reach
-            // the rows that must not see it, so such value rows (rare) are taken out of the stage and added to
-            // the rows that do see them one by one below.
-            const bool check = a.T > 1 && g.b >= 0 && min(stage0 + KEYS, t_end) > lim_min;
-            if (check || stage0 + KEYS > t_end) {
-              if (tid < KEYS / 32) s_bad[it & 1][tid] = 0;
-              named_sync<1, kConsumers>();
-#pragma unroll 4
-              for (int ci = tid; ci < KEYS * CH; ci += kConsumers) {
-                const int r = ci / CH, c = ci % CH;
-                uint4* x = reinterpret_cast<uint4*>(smem + (vbuf - ring) + (c >> 3) * HALFB + r * 128 + (((c & 7) ^ (r & 7)) << 4));
-                if (stage0 + r >= t_end) *x = make_uint4(0, 0, 0, 0);
-                else if (check && stage0 + r >= lim_min && nonfinite8<T>(*x)) atomicOr(&s_bad[it & 1][r >> 5], 1u << (r & 31));
-              }
-              fence_proxy_async();   // the slot's next tensor copy comes after these writes
-              named_sync<1, kConsumers>();
-              if (check) {
+          if (blk == 0) landed = landed && mbar_wait(full + 8 * vs, ((2 * it + 1) / kSlots) & 1);
+          // The keys at the end: value rows past it become zeros. And keys that some rows of the tile see and
+          // others do not (the newest T - 1): a zero weight times an infinite or NaN value would reach the
+          // rows that must not see it, so such value rows (rare) are taken out of the stage (`bad`) and added
+          // to the rows that do see them one by one below. Every warp clears the rows that it multiplies.
+          uint32_t bad = 0;
+          const bool check = a.T > 1 && g.b >= 0 && min(key0 + WB, t_end) > lim_min;
+          if (!idle && (check || key0 + WB > t_end)) {
+            constexpr int PASS = 32 / CH;   // rows per pass of the warp
+            const int c = lane % CH;
+            if (check) {
 #pragma unroll
-                for (int j = 0; j < KEYS / 32; ++j) any_bad |= s_bad[it & 1][j] != 0;
-                if (any_bad) {
-                  for (int ci = tid; ci < KEYS * CH; ci += kConsumers) {
-                    const int r = ci / CH, c = ci % CH;
-                    if (s_bad[it & 1][r >> 5] >> (r & 31) & 1)
-                      *reinterpret_cast<uint4*>(smem + (vbuf - ring) + (c >> 3) * HALFB + r * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
-                  }
-                  fence_proxy_async();
-                  named_sync<1, kConsumers>();
-                }
+              for (int p = 0; p < WB / PASS; ++p) {
+                const int r = lead + p * PASS + lane / CH;
+                const uint4 x = *reinterpret_cast<const uint4*>(smem + (vbuf - ring) + (c >> 3) * HALFB + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+                const uint32_t hit = __ballot_sync(0xffffffffu, stage0 + r >= lim_min && stage0 + r < t_end && nonfinite8<T>(x));
+#pragma unroll
+                for (int y = 0; y < PASS; ++y)
+                  if (hit >> (y * CH) & (CH == 8 ? 0xFFu : 0xFFFFu)) bad |= 1u << (p * PASS + y);
               }
+              // the warps of other row tiles look at the same rows: all have seen them before any clears them
+              if (RW > 1 && bad) asm volatile("bar.sync %0, %1;\n" ::"r"(2 + kw), "n"(RW * 32) : "memory");
             }
+#pragma unroll
+            for (int p = 0; p < WB / PASS; ++p) {
+              const int i = p * PASS + lane / CH, r = lead + i;
+              if (stage0 + r >= t_end || (bad >> i & 1))
+                *reinterpret_cast<uint4*>(smem + (vbuf - ring) + (c >> 3) * HALFB + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async();   // the slot's next tensor copy comes after these writes
+            __syncwarp();
           }
           if (!idle) {
 #pragma unroll
@@ -535,12 +567,12 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
                 Mma<T>::run(o[np + 1], pa[0], pa[1], pa[2], pa[3], v2, v3);
               }
             }
-            if (any_bad) {   // the value rows taken out above, for the rows that see them
+            if (bad) {   // the value rows taken out above, for the rows that see them
 #pragma unroll
               for (int n = 0; n < WB / 8; ++n) {
                 for (int col = 0; col < 8; ++col) {
                   const int r = lead + 8 * n + col;
-                  if (!(s_bad[it & 1][r >> 5] >> (r & 31) & 1)) continue;
+                  if (!(bad >> (8 * n + col) & 1)) continue;
                   const int src = (lane & ~3) | (col >> 1);
                   const float p0 = __shfl_sync(0xffffffffu, (col & 1) ? s[n][1] : s[n][0], src);
                   const float p1 = __shfl_sync(0xffffffffu, (col & 1) ? s[n][3] : s[n][2], src);
@@ -621,31 +653,43 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
           }
         }
       } else {
-#pragma unroll
-        for (int hf = 0; hf < HALVES; ++hf) {   // 64 elements at a time through the merge buffer
-          if (hf > 0) named_sync<1, kConsumers>();
+        // up to 8 rows (the usual decode) go through the merge buffer at once, more 64 elements at a time
+        auto merge = [&](auto width, int col0) {
+          constexpr int WIDTH = decltype(width)::value, PAD = WIDTH + 8;
+          const int limit = WIDTH == D && D > 64 ? 8 : 16;   // rows of a warp's part of the buffer
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            float* dst = s_o + (warp * 16 + g8 + 8 * r) * kOPad + 2 * tq;
-            if (16 * rw + g8 + 8 * r < g.nrows) {
+            float* dst = s_o + (warp * limit + g8 + 8 * r) * PAD + 2 * tq;
+            if (g8 + 8 * r < limit && 16 * rw + g8 + 8 * r < g.nrows) {
 #pragma unroll
-              for (int n = 0; n < 8; ++n)
-                *reinterpret_cast<float2*>(dst + 8 * n) = make_float2(o[8 * hf + n][2 * r] * factor[r], o[8 * hf + n][2 * r + 1] * factor[r]);
+              for (int n = 0; n < NTILES; ++n) {
+                if (8 * n < col0 || 8 * n >= col0 + WIDTH) continue;
+                *reinterpret_cast<float2*>(dst + 8 * n - col0) = make_float2(o[n][2 * r] * factor[r], o[n][2 * r + 1] * factor[r]);
+              }
             }
           }
           named_sync<1, kConsumers>();
-          for (int row = warp; row < g.nrows; row += kWarps) {
-            const int d = 2 * lane, w0 = row / 16, rr = row % 16;
+          for (int idx = tid; idx < g.nrows * (WIDTH / 2); idx += kConsumers) {
+            const int row = idx / (WIDTH / 2), d = 2 * (idx % (WIDTH / 2)), w0 = row / 16, rr = row % 16;
             float2 v = make_float2(0.f, 0.f);
 #pragma unroll
             for (int k = 0; k < KW; ++k) {
-              const float2 x = *reinterpret_cast<const float2*>(s_o + ((k * RW + w0) * 16 + rr) * kOPad + d);
+              const float2 x = *reinterpret_cast<const float2*>(s_o + ((k * RW + w0) * limit + rr) * PAD + d);
               v.x += x.x;
               v.y += x.y;
             }
             const int64_t at = s_at[row];
-            if (g.kind == 0) store_out2<T>(a, at + 64 * hf + d, v.x, v.y);
-            else *reinterpret_cast<float2*>(a.acc + at * D + 64 * hf + d) = v;
+            if (g.kind == 0) store_out2<T>(a, at + col0 + d, v.x, v.y);
+            else *reinterpret_cast<float2*>(a.acc + at * D + col0 + d) = v;
+          }
+        };
+        if (D == 64 || g.nrows <= 8) {
+          merge(std::integral_constant<int, D>{}, 0);
+        } else {
+#pragma unroll
+          for (int hf = 0; hf < HALVES; ++hf) {
+            if (hf > 0) named_sync<1, kConsumers>();
+            merge(std::integral_constant<int, 64>{}, 64 * hf);
           }
         }
       }
@@ -654,37 +698,36 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
   if (a.after_prefix) pdl_wait();   // this launch completes after the prefix's, so the combine sees both
 }
 
-// Merges the entries of 16 rows of a (sequence, KV head): a block of 128 threads, four elements a thread.
-constexpr int kMergeRows = 16;
+// Merges rows' entries: a block of 128 threads for 512 / D rows of a (sequence, KV head), four elements a thread.
+// A thread reads its row's (m, l) along with the sums and keeps a running maximum, so that one round trip to
+// memory follows the streaming kernel's end; the rest is done while that kernel still runs (its shared memory
+// is sized to leave room for these blocks).
 template <typename T, int D, int RW>
-__global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constant__ PagedAttnArgs a) {
-  constexpr int ROWS = 16 * RW, QUADS = D / 4;
+__global__ void __launch_bounds__(128, 6) paged_combine_kernel(const __grid_constant__ PagedAttnArgs a) {
+  constexpr int ROWS = 16 * RW, QUADS = D / 4, BLOCK_ROWS = 128 / QUADS;
   constexpr int MOST = kMaxParts + kMaxCtas + 2;   // a prefix unit's and an own unit's CTAs have at most one in common
-  __shared__ int s_sum[kMaxBatch + 1], s_warp[4];
-  __shared__ int64_t s_entry[MOST];            // entry of the first row; the next rows follow at a step of `step`
-  __shared__ float s_f[kMergeRows][MOST];      // factors
-  __shared__ float s_inv[kMergeRows];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  __shared__ int s_sum[kMaxBatch + 1], s_len[kMaxBatch], s_warp[4];
+  __shared__ int64_t s_entry[MOST];   // entry of the first row, or -1 - (its block of R rows in the output's order)
+  const int tid = threadIdx.x;
   pdl_launch_dependents();
   // the lengths are inputs of the whole call, complete before its first kernel began
   Line<D, RW> line(a);
-  scan_stages<D, RW, 128>(a, s_sum, s_warp);
+  scan_stages<D, RW, 128>(a, s_sum, s_len, s_warp);
   line.close(a, s_sum[a.B]);
   const int64_t R = all_rows(a);
   const int b = blockIdx.x / a.kv.KVH, kvh = blockIdx.x - b * a.kv.KVH;
-  const Span sp = span_of(a, b);
+  const Span sp = span_of(a, s_len[b]);
   const int stages = s_sum[b + 1] - s_sum[b];
   bool waited = false;
-  const int stop = min(a.rows, (static_cast<int>(blockIdx.y) + 1) * kMergeRows);
-  for (int row0 = blockIdx.y * kMergeRows, n; row0 < stop; row0 += n) {
+  const int stop = min(a.rows, (static_cast<int>(blockIdx.y) + 1) * BLOCK_ROWS);
+  for (int row0 = blockIdx.y * BLOCK_ROWS, n; row0 < stop; row0 += n) {
     // n rows of one unit (and of one unit of the prefix)
     const int pr = b * a.rows + row0;
     n = stop - row0;
     if (sp.shares && line.tiles_p > 0) n = min(n, ROWS - pr % ROWS);
     int ne = 0;
     bool written = false;   // by the streaming kernel
-    // a unit's entries: one whole part, or a slot of every CTA that shares it. Entry < 0: -1 - (index of the
-    // whole part's first R block), whose rows follow the output's order
+    // a unit's entries: one whole part, or a slot of every CTA that shares it
     auto unit = [&](int p0, int count, int r, int block, bool direct) {
       if (count == 0) return;
       const int c0 = line.owner(p0), c1 = line.owner(p0 + count - 1);
@@ -711,54 +754,47 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constan
     if (!waited) pdl_wait();
     waited = true;
     if (written) continue;
-    auto entry_of = [&](int e, int r) -> int64_t {
-      const int64_t x = s_entry[e];
-      if (x >= 0) return x + r;
-      const int t = (row0 + r) / a.G;
-      return (-1 - x) * R + (static_cast<int64_t>(b) * a.T + t) * a.H + kvh * a.G + row0 + r - t * a.G;
-    };
     __syncthreads();
-    for (int r = warp; r < n; r += 4) {   // a warp per row: the entries' factors
-      float mx = -INFINITY;
-      for (int e = lane; e < ne; e += 32) mx = fmaxf(mx, a.ml[entry_of(e, r) * 2]);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      float l = 0.f;
-      for (int e = lane; e < ne; e += 32) {
-        const float2 x = *reinterpret_cast<const float2*>(a.ml + entry_of(e, r) * 2);
-        const float f = x.x == -INFINITY ? 0.f : exp2_fast(x.x - mx);
-        s_f[r][e] = f;
-        l += f * x.y;
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-      if (lane == 0) s_inv[r] = l == 0.f ? 0.f : 1.f / l;   // a row that sees no key: zeros
-    }
-    __syncthreads();
-#pragma unroll 1
-    for (int item = tid; item < n * QUADS; item += 128) {
-      const int r = item / QUADS, d = (item - r * QUADS) * 4;
+    const int r = tid / QUADS, d = (tid - r * QUADS) * 4;
+    if (r < n) {
+      const int t = (row0 + r) / a.G, head = kvh * a.G + row0 + r - t * a.G;
+      const int64_t index = (static_cast<int64_t>(b) * a.T + t) * a.H + head;
+      float m = -INFINITY, l = 0.f;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
       for (int e = 0; e < ne; e += 8) {   // eight entries in flight
         float4 x[8];
+        float2 ml[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (e + k < ne) x[k] = *reinterpret_cast<const float4*>(a.acc + entry_of(e + k, r) * D + d);
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
+        for (int k = 0; k < 8; ++k) {
+          ml[k] = make_float2(-INFINITY, 0.f);
+          x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
           if (e + k < ne) {
-            const float f = s_f[r][e + k];
-            v.x = fmaf(f, x[k].x, v.x); v.y = fmaf(f, x[k].y, v.y);
-            v.z = fmaf(f, x[k].z, v.z); v.w = fmaf(f, x[k].w, v.w);
+            const int64_t s = s_entry[e + k], at = s >= 0 ? s + r : (-1 - s) * R + index;
+            ml[k] = *reinterpret_cast<const float2*>(a.ml + at * 2);
+            x[k] = *reinterpret_cast<const float4*>(a.acc + at * D + d);
           }
+        }
+        float mx = m;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) mx = fmaxf(mx, ml[k].x);
+        const float keep = m == -INFINITY ? 0.f : exp2_fast(m - mx);
+        m = mx;
+        l *= keep;
+        v.x *= keep; v.y *= keep; v.z *= keep; v.w *= keep;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float f = ml[k].x == -INFINITY ? 0.f : exp2_fast(ml[k].x - mx);
+          l = fmaf(f, ml[k].y, l);
+          v.x = fmaf(f, x[k].x, v.x); v.y = fmaf(f, x[k].y, v.y);
+          v.z = fmaf(f, x[k].z, v.z); v.w = fmaf(f, x[k].w, v.w);
+        }
       }
-      const float inv = s_inv[r];
-      const int t = (row0 + r) / a.G;
-      const int64_t at = b * a.so_b + t * a.so_t + static_cast<int64_t>(kvh * a.G + row0 + r - t * a.G) * a.so_h + d;
+      const float inv = l == 0.f ? 0.f : 1.f / l;   // a row that sees no key: zeros
+      const int64_t at = b * a.so_b + t * a.so_t + static_cast<int64_t>(head) * a.so_h + d;
       store_out2<T>(a, at, v.x * inv, v.y * inv);
       store_out2<T>(a, at + 2, v.z * inv, v.w * inv);
     }
-    __syncthreads();   // the next rows reuse the tables
+    __syncthreads();   // the next rows reuse the table
   }
   if (!waited) pdl_wait();
 }
@@ -870,7 +906,7 @@ int launch_stream(const PoolMaps& maps, const PagedAttnArgs& a, bool combine, bo
   }
   int st = launch_kernel(kern, dim3(a.ctas), dim3(kThreads), bytes, s, pdl || a.after_prefix, maps, a);
   if (st != B2D_OK || !combine) return st;
-  return launch_kernel(paged_combine_kernel<T, D, RW>, dim3(a.B * a.kv.KVH, (a.rows + kMergeRows - 1) / kMergeRows),
+  return launch_kernel(paged_combine_kernel<T, D, RW>, dim3(a.B * a.kv.KVH, (a.rows + 512 / D - 1) / (512 / D)),
                        dim3(128), 0, s, true, a);
 }
 

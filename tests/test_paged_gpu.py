@@ -194,6 +194,36 @@ def test_attention_lengths_beyond_the_table_and_bad_pages():
     c.check(c.run())
 
 
+@pytest.mark.parametrize("H,KVH,T,D,lens", [(8, 2, 4, 128, [130, 64, 7]), (16, 2, 4, 128, [193, 66, 4]),
+                                            (16, 1, 4, 64, [129, 260, 5]), (4, 1, 3, 64, [128, 2, 300]),
+                                            (16, 1, 16, 128, [70, 16, 5])])
+@pytest.mark.parametrize("value", [float("inf"), NAN])
+def test_attention_masked_infinities_and_nans(H, KVH, T, D, lens, value):
+    """An infinite or NaN key and value of the newest token reaches no query before it, and every later query
+    that sees it (a NaN key, an infinite value) is not finite."""
+    c = Case(lens, H=H, KVH=KVH, T=T, D=D, dtype=BF16, seed=T + D)
+    clean = c.run()
+    for b, n in enumerate(lens):
+        page = c.table[b, (n - 1) // 16].long().item()
+        c.kd[page, :, (n - 1) % 16, ::3] = value
+        c.vd[page, :, (n - 1) % 16, 1::2] = value
+    got = c.run()
+    assert torch.equal(got[:, :-1], clean[:, :-1])
+    assert not torch.isfinite(got[:, -1, :, 1::2]).any()
+
+
+def test_attention_infinite_value_alone():
+    """An infinite value among the newest tokens: the queries that see it get it, in its elements only."""
+    c = Case([70, 140], H=8, KVH=2, T=3, seed=40)
+    clean = c.run()
+    for b, n in enumerate([70, 140]):
+        c.vd[c.table[b, (n - 2) // 16].long().item(), :, (n - 2) % 16, 5] = -float("inf")
+    got = c.run()
+    assert torch.equal(got[:, 0], clean[:, 0]) and (got[:, 1:, :, 5] == -float("inf")).all()
+    got[:, 1:, :, 5] = clean[:, 1:, :, 5]
+    assert torch.allclose(got.float(), clean.float(), rtol=2.0 ** -9, atol=2.0 ** -9)   # summed in another order
+
+
 def test_attention_empty_calls():
     kv = PagedKV(torch.zeros(2, 2, 16, 64, dtype=F16, device=DEV), torch.zeros(2, 2, 16, 64, dtype=F16, device=DEV))
     t0 = torch.zeros(0, 3, dtype=torch.int32, device=DEV)
