@@ -5,7 +5,7 @@
 // o[b, t, h] = sum_{j < limit} softmax_j(scale q.k_j) v_j, limit = seqlens[b] - T + 1 + t. Key j lies in
 // prefix_table's pages for j < prefix_len and in page_table[b]'s behind.
 //
-// Streaming kernel. A unit of work is (sequence, KV head, tile of 16 RW rows): rows are the T x G query vectors
+// Streaming kernel. A unit of work is (sequence, KV head, tile of up to 32 rows): rows are the T x G query vectors
 // that read this KV head (row = t G + g), so K and V are read once for all of them. The units' stages (64 keys
 // of 128, 128 keys of 64) form one line, of which every CTA (two per SM) takes an equal share: a ragged batch
 // is balanced from its lengths on the device, and a CTA's ring never drains between two units.
@@ -13,16 +13,18 @@
 //    up one stage ahead and issue one tensor copy per (page, 64 elements), 128-byte swizzled, so that the
 //    ldmatrix reads hit 8 distinct bank groups; completion on mbarriers. Pages that tensor copies do not fit
 //    (sizes that neither divide nor are divided by 64, ...) take 16-byte cp.async from the same warp.
-//  * Consumer warp (rw, kw) takes rows [16 rw, 16 rw + 16) and its share of each stage's keys: S = Q K^T and
-//    O += P V by mma.sync m16n8k16 (fp32 accumulate), online softmax in the log2 domain; the key warps meet in
-//    shared memory at a unit's end. P is rounded to the cache's dtype for the second product, as its V operand
-//    is; the sum of the weights is taken before that rounding, in fp32. Value rows at or past the length are
+//  * Each of four consumer warps takes a quarter of a stage's keys, transposed so that few rows waste little of
+//    the products: S^T = K Q^T and O^T += V^T P^T by mma.sync m16n8k16 (fp32 accumulate) with 16 keys (16
+//    elements) as M and 8 rows as N. Online softmax in the log2 domain; the warps meet in shared memory at a
+//    unit's end. P is rounded to the cache's dtype for the second product, as its V operand is; the sum of the
+//    weights is taken before that rounding, in fp32. The running maximum moves only when a score exceeds it
+//    by 2^8 (weights up to 256 are as exact), so O is rarely rescaled. Value rows at or past the length are
 //    set to zero before they are multiplied (a zero weight times a stale NaN would not be zero).
 //  * A unit that one CTA finishes is written out; the parts of a unit that several CTAs share go to the
 //    workspace as (O, m, l), and the combine kernel (a programmatic dependent) merges them in CTA order.
 // Short calls give whole units to CTAs and need no combine.
 //
-// Shared prefix: all sequences' rows form one row axis, [0, B T G), over the prefix's pages -- up to 64 rows as
+// Shared prefix: all sequences' rows form one row axis, [0, B T G), over the prefix's pages -- up to 32 rows as
 // further units of the streaming kernel, more on tcgen05 (csrc/paged_prefix.cu, a launch of its own); the
 // sequences' units start behind the prefix, and the combine merges both. A sequence with a query that does not
 // see the whole shared part is computed from position 0 by its own units.
@@ -46,12 +48,11 @@ constexpr int kMaxCtas = 320;
 constexpr float kLazy = 8.f;                    // log2 of the largest weight before the running maximum moves
 constexpr float kLog2e = 1.4426950408889634f;
 
-constexpr int kMergeBytes = kWarps * 16 * 72 * 4;   // a warp's 16 rows of 64 floats (or 8 of 128), padded by 8
 template <int D>
 __host__ __device__ constexpr int stage_keys() { return kSlotBytes / (D * 2); }
-template <int D, int RW>
+template <int D, int NT>
 __host__ __device__ constexpr uint32_t smem_bytes() {
-  return kSlots * kSlotBytes + 16 * RW * D * 2 /* Q */ + (RW < 4 ? kMergeBytes : 0) + 1024;
+  return kSlots * kSlotBytes + 8 * NT * D * 2 /* Q */ + kWarps * 8 * (D + 4) * 4 /* merge */ + 1024;
 }
 
 // any infinity or NaN among 8 values
@@ -104,9 +105,9 @@ __device__ __forceinline__ Span span_of(const PagedAttnArgs& a, int len) {
 // The line of all units' stages: the prefix's units first (where the streaming kernel takes them), then the
 // sequences' in order, KV head by KV head and row tile by row tile. In whole mode a unit counts as one stage.
 // CTA c takes the positions [share(c), share(c + 1)); the host has checked that they fit 31 bits.
-template <int D, int RW>
+template <int D, int NT>
 struct Line {
-  static constexpr int KEYS = stage_keys<D>(), ROWS = 16 * RW;
+  static constexpr int KEYS = stage_keys<D>(), ROWS = 8 * NT;
   int tiles, units, tiles_p, stages_p, base, ctas, quota, extra;
   __device__ __forceinline__ Line(const PagedAttnArgs& a) {
     tiles = (a.rows + ROWS - 1) / ROWS;
@@ -135,7 +136,7 @@ struct Line {
 
 // The sequences' lengths into s_len and the exclusive running sums of their stages into s_sum[0 .. B] (all
 // THREADS of the block take part).
-template <int D, int RW, int THREADS>
+template <int D, int NT, int THREADS>
 __device__ __forceinline__ void scan_stages(const PagedAttnArgs& a, int* s_sum, int* s_len, int* s_warp) {
   constexpr int W = THREADS / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -143,7 +144,7 @@ __device__ __forceinline__ void scan_stages(const PagedAttnArgs& a, int* s_sum, 
   for (int b0 = 0; b0 < a.B; b0 += THREADS) {
     const int b = b0 + tid;
     const int len = b < a.B ? length_of(a, b) : 0;
-    const int own = b < a.B ? Line<D, RW>::stages_of(a, len) : 0;
+    const int own = b < a.B ? Line<D, NT>::stages_of(a, len) : 0;
     int v = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -175,10 +176,10 @@ struct Segment {
   int kind;                      // 0: the final output, 1: a whole part, 2: a part of a unit shared with other CTAs
 };
 // Segment at position pos of a share that ends at `end`; its number of positions in n.
-template <int D, int RW>
-__device__ __forceinline__ Segment segment_at(const PagedAttnArgs& a, const Line<D, RW>& line, const int* s_sum,
+template <int D, int NT>
+__device__ __forceinline__ Segment segment_at(const PagedAttnArgs& a, const Line<D, NT>& line, const int* s_sum,
                                               const int* s_len, int pos, int end, int& n) {
-  constexpr int KEYS = stage_keys<D>(), ROWS = 16 * RW;
+  constexpr int KEYS = stage_keys<D>(), ROWS = 8 * NT;
   Segment g;
   int u, s0, stages, tile, first = 0, last;
   bool shares = true;
@@ -223,28 +224,29 @@ __device__ __forceinline__ Segment segment_at(const PagedAttnArgs& a, const Line
   return g;
 }
 
+// r / G for a sequence's rows (r < 256, G <= 16: exact)
+__device__ __forceinline__ int div_g(const PagedAttnArgs& a, int r) { return r * a.inv_g >> 16; }
 // Row r of a unit -> its (b, t, head).
 struct Row {
   int b, t, head;
 };
 __device__ __forceinline__ Row row_of(const PagedAttnArgs& a, int b, int kvh, int r) {
-  const int rb = b < 0 ? r / a.rows : b, rr = b < 0 ? r - rb * a.rows : r, t = rr / a.G;
+  const int rb = b < 0 ? r / a.rows : b, rr = b < 0 ? r - rb * a.rows : r, t = div_g(a, rr);
   return Row{rb, t, kvh * a.G + rr - t * a.G};
 }
 __device__ __forceinline__ int64_t all_rows(const PagedAttnArgs& a) { return static_cast<int64_t>(a.B) * a.T * a.H; }
 
-template <typename T, int D, int RW>
+template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_constant__ PoolMaps maps,
                                                                    const __grid_constant__ PagedAttnArgs a) {
   constexpr int KEYS = stage_keys<D>();
-  constexpr int KW = kWarps / RW;       // warps that share a row tile and split a stage's keys
-  constexpr int WK = KEYS / KW;         // keys of a stage that a warp takes,
-  constexpr int WB = WK < 32 ? WK : 32; // at most 32 at a time
-  constexpr int ROWS = 16 * RW;
-  constexpr int KSTEPS = D / 16, NTILES = D / 8, CH = D / 8, HALVES = D / 64;
+  constexpr int WK = KEYS / kWarps, MT = WK / 16;   // keys of a stage that a warp takes, in tiles of 16
+  constexpr int ROWS = 8 * NT;
+  constexpr int KSTEPS = D / 16, DT = D / 16, CH = D / 8, HALVES = D / 64;
+  constexpr bool Q_REGS = NT * KSTEPS <= 16;        // Q stays in registers (else it is read per stage)
   constexpr uint32_t HALFB = KEYS * 128;   // a slot's 64-element column
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  __shared__ float s_m[kWarps][16], s_l[kWarps][16];
+  __shared__ float s_m[kWarps][ROWS], s_l[kWarps][ROWS];
   __shared__ __align__(8) uint64_t s_bar[2 * kSlots + 2];
   __shared__ int s_sum[kMaxBatch + 1], s_len[kMaxBatch], s_warp[kThreads / 32];
   __shared__ Segment s_seg;
@@ -270,8 +272,8 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
   }
   if (!a.after_prefix) pdl_wait();   // behind the prefix launch the inputs are complete
   pdl_launch_dependents();
-  Line<D, RW> line(a);
-  scan_stages<D, RW, kThreads>(a, s_sum, s_len, s_warp);   // (its barriers also publish the mbarriers)
+  Line<D, NT> line(a);
+  scan_stages<D, NT, kThreads>(a, s_sum, s_len, s_warp);   // (its barriers also publish the mbarriers)
   line.close(a, s_sum[a.B]);
   const int first = line.share(blockIdx.x), end = line.share(blockIdx.x + 1);
 
@@ -307,28 +309,24 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
       const int split_at = g.b < 0 ? 0 : a.prefix_len;   // positions before it lie in prefix_table's pages
       const int nst = (t_end - t_begin + KEYS - 1) / KEYS;
       // Q rows of the tile, behind the first stage's copies: [64-element column][row][128 bytes] swizzled; rows
-      // past the end are zeros. Lane l owns the addresses of rows l and l + 32.
+      // past the end are zeros. Lane l owns the address of row l.
       auto send_q = [&]() {
         if (seg > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait(q_empty, (seg - 1) & 1));
         if (!ok) return;
-#pragma unroll
-      for (int r0 = 0; r0 < ROWS; r0 += 32) {
-        const int mine = r0 + lane;
         int64_t off = -1;
-        if (mine < g.nrows) {
-          const Row x = row_of(a, g.b, g.kvh, g.row0 + mine);
+        if (lane < g.nrows) {
+          const Row x = row_of(a, g.b, g.kvh, g.row0 + lane);
           off = x.b * a.sq_b + x.t * a.sq_t + static_cast<int64_t>(x.head) * a.sq_h;
         }
 #pragma unroll
-        for (int i = 0; i < (ROWS < 32 ? ROWS : 32) / 4; ++i) {
-          const int rr = 4 * i + lane / 8, r = r0 + rr, c = lane & 7;
-          const int64_t o = __shfl_sync(0xffffffffu, off, rr);
+        for (int i = 0; i < ROWS / 4; ++i) {
+          const int r = 4 * i + lane / 8, c = lane & 7;
+          const int64_t o = __shfl_sync(0xffffffffu, off, r);
           const T* src = static_cast<const T*>(a.q) + (o < 0 ? 0 : o + c * 8);
 #pragma unroll
           for (int col = 0; col < HALVES; ++col)
             cp_async16_zfill(q_s + col * (ROWS * 128) + r * 128 + ((c ^ (r & 7)) << 4), src + (o < 0 ? 0 : 64 * col), o >= 0);
         }
-      }
       if (lane == 0) {
         s_seg = g;
         mbar_arrive(q_full);
@@ -397,13 +395,12 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
     }
     cp_async_wait<0>();
   } else {
-    // ---- consumers
-    const int rw = warp % RW, kw = warp / RW;
+    // ---- consumers: keys are the products' M axis (16 of a warp's keys), rows their N axis (8 per tile)
     const int g8 = lane >> 2, tq = lane & 3, mi = lane >> 3, ri = lane & 7;
+    const int lead = warp * WK;   // this warp's keys of a stage
     int it = 0, seg = 0;
     bool landed = true;
     for (int pos = first; pos < end; ++seg) {
-      uint32_t qa[KSTEPS][4];   // Q fragments of the warp's 16 rows
       // (the last unit's readers are done with s_at, s_m, s_o behind this barrier)
       landed = named_all<1, kConsumers>(landed && mbar_wait(q_full, seg & 1));
       Segment g = s_seg;
@@ -411,13 +408,20 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
         int n;
         g = segment_at(a, line, s_sum, s_len, pos, end, n);
       }
+      uint32_t qb[NT][KSTEPS][2];   // Q as the B operand: row 8 n + g8, elements 16 j + 2 tq ..
+      auto load_q = [&](int n, int j) {   // two k-steps at a time
+        const int r = 8 * n + ri, c = 2 * j + mi;
+        ldsm_x4(q_s + (c >> 3) * (ROWS * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), qb[n][j][0], qb[n][j][1],
+                qb[n][j + 1][0], qb[n][j + 1][1]);
+      };
+      if constexpr (Q_REGS) {
 #pragma unroll
-      for (int j = 0; j < KSTEPS; ++j) {
-        const int r = 16 * rw + (mi & 1) * 8 + ri, c = 2 * j + (mi >> 1);
-        ldsm_x4(q_s + (c >> 3) * (ROWS * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), qa[j][0], qa[j][1], qa[j][2], qa[j][3]);
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < KSTEPS; j += 2) load_q(n, j);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_empty);
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_empty);
       const int t_begin = g.t_begin, t_end = g.t_end, nst = (t_end - t_begin + KEYS - 1) / KEYS;
       const bool opens = pos == first;   // the unit may have begun in an earlier CTA
       pos += a.whole ? 1 : nst;
@@ -428,167 +432,169 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
                     : g.kind == 1 ? (a.nparts + (g.b < 0 ? 1 : 0)) * all_rows(a) + index
                                   : a.slot0 + (static_cast<int64_t>(blockIdx.x) * 2 + (opens ? 0 : 1)) * ROWS + tid;
       }
-      int lim[2], lim_min;   // keys that this thread's two rows see; below lim_min no row is masked
-      if (g.b < 0) {
-        lim[0] = lim[1] = lim_min = g.limit;
-      } else if (a.T == 1) {
-        lim[0] = lim[1] = lim_min = g.limit;
-      } else {
-        lim_min = g.limit + g.row0 / a.G;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) lim[h] = g.limit + (g.row0 + min(16 * rw + g8 + 8 * h, g.nrows - 1)) / a.G;
-      }
+      // keys that this thread's rows 8 n + 2 tq + e see; below lim_min no row is masked
+      const bool causal = g.b >= 0 && a.T > 1;
+      const int lim_min = causal ? g.limit + div_g(a, g.row0) : g.limit;
+      auto lim = [&](int n, int e) { return causal ? g.limit + div_g(a, g.row0 + min(8 * n + 2 * tq + e, g.nrows - 1)) : g.limit; };
 
-      float o[NTILES][4];
+      float o[DT][NT][4];   // element 16 m + g8 (+ 8), row 8 n + 2 tq (+ 1)
 #pragma unroll
-      for (int n = 0; n < NTILES; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-      float m_run[2] = {-INFINITY, -INFINITY};   // log2 domain
-      float l_run[2] = {0.f, 0.f};               // this thread's keys only
+      for (int m = 0; m < DT; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) o[m][n][0] = o[m][n][1] = o[m][n][2] = o[m][n][3] = 0.f;
+      float m_run[NT][2], l_run[NT][2];   // log2 domain; the sum over this thread's keys only
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        m_run[n][0] = m_run[n][1] = -INFINITY;
+        l_run[n][0] = l_run[n][1] = 0.f;
+      }
 
       for (int i = 0; i < nst; ++i, ++it) {
         const int ks = (2 * it) % kSlots, vs = (2 * it + 1) % kSlots;
         const uint32_t kbuf = ring + ks * kSlotBytes, vbuf = ring + vs * kSlotBytes;
-        const int stage0 = t_begin + i * KEYS;
+        const int key0 = t_begin + i * KEYS + lead;   // this warp's first key
+        const bool idle = key0 >= t_end;
+        float s[MT][NT][4];   // key 16 mt + g8 (+ 8), row 8 n + 2 tq (+ 1)
         landed = landed && mbar_wait(full + 8 * ks, (2 * it / kSlots) & 1);
+        if (!idle) {
+          // with one row tile, even and odd k-steps in sums of their own: short chains of dependent products
+          constexpr int SETS = NT == 1 ? 2 : 1;
+          float sum[SETS][MT][NT][4];
 #pragma unroll
-        for (int blk = 0; blk < WK / WB; ++blk) {
-          const int lead = kw * WK + blk * WB, key0 = stage0 + lead;   // this warp's keys
-          const bool idle = key0 >= t_end;
-          const bool masked = key0 + WB > min(lim_min, t_end);
-          float s[WB / 8][4];
-          float msafe[2];
-          if (!idle) {
-            // 16 keys per ldmatrix; even and odd k-steps in sums of their own, so that short chains of
-            // dependent products alternate
-            float s2[WB / 8][4];
+          for (int x = 0; x < SETS; ++x)
 #pragma unroll
-            for (int n = 0; n < WB / 8; ++n)
+            for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-              for (int c = 0; c < 4; ++c) s[n][c] = s2[n][c] = 0.f;
+              for (int n = 0; n < NT; ++n) sum[x][mt][n][0] = sum[x][mt][n][1] = sum[x][mt][n][2] = sum[x][mt][n][3] = 0.f;
 #pragma unroll
-            for (int j = 0; j < KSTEPS; ++j)
+          for (int j = 0; j < KSTEPS; ++j) {
+            if (!Q_REGS && j % 2 == 0) {
 #pragma unroll
-              for (int n = 0; n < WB / 8; n += 2) {
-                const int r = lead + 8 * n + 8 * (mi >> 1) + ri, c = 2 * j + (mi & 1);
-                uint32_t b0, b1, b2, b3;
-                ldsm_x4(kbuf + (c >> 3) * HALFB + r * 128 + (((c & 7) ^ (r & 7)) << 4), b0, b1, b2, b3);
-                Mma<T>::run((j & 1) ? s2[n] : s[n], qa[j][0], qa[j][1], qa[j][2], qa[j][3], b0, b1);
-                Mma<T>::run((j & 1) ? s2[n + 1] : s[n + 1], qa[j][0], qa[j][1], qa[j][2], qa[j][3], b2, b3);
-              }
-            float tmax[2] = {-INFINITY, -INFINITY};
+              for (int n = 0; n < NT; ++n) load_q(n, j);
+            }
 #pragma unroll
-            for (int n = 0; n < WB / 8; ++n)
+            for (int mt = 0; mt < MT; ++mt) {
+              const int r = lead + 16 * mt + (mi & 1) * 8 + ri, c = 2 * j + (mi >> 1);
+              uint32_t k0, k1, k2, k3;
+              ldsm_x4(kbuf + (c >> 3) * HALFB + r * 128 + (((c & 7) ^ (r & 7)) << 4), k0, k1, k2, k3);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) Mma<T>::run(sum[j % SETS][mt][n], k0, k1, k2, k3, qb[n][j][0], qb[n][j][1]);
+            }
+          }
+          const bool masked = key0 + WK > min(lim_min, t_end);
+          float tmax[NT][2];
+          bool move = false;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            tmax[n][0] = tmax[n][1] = -INFINITY;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
               for (int c = 0; c < 4; ++c) {
-                const int tok = key0 + 8 * n + 2 * tq + (c & 1);
-                s[n][c] = (s[n][c] + s2[n][c]) * a.scale_log2;
-                if (masked && (tok >= lim[c >> 1] || tok >= t_end)) s[n][c] = -INFINITY;
-                tmax[c >> 1] = fmaxf(tmax[c >> 1], s[n][c]);
+                float x = sum[0][mt][n][c];
+                if constexpr (SETS == 2) x += sum[SETS - 1][mt][n][c];
+                x *= a.scale_log2;
+                if (masked) {
+                  const int tok = key0 + 16 * mt + g8 + 8 * (c >> 1);
+                  if (tok >= lim(n, c & 1) || tok >= t_end) x = -INFINITY;
+                }
+                s[mt][n][c] = x;
+                tmax[n][c & 1] = fmaxf(tmax[n][c & 1], x);
               }
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              tmax[r] = fmaxf(tmax[r], __shfl_xor_sync(0xffffffffu, tmax[r], 1));
-              tmax[r] = fmaxf(tmax[r], __shfl_xor_sync(0xffffffffu, tmax[r], 2));
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+              for (int x = 4; x < 32; x <<= 1) tmax[n][e] = fmaxf(tmax[n][e], __shfl_xor_sync(0xffffffffu, tmax[n][e], x));
+              move |= tmax[n][e] > m_run[n][e] + kLazy;
             }
-            // the running maximum moves only when a score passes it by kLazy (or is the first)
-            if (__any_sync(0xffffffffu, tmax[0] > m_run[0] + kLazy || tmax[1] > m_run[1] + kLazy)) {
+          }
+          // the running maximum moves only when a score passes it by kLazy (or is the first)
+          if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
-              for (int r = 0; r < 2; ++r) {
-                const bool move = tmax[r] > m_run[r] + kLazy;
-                const float alpha = move ? exp2_fast(m_run[r] - tmax[r]) : 1.f;   // m_run = -inf: 0
-                if (move) m_run[r] = tmax[r];
-                l_run[r] *= alpha;
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int n = 0; n < NTILES; ++n) {
-                  o[n][2 * r] *= alpha;
-                  o[n][2 * r + 1] *= alpha;
+              for (int e = 0; e < 2; ++e) {
+                const bool up = tmax[n][e] > m_run[n][e] + kLazy;
+                const float alpha = up ? exp2_fast(m_run[n][e] - tmax[n][e]) : 1.f;   // m_run = -inf: 0
+                if (up) m_run[n][e] = tmax[n][e];
+                l_run[n][e] *= alpha;
+#pragma unroll
+                for (int m = 0; m < DT; ++m) {
+                  o[m][n][e] *= alpha;
+                  o[m][n][2 + e] *= alpha;
                 }
               }
-            }
-#pragma unroll
-            for (int r = 0; r < 2; ++r) msafe[r] = m_run[r] == -INFINITY ? 0.f : m_run[r];
           }
-          if (blk == WK / WB - 1) {   // the warp is done with K
-            __syncwarp();
-            if (lane == 0) mbar_arrive(empty + 8 * ks);
+        }
+        __syncwarp();   // the warp is done with K (and, after the last stage, with Q)
+        if (lane == 0) {
+          mbar_arrive(empty + 8 * ks);
+          if (!Q_REGS && i == nst - 1) mbar_arrive(q_empty);
+        }
+        landed = landed && mbar_wait(full + 8 * vs, ((2 * it + 1) / kSlots) & 1);
+        // The keys at the end: value rows past it become zeros. And keys that some rows of the tile see and
+        // others do not (the newest T - 1): a zero weight times an infinite or NaN value would reach the rows
+        // that must not see it, so such value rows (rare) are taken out of the stage (`bad`) and added to the
+        // rows that do see them one by one below. A warp alone reads its keys' rows.
+        uint32_t bad = 0;
+        const bool check = causal && min(key0 + WK, t_end) > lim_min;
+        if (!idle && (check || key0 + WK > t_end)) {
+          constexpr int PASS = 32 / CH;   // rows per pass of the warp
+          const int c = lane % CH;
+#pragma unroll
+          for (int p = 0; p < WK / PASS; ++p) {
+            const int y = p * PASS + lane / CH, r = lead + y, tok = key0 + y;
+            uint4* const x = reinterpret_cast<uint4*>(smem + (vbuf - ring) + (c >> 3) * HALFB + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+            const uint32_t hit = __ballot_sync(0xffffffffu, check && tok >= lim_min && tok < t_end && nonfinite8<T>(*x));
+#pragma unroll
+            for (int z = 0; z < PASS; ++z)
+              if (hit >> (z * CH) & (CH == 8 ? 0xFFu : 0xFFFFu)) bad |= 1u << (p * PASS + z);
+            if (tok >= t_end || (bad >> y & 1)) *x = make_uint4(0, 0, 0, 0);
           }
-          if (blk == 0) landed = landed && mbar_wait(full + 8 * vs, ((2 * it + 1) / kSlots) & 1);
-          // The keys at the end: value rows past it become zeros. And keys that some rows of the tile see and
-          // others do not (the newest T - 1): a zero weight times an infinite or NaN value would reach the
-          // rows that must not see it, so such value rows (rare) are taken out of the stage (`bad`) and added
-          // to the rows that do see them one by one below. Every warp clears the rows that it multiplies.
-          uint32_t bad = 0;
-          const bool check = a.T > 1 && g.b >= 0 && min(key0 + WB, t_end) > lim_min;
-          if (!idle && (check || key0 + WB > t_end)) {
-            constexpr int PASS = 32 / CH;   // rows per pass of the warp
-            const int c = lane % CH;
-            if (check) {
+          fence_proxy_async();   // the slot's next tensor copy comes after these writes
+          __syncwarp();
+        }
+        if (!idle) {
 #pragma unroll
-              for (int p = 0; p < WB / PASS; ++p) {
-                const int r = lead + p * PASS + lane / CH;
-                const uint4 x = *reinterpret_cast<const uint4*>(smem + (vbuf - ring) + (c >> 3) * HALFB + r * 128 + (((c & 7) ^ (r & 7)) << 4));
-                const uint32_t hit = __ballot_sync(0xffffffffu, stage0 + r >= lim_min && stage0 + r < t_end && nonfinite8<T>(x));
+          for (int mt = 0; mt < MT; ++mt) {
+            uint32_t pb[NT][2];   // P as the B operand: row 8 n + g8, keys 2 tq .. (+ 8)
 #pragma unroll
-                for (int y = 0; y < PASS; ++y)
-                  if (hit >> (y * CH) & (CH == 8 ? 0xFFu : 0xFFFFu)) bad |= 1u << (p * PASS + y);
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                const float mr = m_run[n][c & 1];
+                s[mt][n][c] = exp2_fast(s[mt][n][c] - (mr == -INFINITY ? 0.f : mr));
+                l_run[n][c & 1] += s[mt][n][c];
               }
-              // the warps of other row tiles look at the same rows: all have seen them before any clears them
-              if (RW > 1 && bad) asm volatile("bar.sync %0, %1;\n" ::"r"(2 + kw), "n"(RW * 32) : "memory");
+              pb[n][0] = transpose8(Dt<T>::pack2(s[mt][n][0], s[mt][n][1]));
+              pb[n][1] = transpose8(Dt<T>::pack2(s[mt][n][2], s[mt][n][3]));
             }
 #pragma unroll
-            for (int p = 0; p < WB / PASS; ++p) {
-              const int i = p * PASS + lane / CH, r = lead + i;
-              if (stage0 + r >= t_end || (bad >> i & 1))
-                *reinterpret_cast<uint4*>(smem + (vbuf - ring) + (c >> 3) * HALFB + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+            for (int m = 0; m < DT; ++m) {
+              const int r = lead + 16 * mt + (mi >> 1) * 8 + ri, c = 2 * m + (mi & 1);
+              uint32_t v0, v1, v2, v3;
+              ldsm_x4_t(vbuf + (c >> 3) * HALFB + r * 128 + (((c & 7) ^ (r & 7)) << 4), v0, v1, v2, v3);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) Mma<T>::run(o[m][n], v0, v1, v2, v3, pb[n][0], pb[n][1]);
             }
-            fence_proxy_async();   // the slot's next tensor copy comes after these writes
-            __syncwarp();
-          }
-          if (!idle) {
+            if (bad >> (16 * mt) & 0xFFFFu) {   // the value rows taken out above, for the rows that see them
+              for (int y = 0; y < 16; ++y) {
+                if (!(bad >> (16 * mt + y) & 1)) continue;
+                const int tok = key0 + 16 * mt + y, pi = a.div.page(tok);
+                const int page = (tok >= a.prefix_len ? a.table + g.b * a.ld_table : a.prefix_table)[pi];
+                const T* v = static_cast<const T*>(a.kv.v) + page * a.kv.sv_p + g.kvh * a.kv.sv_h + a.div.slot(tok, pi) * a.kv.sv_s + g8;
 #pragma unroll
-            for (int u = 0; u < WB / 16; ++u) {   // 16 keys at a time
-              uint32_t pa[4];
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                float(&p)[4] = s[2 * u + h];
+                  for (int e = 0; e < 2; ++e) {
+                    const float w = __shfl_sync(0xffffffffu, y < 8 ? s[mt][n][e] : s[mt][n][2 + e], (y & 7) * 4 + tq);
+                    if (tok >= lim(n, e)) continue;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) p[c] = exp2_fast(p[c] - msafe[c >> 1]);
-                l_run[0] += p[0] + p[1];
-                l_run[1] += p[2] + p[3];
-                pa[2 * h] = Dt<T>::pack2(p[0], p[1]);
-                pa[2 * h + 1] = Dt<T>::pack2(p[2], p[3]);
-              }
-#pragma unroll
-              for (int np = 0; np < NTILES; np += 2) {
-                const int r = lead + 16 * u + 8 * (mi & 1) + ri, c = np + (mi >> 1);
-                uint32_t v0, v1, v2, v3;
-                ldsm_x4_t(vbuf + (c >> 3) * HALFB + r * 128 + (((c & 7) ^ (r & 7)) << 4), v0, v1, v2, v3);
-                Mma<T>::run(o[np], pa[0], pa[1], pa[2], pa[3], v0, v1);
-                Mma<T>::run(o[np + 1], pa[0], pa[1], pa[2], pa[3], v2, v3);
-              }
-            }
-            if (bad) {   // the value rows taken out above, for the rows that see them
-#pragma unroll
-              for (int n = 0; n < WB / 8; ++n) {
-                for (int col = 0; col < 8; ++col) {
-                  const int r = lead + 8 * n + col;
-                  if (!(bad >> (8 * n + col) & 1)) continue;
-                  const int src = (lane & ~3) | (col >> 1);
-                  const float p0 = __shfl_sync(0xffffffffu, (col & 1) ? s[n][1] : s[n][0], src);
-                  const float p1 = __shfl_sync(0xffffffffu, (col & 1) ? s[n][3] : s[n][2], src);
-                  const int tok = stage0 + r, pi = a.div.page(tok);
-                  const int page = (tok >= a.prefix_len ? a.table + g.b * a.ld_table : a.prefix_table)[pi];
-                  const T* v = static_cast<const T*>(a.kv.v) + page * a.kv.sv_p + g.kvh * a.kv.sv_h +
-                               a.div.slot(tok, pi) * a.kv.sv_s + 2 * tq;
-#pragma unroll
-                  for (int d = 0; d < NTILES; ++d)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                      const float x = Dt<T>::to_f32(v[8 * d + e]);
-                      if (tok < lim[0]) o[d][e] += p0 * x;
-                      if (tok < lim[1]) o[d][2 + e] += p1 * x;
+                    for (int m = 0; m < DT; ++m) {
+                      o[m][n][e] += w * Dt<T>::to_f32(v[16 * m]);
+                      o[m][n][2 + e] += w * Dt<T>::to_f32(v[16 * m + 8]);
                     }
-                }
+                  }
               }
             }
           }
@@ -596,100 +602,65 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
         __syncwarp();
         if (lane == 0) mbar_arrive(empty + 8 * vs);
       }
+      if (!Q_REGS && nst == 0) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_empty);
+      }
 
-      // ---- the unit's (or this CTA's part of it) result
-      if (!landed) l_run[0] = l_run[1] = NAN;
+      // ---- the unit's (or this CTA's part of it) result: the key warps meet in shared memory
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 1);
-        l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 2);
-      }
-      if constexpr (KW > 1) {
-        if (tq == 0) {
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            s_m[warp][g8 + 8 * r] = m_run[r];
-            s_l[warp][g8 + 8 * r] = l_run[r];
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) l_run[n][e] += __shfl_xor_sync(0xffffffffu, l_run[n][e], x);
+          if (g8 == 0) {
+            s_m[warp][8 * n + 2 * tq + e] = m_run[n][e];
+            s_l[warp][8 * n + 2 * tq + e] = landed ? l_run[n][e] : NAN;
           }
         }
-      }
-      named_sync<1, kConsumers>();
-      // factor of this thread's rows, from the key warps' maxima; (m, l) of the tile's row by its first warp
-      float factor[2];
+      landed = named_all<1, kConsumers>(landed);
+      constexpr int PAD = D + 4;   // the rows 2 tq of the accumulators' columns fall into different banks
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        float mx = m_run[r], l = l_run[r];
-        if constexpr (KW > 1) {
-          mx = -INFINITY;
-          l = 0.f;
+      for (int n = 0; n < NT; ++n) {
+        if (8 * n >= g.nrows) break;
+        if (n > 0) named_sync<1, kConsumers>();
 #pragma unroll
-          for (int k = 0; k < KW; ++k) mx = fmaxf(mx, s_m[k * RW + rw][g8 + 8 * r]);
+        for (int e = 0; e < 2; ++e) {
+          const int row = 8 * n + 2 * tq + e;
+          float mx = -INFINITY, l = 0.f;
 #pragma unroll
-          for (int k = 0; k < KW; ++k) {
-            const float m = s_m[k * RW + rw][g8 + 8 * r];
-            l += (m == -INFINITY ? 0.f : exp2_fast(m - mx)) * s_l[k * RW + rw][g8 + 8 * r];
+          for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, s_m[w][row]);
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) l += (s_m[w][row] == -INFINITY ? 0.f : exp2_fast(s_m[w][row] - mx)) * s_l[w][row];
+          if (!landed) l = NAN;
+          float factor = m_run[n][e] == -INFINITY ? 1.f : exp2_fast(m_run[n][e] - mx);
+          // a row that sees no key: zeros (l is NaN, not 0, where a visible score is)
+          if (g.kind == 0) factor *= l == 0.f ? 0.f : 1.f / l;
+          else if (g8 == 0 && warp == 0 && row < g.nrows) *reinterpret_cast<float2*>(a.ml + s_at[row] * 2) = make_float2(mx, l);
+          float* dst = s_o + (warp * 8 + 2 * tq + e) * PAD + g8;
+#pragma unroll
+          for (int m = 0; m < DT; ++m) {
+            dst[16 * m] = o[m][n][e] * factor;
+            dst[16 * m + 8] = o[m][n][2 + e] * factor;
           }
         }
-        factor[r] = KW == 1 || m_run[r] == -INFINITY ? 1.f : exp2_fast(m_run[r] - mx);
-        // a row that sees no key: zeros (l is NaN, not 0, where a visible score is)
-        if (g.kind == 0) factor[r] *= l == 0.f ? 0.f : 1.f / l;
-        const int row = 16 * rw + g8 + 8 * r;
-        if (g.kind != 0 && tq == 0 && kw == 0 && row < g.nrows)
-          *reinterpret_cast<float2*>(a.ml + s_at[row] * 2) = make_float2(mx, l);
-      }
-      if constexpr (KW == 1) {
+        named_sync<1, kConsumers>();
+        const int live = min(g.nrows - 8 * n, 8);
+        for (int idx = tid; idx < live * (D / 4); idx += kConsumers) {
+          const int row = idx / (D / 4), d = 4 * (idx % (D / 4));
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int row = 16 * rw + g8 + 8 * r;
-          if (row < g.nrows) {
-            const int64_t at = s_at[row];
-#pragma unroll
-            for (int n = 0; n < NTILES; ++n) {
-              const float x = o[n][2 * r] * factor[r], y = o[n][2 * r + 1] * factor[r];
-              const int d = 8 * n + 2 * tq;
-              if (g.kind == 0) store_out2<T>(a, at + d, x, y);
-              else *reinterpret_cast<float2*>(a.acc + at * D + d) = make_float2(x, y);
-            }
+          for (int w = 0; w < kWarps; ++w) {
+            const float4 x = *reinterpret_cast<const float4*>(s_o + (w * 8 + row) * PAD + d);
+            v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
           }
-        }
-      } else {
-        // up to 8 rows (the usual decode) go through the merge buffer at once, more 64 elements at a time
-        auto merge = [&](auto width, int col0) {
-          constexpr int WIDTH = decltype(width)::value, PAD = WIDTH + 8;
-          const int limit = WIDTH == D && D > 64 ? 8 : 16;   // rows of a warp's part of the buffer
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            float* dst = s_o + (warp * limit + g8 + 8 * r) * PAD + 2 * tq;
-            if (g8 + 8 * r < limit && 16 * rw + g8 + 8 * r < g.nrows) {
-#pragma unroll
-              for (int n = 0; n < NTILES; ++n) {
-                if (8 * n < col0 || 8 * n >= col0 + WIDTH) continue;
-                *reinterpret_cast<float2*>(dst + 8 * n - col0) = make_float2(o[n][2 * r] * factor[r], o[n][2 * r + 1] * factor[r]);
-              }
-            }
-          }
-          named_sync<1, kConsumers>();
-          for (int idx = tid; idx < g.nrows * (WIDTH / 2); idx += kConsumers) {
-            const int row = idx / (WIDTH / 2), d = 2 * (idx % (WIDTH / 2)), w0 = row / 16, rr = row % 16;
-            float2 v = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int k = 0; k < KW; ++k) {
-              const float2 x = *reinterpret_cast<const float2*>(s_o + ((k * RW + w0) * limit + rr) * PAD + d);
-              v.x += x.x;
-              v.y += x.y;
-            }
-            const int64_t at = s_at[row];
-            if (g.kind == 0) store_out2<T>(a, at + col0 + d, v.x, v.y);
-            else *reinterpret_cast<float2*>(a.acc + at * D + col0 + d) = v;
-          }
-        };
-        if (D == 64 || g.nrows <= 8) {
-          merge(std::integral_constant<int, D>{}, 0);
-        } else {
-#pragma unroll
-          for (int hf = 0; hf < HALVES; ++hf) {
-            if (hf > 0) named_sync<1, kConsumers>();
-            merge(std::integral_constant<int, 64>{}, 64 * hf);
+          const int64_t at = s_at[8 * n + row];
+          if (g.kind == 0) {
+            store_out2<T>(a, at + d, v.x, v.y);
+            store_out2<T>(a, at + d + 2, v.z, v.w);
+          } else {
+            *reinterpret_cast<float4*>(a.acc + at * D + d) = v;
           }
         }
       }
@@ -702,17 +673,17 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
 // A thread reads its row's (m, l) along with the sums and keeps a running maximum, so that one round trip to
 // memory follows the streaming kernel's end; the rest is done while that kernel still runs (its shared memory
 // is sized to leave room for these blocks).
-template <typename T, int D, int RW>
+template <typename T, int D, int NT>
 __global__ void __launch_bounds__(128, 6) paged_combine_kernel(const __grid_constant__ PagedAttnArgs a) {
-  constexpr int ROWS = 16 * RW, QUADS = D / 4, BLOCK_ROWS = 128 / QUADS;
+  constexpr int ROWS = 8 * NT, QUADS = D / 4, BLOCK_ROWS = 128 / QUADS;
   constexpr int MOST = kMaxParts + kMaxCtas + 2;   // a prefix unit's and an own unit's CTAs have at most one in common
   __shared__ int s_sum[kMaxBatch + 1], s_len[kMaxBatch], s_warp[4];
   __shared__ int64_t s_entry[MOST];   // entry of the first row, or -1 - (its block of R rows in the output's order)
   const int tid = threadIdx.x;
   pdl_launch_dependents();
   // the lengths are inputs of the whole call, complete before its first kernel began
-  Line<D, RW> line(a);
-  scan_stages<D, RW, 128>(a, s_sum, s_len, s_warp);
+  Line<D, NT> line(a);
+  scan_stages<D, NT, 128>(a, s_sum, s_len, s_warp);
   line.close(a, s_sum[a.B]);
   const int64_t R = all_rows(a);
   const int b = blockIdx.x / a.kv.KVH, kvh = blockIdx.x - b * a.kv.KVH;
@@ -757,7 +728,7 @@ __global__ void __launch_bounds__(128, 6) paged_combine_kernel(const __grid_cons
     __syncthreads();
     const int r = tid / QUADS, d = (tid - r * QUADS) * 4;
     if (r < n) {
-      const int t = (row0 + r) / a.G, head = kvh * a.G + row0 + r - t * a.G;
+      const int t = div_g(a, row0 + r), head = kvh * a.G + row0 + r - t * a.G;
       const int64_t index = (static_cast<int64_t>(b) * a.T + t) * a.H + head;
       float m = -INFINITY, l = 0.f;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -837,11 +808,11 @@ int box_rows(const b2d_paged_kv& kv, int prefix_len) {
   return prefix_len % rows == 0 ? rows : 0;
 }
 
-int row_warps(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+int row_tiles(int64_t rows) { return rows < 32 ? static_cast<int>((rows + 7) / 8) : 4; }   // of 8, in a unit
 
 // How a call is cut.
 struct Plan {
-  int shared, tc5, splits, nparts, rw, ctas, whole, combine, fits;
+  int shared, tc5, splits, nparts, nt, ctas, whole, combine, fits;
   int64_t slot0, entries;
   size_t bytes;
 };
@@ -851,7 +822,7 @@ Plan make_plan(const b2d_paged_kv* kv, int B, int T, int H, int pages_per_seq, i
   const int64_t reach = static_cast<int64_t>(pages_per_seq) * kv->page_size;
   const int64_t rows = static_cast<int64_t>(T) * (H / kv->KVH), all = B * rows;
   p.shared = B > 1 ? prefix_len / 64 * 64 : 0;   // one sequence has nothing to share; the rest of 64 is read per sequence
-  p.tc5 = p.shared >= 128 && all > 64 && box_rows(*kv, prefix_len) > 0;
+  p.tc5 = p.shared >= 128 && all > 32 && box_rows(*kv, prefix_len) > 0;
   if (p.tc5) {
     // one CTA per SM, at least two tiles of 128 keys each
     const int64_t groups = kv->KVH * ((all + 255) / 256), tiles = (p.shared + 127) / 128;
@@ -863,8 +834,8 @@ Plan make_plan(const b2d_paged_kv* kv, int B, int T, int H, int pages_per_seq, i
     p.nparts = p.splits * per;
   }
   const bool streams_prefix = p.shared > 0 && !p.tc5;
-  p.rw = row_warps(streams_prefix ? all : rows);
-  const int tile = 16 * p.rw, keys_per_stage = kSlotBytes / (kv->D * 2);
+  p.nt = row_tiles(streams_prefix ? all : rows);
+  const int tile = 8 * p.nt, keys_per_stage = kSlotBytes / (kv->D * 2);
   int64_t keys = max_len > 0 && max_len < reach ? max_len : reach;
   if (keys < prefix_len) keys = prefix_len;
   // the most stages that there can be
@@ -889,10 +860,10 @@ Plan make_plan(const b2d_paged_kv* kv, int B, int T, int H, int pages_per_seq, i
   return p;
 }
 
-template <typename T, int D, int RW>
+template <typename T, int D, int NT>
 int launch_stream(const PoolMaps& maps, const PagedAttnArgs& a, bool combine, bool pdl, cudaStream_t s) {
-  auto kern = paged_stream_kernel<T, D, RW>;
-  constexpr uint32_t bytes = smem_bytes<D, RW>();
+  auto kern = paged_stream_kernel<T, D, NT>;
+  constexpr uint32_t bytes = smem_bytes<D, NT>();
   static bool configured[64] = {};   // per device; setting it twice is harmless
   int dev = 0;
   cudaGetDevice(&dev);
@@ -906,7 +877,7 @@ int launch_stream(const PoolMaps& maps, const PagedAttnArgs& a, bool combine, bo
   }
   int st = launch_kernel(kern, dim3(a.ctas), dim3(kThreads), bytes, s, pdl || a.after_prefix, maps, a);
   if (st != B2D_OK || !combine) return st;
-  return launch_kernel(paged_combine_kernel<T, D, RW>, dim3(a.B * a.kv.KVH, (a.rows + 512 / D - 1) / (512 / D)),
+  return launch_kernel(paged_combine_kernel<T, D, NT>, dim3(a.B * a.kv.KVH, (a.rows + 512 / D - 1) / (512 / D)),
                        dim3(128), 0, s, true, a);
 }
 
@@ -923,9 +894,12 @@ int run(PagedAttnArgs& a, const Plan& p, bool pdl, cudaStream_t s) {
   } else if (p.tc5) {   // tensor maps refused: every sequence reads the prefix itself
     a.shared = 0;
   }
-  if (p.rw == 1) return launch_stream<T, D, 1>(maps, a, p.combine, pdl, s);
-  if (p.rw == 2) return launch_stream<T, D, 2>(maps, a, p.combine, pdl, s);
-  return launch_stream<T, D, 4>(maps, a, p.combine, pdl, s);
+  switch (p.nt) {
+    case 1: return launch_stream<T, D, 1>(maps, a, p.combine, pdl, s);
+    case 2: return launch_stream<T, D, 2>(maps, a, p.combine, pdl, s);
+    case 3: return launch_stream<T, D, 3>(maps, a, p.combine, pdl, s);
+    default: return launch_stream<T, D, 4>(maps, a, p.combine, pdl, s);
+  }
 }
 
 int check_shapes(const b2d_paged_kv* kv, int B, int T, int H, int pages_per_seq, int prefix_len, int max_len) {
@@ -983,7 +957,7 @@ extern "C" int b2d_paged_attention(const b2d_paged_kv* kv, const void* q, int64_
     a.so_b = so_b; a.so_t = so_t; a.so_h = so_h;
     a.kv = *kv; a.div = page_div(kv->page_size);
     a.pages_per_seq = pages_per_seq; a.prefix_len = prefix_len;
-    a.B = n; a.T = T; a.H = H; a.G = H / kv->KVH; a.rows = T * a.G;
+    a.B = n; a.T = T; a.H = H; a.G = H / kv->KVH; a.rows = T * a.G; a.inv_g = (65536 + a.G - 1) / a.G;
     a.scale_log2 = scale * kLog2e;
     a.shared = p.shared; a.nparts = p.nparts; a.splits = p.splits; a.ctas = p.ctas; a.whole = p.whole; a.slot0 = p.slot0;
     a.out_f32 = out_dtype == B2D_F32;

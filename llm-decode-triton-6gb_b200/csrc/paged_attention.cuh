@@ -19,6 +19,7 @@ struct PagedAttnArgs {
   b2d_paged_kv kv;
   PageDiv div;
   int pages_per_seq, prefix_len, B, T, H, G, rows;   // rows = T G: query vectors of a sequence and KV head
+  int inv_g;        // 2^16 / G, rounded up
   float scale_log2;
   int shared;       // positions [0, shared) are computed once for the batch (0: none are)
   int nparts;       // partials of the tcgen05 prefix launch (0: the streaming kernel takes the prefix)

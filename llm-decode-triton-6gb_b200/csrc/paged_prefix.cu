@@ -1,6 +1,6 @@
 // Attention over a prefix that the whole batch shares, on the 5th-generation tensor cores (sm_100a): the
 // queries of all sequences that read one KV head form one row axis, so the prefix is read once for up to 256
-// rows and the two products are 128 x 128 x 128 matrix products. Used from more than 64 rows on (below, the
+// rows and the two products are 128 x 128 x 128 matrix products. Used from more than 32 rows on (below, the
 // mma.sync kernel of csrc/paged_attention.cu is bound by the same bytes); leaves (O, m, l) per row and split
 // of the keys, which that file's per-sequence kernel takes in.
 //

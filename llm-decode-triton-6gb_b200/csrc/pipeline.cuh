@@ -59,6 +59,12 @@ __device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t& r0, uint32_t&
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];\n"
                : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(addr) : "memory");
 }
+// Transposes an 8 x 8 matrix of 16-bit values held two per lane (lane l: row l / 4, columns 2 (l % 4), + 1).
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
+  return y;
+}
 // 2^x (the hardware's approximation: 2 units in the last place, results below 2^-126 become 0)
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
