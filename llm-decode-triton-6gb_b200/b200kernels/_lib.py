@@ -155,28 +155,24 @@ def ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
 
 
-def cuda_index(device) -> int:
-    """The device's index; raises for tensors that are not on a GPU."""
-    import torch
-    if device.type != "cuda":
-        raise ValueError(f"the tensors are on {device}; the kernels run on a CUDA device only")
-    return device.index if device.index is not None else torch.cuda.current_device()
+_binding = None
 
 
-def on_device(index: int):
-    """Context that makes device ``index`` current (the library launches on the current device)."""
-    import contextlib
-
-    import torch
-    return contextlib.nullcontext() if torch.cuda.current_device() == index else torch.cuda.device(index)
-
-
-def call_on(index: int, name: str, *args) -> None:
-    """``call`` an entry point whose last argument is the stream, on device ``index`` and torch's current
-    stream there, whichever device is current."""
-    import torch
-    if torch.cuda.current_device() == index:
-        call(name, *args, torch.cuda.current_stream(index).cuda_stream)
-    else:
-        with torch.cuda.device(index):
-            call(name, *args, torch.cuda.current_stream(index).cuda_stream)
+def binding():
+    """The CPython module of csrc/binding.cpp (the checks and calls of the paged-cache and draft-verification
+    entry points), bound to the library's functions; raises if it has not been built."""
+    global _binding
+    if _binding is None:
+        import importlib.machinery
+        import importlib.util
+        path = LIB_PATH.parent / "_binding.so"
+        if not path.exists():
+            raise RuntimeError(f"{path} is missing: build it with `python llm-decode-triton-6gb_b200/build.py`")
+        lib = load()
+        loader = importlib.machinery.ExtensionFileLoader("_binding", str(path))
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_binding", loader))
+        loader.exec_module(module)
+        module.bind(*(C.cast(getattr(lib, f), C.c_void_p).value for f in (
+            "b2d_paged_rope_append", "b2d_paged_attention_workspace_bytes", "b2d_paged_attention", "b2d_verify_drafts")))
+        _binding = module
+    return _binding

@@ -18,6 +18,7 @@ REPO_ROOT = PKG_ROOT.parent
 CSRC = PKG_ROOT / "csrc"
 INCLUDE = REPO_ROOT / "include"
 LIB_PATH = PKG_ROOT / "b200kernels" / "libb200decode.so"
+BINDING_PATH = PKG_ROOT / "b200kernels" / "_binding.so"   # CPython module of csrc/binding.cpp
 SOURCES = ["capi.cu", "nf4_gemm.cu", "nf4_gemm_tma.cu", "nf4_tc5.cu", "nf4_format.cu", "gqa_decode.cu", "decode_glue.cu", "tp_allreduce.cu", "lm_head.cu",
            "paged_append.cu", "paged_attention.cu", "paged_prefix.cu", "verify_drafts.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -31,10 +32,10 @@ def nvcc_path() -> str:
 
 
 def needs_build() -> bool:
-    if not LIB_PATH.exists():
+    if not LIB_PATH.exists() or not BINDING_PATH.exists():
         return True
-    t = LIB_PATH.stat().st_mtime
-    deps = [CSRC / s for s in SOURCES] + list(CSRC.glob("*.cuh")) + [INCLUDE / "b200decode.h", Path(__file__)]
+    t = min(LIB_PATH.stat().st_mtime, BINDING_PATH.stat().st_mtime)
+    deps = [CSRC / s for s in SOURCES] + [CSRC / "binding.cpp"] + list(CSRC.glob("*.cuh")) + [INCLUDE / "b200decode.h", Path(__file__)]
     return any(p.stat().st_mtime > t for p in deps if p.exists())
 
 
@@ -43,6 +44,24 @@ def _compile(src: Path, obj: Path, verbose: bool) -> subprocess.CompletedProcess
            "-o", str(obj), str(src)]
     if verbose:
         cmd.insert(1, "-Xptxas=-v")
+        print(" ".join(cmd))
+    return subprocess.run(cmd, capture_output=True, text=True)
+
+
+def _build_binding(out: Path, verbose: bool) -> subprocess.CompletedProcess:
+    """The CPython module against this interpreter's torch (its libraries are loaded by `import torch`)."""
+    import sysconfig
+
+    import torch
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc_path()).resolve().parent.parent
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}",
+           f"-I{root / 'include'}", f"-I{root / 'include/torch/csrc/api/include'}", f"-I{cuda / 'include'}",
+           f"-I{sysconfig.get_paths()['include']}", "-o", str(out), str(CSRC / "binding.cpp"),
+           f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python",
+           f"-Wl,-rpath,{root / 'lib'}"]
+    if verbose:
         print(" ".join(cmd))
     return subprocess.run(cmd, capture_output=True, text=True)
 
@@ -56,8 +75,10 @@ def build(verbose: bool = False, force: bool = False) -> Path:
     from concurrent.futures import ThreadPoolExecutor
     with tempfile.TemporaryDirectory(dir=LIB_PATH.parent) as tmp:
         objs = [Path(tmp) / (Path(s).stem + ".o") for s in SOURCES]
-        with ThreadPoolExecutor(max_workers=min(len(SOURCES), os.cpu_count() or 1)) as ex:
+        with ThreadPoolExecutor(max_workers=min(len(SOURCES) + 1, os.cpu_count() or 1)) as ex:
+            binding = ex.submit(_build_binding, Path(tmp) / BINDING_PATH.name, verbose)
             results = list(ex.map(lambda so: _compile(CSRC / so[0], so[1], verbose), zip(SOURCES, objs)))
+            results.append(binding.result())
         failed = False
         for res in results:
             if verbose or res.returncode != 0:
@@ -65,7 +86,7 @@ def build(verbose: bool = False, force: bool = False) -> Path:
                 sys.stderr.write(res.stderr)
             failed |= res.returncode != 0
         if failed:
-            raise RuntimeError("nvcc failed")
+            raise RuntimeError("the compiler failed")
         cmd = [nvcc_path(), "-shared", *ARCH, "-cudart", "shared", "-o", str(LIB_PATH) + ".tmp", *map(str, objs)]
         res = subprocess.run(cmd, capture_output=True, text=True)
         if verbose or res.returncode != 0:
@@ -73,6 +94,7 @@ def build(verbose: bool = False, force: bool = False) -> Path:
             sys.stderr.write(res.stderr)
         if res.returncode != 0:
             raise RuntimeError(f"nvcc link failed with exit code {res.returncode}")
+        os.replace(Path(tmp) / BINDING_PATH.name, BINDING_PATH)
     os.replace(str(LIB_PATH) + ".tmp", LIB_PATH)
     return LIB_PATH
 
