@@ -6,16 +6,21 @@
 // Only the row that the draw needs is read (V values of p, and of q after a refusal), not all K + 1.
 // Every product, sum and comparison is in 64 bits: with fp32 running sums over 10^5 weights the border
 // between two tokens moves by more than a small token's own weight.
-//  1. thread i < n tests draft i; the first refusal is the lowest clear bit of a ballot;
-//  2. every warp sums its contiguous piece of the row;
-//  3. the pieces are scanned in order; the warp whose piece holds the target walks it 32 values at a time.
+// A sequence takes a thread-block cluster of up to 8 CTAs:
+//  1. thread i < n tests draft i (in every CTA: the few loads are cheaper than an exchange); the first refusal
+//     is the lowest clear bit of a ballot;
+//  2. every warp sums its contiguous piece of the row (loads of 8 steps in flight), and the pieces' sums meet
+//     through distributed shared memory;
+//  3. a warp of each CTA scans them; the CTA that holds the target sums the piece again in 256 chunks (from
+//     L2), scans those, and the thread that holds the target walks its chunk.
 #include "common.cuh"
 
 namespace b2d {
 namespace {
 
-constexpr int kVerifyThreads = 1024;
+constexpr int kVerifyThreads = 256;
 constexpr int kVerifyWarps = kVerifyThreads / 32;
+constexpr int kVerifyCluster = 8;
 constexpr int kMaxDrafts = 31;
 
 struct VerifyArgs {
@@ -47,19 +52,35 @@ __device__ __forceinline__ double warp_sum(double v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+__device__ __forceinline__ double warp_scan(double v, int lane) {   // inclusive
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double up = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += up;
+  }
+  return v;
+}
+__device__ __forceinline__ double ld_dsmem_f64(uint32_t local_addr, int rank) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(remote) : "r"(local_addr), "r"(rank));
+  double v;
+  asm volatile("ld.shared::cluster.f64 %0, [%1];\n" : "=d"(v) : "r"(remote) : "memory");
+  return v;
+}
 
 template <typename P>
 __global__ void __launch_bounds__(kVerifyThreads) verify_drafts_kernel(const VerifyArgs a) {
   pdl_launch_dependents();
   pdl_wait();
-  __shared__ int s_accepted;
-  __shared__ double s_sum[kVerifyWarps], s_start[kVerifyWarps];
-  __shared__ double s_total;
-  __shared__ int s_owner, s_last;
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  __shared__ int s_accepted, s_owner, s_place[kVerifyWarps];
+  __shared__ double s_sum[kVerifyWarps];   // read by the cluster
+  __shared__ double s_start, s_total, s_scan[kVerifyWarps];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int ranks = cluster_size(), rank = cluster_rank(), b = static_cast<int>(blockIdx.x) / ranks;
   const int n = a.draft_lens ? max(0, min(a.K, a.draft_lens[b])) : a.K;
   const P* target = static_cast<const P*>(a.target) + b * a.st_b;
   const P* probs = a.probs ? static_cast<const P*>(a.probs) + b * a.sd_b : nullptr;
+  const double u_draw = static_cast<double>(a.u[b * a.ld_u + a.K]);
   if (warp == 0) {
     bool ok = false;
     if (lane < n) {
@@ -69,77 +90,141 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafts_kernel(const Ver
         ok = static_cast<double>(a.u[b * a.ld_u + lane]) * q < to_f64<P>(target[lane * a.st_k + x]);
       }
     }
-    const uint32_t refused = ~__ballot_sync(0xffffffffu, ok);   // lanes >= n count as refused
-    if (lane == 0) {
-      const int acc = min(n, __ffs(refused) - 1);
-      s_accepted = refused ? acc : n;
-    }
+    const uint32_t refused = ~__ballot_sync(0xffffffffu, ok);   // lanes >= n count as refused (n <= 31)
+    if (lane == 0) s_accepted = __ffs(refused) - 1;
   }
   __syncthreads();
   const int acc = s_accepted;
   const P* p = target + acc * a.st_k;
   const P* q = acc < n && probs ? probs + acc * a.sd_k : nullptr;
   int64_t x = acc < n && !probs ? a.draft[b * a.ld_tokens + acc] : -1;
-  const int piece = ((a.V + kVerifyWarps - 1) / kVerifyWarps + 31) / 32 * 32;
-  const int v0 = min(a.V, warp * piece), v1 = min(a.V, v0 + piece);
+  const int pieces = ranks * kVerifyWarps, piece = (a.V + pieces - 1) / pieces;
+  const int v0 = min(a.V, (rank * kVerifyWarps + warp) * piece), v1 = min(a.V, v0 + piece);
   for (int pass = 0;; ++pass) {
     double sum = 0.0;
-    for (int v = v0 + lane; v < v1; v += 32) sum += weight<P>(p, q, x, v);
+    for (int base = v0 + lane; base < v1; base += 256) {
+      P pv[8], qv[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int v = base + 32 * i;
+        pv[i] = v < v1 ? p[v] : P(0.f);
+        qv[i] = v < v1 && q ? q[v] : P(0.f);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const double w = base + 32 * i == x ? 0.0 : to_f64<P>(pv[i]) - to_f64<P>(qv[i]);
+        if (w > 0.0) sum += w;
+      }
+    }
     sum = warp_sum(sum);
     if (lane == 0) s_sum[warp] = sum;
-    __syncthreads();
-    if (tid == 0) {
-      double run = 0.0;
-      for (int w = 0; w < kVerifyWarps; ++w) {
-        s_start[w] = run;
-        run += s_sum[w];
+    if (ranks > 1) cluster_sync();
+    else __syncthreads();
+    if (warp == 0) {   // up to 64 pieces, two a lane
+      double w[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int e = 2 * lane + i;
+        w[i] = e >= pieces ? 0.0
+               : ranks > 1 ? ld_dsmem_f64(static_cast<uint32_t>(__cvta_generic_to_shared(&s_sum[e % kVerifyWarps])), e / kVerifyWarps)
+                           : s_sum[e];
       }
-      s_total = run;
-      const double goal = static_cast<double>(a.u[b * a.ld_u + a.K]) * run;
-      int owner = -1, last = -1;
-      for (int w = 0; w < kVerifyWarps; ++w) {
-        if (s_sum[w] > 0.0) last = w;
-        if (owner < 0 && s_start[w] + s_sum[w] > goal) owner = w;
+      const double incl = warp_scan(w[0] + w[1], lane), start = incl - (w[0] + w[1]);
+      const double total = __shfl_sync(0xffffffffu, incl, 31), goal = u_draw * total;
+      const uint32_t above0 = __ballot_sync(0xffffffffu, w[0] > 0.0 && start + w[0] > goal);
+      const uint32_t above1 = __ballot_sync(0xffffffffu, w[1] > 0.0 && incl > goal);
+      const uint32_t some0 = __ballot_sync(0xffffffffu, w[0] > 0.0), some1 = __ballot_sync(0xffffffffu, w[1] > 0.0);
+      int owner = -1;   // the first piece whose end is above the goal, else the last one with any weight
+      if (above0 | above1) {
+        const int l = __ffs(above0 | above1) - 1;
+        owner = 2 * l + ((above0 >> l & 1) ? 0 : 1);
+      } else if (some0 | some1) {
+        const int l = 31 - __clz(some0 | some1);
+        owner = 2 * l + ((some1 >> l & 1) ? 1 : 0);
       }
-      s_owner = owner < 0 ? last : owner;   // no piece reaches the goal: the last one with any weight
-      s_last = last;
+      const double begin0 = __shfl_sync(0xffffffffu, start, max(owner, 0) >> 1);
+      const double first = __shfl_sync(0xffffffffu, w[0], max(owner, 0) >> 1);
+      if (lane == 0) {
+        s_owner = owner;
+        s_total = total;
+        s_start = (owner & 1) ? begin0 + first : begin0;
+      }
     }
-    __syncthreads();
+    if (ranks > 1) cluster_sync();   // the sums are read; also a barrier of this CTA
+    else __syncthreads();
     if (s_total > 0.0 || pass == 1 || acc == n) break;
     q = nullptr;   // max(p - q, 0) is zero everywhere: draw from p
     x = -1;
-    __syncthreads();
   }
   const int owner = s_owner;
-  if (tid < a.K + 1 && tid != acc) a.tokens[b * a.ld_out + tid] = tid < acc ? a.draft[b * a.ld_tokens + tid] : -1;
-  if (tid == 0 && a.accepted) a.accepted[b] = acc;
-  if (owner < 0) {
-    if (tid == 0) a.tokens[b * a.ld_out + acc] = -1;
-    return;
+  if (rank == 0) {
+    if (tid < a.K + 1 && tid != acc) a.tokens[b * a.ld_out + tid] = tid < acc ? a.draft[b * a.ld_tokens + tid] : -1;
+    if (tid == 0 && a.accepted) a.accepted[b] = acc;
+    if (owner < 0 && tid == 0) a.tokens[b * a.ld_out + acc] = -1;
   }
-  if (warp != owner) return;
-  const double goal = static_cast<double>(a.u[b * a.ld_u + a.K]) * s_total;
-  double run = s_start[warp];
-  int found = -1, last = -1;
-  for (int base = v0; base < v1; base += 32) {
-    const int v = base + lane;
-    const double w = v < v1 ? weight<P>(p, q, x, v) : 0.0;
-    double scan = w;
+  if (owner < 0 || owner / kVerifyWarps != rank) return;
+  // ---- the owner's piece in 256 chunks, one a thread
+  const double goal = u_draw * s_total;
+  const int o0 = min(a.V, owner * piece), o1 = min(a.V, o0 + piece), chunk = (piece + kVerifyThreads - 1) / kVerifyThreads;
+  const int c0 = min(o1, o0 + tid * chunk), c1 = min(o1, c0 + chunk);
+  double sum = 0.0;
+#pragma unroll 4
+  for (int v = c0; v < c1; ++v) sum += weight<P>(p, q, x, v);
+  const double incl = warp_scan(sum, lane);
+  if (lane == 31) s_scan[warp] = incl;
+  __syncthreads();
+  double run = s_start;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double up = __shfl_up_sync(0xffffffffu, scan, o);
-      if (lane >= o) scan += up;
+  for (int w = 0; w < kVerifyWarps; ++w)
+    if (w < warp) run += s_scan[w];
+  const uint32_t above = __ballot_sync(0xffffffffu, sum > 0.0 && run + incl > goal);
+  const uint32_t some = __ballot_sync(0xffffffffu, sum > 0.0);
+  // the first thread whose end is above the goal, else the last one with any weight (as 2 T - thread)
+  constexpr int T2 = 2 * kVerifyThreads;
+  if (lane == 0)
+    s_place[warp] = above ? 32 * warp + __ffs(above) - 1 : some ? T2 - (32 * warp + 31 - __clz(some)) : T2 + 1;
+  __syncthreads();
+  int place = s_place[0];
+#pragma unroll
+  for (int w = 1; w < kVerifyWarps; ++w) place = min(place, s_place[w]);
+  if (place > T2 || tid != (place < kVerifyThreads ? place : T2 - place)) return;
+  run += incl - sum;
+  int found = -1, last = -1;
+  for (int v = c0; v < c1; ++v) {
+    const double w = weight<P>(p, q, x, v);
+    if (w > 0.0) {
+      last = v;
+      run += w;
+      if (run > goal) {
+        found = v;
+        break;
+      }
     }
-    const uint32_t some = __ballot_sync(0xffffffffu, w > 0.0);
-    if (some) last = base + 31 - __clz(some);
-    const uint32_t above = __ballot_sync(0xffffffffu, w > 0.0 && run + scan > goal);
-    if (above) {
-      found = base + __ffs(above) - 1;
-      break;
-    }
-    run += __shfl_sync(0xffffffffu, scan, 31);
   }
-  if (lane == 0) a.tokens[b * a.ld_out + acc] = found >= 0 ? found : last;
+  a.tokens[b * a.ld_out + acc] = found >= 0 ? found : last;
+}
+
+template <typename P>
+int launch_verify(const VerifyArgs& a, int B, int ranks, bool pdl, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(B) * ranks);
+  cfg.blockDim = dim3(kVerifyThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ranks;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, verify_drafts_kernel<P>, a);
+  if (e != cudaSuccess) {
+    set_cuda_error(e);
+    return B2D_ERR_LAUNCH;
+  }
+  return launch_status();
 }
 
 }  // namespace
@@ -168,8 +253,11 @@ extern "C" int b2d_verify_drafts(const int64_t* draft_tokens, int64_t ld_tokens,
                      uniforms, ld_u, tokens, ld_out, accepted, K, V};
   const bool pdl = (flags & B2D_LAUNCH_PDL) != 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const dim3 grid(static_cast<unsigned>(B)), block(kVerifyThreads);
-  if (probs_dtype == B2D_F32) return launch_kernel(verify_drafts_kernel<float>, grid, block, 0, s, pdl, a);
-  if (probs_dtype == B2D_F16) return launch_kernel(verify_drafts_kernel<__half>, grid, block, 0, s, pdl, a);
-  return launch_kernel(verify_drafts_kernel<__nv_bfloat16>, grid, block, 0, s, pdl, a);
+  // CTAs of a sequence: as many as fit the SMs at once (four each), with at least 1024 tokens
+  int ranks = 1;
+  while (ranks < kVerifyCluster && static_cast<int64_t>(B) * ranks * 2 <= 4 * di.sm_count && V / (ranks * 2) >= 1024) ranks *= 2;
+  if (static_cast<int64_t>(B) * ranks > (int64_t(1) << 31) - 1) return B2D_ERR_SHAPE;
+  if (probs_dtype == B2D_F32) return launch_verify<float>(a, B, ranks, pdl, s);
+  if (probs_dtype == B2D_F16) return launch_verify<__half>(a, B, ranks, pdl, s);
+  return launch_verify<__nv_bfloat16>(a, B, ranks, pdl, s);
 }
