@@ -4,17 +4,18 @@
 // mma.sync kernel of csrc/paged_attention.cu is bound by the same bytes); leaves (O, m, l) per row and split
 // of the keys, which that file's per-sequence kernel takes in.
 //
-// A CTA owns (256 rows as two tiles of 128, KV head, split). Per tile of 128 keys and row tile:
-//   S = Q K^T     tcgen05.mma kind::f16, M = N = 128, both operands K-major in shared memory, S in TMEM
-//   softmax       one warpgroup per row tile, one thread per row (tcgen05.ld brings the row's 128 scores into
+// A CTA owns (256 rows as two tiles of 128, KV head, split). Per 64 keys and row tile:
+//   S = Q K^T     tcgen05.mma kind::f16, M = 128, N = 64, both operands K-major in shared memory, S in TMEM
+//   softmax       one warpgroup per row tile, one thread per row (tcgen05.ld brings the row's 64 scores into
 //                 registers); P is rounded to the cache's dtype and overwrites S in TMEM
 //   O += P V      P from TMEM, V from shared memory (MN-major), O in TMEM
-// One elected thread issues all products; while it works for one row tile, the other tile's warpgroup is in
-// its softmax. With 128 rows or fewer both warpgroups take the same rows and alternate over the key tiles.
-// The running maximum moves only when a score exceeds it by 2^8 (weights up to 256 are as exact in fp32 and
-// in both 16-bit types), so O in TMEM is rarely rescaled. K and V come as 128-byte-swizzled tensor copies,
-// page by page, through a ring of four 128-key tiles.
-// TMEM columns: S/P of the two warpgroups at 0 and 128, their O at 256 and 256 + D.
+// Each warpgroup has two S buffers, so the product for the next 64 keys is under way while it works: with one
+// buffer of 128 keys the warpgroup waited as long as it worked (2.33 us per 128 keys and 256 rows). A warp per warpgroup issues its
+// products. With 128 rows or fewer both warpgroups take the same rows and alternate over the
+// key tiles. The running maximum moves only when a score exceeds it by 2^8 (weights up to 256 are as exact in
+// fp32 and in both 16-bit types), so O in TMEM is rarely rescaled. K and V come as 128-byte-swizzled tensor
+// copies, page by page, through a ring of four 128-key tiles.
+// TMEM columns: S/P buffers of the two warpgroups at 0, 64 and 128, 192, their O at 256 and 256 + D.
 #include <type_traits>
 
 #include "paged_attention.cuh"
@@ -23,10 +24,11 @@
 namespace b2d {
 namespace {
 
-constexpr int kTile = 128;                  // keys of a tile, rows of a row tile
+constexpr int kTile = 128;                  // keys of a copied tile, rows of a row tile
+constexpr int kSub = 64;                    // keys of a product
 constexpr int kSoftmax = 256;               // softmax threads (two warpgroups)
-constexpr int kProducer = 8, kIssuer = 9;   // warps
-constexpr int kPrefixThreads = 384;         // the third warpgroup: producer, issuer, two idle warps
+constexpr int kProducer = 8, kIssuer = 9;   // warps: one producer, an issuer per warpgroup
+constexpr int kPrefixThreads = 352;
 constexpr int kRing = 4;                    // K or V tiles in flight
 constexpr uint32_t kTmemCols = 512;
 constexpr float kLazy = 8.f;                // log2 of the largest weight before the maximum moves
@@ -37,6 +39,13 @@ __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar) : "memory");
+}
+// One lane of a converged warp. The issuing code runs warp-uniformly around it, so that descriptors and addresses
+// stay in uniform registers: from a single divergent lane a product took 90 cycles to issue.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n selp.u32 %0, 1, 0, e;\n}\n" : "=r"(p));
+  return p != 0;
 }
 // 32 TMEM columns of this thread's lane
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
@@ -83,18 +92,19 @@ __host__ __device__ constexpr uint32_t idesc() {
          ((std::is_same<T, __half>::value ? 0u : 1u) << 10) | ((B_MN ? 1u : 0u) << 16) |
          (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+// D (+)= A B; A from shared memory (ss) or TMEM (ts)
+template <bool ADD>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n}\n"
-      ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(accumulate), "r"(0u)
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+      ::"r"(d), "l"(a), "l"(b), "r"(id), "n"(ADD ? 1 : 0)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+template <bool ADD>
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n}\n"
-      ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(accumulate), "r"(0u)
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+      ::"r"(d), "r"(a), "l"(b), "r"(id), "n"(ADD ? 1 : 0)
       : "memory");
 }
 
@@ -107,32 +117,45 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kPrefixThreads, 1) paged_prefix_kernel(const __grid_constant__ PoolMaps maps,
                                                                          const __grid_constant__ PagedAttnArgs a) {
   constexpr uint32_t TILEB = kTile * D * 2, COLB = kTile * 128;   // a K, V or Q tile; its 64-element column
+  constexpr uint32_t SUBB = kSub * 128;                           // 64 keys of a column
   constexpr int HALVES = D / 64;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t s_bar[2 * kRing + 7];
+  __shared__ __align__(8) uint64_t s_bar[2 * kRing + 12];
   __shared__ uint32_t s_tmem;
+  __shared__ int64_t s_q[kSoftmax];   // per row: offset of its query, -1 past the end
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint8_t* const smem = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
   const uint32_t q_s = smem_u32(smem), ring = q_s + 2 * TILEB;
-  const uint32_t full = smem_u32(s_bar), empty = full + 8 * kRing, s_full = empty + 8 * kRing, p_full = s_full + 16,
-                 o_full = p_full + 16, q_full = o_full + 16;
+  // barriers: ring slots full / empty; scores ready and weights ready per warpgroup and buffer; products into O
+  const uint32_t full = smem_u32(s_bar), empty = full + 8 * kRing, s_full = empty + 8 * kRing, p_full = s_full + 32,
+                 o_full = p_full + 32, q_full = o_full + 16, done = q_full + 8;
 
   const int rows = a.B * a.rows;
   const bool pair = rows > kTile;          // two row tiles; else one, whose key tiles the warpgroups share
   const int kvh = blockIdx.y, split = blockIdx.x % a.splits, row0 = static_cast<int>(blockIdx.x) / a.splits * (2 * kTile);
   const int ktiles = (a.shared + kTile - 1) / kTile;
   const int t0 = ktiles * split / a.splits, n = ktiles * (split + 1) / a.splits - t0;   // this split's key tiles
+  const int subs = min(2 * n, a.shared / kSub - 2 * t0);                                // and steps of 64 keys
+  // steps of warpgroup w: tile of step u, and how many
+  auto tile_of = [&](int w, int u) { return pair ? u >> 1 : 2 * (u >> 1) + w; };
+  auto steps_of = [&](int w) {
+    if (pair) return subs;
+    const int tiles = (n + 1 - w) / 2;   // tiles w, w + 2, ...
+    return 2 * tiles - (tiles > 0 && 2 * tile_of(w, 2 * tiles - 1) + 1 >= subs ? 1 : 0);
+  };
   if (tid == 0) {
     for (int i = 0; i < kRing; ++i) {
       mbar_init(full + 8 * i, 1);
-      mbar_init(empty + 8 * i, 1);
+      mbar_init(empty + 8 * i, pair ? 2 : 1);   // the issuers that use a slot
     }
-    for (int w = 0; w < 2; ++w) {
-      mbar_init(s_full + 8 * w, 1);
-      mbar_init(p_full + 8 * w, kTile);
-      mbar_init(o_full + 8 * w, 1);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(s_full + 8 * i, 1);
+      mbar_init(p_full + 8 * i, kTile);
     }
+    mbar_init(o_full, 1);
+    mbar_init(o_full + 8, 1);
     mbar_init(q_full, kSoftmax);
+    mbar_init(done, 2);
     fence_mbar_init();
   }
   if (warp == kIssuer) {
@@ -149,12 +172,11 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) paged_prefix_kernel(const _
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = s_tmem;
+  // All of TMEM is this CTA's, so its base is column 0: a constant, which keeps the products' addresses in
+  // uniform registers (were it ever another, the rows would be NaN)
+  constexpr uint32_t tmem = 0;
 
-  // Registers: 168 a thread at launch (64,512 in all); the softmax takes 208 and the rest 80 (63,488).
-  if (warp >= kProducer) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;\n");
-  if (warp > kIssuer) {
-  } else if (warp == kProducer) {
+  if (warp == kProducer) {
     // ---- K and V tiles in the order in which the issuer uses them; a lane per (64-element column, box)
     const int bp = a.box_rows, boxes = kTile / bp, col = lane / boxes, box = lane - col * boxes;
     int unit = 0;
@@ -180,140 +202,138 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) paged_prefix_kernel(const _
         tma_load_4d(dst, is_v ? &maps.v : &maps.k, 64 * col, a.div.slot(tok, a.div.page(tok)), kvh, page, full + 8 * slot);
       ++unit;
     };
-    const int ahead = pair ? 1 : 2;   // score products that run ahead of the first P V
-    for (int i = 0; i < ahead && i < n; ++i) load(false, i);
+    // behind the first tile the copies wait for Q: ahead of its loads they would hold them up (8 us)
+    const int ahead = pair ? 1 : 2;   // tiles of scores that run ahead of the first P V
+    for (int i = 0; i < ahead && i < n; ++i) {
+      load(false, i);
+      if (i == 0) mbar_wait(q_full, 0);
+    }
     for (int i = 0; i < n; ++i) {
       load(true, i);
       if (i + ahead < n) load(false, i + ahead);
     }
-  } else if (warp == kIssuer) {
-    if (lane == 0 && n > 0) {
-      constexpr uint32_t ID_S = idesc<T, kTile, false>(), ID_O = idesc<T, D, true>();
-      int unit = 0, done[2] = {0, 0};   // ring position; tiles whose P V is issued, per warpgroup
-      auto take = [&]() -> uint32_t {
-        const uint32_t slot = unit % kRing;
-        mbar_wait(full + 8 * slot, (unit / kRing) & 1);
-        ++unit;
-        return slot;
-      };
-      auto scores = [&](int w, uint32_t slot) {   // S_w = Q K^T
-        const uint32_t qa = q_s + (pair ? w * TILEB : 0u), kb = ring + slot * TILEB;
+  } else if (warp >= kIssuer) {
+    // ---- the products of warpgroup w, in the order that its buffers need: P V of a step, then the scores of the
+    // step after the next, which overwrite that P (the tensor core takes a thread's products in order)
+    const int w = warp - kIssuer, steps = steps_of(w);
+    constexpr uint32_t ID_S = idesc<T, kSub, false>(), ID_O = idesc<T, D, true>();
+    const int ahead = pair ? 1 : 2;
+    // the producer's position of a K or V tile
+    auto unit_k = [&](int tile) { return tile < ahead ? tile : 2 * tile - ahead + 1; };
+    auto unit_v = [&](int tile) { return min(tile + ahead, n) + tile; };
+    auto ready = [&](int unit) {
+      mbar_wait(full + 8 * (unit % kRing), (unit / kRing) & 1);
+      return static_cast<uint32_t>(unit % kRing);
+    };
+    auto scores = [&](int u) {   // S_w[u & 1] = Q K^T for step u
+      const uint32_t slot = ready(unit_k(tile_of(w, u)));
+      const uint32_t qa = q_s + (pair ? w * TILEB : 0u), kb = ring + slot * TILEB + (u & 1) * SUBB;
+      if (elect_one()) {
+        const uint32_t d = tmem + 128 * w + 64 * (u & 1);
+        const uint64_t qd = desc_k_major(qa), kd = desc_k_major(kb);   // addresses count 16 bytes: + offset / 16
+        mma_ss<false>(d, qd, kd, ID_S);
 #pragma unroll
-        for (int j = 0; j < D / 16; ++j)
-          mma_ss(tmem + 128 * w, desc_k_major(qa + (j >> 2) * COLB + (j & 3) * 32),
-                 desc_k_major(kb + (j >> 2) * COLB + (j & 3) * 32), ID_S, j != 0);
-        mma_commit(s_full + 8 * w);
-      };
-      auto values = [&](int w, uint32_t slot, int tile) {   // O_w += P_w V
-        mbar_wait(p_full + 8 * w, done[w] & 1);
-        tc_fence_after();
-        const uint32_t vb = ring + slot * TILEB;
-        const int steps = min(kTile, a.shared - (t0 + tile) * kTile) / 16;
-        for (int j = 0; j < steps; ++j)
-          mma_ts(tmem + 256 + D * w, tmem + 128 * w + 8 * j, desc_mn_major(vb + 2048 * j, COLB), ID_O,
-                 done[w] != 0 || j != 0);
-        ++done[w];
-      };
+        for (int j = 1; j < D / 16; ++j) {
+          const uint32_t off = ((j >> 2) * COLB + (j & 3) * 32) >> 4;
+          mma_ss<true>(d, qd + off, kd + off, ID_S);
+        }
+        mma_commit(s_full + 16 * w + 8 * (u & 1));
+        if (u % 2 == 1 || u == steps - 1) mma_commit(empty + 8 * slot);   // the tile's last use
+      }
+      __syncwarp();
+    };
+    auto values = [&](int u) {   // O_w += P_w V for step u
+      const uint32_t slot = ready(unit_v(tile_of(w, u)));
+      mbar_wait(p_full + 16 * w + 8 * (u & 1), (u >> 1) & 1);
+      tc_fence_after();
+      const uint32_t vb = ring + slot * TILEB + (u & 1) * SUBB;
+      if (elect_one()) {
+        const uint32_t d = tmem + 256 + D * w, p = tmem + 128 * w + 64 * (u & 1);
+        const uint64_t vd = desc_mn_major(vb, COLB);
+        if (u == 0) mma_ts<false>(d, p, vd, ID_O);
+        else mma_ts<true>(d, p, vd, ID_O);
+#pragma unroll
+        for (int j = 1; j < kSub / 16; ++j) mma_ts<true>(d, p + 8 * j, vd + (2048 * j >> 4), ID_O);
+        mma_commit(o_full + 8 * w);
+        if (u % 2 == 1 || u == steps - 1) mma_commit(empty + 8 * slot);
+      }
+      __syncwarp();
+    };
+    if (n > 0) {
       mbar_wait(q_full, 0);
       tc_fence_after();
-      if (pair) {
-        uint32_t ks = take();
-        scores(0, ks);
-        scores(1, ks);
-        mma_commit(empty + 8 * ks);
-        for (int i = 0; i < n; ++i) {
-          const uint32_t vs = take();
-          const bool more = i + 1 < n;
-          values(0, vs, i);
-          if (more) {
-            ks = take();
-            scores(0, ks);
-          }
-          values(1, vs, i);
-          mma_commit(empty + 8 * vs);
-          if (more) {
-            scores(1, ks);
-            mma_commit(empty + 8 * ks);
-          }
-        }
-      } else {
-        for (int i = 0; i < 2 && i < n; ++i) {
-          const uint32_t ks = take();
-          scores(i, ks);
-          mma_commit(empty + 8 * ks);
-        }
-        for (int i = 0; i < n; ++i) {
-          const uint32_t vs = take();
-          values(i & 1, vs, i);
-          mma_commit(empty + 8 * vs);
-          if (i + 2 < n) {
-            const uint32_t ks = take();
-            scores(i & 1, ks);
-            mma_commit(empty + 8 * ks);
-          }
-        }
+      for (int u = 0; u < 2 && u < steps; ++u) scores(u);
+      for (int u = 0; u < steps; ++u) {
+        values(u);
+        if (u + 2 < steps) scores(u + 2);
       }
-      mma_commit(o_full);
-      mma_commit(o_full + 8);
+      if (elect_one()) mma_commit(done);
     }
     __syncwarp();
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;\n");
     // ---- softmax: warpgroup w, thread = row (TMEM lane)
     const int w = warp >> 2, r = tid & (kTile - 1);
-    const int row = row0 + (pair ? w * kTile : 0) + r;
-    const bool live = row < rows;
-    const int qb = row / a.rows, qr = row - qb * a.rows, t = qr / a.G, head = kvh * a.G + qr - t * a.G;
-    if (pair || w == 0) {
-      // this thread's row of Q into the K-major tile; a negative scale is moved into Q's sign
-      const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
-      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + qb * a.sq_b + t * a.sq_t +
-                                                        static_cast<int64_t>(head) * a.sq_h);
-      uint8_t* dst = smem + (pair ? w * TILEB : 0u) + r * 128;
-#pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        uint4 x = live ? src[c] : make_uint4(0, 0, 0, 0);
-        x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
-        *reinterpret_cast<uint4*>(dst + (c >> 3) * COLB + (((c & 7) ^ (r & 7)) << 4)) = x;
+    {
+      // Q into the K-major tiles, 16 bytes a copy
+      constexpr int CH = D / 8;
+      const int tile_rows = pair ? 2 * kTile : kTile;
+      {
+        const int row = row0 + tid, qb = row / a.rows, qr = row - qb * a.rows, t = qr * a.inv_g >> 16;
+        s_q[tid] = row < rows ? qb * a.sq_b + t * a.sq_t + static_cast<int64_t>(kvh * a.G + qr - t * a.G) * a.sq_h : -1;
       }
+      named_sync<1, kSoftmax>();
+#pragma unroll 1
+      for (int i = tid; i < tile_rows * CH; i += kSoftmax) {
+        const int qrow = i / CH, c = i % CH, tr = qrow & (kTile - 1);
+        const int64_t off = s_q[qrow];
+        cp_async16_zfill(q_s + (qrow >> 7) * TILEB + (c >> 3) * COLB + tr * 128 + (((c & 7) ^ (tr & 7)) << 4),
+                         static_cast<const T*>(a.q) + (off < 0 ? 0 : off + c * 8), off >= 0);
+      }
+      cp_async_commit();
+      cp_async_wait<0>();
       fence_proxy_async();
     }
     mbar_arrive(q_full);
-    const float scale = fabsf(a.scale_log2);
+    const float scale = a.scale_log2;
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
     const uint32_t st = tmem + lanes + 128 * w, ot = tmem + lanes + 256 + D * w;
-    const int mine = pair ? n : (n + 1 - w) / 2;   // key tiles of this warpgroup
+    const int steps = steps_of(w);
     float m_run = 0.f, l[4] = {0.f, 0.f, 0.f, 0.f};
-    bool landed = true;
-    for (int i = 0; i < mine; ++i) {
-      const int tile = pair ? i : 2 * i + w;
-      const int valid = min(kTile, a.shared - (t0 + tile) * kTile);
-      landed = mbar_wait(s_full + 8 * w, i & 1) && landed;
+    bool landed = s_tmem == tmem;
+    for (int u = 0; u < steps; ++u) {
+      const uint32_t sb = st + 64 * (u & 1);
+      landed = landed && mbar_wait(s_full + 16 * w + 8 * (u & 1), (u >> 1) & 1);
       __syncwarp();
       tc_fence_after();
-      uint32_t s[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(st + 32 * c, s[c]);
+      uint32_t s[2][32];
+      tmem_ld32(sb, s[0]);
+      tmem_ld32(sb + 32, s[1]);
       tmem_wait_ld();
-      if (valid < kTile) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (32 * c + j >= valid) s[c][j] = __float_as_uint(-INFINITY);
-      }
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
       for (int j = 0; j < 32; ++j)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) mx[c] = fmaxf(mx[c], __uint_as_float(s[c][j]));
+        for (int c = 0; c < 2; ++c) mx[2 * c + (j & 1)] = fmaxf(mx[2 * c + (j & 1)], __uint_as_float(s[c][j]));
+      if (scale < 0.f) {   // the largest product has the smallest score
+#pragma unroll
+        for (int c = 0; c < 4; ++c) mx[c] = INFINITY;
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) mx[2 * c + (j & 1)] = fminf(mx[2 * c + (j & 1)], __uint_as_float(s[c][j]));
+        mx[0] = fminf(fminf(mx[0], mx[1]), fminf(mx[2], mx[3]));
+        mx[1] = mx[2] = mx[3] = mx[0];
+      }
       const float m_new = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
-      if (i == 0) {
+      if (u == 0) {
         m_run = m_new == -INFINITY ? 0.f : m_new;
       } else if (__any_sync(0xffffffffu, m_new > m_run + kLazy)) {
-        // the products into O have completed: the commit behind S covers them
-        const float alpha = m_new > m_run + kLazy ? exp2_fast(m_run - m_new) : 1.f;
-        if (m_new > m_run + kLazy) m_run = m_new;
+        landed = landed && mbar_wait(o_full + 8 * w, (u - 1) & 1);   // the products into O so far
+        __syncwarp();
+        tc_fence_after();
+        const bool move = m_new > m_run + kLazy;
+        const float alpha = move ? exp2_fast(m_run - m_new) : 1.f;
+        if (move) m_run = m_new;
 #pragma unroll
         for (int c = 0; c < 4; ++c) l[c] *= alpha;
 #pragma unroll
@@ -327,7 +347,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) paged_prefix_kernel(const _
         }
       }
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {   // 32 scores -> 16 columns of P
+      for (int c = 0; c < 2; ++c) {   // 32 scores -> 16 columns of P
         uint32_t p[16];
 #pragma unroll
         for (int j = 0; j < 32; j += 2) {
@@ -337,37 +357,50 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) paged_prefix_kernel(const _
           l[(j & 2) + 1] += p1;
           p[j / 2] = Dt<T>::pack2(p0, p1);
         }
-        tmem_st16(st + 16 * c, p);
+        tmem_st16(sb + 16 * c, p);
       }
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(p_full + 8 * w);
+      mbar_arrive(p_full + 16 * w + 8 * (u & 1));
     }
-    if (mine > 0) {
-      landed = mbar_wait(o_full + 8 * w, 0) && landed;
-      __syncwarp();
-      tc_fence_after();
-    }
-    const int64_t all_rows = static_cast<int64_t>(a.B) * a.T * a.H;
-    const int64_t out = (static_cast<int64_t>(pair ? split : 2 * split + w)) * all_rows +
-                        (static_cast<int64_t>(qb) * a.T + t) * a.H + head;
+    // ---- the partials. Both warpgroups' products are done, so the ring is free: rows pass through it (16-byte
+    // chunk c of row r at c ^ r) and leave as whole lines
+    if (n > 0) landed = landed && mbar_wait(done, 0);
+    __syncwarp();
+    tc_fence_after();
+    const int64_t all = static_cast<int64_t>(a.B) * a.T * a.H;
+    const int row = row0 + (pair ? w * kTile : 0) + r;
+    const int qb = row / a.rows, qr = row - qb * a.rows, t = qr * a.inv_g >> 16;
+    const int64_t out = row >= rows ? -1 : static_cast<int64_t>(pair ? split : 2 * split + w) * all +
+                                              (static_cast<int64_t>(qb) * a.T + t) * a.H + kvh * a.G + qr - t * a.G;
     float sum = (l[0] + l[1]) + (l[2] + l[3]);
     if (!landed) sum = NAN;
-    if (live) *reinterpret_cast<float2*>(a.ml + out * 2) = make_float2(mine > 0 ? m_run : -INFINITY, sum);
-    if (mine > 0) {
+    if (out >= 0) *reinterpret_cast<float2*>(a.ml + out * 2) = make_float2(steps > 0 ? m_run : -INFINITY, sum);
+    constexpr int OC = D / 4;   // 16-byte chunks of a row
+    uint8_t* const stage = smem + 2 * TILEB + warp * (32 * D * 4);
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t x[32];
+    for (int c = 0; c < D / 32; ++c) {
+      uint32_t x[32];
+      if (steps > 0) {
         tmem_ld32(ot + 32 * c, x);
         tmem_wait_ld();
-        if (live) {
-          uint4* dst = reinterpret_cast<uint4*>(a.acc + out * D + 32 * c);
+      } else {   // an entry that never counts, but is multiplied by zero
 #pragma unroll
-          for (int j = 0; j < 8; ++j) dst[j] = make_uint4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
-        }
+        for (int j = 0; j < 32; ++j) x[j] = 0;
       }
-    } else if (live) {   // an entry that never counts, but is multiplied by zero
-      for (int c = 0; c < D / 4; ++c) reinterpret_cast<uint4*>(a.acc + out * D)[c] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        *reinterpret_cast<uint4*>(stage + lane * (D * 4) + (((8 * c + j) ^ (lane & (OC - 1))) << 4)) =
+            make_uint4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
+    }
+    __syncwarp();
+#pragma unroll 8
+    for (int i = 0; i < OC; ++i) {   // 32 chunks a step: 32 / OC rows
+      const int rr = i * (32 / OC) + lane / OC, c = lane % OC;
+      const int64_t to = __shfl_sync(0xffffffffu, out, rr);
+      if (to >= 0)
+        *reinterpret_cast<uint4*>(a.acc + to * D + 4 * c) =
+            *reinterpret_cast<const uint4*>(stage + rr * (D * 4) + ((c ^ (rr & (OC - 1))) << 4));
     }
   }
   tc_fence_before();

@@ -144,6 +144,35 @@ def test_attention_shared_prefix(B, T, H, KVH, prefix, ps, dtype):
     c.check(c.run(out_dtype=F32))
 
 
+@pytest.mark.parametrize("B,T,H,KVH,D,prefix,ps,extra", [
+    (12, 1, 6, 2, 128, 64, 16, 40),      # 36 rows: one step of 64 keys would do, the streaming kernel takes it
+    (12, 1, 6, 2, 128, 128, 8, 40), (12, 1, 6, 2, 128, 192, 64, 40), (30, 1, 8, 2, 64, 320, 32, 70),
+    (16, 2, 8, 2, 128, 2048, 16, 33),    # 128 rows, several splits, a table of small pages
+    (17, 2, 4, 1, 64, 1984, 16, 33),     # 136 rows: the second row tile almost empty
+    (16, 4, 12, 2, 128, 960, 192, 90),   # 384 rows: a second pair of row tiles; pages of three boxes
+    (65, 2, 4, 1, 128, 4160, 64, 20)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_attention_prefix_on_tensor_cores(B, T, H, KVH, D, prefix, ps, extra, dtype):
+    g = torch.Generator().manual_seed(B + prefix)
+    lens = (prefix + torch.randint(T, extra, (B,), generator=g)).tolist()
+    lens[2], lens[3] = 0, prefix // 2
+    c = Case(lens, H=H, KVH=KVH, T=T, D=D, prefix=prefix, ps=ps, dtype=dtype, seed=B)
+    c.check(c.run())
+    c.scale = -c.scale                   # a negative scale
+    c.check(c.run(scale=c.scale))
+
+
+def test_attention_prefix_rising_scores():
+    """Scores that grow along the prefix: the running maximum moves again and again."""
+    c = Case([1300 + i for i in range(20)], H=8, KVH=2, T=2, D=64, prefix=1280, ps=64, dtype=BF16, seed=50)
+    direction = torch.randn(64, generator=torch.Generator().manual_seed(1)).sign()
+    c.q = (c.q.float() * 0.2 + direction).bfloat16()
+    for i, page in enumerate(c.prefix_table.tolist()):
+        c.k[page] = (c.k[page].float() * 0.2 + direction * (0.3 * i)).bfloat16()
+    c.kd.copy_(c.k)
+    c.check(c.run())
+
+
 def test_attention_prefix_heads_of_64():
     c = Case([600 + 7 * i for i in range(24)], H=12, KVH=2, D=64, T=3, prefix=576, ps=32, dtype=BF16, seed=3)
     c.check(c.run())
