@@ -102,27 +102,32 @@ __device__ __forceinline__ Span span_of(const PagedAttnArgs& a, int len) {
   return s;
 }
 
-// The line of all units' stages: the prefix's units first (where the streaming kernel takes them), then the
-// sequences' in order, KV head by KV head and row tile by row tile. In whole mode a unit counts as one stage.
-// CTA c takes the positions [share(c), share(c + 1)); the host has checked that they fit 31 bits.
+// The line of all units' work: the prefix's units first (where the streaming kernel takes them), then the
+// sequences' in order, KV head by KV head and row tile by row tile. A unit takes `lead` positions, what its start
+// and end cost in stages, and one for each of its stages; one without keys takes none. CTA c takes the
+// positions [share(c), share(c + 1)); the host has checked that they fit 31 bits. In whole mode a unit is one
+// position.
 template <int D, int NT>
 struct Line {
   static constexpr int KEYS = stage_keys<D>(), ROWS = 8 * NT;
-  int tiles, units, tiles_p, stages_p, base, ctas, quota, extra;
+  // measured: a unit's start and end cost 1.3 us with one row tile and 4 us with more, a stage 1 us (1.6 with
+  // three row tiles)
+  static constexpr int LEAD = NT == 1 ? 2 : NT == 2 ? 4 : 3;
+  int tiles, units, tiles_p, cost_p, base, ctas, quota, extra;
   __device__ __forceinline__ Line(const PagedAttnArgs& a) {
     tiles = (a.rows + ROWS - 1) / ROWS;
     units = a.kv.KVH * tiles;
     const bool streams = a.shared > 0 && a.nparts == 0;
     tiles_p = streams ? (a.B * a.rows + ROWS - 1) / ROWS : 0;
-    stages_p = streams ? (a.shared + KEYS - 1) / KEYS : 0;
-    base = a.kv.KVH * tiles_p * stages_p;
+    cost_p = streams ? (a.shared + KEYS - 1) / KEYS + LEAD : 0;
+    base = a.kv.KVH * tiles_p * cost_p;
   }
-  static __device__ __forceinline__ int stages_of(const PagedAttnArgs& a, int len) {
+  static __device__ __forceinline__ int cost_of(const PagedAttnArgs& a, int len) {
     const Span s = span_of(a, len);
-    return a.whole ? 1 : (s.len - s.begin + KEYS - 1) / KEYS;
+    return a.whole ? 1 : s.len > s.begin ? (s.len - s.begin + KEYS - 1) / KEYS + LEAD : 0;
   }
-  __device__ __forceinline__ void close(const PagedAttnArgs& a, int stages) {   // of all sequences
-    const int total = base + stages * units;
+  __device__ __forceinline__ void close(const PagedAttnArgs& a, int cost) {   // of all sequences
+    const int total = base + cost * units;
     ctas = min(total, a.ctas);   // the CTAs with a share, none of them empty
     quota = ctas > 0 ? total / ctas : 0;
     extra = total - quota * ctas;   // so many CTAs take one position more
@@ -134,17 +139,17 @@ struct Line {
   }
 };
 
-// The sequences' lengths into s_len and the exclusive running sums of their stages into s_sum[0 .. B] (all
+// The sequences' lengths into s_len and the exclusive running sums of their units' cost into s_sum[0 .. B] (all
 // THREADS of the block take part).
 template <int D, int NT, int THREADS>
-__device__ __forceinline__ void scan_stages(const PagedAttnArgs& a, int* s_sum, int* s_len, int* s_warp) {
+__device__ __forceinline__ void scan_costs(const PagedAttnArgs& a, int* s_sum, int* s_len, int* s_warp) {
   constexpr int W = THREADS / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int run = 0;
   for (int b0 = 0; b0 < a.B; b0 += THREADS) {
     const int b = b0 + tid;
     const int len = b < a.B ? length_of(a, b) : 0;
-    const int own = b < a.B ? Line<D, NT>::stages_of(a, len) : 0;
+    const int own = b < a.B ? Line<D, NT>::cost_of(a, len) : 0;
     int v = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -173,20 +178,22 @@ __device__ __forceinline__ void scan_stages(const PagedAttnArgs& a, int* s_sum, 
 struct Segment {
   int b, kvh, row0, nrows;       // b < 0: the prefix
   int t_begin, t_end, limit;     // query t sees the keys before limit + t (the prefix: before t_end)
-  int kind;                      // 0: the final output, 1: a whole part, 2: a part of a unit shared with other CTAs
+  int kind;                      // 0: the final output, 1: a whole part, 2 / 3: the end (or middle) / the start of
+                                 // a unit shared with other CTAs, < 0: none
+  int next;                      // position behind it
 };
-// Segment at position pos of a share that ends at `end`; its number of positions in n.
+// The segment at position pos of a share that ends at `end`; none where only a unit's lead lies in the share.
 template <int D, int NT>
 __device__ __forceinline__ Segment segment_at(const PagedAttnArgs& a, const Line<D, NT>& line, const int* s_sum,
-                                              const int* s_len, int pos, int end, int& n) {
+                                              const int* s_len, int pos, int end) {
   constexpr int KEYS = stage_keys<D>(), ROWS = 8 * NT;
   Segment g;
-  int u, s0, stages, tile, first = 0, last;
+  int u, cost, tile, start, first = 0, last;   // start: the unit's first position
   bool shares = true;
   if (pos < line.base) {
-    stages = line.stages_p;
-    u = pos / stages;
-    s0 = pos - u * stages;
+    cost = line.cost_p;
+    u = pos / cost;
+    start = u * cost;
     g.b = -1;
     g.kvh = u / line.tiles_p;
     tile = u - g.kvh * line.tiles_p;
@@ -195,11 +202,9 @@ __device__ __forceinline__ Segment segment_at(const PagedAttnArgs& a, const Line
     g.nrows = min(a.B * a.rows - tile * ROWS, ROWS);
   } else {
     int lo = 0, hi = a.B - 1;   // the last sequence that starts at or before pos
-    pos -= line.base;
-    end -= line.base;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (s_sum[mid] * line.units <= pos) lo = mid;
+      if (line.base + s_sum[mid] * line.units <= pos) lo = mid;
       else hi = mid - 1;
     }
     g.b = lo;
@@ -208,19 +213,27 @@ __device__ __forceinline__ Segment segment_at(const PagedAttnArgs& a, const Line
     last = s.len;
     shares = s.shares;
     g.limit = s.len - a.T + 1;
-    stages = s_sum[lo + 1] - s_sum[lo];
-    const int rest = pos - s_sum[lo] * line.units;
-    u = rest / stages;
-    s0 = rest - u * stages;
+    cost = s_sum[lo + 1] - s_sum[lo];
+    start = line.base + s_sum[lo] * line.units;
+    u = (pos - start) / cost;
+    start += u * cost;
     g.kvh = line.tiles == 1 ? u : u / line.tiles;
     tile = u - g.kvh * line.tiles;
     g.nrows = min(a.rows - tile * ROWS, ROWS);
   }
-  n = min(end - pos, stages - s0);
   g.row0 = tile * ROWS;
-  g.t_begin = first + s0 * KEYS;
-  g.t_end = a.whole ? last : max(g.t_begin, min(last, g.t_begin + n * KEYS));
-  g.kind = n < stages ? 2 : shares ? 1 : 0;
+  g.next = min(end, start + cost);
+  if (a.whole) {
+    g.t_begin = first;
+    g.t_end = last;
+    g.kind = 0;
+  } else {
+    const int stages = cost - Line<D, NT>::LEAD, s0 = max(pos - start - Line<D, NT>::LEAD, 0);
+    const int s1 = g.next - start - Line<D, NT>::LEAD;
+    g.t_begin = first + s0 * KEYS;
+    g.t_end = min(last, first + s1 * KEYS);
+    g.kind = s1 <= s0 ? -1 : s0 > 0 ? 2 : s1 < stages ? 3 : shares ? 1 : 0;
+  }
   return g;
 }
 
@@ -273,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
   if (!a.after_prefix) pdl_wait();   // behind the prefix launch the inputs are complete
   pdl_launch_dependents();
   Line<D, NT> line(a);
-  scan_stages<D, NT, kThreads>(a, s_sum, s_len, s_warp);   // (its barriers also publish the mbarriers)
+  scan_costs<D, NT, kThreads>(a, s_sum, s_len, s_warp);   // (its barriers also publish the mbarriers)
   line.close(a, s_sum[a.B]);
   const int first = line.share(blockIdx.x), end = line.share(blockIdx.x + 1);
 
@@ -290,20 +303,24 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
       if (kv > 1 || tok >= g.t_end) return -1;
       return __ldg((g.b >= 0 && tok >= a.prefix_len ? a.table + g.b * a.ld_table : a.prefix_table) + a.div.page(tok));
     };
-    Segment ahead;         // the next segment, found while this one's copies are under way,
-    int ahead_n = 0, ahead_page = -1;   // and the pages of its first stage
-    if (first < end) {
-      ahead = segment_at(a, line, s_sum, s_len, first, end, ahead_n);
-      if (bp) ahead_page = lookup(ahead, 0);
-    }
-    for (int pos = first; pos < end && ok; ++seg) {
-      const Segment g = ahead;
-      int next = ahead_page;
-      pos += ahead_n;
-      if (pos < end) {
-        ahead = segment_at(a, line, s_sum, s_len, pos, end, ahead_n);
-        if (bp) ahead_page = lookup(ahead, 0);
+    // the next segment, found while this one's copies are under way, and the pages of its first stage
+    Segment ahead;
+    int ahead_page = -1;
+    auto find = [&](int pos) {
+      ahead.kind = -1;
+      while (pos < end) {
+        ahead = segment_at(a, line, s_sum, s_len, pos, end);
+        if (ahead.kind >= 0) break;
+        pos = ahead.next;
       }
+      if (bp && ahead.kind >= 0) ahead_page = lookup(ahead, 0);
+    };
+    find(first);
+    while (ahead.kind >= 0 && ok) {
+      Segment g = ahead;
+      int next = ahead_page;
+      find(g.next);
+      if (ahead.kind < 0) g.next = end;   // the consumers stop behind it
       const int t_begin = g.t_begin, t_end = g.t_end;
       const int32_t* table = g.b < 0 ? a.prefix_table : a.table + g.b * a.ld_table;
       const int split_at = g.b < 0 ? 0 : a.prefix_len;   // positions before it lie in prefix_table's pages
@@ -392,6 +409,14 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
           if (i == 0) send_q();
         }
       }
+      ++seg;
+    }
+    if (seg == 0) {   // nothing in this share
+      if (lane == 0) {
+        s_seg = ahead;
+        mbar_arrive(q_full);
+      }
+      mbar_arrive(q_full);
     }
     cp_async_wait<0>();
   } else {
@@ -404,9 +429,11 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
       // (the last unit's readers are done with s_at, s_m, s_o behind this barrier)
       landed = named_all<1, kConsumers>(landed && mbar_wait(q_full, seg & 1));
       Segment g = s_seg;
-      if (!landed) {   // a wait ran out: NaN for what is left
-        int n;
-        g = segment_at(a, line, s_sum, s_len, pos, end, n);
+      if (!landed) g = segment_at(a, line, s_sum, s_len, pos, end);   // a wait ran out: NaN for what is left
+      pos = g.next;
+      if (g.kind < 0) {
+        if (landed) break;
+        continue;
       }
       uint32_t qb[NT][KSTEPS][2];   // Q as the B operand: row 8 n + g8, elements 16 j + 2 tq ..
       auto load_q = [&](int n, int j) {   // two k-steps at a time
@@ -423,14 +450,12 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
         if (lane == 0) mbar_arrive(q_empty);
       }
       const int t_begin = g.t_begin, t_end = g.t_end, nst = (t_end - t_begin + KEYS - 1) / KEYS;
-      const bool opens = pos == first;   // the unit may have begun in an earlier CTA
-      pos += a.whole ? 1 : nst;
       if (tid < g.nrows) {
         const Row x = row_of(a, g.b, g.kvh, g.row0 + tid);
         const int64_t index = (static_cast<int64_t>(x.b) * a.T + x.t) * a.H + x.head;
         s_at[tid] = g.kind == 0   ? x.b * a.so_b + x.t * a.so_t + static_cast<int64_t>(x.head) * a.so_h
                     : g.kind == 1 ? (a.nparts + (g.b < 0 ? 1 : 0)) * all_rows(a) + index
-                                  : a.slot0 + (static_cast<int64_t>(blockIdx.x) * 2 + (opens ? 0 : 1)) * ROWS + tid;
+                                  : a.slot0 + (static_cast<int64_t>(blockIdx.x) * 2 + (g.kind - 2)) * ROWS + tid;
       }
       // keys that this thread's rows 8 n + 2 tq + e see; below lim_min no row is masked
       const bool causal = g.b >= 0 && a.T > 1;
@@ -683,12 +708,12 @@ __global__ void __launch_bounds__(128, 6) paged_combine_kernel(const __grid_cons
   pdl_launch_dependents();
   // the lengths are inputs of the whole call, complete before its first kernel began
   Line<D, NT> line(a);
-  scan_stages<D, NT, 128>(a, s_sum, s_len, s_warp);
+  scan_costs<D, NT, 128>(a, s_sum, s_len, s_warp);
   line.close(a, s_sum[a.B]);
   const int64_t R = all_rows(a);
   const int b = blockIdx.x / a.kv.KVH, kvh = blockIdx.x - b * a.kv.KVH;
   const Span sp = span_of(a, s_len[b]);
-  const int stages = s_sum[b + 1] - s_sum[b];
+  const int cost = s_sum[b + 1] - s_sum[b];
   bool waited = false;
   const int stop = min(a.rows, (static_cast<int>(blockIdx.y) + 1) * BLOCK_ROWS);
   for (int row0 = blockIdx.y * BLOCK_ROWS, n; row0 < stop; row0 += n) {
@@ -699,16 +724,16 @@ __global__ void __launch_bounds__(128, 6) paged_combine_kernel(const __grid_cons
     int ne = 0;
     bool written = false;   // by the streaming kernel
     // a unit's entries: one whole part, or a slot of every CTA that shares it
-    auto unit = [&](int p0, int count, int r, int block, bool direct) {
-      if (count == 0) return;
-      const int c0 = line.owner(p0), c1 = line.owner(p0 + count - 1);
+    auto unit = [&](int start, int cost, int r, int block, bool direct) {
+      if (cost == 0) return;
+      const int p0 = start + Line<D, NT>::LEAD, c0 = line.owner(p0), c1 = line.owner(start + cost - 1);
       if (c0 == c1) {
         if (direct) written = true;
         else if (tid == 0) s_entry[ne] = -1 - block;
         ne += !direct;
       } else {
         for (int c = c0 + tid; c <= c1; c += 128)
-          s_entry[ne + c - c0] = a.slot0 + (static_cast<int64_t>(c) * 2 + (line.share(c) < p0 ? 1 : 0)) * ROWS + r;
+          s_entry[ne + c - c0] = a.slot0 + (static_cast<int64_t>(c) * 2 + (line.share(c) <= p0 ? 1 : 0)) * ROWS + r;
         ne += c1 - c0 + 1;
       }
     };
@@ -717,10 +742,10 @@ __global__ void __launch_bounds__(128, 6) paged_combine_kernel(const __grid_cons
         if (tid < a.nparts) s_entry[tid] = -1 - tid;
         ne = a.nparts;
       } else {
-        unit((kvh * line.tiles_p + pr / ROWS) * line.stages_p, line.stages_p, pr % ROWS, a.nparts + 1, false);
+        unit((kvh * line.tiles_p + pr / ROWS) * line.cost_p, line.cost_p, pr % ROWS, a.nparts + 1, false);
       }
     }
-    unit(line.base + s_sum[b] * line.units + (kvh * line.tiles + row0 / ROWS) * stages, stages, row0 % ROWS, a.nparts,
+    unit(line.base + s_sum[b] * line.units + (kvh * line.tiles + row0 / ROWS) * cost, cost, row0 % ROWS, a.nparts,
          !sp.shares);
     if (!waited) pdl_wait();
     waited = true;
@@ -844,7 +869,7 @@ Plan make_plan(const b2d_paged_kv* kv, int B, int T, int H, int pages_per_seq, i
   const int64_t most = units * ((keys - p.shared + keys_per_stage - 1) / keys_per_stage) +
                        units_p * ((p.shared + keys_per_stage - 1) / keys_per_stage);
   const int64_t longest = reach > prefix_len ? reach : prefix_len;
-  p.fits = (units + units_p) * ((longest + keys_per_stage - 1) / keys_per_stage + 1) < (int64_t(1) << 31);
+  p.fits = (units + units_p) * ((longest + keys_per_stage - 1) / keys_per_stage + 4) < (int64_t(1) << 31);
   p.whole = keys <= keys_per_stage && p.shared == 0;
   int64_t ctas = p.whole ? units : most;
   if (ctas > 2 * sm) ctas = 2 * sm;
