@@ -385,7 +385,7 @@ typedef struct {
  * (row stride ld_cs) in the cache's dtype or F32 (cs_dtype). q_out may alias q. A token whose sequence is
  * outside [0, B) or whose position is outside [0, S_max) is padding: nothing of it is written; one whose
  * page is outside the table or the pool gets its q_out only. Two tokens of a call must not share a slot.
- * D % 16 == 0, D <= 256, H % KVH == 0; 16-byte aligned pointers (weights too), strides % 8 == 0.
+ * D % 16 == 0, D <= 256, H % KVH == 0, H < 65536; 16-byte aligned pointers (weights too), strides % 8 == 0.
  * flags: B2D_LAUNCH_PDL. */
 int b2d_paged_rope_append(const b2d_paged_kv* kv, const void* q, int64_t sq_n, int64_t sq_h,
                           const void* k, int64_t sk_n, int64_t sk_h, const void* v, int64_t sv_n, int64_t sv_h,
@@ -405,7 +405,8 @@ int b2d_paged_rope_append(const b2d_paged_kv* kv, const void* q, int64_t sq_n, i
  * multiplied once for the whole batch; page_table's entries for them are not read. prefix_len 0: none.
  * max_len: an upper bound of seqlens known to the host (0: the page table's reach); it only guides the
  * split over the SMs, longer sequences stay right.
- * D 64 or 128; H / KVH in 1..16; T in 1..16; 16-byte aligned q, strides % 8 == 0.
+ * D 64 or 128; H / KVH in 1..16; T in 1..16; 16-byte aligned q, strides % 8 == 0; the page table reaches less
+ * than 2^31 - 1024 positions.
  * workspace: b2d_paged_attention_workspace_bytes bytes for the same sizes (it may be 0), 16-byte aligned;
  * calls that may overlap need separate ones. No initial contents are needed. flags: B2D_LAUNCH_PDL. */
 size_t b2d_paged_attention_workspace_bytes(const b2d_paged_kv* kv, int B, int T, int H, int pages_per_seq,
@@ -429,7 +430,7 @@ int b2d_paged_attention(const b2d_paged_kv* kv, const void* q, int64_t sq_b, int
  *   tokens[b] = x_0 .. x_{a-1}, next, -1 ...  (int64 [B, K+1], row stride ld_out), accepted[b] = a (int32)
  * The tokens so drawn are distributed as the target's own. A negative or NaN weight counts as zero; a row
  * without any weight gives -1. Sums, products and comparisons are in 64 bits. probs_dtype F32, F16 or BF16
- * for both; V >= 1; 0 <= K <= 31; strides of the K dimension may be anything, V is contiguous.
+ * for both; 1 <= V <= 2^30; 0 <= K <= 31; strides of the K dimension may be anything, V is contiguous.
  * accepted may be NULL. flags: B2D_LAUNCH_PDL. */
 int b2d_verify_drafts(const int64_t* draft_tokens, int64_t ld_tokens, const int32_t* draft_lens,
                       const void* target_probs, int64_t st_b, int64_t st_k,

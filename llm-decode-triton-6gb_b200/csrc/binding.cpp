@@ -84,6 +84,10 @@ void check_shape(const at::Tensor& t, const char* name, at::IntArrayRef shape) {
     bad_value(s.str());
   }
 }
+int narrow(int64_t v, const char* name) {   // a size that the C ABI takes as an int
+  if (v > INT32_MAX) bad_value(std::string(name) + " is too large: " + std::to_string(v));
+  return static_cast<int>(v);
+}
 void check_last(const at::Tensor& t, const char* name) {
   if (t.numel() > 0 && t.size(-1) > 1 && t.stride(-1) != 1)
     bad_value(std::string("the last dimension of ") + name + " must be contiguous, got " + show(t));
@@ -192,10 +196,10 @@ PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t na) {
     const int st = g_append(kv, q.const_data_ptr(), q.stride(0), q.stride(1), k.const_data_ptr(), k.stride(0), k.stride(1),
                             v.const_data_ptr(), v.stride(0), v.stride(1), static_cast<const int64_t*>(positions.const_data_ptr()),
                             static_cast<const int32_t*>(ptr(seq)), static_cast<const int32_t*>(table.const_data_ptr()),
-                            table.stride(0), static_cast<int>(table.size(1)), static_cast<int>(B), cos.const_data_ptr(),
-                            sin.const_data_ptr(), cos.stride(0), static_cast<int>(cos.size(0)), code(cos.scalar_type()),
+                            table.stride(0), narrow(table.size(1), "page_table"), narrow(B, "page_table"), cos.const_data_ptr(),
+                            sin.const_data_ptr(), cos.stride(0), narrow(cos.size(0), "cos"), code(cos.scalar_type()),
                             ptr(qw), ptr(kw), static_cast<float>(number(a[12])), out.mutable_data_ptr(), out.stride(0),
-                            out.stride(1), static_cast<int>(N), static_cast<int>(H), integer32(a[13], "flags"), on.stream);
+                            out.stride(1), narrow(N, "q"), narrow(H, "q"), integer32(a[13], "flags"), on.stream);
     if (st != B2D_OK) return PyLong_FromLong(st);
     return a[8] == Py_None ? THPVariable_Wrap(made) : given(a[8]);
   });
@@ -249,10 +253,10 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t na) {
     check_cuda(dev);
     check_pool(dev, a[12]);
     const OnDevice on(dev);
-    const int per_seq = static_cast<int>(table.size(1));
+    const int per_seq = narrow(table.size(1), "page_table"), b = narrow(B, "q"), tn = narrow(T, "q"), h = narrow(H, "q");
     at::Tensor scratch;
     if (!ws) {
-      const size_t n = g_workspace(kv, static_cast<int>(B), static_cast<int>(T), static_cast<int>(H), per_seq, prefix_len, max_len);
+      const size_t n = g_workspace(kv, b, tn, h, per_seq, prefix_len, max_len);
       if (n > 0) scratch = at::empty({static_cast<int64_t>(n)}, q.options().dtype(at::kByte));
       ws = &scratch;
     }
@@ -261,7 +265,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t na) {
     const int st = g_attention(kv, q.const_data_ptr(), q.stride(0), q.stride(1), q.stride(2),
                                static_cast<const int32_t*>(table.const_data_ptr()), table.stride(0), per_seq,
                                static_cast<const int32_t*>(lens.const_data_ptr()), static_cast<const int32_t*>(ptr(prefix)),
-                               prefix_len, max_len, static_cast<int>(B), static_cast<int>(T), static_cast<int>(H),
+                               prefix_len, max_len, b, tn, h,
                                static_cast<float>(scale), out.mutable_data_ptr(), out.stride(0), out.stride(1), out.stride(2),
                                code(out.scalar_type()), has ? ws->mutable_data_ptr() : nullptr,
                                has ? static_cast<size_t>(ws->nbytes()) : 0, integer32(a[11], "flags"), on.stream);
@@ -279,8 +283,8 @@ PyObject* attention_workspace(PyObject*, PyObject* const* a, Py_ssize_t na) {
     check_table(table, "page_table", 2);
     check_cuda(q.device());
     const OnDevice on(q.device());
-    const size_t n = g_workspace(pool(a[0]), static_cast<int>(q.size(0)), static_cast<int>(q.size(1)), static_cast<int>(q.size(2)),
-                                 static_cast<int>(table.size(1)), integer32(a[3], "prefix_len"), integer32(a[4], "max_len"));
+    const size_t n = g_workspace(pool(a[0]), narrow(q.size(0), "q"), narrow(q.size(1), "q"), narrow(q.size(2), "q"),
+                                 narrow(table.size(1), "page_table"), integer32(a[3], "prefix_len"), integer32(a[4], "max_len"));
     return THPVariable_Wrap(at::empty({static_cast<int64_t>(n)}, q.options().dtype(at::kByte)));
   });
 }
@@ -330,7 +334,7 @@ PyObject* verify(PyObject*, PyObject* const* a, Py_ssize_t na) {
                             ptr(probs), probs ? probs->stride(0) : 0, probs ? probs->stride(1) : 0, code(dt),
                             static_cast<const float*>(u.const_data_ptr()), B > 1 ? u.stride(0) : K + 1,
                             static_cast<int64_t*>(tok.mutable_data_ptr()), B > 1 ? tok.stride(0) : K + 1,
-                            static_cast<int32_t*>(acc.mutable_data_ptr()), static_cast<int>(B), static_cast<int>(K),
+                            static_cast<int32_t*>(acc.mutable_data_ptr()), narrow(B, "draft_tokens"), static_cast<int>(K),
                             static_cast<int>(V), integer32(a[7], "flags"), on.stream);
     if (st != B2D_OK) return PyLong_FromLong(st);
     PyObject* t = a[5] == Py_None ? THPVariable_Wrap(made_t) : given(a[5]);

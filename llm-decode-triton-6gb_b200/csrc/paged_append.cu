@@ -268,7 +268,7 @@ extern "C" int b2d_paged_rope_append(const b2d_paged_kv* kv, const void* q, int6
   if ((st = check_paged_kv(kv)) != B2D_OK) return st;
   if (N < 0 || H < 0 || B < 0 || S_max < 0 || pages_per_seq < 0) return B2D_ERR_ARG;
   if (cs_dtype != kv->dtype && cs_dtype != B2D_F32) return B2D_ERR_DTYPE;
-  if (kv->D % 16 != 0 || kv->D < 16 || kv->D > 256 || H % kv->KVH != 0) return B2D_ERR_SHAPE;
+  if (kv->D % 16 != 0 || kv->D < 16 || kv->D > 256 || H % kv->KVH != 0 || H > 65535) return B2D_ERR_SHAPE;
   if (N == 0) return B2D_OK;
   if (B == 0 || (!seq_ids && N % B != 0) || ld_table < 0 || ld_cs < 0) return B2D_ERR_SHAPE;
   if (!q || !k || !v || !positions || !page_table || !cos || !sin || !q_out) return B2D_ERR_ARG;

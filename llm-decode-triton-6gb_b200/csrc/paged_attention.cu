@@ -932,7 +932,9 @@ int check_shapes(const b2d_paged_kv* kv, int B, int T, int H, int pages_per_seq,
   if (st != B2D_OK) return st;
   if (B < 0 || T < 0 || H < 0 || pages_per_seq < 0 || prefix_len < 0 || max_len < 0) return B2D_ERR_ARG;
   if ((kv->D != 64 && kv->D != 128) || H % kv->KVH != 0 || H / kv->KVH > kMaxG || T > kMaxT) return B2D_ERR_SHAPE;
-  if (static_cast<int64_t>(pages_per_seq) * kv->page_size >= (int64_t(1) << 31) || kv->KVH > 65535) return B2D_ERR_SHAPE;
+  // positions and their sums with a stage's keys fit 31 bits
+  constexpr int64_t most = (int64_t(1) << 31) - 1024;
+  if (static_cast<int64_t>(pages_per_seq) * kv->page_size > most || prefix_len > most || kv->KVH > 65535) return B2D_ERR_SHAPE;
   return B2D_OK;
 }
 
@@ -946,7 +948,10 @@ extern "C" size_t b2d_paged_attention_workspace_bytes(const b2d_paged_kv* kv, in
   if (check_shapes(kv, B, T, H, pages_per_seq, prefix_len, max_len) != B2D_OK || B == 0 || T == 0 || H == 0) return 0;
   DeviceInfo di;
   if (device_info(&di) != B2D_OK) return 0;
-  return make_plan(kv, B < kMaxBatch ? B : kMaxBatch, T, H, pages_per_seq, prefix_len, max_len, di.sm_count).bytes;
+  // the launches of a large batch: full ones and a rest
+  const size_t full = B >= kMaxBatch ? make_plan(kv, kMaxBatch, T, H, pages_per_seq, prefix_len, max_len, di.sm_count).bytes : 0;
+  const size_t rest = B % kMaxBatch ? make_plan(kv, B % kMaxBatch, T, H, pages_per_seq, prefix_len, max_len, di.sm_count).bytes : 0;
+  return full > rest ? full : rest;
 }
 
 extern "C" int b2d_paged_attention(const b2d_paged_kv* kv, const void* q, int64_t sq_b, int64_t sq_t, int64_t sq_h,

@@ -258,7 +258,7 @@ extern "C" int b2d_verify_drafts(const int64_t* draft_tokens, int64_t ld_tokens,
                                  void* stream) {
   if (B < 0 || K < 0 || V < 0) return B2D_ERR_ARG;
   if (probs_dtype != B2D_F32 && probs_dtype != B2D_F16 && probs_dtype != B2D_BF16) return B2D_ERR_DTYPE;
-  if (K > kMaxDrafts || V == 0 || ld_tokens < 0 || ld_u < 0 || ld_out < K + 1) return B2D_ERR_SHAPE;
+  if (K > kMaxDrafts || V == 0 || V > (1 << 30) || ld_tokens < 0 || ld_u < 0 || ld_out < K + 1) return B2D_ERR_SHAPE;
   if (B == 0) return B2D_OK;
   if ((!draft_tokens && K > 0) || !target_probs || !uniforms || !tokens) return B2D_ERR_ARG;
   const int size = probs_dtype == B2D_F32 ? 4 : 2;

@@ -145,7 +145,7 @@ def test_c_attention_checks():
     assert call(q=None) == ARG and call(lens=None) == ARG and call(out=None) == ARG and call(table=None) == ARG
     assert call(pl=4) == ARG and call(pl=-1) == ARG and call(B=-1) == ARG
     assert call(q=P + 2) == ALIGN and call(sq=(256, 256, 60)) == ALIGN
-    assert call(d=desc(page_size=1024), per=1 << 21) == SHAPE
+    assert call(d=desc(page_size=1024), per=1 << 21) == SHAPE and call(pl=2 ** 31 - 1, pt=P) == SHAPE
 
 
 def test_c_append_checks():
@@ -156,7 +156,7 @@ def test_c_append_checks():
                                          32, cdt, qw, None, 1e-6, P, 256, 64, N, H, 0, None)
     assert call(N=0) == OK
     assert call(d=desc(D=40)) == SHAPE and call(d=desc(D=272)) == SHAPE and call(H=5) == SHAPE
-    assert call(B=0) == SHAPE and call(N=3, B=2) == SHAPE
+    assert call(B=0) == SHAPE and call(N=3, B=2) == SHAPE and call(H=65536) == SHAPE
     assert call(cdt=1) == DTYPE and call(N=-1) == ARG and call(q=None) == ARG and call(pos=None) == ARG
     assert call(ksn=124) == ALIGN and call(ldcs=60) == ALIGN and call(qw=P + 4) == ALIGN and call(cs=P + 8) == ALIGN
 
@@ -167,7 +167,7 @@ def test_c_verify_checks():
     def call(draft=P, tp=P, dt=2, u=P, out=P, ldo=5, B=1, K=4, V=10):
         return lib.b2d_verify_drafts(draft, 4, None, tp, 50, 10, None, 0, 0, dt, u, 5, out, ldo, None, B, K, V, 0, None)
     assert call(B=0) == OK
-    assert call(K=32, ldo=33) == SHAPE and call(V=0) == SHAPE and call(ldo=4) == SHAPE and call(dt=5) == DTYPE
+    assert call(K=32, ldo=33) == SHAPE and call(V=0) == SHAPE and call(V=2 ** 30 + 1) == SHAPE and call(ldo=4) == SHAPE and call(dt=5) == DTYPE
     assert call(draft=None) == ARG and call(tp=None) == ARG and call(u=None) == ARG and call(out=None) == ARG
     assert call(B=-1) == ARG and call(draft=P + 4) == ALIGN and call(tp=P + 2) == ALIGN
 

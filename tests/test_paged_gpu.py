@@ -341,6 +341,46 @@ def test_attention_two_graphs_replayed_at_once():
     cs[0].check(outs[0])
 
 
+@pytest.mark.parametrize("B,T,prefix", [(300, 1, 0), (300, 1, 128), (261, 3, 192), (257, 1, 64)])
+def test_attention_large_batches(B, T, prefix):
+    """More sequences than one launch takes."""
+    g = torch.Generator().manual_seed(B)
+    lens = (prefix + torch.randint(0, 70, (B,), generator=g)).tolist()
+    c = Case(lens, H=4, KVH=2, D=64, T=T, prefix=prefix, seed=B, dtype=BF16)
+    c.check(c.run())
+
+
+def test_attention_programmatic_launches():
+    """The calls as programmatic dependents of one another, in a captured chain, give the same bits."""
+    for prefix, T in ((0, 1), (512, 3)):
+        c = Case([600 + 31 * i for i in range(12)], H=8, KVH=2, T=T, prefix=prefix, seed=60)
+        q, table, lens = c.q.to(DEV), c.table.to(DEV), c.lens.to(DEV)
+        kw = dict(prefix_table=c.prefix_table.to(DEV), prefix_len=prefix) if prefix else {}
+        N = 12 * T
+        pos = (c.lens[:, None] - T + torch.arange(T)).reshape(-1).long().to(DEV)
+        g = torch.Generator().manual_seed(6)
+        k, v = (torch.randn(N, 2, 128, generator=g).half().to(DEV) for _ in range(2))
+        cos, sin = (torch.rand(1024, 128, generator=g).to(DEV) for _ in range(2))
+
+        def chain(flags):
+            qr = paged_rope_append(c.cache, q.view(N, 8, 128), k, v, pos, table, cos, sin, flags=flags)
+            out = paged_attention(c.cache, qr.view(12, T, 8, 128), table, lens, flags=flags, **kw)
+            probs = torch.softmax(out.float().view(12, T, -1), -1).contiguous()
+            return out, verify_drafts(torch.zeros(12, T - 1, dtype=torch.int64, device=DEV), probs,
+                                      torch.full((12, T), 0.3, device=DEV), flags=flags)
+
+        want = chain(0)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = [chain(_lib.LAUNCH_PDL) for _ in range(3)]
+        for _ in range(5):
+            graph.replay()
+        torch.cuda.synchronize()
+        for out, (tok, acc) in got:
+            assert torch.equal(out, want[0]) and torch.equal(tok, want[1][0]) and torch.equal(acc, want[1][1])
+
+
 def test_attention_caller_workspace():
     c = Case([900 + i for i in range(20)], T=2, prefix=512, seed=30)
     ws = paged_attention_workspace(c.cache, c.q.to(DEV), c.table.to(DEV), prefix_len=512)
