@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
       if (kv > 1 || tok >= g.t_end) return -1;
       return __ldg((g.b >= 0 && tok >= a.prefix_len ? a.table + g.b * a.ld_table : a.prefix_table) + a.div.page(tok));
     };
-    // the next segment, found while this one's copies are under way, and the pages of its first stage
+    // the next segment, found while this one's first copies are under way, and the pages of its first stage
     Segment ahead;
     int ahead_page = -1;
     auto find = [&](int pos) {
@@ -316,11 +316,11 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
       if (bp && ahead.kind >= 0) ahead_page = lookup(ahead, 0);
     };
     find(first);
+    int behind = first;   // position behind the last segment
     while (ahead.kind >= 0 && ok) {
-      Segment g = ahead;
+      const Segment g = ahead;
       int next = ahead_page;
-      find(g.next);
-      if (ahead.kind < 0) g.next = end;   // the consumers stop behind it
+      behind = g.next;
       const int t_begin = g.t_begin, t_end = g.t_end;
       const int32_t* table = g.b < 0 ? a.prefix_table : a.table + g.b * a.ld_table;
       const int split_at = g.b < 0 ? 0 : a.prefix_len;   // positions before it lie in prefix_table's pages
@@ -329,7 +329,10 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
       // past the end are zeros. Lane l owns the address of row l.
       auto send_q = [&]() {
         if (seg > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait(q_empty, (seg - 1) & 1));
-        if (!ok) return;
+        if (!ok) {
+          ahead.kind = -1;
+          return;
+        }
         int64_t off = -1;
         if (lane < g.nrows) {
           const Row x = row_of(a, g.b, g.kvh, g.row0 + lane);
@@ -344,11 +347,12 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
           for (int col = 0; col < HALVES; ++col)
             cp_async16_zfill(q_s + col * (ROWS * 128) + r * 128 + ((c ^ (r & 7)) << 4), src + (o < 0 ? 0 : 64 * col), o >= 0);
         }
-      if (lane == 0) {
-        s_seg = g;
-        mbar_arrive(q_full);
-      }
-      mbar_arrive_cp_async(q_full);
+        if (lane == 0) {
+          s_seg = g;
+          mbar_arrive(q_full);
+        }
+        mbar_arrive_cp_async(q_full);
+        find(g.next);
       };
       if (nst == 0) send_q();
       if (a.box_rows) {
@@ -411,8 +415,11 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
       }
       ++seg;
     }
-    if (seg == 0) {   // nothing in this share
+    if (ok && behind < end) {   // only a unit's lead is left: the consumers stop
+      if (seg > 0) __all_sync(0xffffffffu, mbar_wait(q_empty, (seg - 1) & 1));
       if (lane == 0) {
+        ahead.kind = -1;
+        ahead.next = end;
         s_seg = ahead;
         mbar_arrive(q_full);
       }

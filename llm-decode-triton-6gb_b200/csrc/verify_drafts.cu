@@ -13,6 +13,8 @@
 //     through distributed shared memory;
 //  3. a warp of each CTA scans them; the CTA that holds the target sums the piece again in 256 chunks (from
 //     L2), scans those, and the thread that holds the target walks its chunk.
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace b2d {
@@ -36,25 +38,41 @@ struct VerifyArgs {
 
 template <typename P> __device__ __forceinline__ double to_f64(P v) { return static_cast<double>(Dt<P>::to_f32(v)); }
 template <> __device__ __forceinline__ double to_f64<float>(float v) { return static_cast<double>(v); }
-// The same for the long sums: the conversion instruction has a small share of the SM's rate and bounded the
-// kernel (46 us for 128 rows of 131071, 1.4x the rest), so normal numbers move their exponent and mantissa
-// into place with integer instructions; zeros become zero, and the rest (rare) is converted.
-template <typename P> __device__ __forceinline__ double widen(P x) {
-  const float v = Dt<P>::to_f32(x);
-  const uint32_t u = __float_as_uint(v), m = u + u;   // without the sign
-  double d = __hiloint2double(static_cast<int>((u & 0x80000000u) | ((m >> 4) + 0x38000000u)), static_cast<int>(u << 29));
-  if (m - 0x01000000u >= 0xFE000000u) d = m == 0 ? 0.0 : static_cast<double>(v);
-  return d;
+// The weights of a row are summed times 2^30: exact, and no fp32 value is subnormal then, so that a positive one
+// widens by moving its exponent and mantissa into place -- the conversion instruction has a small share of the
+// SM's rate and bounded the kernel. (An infinity counts as 2^128.)
+constexpr float kWeightScale = 1073741824.f;
+__device__ __forceinline__ double widen(float x) {   // x > 0 and normal
+  const uint32_t u = __float_as_uint(x);
+  return __hiloint2double(static_cast<int>((u >> 3) + 0x38000000u), static_cast<int>(u << 29));
 }
-
-// The weight of token v: p (q null and x < 0), max(p - q, 0), or p with the drafted token x left out.
-// NaN and negative weights count as zero.
+// 2^30 (p - q) for a negative q (no probability; out of line, so that its conversions stay off the usual path)
+__device__ __noinline__ double weight_of_negative(float p, float q) {
+  return (static_cast<double>(p) - static_cast<double>(q)) * static_cast<double>(kWeightScale);
+}
+// sum += 2^30 max(p - q, 0); NaN counts as zero. HAS_Q false: q is zero.
+template <bool HAS_Q>
+__device__ __forceinline__ void add_weight(float p, float q, double& sum) {
+  if constexpr (HAS_Q) {
+    if (p > q) {
+      if (q >= 0.f) {
+        const double wide = widen(q * kWeightScale);
+        sum += widen(p * kWeightScale) - (q == 0.f ? 0.0 : wide);
+      } else {
+        sum += weight_of_negative(p, q);
+      }
+    }
+  } else {
+    if (p > 0.f) sum += widen(p * kWeightScale);
+  }
+}
+// The same weight for token v of a row: max(p - q, 0), or p with the drafted token x left out (q null).
 template <typename P>
 __device__ __forceinline__ double weight(const P* p, const P* q, int64_t x, int v) {
-  double w = to_f64<P>(p[v]);
-  if (q) w -= to_f64<P>(q[v]);
-  else if (v == x) w = 0.0;
-  return w > 0.0 ? w : 0.0;
+  double w = 0.0;
+  if (q) add_weight<true>(Dt<P>::to_f32(p[v]), Dt<P>::to_f32(q[v]), w);
+  else if (v != x) add_weight<false>(Dt<P>::to_f32(p[v]), 0.f, w);
+  return w;
 }
 
 __device__ __forceinline__ double warp_sum(double v) {
@@ -112,29 +130,34 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_drafts_kernel(const 
   const int v0 = min(a.V, (rank * kVerifyWarps + warp) * piece), v1 = min(a.V, v0 + piece);
   for (int pass = 0;; ++pass) {
     double sum = 0.0;
-    P pv[2][8], qv[2][8];   // 8 steps of 32 values are added while the next 8 are under way
-    auto load = [&](int set, int base) {
+    auto add_piece = [&](auto has_q) {
+      constexpr bool HAS_Q = decltype(has_q)::value;
+      P pv[2][8], qv[2][8];   // 8 steps of 32 values are added while the next 8 are under way
+      auto load = [&](int set, int base) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int v = base + 32 * i;
-        pv[set][i] = v < v1 ? p[v] : P(0.f);
-        qv[set][i] = v < v1 && q ? q[v] : P(0.f);
+        for (int i = 0; i < 8; ++i) {
+          const int v = base + 32 * i;
+          pv[set][i] = v < v1 ? p[v] : P(0.f);
+          if constexpr (HAS_Q) qv[set][i] = v < v1 ? q[v] : P(0.f);
+        }
+      };
+      auto add = [&](int set, int base) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if constexpr (HAS_Q) add_weight<true>(Dt<P>::to_f32(pv[set][i]), Dt<P>::to_f32(qv[set][i]), sum);
+          else add_weight<false>(base + 32 * i == x ? 0.f : Dt<P>::to_f32(pv[set][i]), 0.f, sum);
+        }
+      };
+      load(0, v0 + lane);
+      for (int base = v0 + lane; base - lane < v1; base += 512) {
+        load(1, base + 256);
+        add(0, base);
+        load(0, base + 512);
+        add(1, base + 256);
       }
     };
-    auto add = [&](int set, int base) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const double w = base + 32 * i == x ? 0.0 : widen<P>(pv[set][i]) - widen<P>(qv[set][i]);
-        if (w > 0.0) sum += w;
-      }
-    };
-    load(0, v0 + lane);
-    for (int base = v0 + lane; base - lane < v1; base += 512) {
-      load(1, base + 256);
-      add(0, base);
-      load(0, base + 512);
-      add(1, base + 256);
-    }
+    if (q) add_piece(std::true_type{});
+    else add_piece(std::false_type{});
     sum = warp_sum(sum);
     if (lane == 0) s_sum[warp] = sum;
     if (ranks > 1) cluster_sync();

@@ -558,6 +558,22 @@ def test_verify_invalid_ids_and_weights():
     run_verify(ids, target, u, draft)
 
 
+def test_verify_tiny_and_negative_weights():
+    """Subnormal probabilities keep their values, zeros on either side too, and a negative draft probability
+    counts as it stands."""
+    g = torch.Generator().manual_seed(8)
+    V = 3000
+    target, draft = torch.rand(4, 2, V, generator=g), torch.rand(4, 1, V, generator=g)
+    target[0] *= 1e-39                   # subnormal throughout, and the draft larger: drawn from the target
+    target[1, :, ::2], draft[1, :, 1::3] = 0.0, 0.0
+    target[2], draft[2] = target[2] * 2e-38, draft[2] * 1e-38   # around the smallest normal number
+    draft[3, :, ::5] *= -1
+    ids = torch.full((4, 1), 7, dtype=torch.int64)
+    for u in (0.0, 0.37, 0.999):
+        run_verify(ids, target, torch.tensor([[1.0, u]] * 4), draft)
+        run_verify(ids, target, torch.tensor([[1.0, u]] * 4))
+
+
 def test_verify_strides_and_buffers():
     ids, target, u, draft = verify_case(3, 4, 257, seed=7)
     wide = torch.zeros(5, 3, 300)                  # [K+1, B, V'] with a longer row
