@@ -652,6 +652,24 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
           }
         }
       landed = named_all<1, kConsumers>(landed);
+      if (tid < g.nrows) {   // (m, l) of a row, and the warps' factors in the place of their maxima
+        float mx = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, s_m[w][tid]);
+        float f[kWarps];
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          f[w] = s_m[w][tid] == -INFINITY ? 0.f : exp2_fast(s_m[w][tid] - mx);
+          l += f[w] * s_l[w][tid];
+        }
+        if (!landed) l = NAN;
+        // a row that sees no key: zeros (l is NaN, not 0, where a visible score is)
+        const float inv = g.kind == 0 ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+        if (g.kind != 0) *reinterpret_cast<float2*>(a.ml + s_at[tid] * 2) = make_float2(mx, l);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) s_m[w][tid] = f[w] * inv;
+      }
+      named_sync<1, kConsumers>();
       constexpr int PAD = D + 4;   // the rows 2 tq of the accumulators' columns fall into different banks
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -659,17 +677,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
         if (n > 0) named_sync<1, kConsumers>();
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int row = 8 * n + 2 * tq + e;
-          float mx = -INFINITY, l = 0.f;
-#pragma unroll
-          for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, s_m[w][row]);
-#pragma unroll
-          for (int w = 0; w < kWarps; ++w) l += (s_m[w][row] == -INFINITY ? 0.f : exp2_fast(s_m[w][row] - mx)) * s_l[w][row];
-          if (!landed) l = NAN;
-          float factor = m_run[n][e] == -INFINITY ? 1.f : exp2_fast(m_run[n][e] - mx);
-          // a row that sees no key: zeros (l is NaN, not 0, where a visible score is)
-          if (g.kind == 0) factor *= l == 0.f ? 0.f : 1.f / l;
-          else if (g8 == 0 && warp == 0 && row < g.nrows) *reinterpret_cast<float2*>(a.ml + s_at[row] * 2) = make_float2(mx, l);
+          const float factor = s_m[warp][8 * n + 2 * tq + e];
           float* dst = s_o + (warp * 8 + 2 * tq + e) * PAD + g8;
 #pragma unroll
           for (int m = 0; m < DT; ++m) {
@@ -878,7 +886,7 @@ Plan make_plan(const b2d_paged_kv* kv, int B, int T, int H, int pages_per_seq, i
   const int64_t longest = reach > prefix_len ? reach : prefix_len;
   p.fits = (units + units_p) * ((longest + keys_per_stage - 1) / keys_per_stage + 4) < (int64_t(1) << 31);
   p.whole = keys <= keys_per_stage && p.shared == 0;
-  int64_t ctas = p.whole ? units : most;
+  int64_t ctas = p.whole ? units : most + 4 * (units + units_p);
   if (ctas > 2 * sm) ctas = 2 * sm;
   if (ctas > kMaxCtas) ctas = kMaxCtas;
   p.ctas = static_cast<int>(ctas < 1 ? 1 : ctas);
