@@ -712,23 +712,32 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
 // Merges rows' entries: a block of 128 threads for 512 / D rows of a (sequence, KV head), four elements a thread.
 // A thread reads its row's (m, l) along with the sums and keeps a running maximum, so that one round trip to
 // memory follows the streaming kernel's end; the rest is done while that kernel still runs (its shared memory
-// is sized to leave room for these blocks).
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(128, 6) paged_combine_kernel(const __grid_constant__ PagedAttnArgs a) {
+// is sized to leave room for these blocks). GROUPS > 1: so many groups of 128 threads share the entries of a
+// unit that many CTAs have cut.
+template <typename T, int D, int NT, int GROUPS>
+__global__ void __launch_bounds__(128 * GROUPS, GROUPS == 1 ? 6 : 1) paged_combine_kernel(const __grid_constant__ PagedAttnArgs a) {
   constexpr int ROWS = 8 * NT, QUADS = D / 4, BLOCK_ROWS = 128 / QUADS;
   constexpr int MOST = kMaxParts + kMaxCtas + 2;   // a prefix unit's and an own unit's CTAs have at most one in common
-  __shared__ int s_sum[kMaxBatch + 1], s_len[kMaxBatch], s_warp[4];
+  __shared__ int s_sum[kMaxBatch + 1], s_len[kMaxBatch], s_warp[4 * GROUPS];
+  __shared__ float4 s_v[GROUPS > 1 ? 128 * GROUPS : 1];   // the groups' sums and (m, l)
+  __shared__ float2 s_ml[GROUPS > 1 ? 128 * GROUPS : 1];
   __shared__ int64_t s_entry[MOST];   // entry of the first row, or -1 - (its block of R rows in the output's order)
   const int tid = threadIdx.x;
   pdl_launch_dependents();
   // the lengths are inputs of the whole call, complete before its first kernel began
   Line<D, NT> line(a);
-  scan_costs<D, NT, 128>(a, s_sum, s_len, s_warp);
+  scan_costs<D, NT, 128 * GROUPS>(a, s_sum, s_len, s_warp);
   line.close(a, s_sum[a.B]);
   const int64_t R = all_rows(a);
   const int b = blockIdx.x / a.kv.KVH, kvh = blockIdx.x - b * a.kv.KVH;
   const Span sp = span_of(a, s_len[b]);
   const int cost = s_sum[b + 1] - s_sum[b];
+  auto put = [&](int b, int t, int head, int d, const float4& v, float l) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;   // a row that sees no key: zeros
+    const int64_t at = b * a.so_b + t * a.so_t + static_cast<int64_t>(head) * a.so_h + d;
+    store_out2<T>(a, at, v.x * inv, v.y * inv);
+    store_out2<T>(a, at + 2, v.z * inv, v.w * inv);
+  };
   bool waited = false;
   const int stop = min(a.rows, (static_cast<int>(blockIdx.y) + 1) * BLOCK_ROWS);
   for (int row0 = blockIdx.y * BLOCK_ROWS, n; row0 < stop; row0 += n) {
@@ -747,7 +756,7 @@ __global__ void __launch_bounds__(128, 6) paged_combine_kernel(const __grid_cons
         else if (tid == 0) s_entry[ne] = -1 - block;
         ne += !direct;
       } else {
-        for (int c = c0 + tid; c <= c1; c += 128)
+        for (int c = c0 + tid; c <= c1; c += 128 * GROUPS)
           s_entry[ne + c - c0] = a.slot0 + (static_cast<int64_t>(c) * 2 + (line.share(c) <= p0 ? 1 : 0)) * ROWS + r;
         ne += c1 - c0 + 1;
       }
@@ -766,13 +775,13 @@ __global__ void __launch_bounds__(128, 6) paged_combine_kernel(const __grid_cons
     waited = true;
     if (written) continue;
     __syncthreads();
-    const int r = tid / QUADS, d = (tid - r * QUADS) * 4;
+    const int group = tid / 128, r = tid % 128 / QUADS, d = (tid % 128 - r * QUADS) * 4;
     if (r < n) {
       const int t = div_g(a, row0 + r), head = kvh * a.G + row0 + r - t * a.G;
       const int64_t index = (static_cast<int64_t>(b) * a.T + t) * a.H + head;
       float m = -INFINITY, l = 0.f;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int e = 0; e < ne; e += 8) {   // eight entries in flight
+      for (int e = 8 * group; e < ne; e += 8 * GROUPS) {   // eight entries in flight
         float4 x[8];
         float2 ml[8];
 #pragma unroll
@@ -800,10 +809,31 @@ __global__ void __launch_bounds__(128, 6) paged_combine_kernel(const __grid_cons
           v.z = fmaf(f, x[k].z, v.z); v.w = fmaf(f, x[k].w, v.w);
         }
       }
-      const float inv = l == 0.f ? 0.f : 1.f / l;   // a row that sees no key: zeros
-      const int64_t at = b * a.so_b + t * a.so_t + static_cast<int64_t>(head) * a.so_h + d;
-      store_out2<T>(a, at, v.x * inv, v.y * inv);
-      store_out2<T>(a, at + 2, v.z * inv, v.w * inv);
+      if constexpr (GROUPS > 1) {
+        s_v[tid] = v;
+        s_ml[tid] = make_float2(m, l);
+      }
+      if constexpr (GROUPS == 1) put(b, t, head, d, v, l);
+    }
+    if constexpr (GROUPS > 1) {
+      __syncthreads();
+      if (group == 0 && r < n) {
+        const int t = div_g(a, row0 + r), head = kvh * a.G + row0 + r - t * a.G;
+        float mx = -INFINITY, l = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < GROUPS; ++k) mx = fmaxf(mx, s_ml[tid + 128 * k].x);
+#pragma unroll
+        for (int k = 0; k < GROUPS; ++k) {
+          const float2 ml = s_ml[tid + 128 * k];
+          const float4 x = s_v[tid + 128 * k];
+          const float f = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - mx);
+          l = fmaf(f, ml.y, l);
+          v.x = fmaf(f, x.x, v.x); v.y = fmaf(f, x.y, v.y);
+          v.z = fmaf(f, x.z, v.z); v.w = fmaf(f, x.w, v.w);
+        }
+        put(b, t, head, d, v, l);
+      }
     }
     __syncthreads();   // the next rows reuse the table
   }
@@ -848,11 +878,15 @@ int box_rows(const b2d_paged_kv& kv, int prefix_len) {
   return prefix_len % rows == 0 ? rows : 0;
 }
 
-int row_tiles(int64_t rows) { return rows < 32 ? static_cast<int>((rows + 7) / 8) : 4; }   // of 8, in a unit
+// Row tiles of 8 in a unit, at most 4: as few units as possible, of equal size (40 rows: two of 24)
+int row_tiles(int64_t rows) {
+  const int64_t units = (rows + 31) / 32, per = (rows + units - 1) / units;
+  return static_cast<int>((per + 7) / 8);
+}
 
 // How a call is cut.
 struct Plan {
-  int shared, tc5, splits, nparts, nt, ctas, whole, combine, fits;
+  int shared, tc5, splits, nparts, nt, ctas, whole, combine, many, fits;
   int64_t slot0, entries;
   size_t bytes;
 };
@@ -891,6 +925,8 @@ Plan make_plan(const b2d_paged_kv* kv, int B, int T, int H, int pages_per_seq, i
   if (ctas > kMaxCtas) ctas = kMaxCtas;
   p.ctas = static_cast<int>(ctas < 1 ? 1 : ctas);
   p.combine = !p.whole;
+  // a unit's parts: with fewer units than CTAs they are many (75 of them: 7 us in one group of threads)
+  p.many = p.ctas > 16 * (units_p > 0 ? units_p : units);
   if (p.combine) {
     const int64_t R = static_cast<int64_t>(B) * T * H;
     p.slot0 = (p.nparts + (p.shared > 0 ? 2 : 0)) * R;
@@ -901,7 +937,7 @@ Plan make_plan(const b2d_paged_kv* kv, int B, int T, int H, int pages_per_seq, i
 }
 
 template <typename T, int D, int NT>
-int launch_stream(const PoolMaps& maps, const PagedAttnArgs& a, bool combine, bool pdl, cudaStream_t s) {
+int launch_stream(const PoolMaps& maps, const PagedAttnArgs& a, bool combine, bool many, bool pdl, cudaStream_t s) {
   auto kern = paged_stream_kernel<T, D, NT>;
   constexpr uint32_t bytes = smem_bytes<D, NT>();
   static bool configured[64] = {};   // per device; setting it twice is harmless
@@ -917,8 +953,9 @@ int launch_stream(const PoolMaps& maps, const PagedAttnArgs& a, bool combine, bo
   }
   int st = launch_kernel(kern, dim3(a.ctas), dim3(kThreads), bytes, s, pdl || a.after_prefix, maps, a);
   if (st != B2D_OK || !combine) return st;
-  return launch_kernel(paged_combine_kernel<T, D, NT>, dim3(a.B * a.kv.KVH, (a.rows + 512 / D - 1) / (512 / D)),
-                       dim3(128), 0, s, true, a);
+  const dim3 grid(a.B * a.kv.KVH, (a.rows + 512 / D - 1) / (512 / D));
+  if (many) return launch_kernel(paged_combine_kernel<T, D, NT, 4>, grid, dim3(512), 0, s, true, a);
+  return launch_kernel(paged_combine_kernel<T, D, NT, 1>, grid, dim3(128), 0, s, true, a);
 }
 
 template <typename T, int D>
@@ -935,10 +972,10 @@ int run(PagedAttnArgs& a, const Plan& p, bool pdl, cudaStream_t s) {
     a.shared = 0;
   }
   switch (p.nt) {
-    case 1: return launch_stream<T, D, 1>(maps, a, p.combine, pdl, s);
-    case 2: return launch_stream<T, D, 2>(maps, a, p.combine, pdl, s);
-    case 3: return launch_stream<T, D, 3>(maps, a, p.combine, pdl, s);
-    default: return launch_stream<T, D, 4>(maps, a, p.combine, pdl, s);
+    case 1: return launch_stream<T, D, 1>(maps, a, p.combine, p.many, pdl, s);
+    case 2: return launch_stream<T, D, 2>(maps, a, p.combine, p.many, pdl, s);
+    case 3: return launch_stream<T, D, 3>(maps, a, p.combine, p.many, pdl, s);
+    default: return launch_stream<T, D, 4>(maps, a, p.combine, p.many, pdl, s);
   }
 }
 
