@@ -3,6 +3,8 @@
     from b200kernels.nf4_gemm import NF4Weight            # fused NF4 dequant + skinny matmul
     from b200kernels.decode_attention import decode_attention   # split-K GQA flash-decoding
     from b200kernels.patch import patch_attention, patch_linear4bit, STATS
+    from b200kernels.paged import PagedKV, paged_rope_append, paged_attention   # paged cache, shared prefix
+    from b200kernels.speculative import verify_drafts           # speculative sampling
 
 Every op runs in ``libb200decode.so`` (C ABI in ``include/b200decode.h``) through ctypes.
 """

@@ -10,8 +10,11 @@
 // heads are always under way: every thread copies its own chunks through two private stages of shared memory
 // (16-byte cp.async), so no thread waits for another. The products w * cos and w * sin are formed once per
 // thread and token and serve all of its heads.
-// Bound by bytes, 2 (H + 2 KVH) D elements a token; one thread per head was bound by instruction issue (80 % of
-// the slots) and by the latency of position -> page -> store at a low occupancy.
+// Measured on B200: 8168 tokens of 32 + 8 + 8 heads of 128 with norms, bf16: 45.0 us, 4.5 TB/s of read and written
+// bytes (copy rate 6.52); 320 tokens 4.9 us; one token 2.4 us (launch and latency). Bound by bytes in the limit,
+// 2 (H + 2 KVH) D elements a token. What is left at 8168 tokens is latency: 16.7 warps per SM are active (shared
+// memory allows 9 blocks) and issue in half of the slots. One head per thread took 49 us, three stages 51, four-element
+// halves 58 to 63 with 80 % of the slots issuing.
 #include "paged.cuh"
 
 namespace b2d {
@@ -124,7 +127,7 @@ __device__ __forceinline__ Pair turn_pair(const Pair& p, const Turn& t, bool nor
 
 // T: cache and activation dtype, C: rotary table type, GROUP: threads of a head (a power of two >= D/16),
 // HEADS: query heads of a thread that are staged (0: a block has one token, whose first heads are loaded straight
-// into registers: 1.8 against 2.5 us for a single token). The groups of a token's blocks (blockIdx.y) take the query
+// into registers: 2.4 against 3.3 us for a single token). The groups of a token's blocks (blockIdx.y) take the query
 // heads in turn; the first groups also the keys, the last ones the values. Heads past the staged ones are
 // loaded when their turn comes.
 template <typename T, typename C, int GROUP, int HEADS>
@@ -238,8 +241,8 @@ int launch_group(const PagedAppendArgs& a, int sm, bool pdl, cudaStream_t s) {
   constexpr int GROUPS = kAppendThreads / GROUP;
   int parts = (a.H + GROUPS - 1) / GROUPS;
   if (parts < 1) parts = 1;
-  // few tokens: a token's heads over several blocks, one query head a thread (320 tokens of 32 heads: 3.8 us
-  // against 5.1 staged; 8168 tokens: 50 us against 45)
+  // few tokens: a token's heads over several blocks, one query head a thread (one token 2.4 us against 3.3 staged, 320 tokens
+  // of 32 heads 4.85 against 5.05; 8168 tokens staged 45, direct 50)
   if (static_cast<int64_t>(a.N) * parts <= 24 * sm) return launch_kernel_of<T, C, GROUP, 0>(a, dim3(a.N, parts), pdl, s);
   if (parts == 1) return launch_kernel_of<T, C, GROUP, 1>(a, dim3(a.N < 16 * sm ? a.N : 16 * sm), pdl, s);
   if (parts == 2) return launch_kernel_of<T, C, GROUP, 2>(a, dim3(a.N < 12 * sm ? a.N : 12 * sm), pdl, s);

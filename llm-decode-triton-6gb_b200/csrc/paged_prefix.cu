@@ -10,11 +10,17 @@
 //                 registers); P is rounded to the cache's dtype and overwrites S in TMEM
 //   O += P V      P from TMEM, V from shared memory (MN-major), O in TMEM
 // Each warpgroup has two S buffers, so the product for the next 64 keys is under way while it works: with one
-// buffer of 128 keys the warpgroup waited as long as it worked (2.33 us per 128 keys and 256 rows). A warp per warpgroup issues its
-// products. With 128 rows or fewer both warpgroups take the same rows and alternate over the
+// buffer of 128 keys the warpgroup waited as long as it worked (2.33 us per 128 keys and 256 rows, by time stamps).
+// A warp per warpgroup issues its products. With 128 rows or fewer both warpgroups take the same rows and alternate over the
 // key tiles. The running maximum moves only when a score exceeds it by 2^8 (weights up to 256 are as exact in
 // fp32 and in both 16-bit types), so O in TMEM is rarely rescaled. K and V come as 128-byte-swizzled tensor
 // copies, page by page, through a ring of four 128-key tiles.
+// Measured on B200 (32 sequences x 4 drafts, 32 / 8 heads of 128, 16384 shared keys, bf16; 34.4 GFLOP): the call
+// takes 65 us by graph replay; with cold caches this kernel is 43.9 us of it, the sequences' own keys 28.3, the
+// combine 14.7. One product of 64 keys and 256 rows after another took about 1.1 us with time stamps in the
+// kernel, which lengthen it; their shared-memory reads alone are estimated at 0.7 and the exponentials at 0.55.
+// The call took 168 us with mma.sync, 83 with the first tcgen05 form. Merging the splits through distributed
+// shared memory before the write: 67.8 against 64.8, not kept.
 // TMEM columns: S/P buffers of the two warpgroups at 0, 64 and 128, 192, their O at 256 and 256 + D.
 #include <type_traits>
 

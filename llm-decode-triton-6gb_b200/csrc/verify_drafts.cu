@@ -13,6 +13,10 @@
 //     through distributed shared memory;
 //  3. a warp of each CTA scans them; the CTA that holds the target sums the piece again in 256 chunks (from
 //     L2), scans those, and the thread that holds the target walks its chunk.
+// Measured on B200 (fp32 probabilities; copy rate 6.52 TB/s): 128 sequences x 131071 tokens 34 us (3.9 TB/s of the
+// rows that are read; 25 warps per SM issue in 48 % of the slots: latency and the phases that wait for one
+// another), 64 x 32768 without draft probabilities 6.8 us, one x 32000 5.4 us (launch and dependent reads).
+// One CTA per sequence took 93, 16.0 and 12.6; clusters with widening by conversions in part 43, 9.4 and 5.7.
 #include <type_traits>
 
 #include "common.cuh"
