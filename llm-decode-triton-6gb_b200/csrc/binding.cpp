@@ -92,6 +92,11 @@ void check_last(const at::Tensor& t, const char* name) {
   if (t.numel() > 0 && t.size(-1) > 1 && t.stride(-1) != 1)
     bad_value(std::string("the last dimension of ") + name + " must be contiguous, got " + show(t));
 }
+// An output whose rows are one memory (an expanded tensor) would be written by several blocks at once.
+void check_output(const at::Tensor& t, const char* name) {
+  for (int64_t d = 0; d < t.dim(); ++d)
+    if (t.size(d) > 1 && t.stride(d) == 0 && t.numel() > 0) bad_value(std::string(name) + " overlaps itself: " + show(t));
+}
 void check_device(const at::Tensor* t, const char* name, const at::Device& d) {
   if (t && t->device() != d) {
     std::ostringstream s;
@@ -189,6 +194,7 @@ PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t na) {
     const at::Tensor& out = a[8] == Py_None ? made : tensor(a[8], "q_out");
     if (out.sizes() != q.sizes() || out.scalar_type() != dt) bad_value("q_out has q's shape and dtype, got " + show(out));
     check_last(out, "q_out");
+    check_output(out, "q_out");
     check_device(&out, "q_out", dev);
     check_cuda(dev);
     check_pool(dev, a[14]);
@@ -246,6 +252,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t na) {
       bad_value("out has q's shape and is fp32 or of the cache's dtype (and of out_dtype), got " + show(out));
     check_last(q, "q");
     check_last(out, "out");
+    check_output(out, "out");
     check_device(&table, "page_table", dev); check_device(&lens, "seqlens", dev); check_device(&out, "out", dev);
     check_device(prefix, "prefix_table", dev);
     const at::Tensor* ws = optional(a[10], "workspace");
@@ -325,6 +332,7 @@ PyObject* verify(PyObject*, PyObject* const* a, Py_ssize_t na) {
     check_last(draft, "draft_tokens");
     check_last(u, "uniforms");
     check_last(tok, "tokens");
+    check_output(tok, "tokens");
     check_device(&draft, "draft_tokens", dev); check_device(probs, "draft_probs", dev); check_device(&u, "uniforms", dev);
     check_device(lens, "draft_lens", dev); check_device(&tok, "tokens", dev); check_device(&acc, "accepted", dev);
     check_cuda(dev);

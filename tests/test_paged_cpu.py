@@ -121,6 +121,16 @@ def desc(**kw):
     return C.byref(_lib.PagedKvDesc(**f))
 
 
+def test_outputs_that_overlap_themselves_are_refused():
+    with pytest.raises(ValueError, match="overlaps itself"):
+        paged_rope_append(pool(), **{**append_args(), "q_out": torch.zeros(1, 4, 64).half().expand(2, 4, 64)})
+    with pytest.raises(ValueError, match="overlaps itself"):
+        paged_attention(pool(), **{**attn_args(), "out": torch.zeros(1, 1, 4, 64).half().expand(2, 1, 4, 64)})
+    with pytest.raises(ValueError, match="overlaps itself"):
+        verify_drafts(torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 4, 10), torch.zeros(2, 4),
+                      tokens=torch.zeros(1, 4, dtype=torch.int64).expand(2, 4))
+
+
 @pytest.mark.parametrize("kw,status", [
     (dict(dtype=2), DTYPE), (dict(page_size=0), SHAPE), (dict(page_size=1025), SHAPE), (dict(KVH=0), SHAPE),
     (dict(k=P + 2), ALIGN), (dict(sv_s=60), ALIGN), (dict(k=None), ARG), (dict(num_pages=-1), ARG), (dict(D=-8), ARG),
