@@ -399,7 +399,7 @@ int b2d_paged_rope_append(const b2d_paged_kv* kv, const void* q, int64_t sq_n, i
  * drafted tokens verified at once). q [B, T, H, D] (strides sq_b, sq_t, sq_h), out likewise in out_dtype
  * (the cache's dtype or F32). seqlens[b] (int32) counts the cached keys of sequence b, its T new tokens
  * included: query t sees the keys before position seqlens[b] - T + 1 + t, and a query that sees none (an
- * empty sequence) gives zeros. seqlens beyond the page table are cut to it.
+ * empty sequence) gives zeros. seqlens beyond the page table are cut to it, or to prefix_len where that is longer.
  * prefix_table / prefix_len: the positions [0, prefix_len) of EVERY sequence are those of the pages
  * prefix_table[0 .. ceil(prefix_len / page_size)) (int32, device) -- a shared system prompt, read and
  * multiplied once for the whole batch; page_table's entries for them are not read. prefix_len 0: none.

@@ -94,15 +94,14 @@ __device__ __forceinline__ void store_out2(const PagedAttnArgs& a, int64_t off, 
   }
 }
 
-// The keys that sequence b computes itself: [begin, len), cut to the page table's reach.
+// The keys that sequence b computes itself: [begin, len), cut to what the page table and the prefix reach.
 struct Span {
   int len, begin;
   bool shares;      // takes the shared prefix's part in
 };
 __device__ __forceinline__ int length_of(const PagedAttnArgs& a, int b) {
   const int64_t reach = static_cast<int64_t>(a.pages_per_seq) * a.kv.page_size;
-  const int len = max(a.seqlens[b], 0);
-  return len > reach ? max(static_cast<int>(reach), a.prefix_len) : len;
+  return min(max(a.seqlens[b], 0), max(static_cast<int>(reach), a.prefix_len));
 }
 __device__ __forceinline__ Span span_of(const PagedAttnArgs& a, int len) {
   Span s;

@@ -223,6 +223,26 @@ def test_attention_lengths_beyond_the_table_and_bad_pages():
     c.check(c.run())
 
 
+@pytest.mark.parametrize("B,T,H,KVH,D,prefix,ps", [
+    (1, 1, 8, 2, 64, 64, 16),            # one sequence: nothing is shared
+    (5, 1, 8, 2, 128, 64, 16), (5, 3, 4, 2, 64, 200, 16), (5, 2, 8, 2, 128, 130, 5),     # prefix units, copies by cp.async last
+    (20, 1, 8, 2, 128, 256, 16), (20, 3, 8, 2, 64, 448, 64), (5, 16, 8, 1, 128, 192, 32)])   # on the tensor cores
+@pytest.mark.parametrize("width", [0, 1, 3])
+def test_attention_page_table_narrower_than_the_prefix(B, T, H, KVH, D, prefix, ps, width):
+    """A table whose entries end inside the prefix (they are not read there): lengths are cut to the prefix's end,
+    never lengthened to it."""
+    reach = max(width * ps, prefix)
+    lens = [min(width * ps + 4, prefix - 1), prefix - 1, prefix, prefix + T + 40, 0, T, prefix // 2, 2 ** 31 - 1]
+    lens = [20] if B == 1 else (lens + [prefix - 1 - i for i in range(B)])[:B]
+    c = Case([min(n, reach) for n in lens], H=H, KVH=KVH, D=D, T=T, ps=ps, prefix=prefix, dtype=BF16, seed=B + width)
+    cut, c.table = c.lens, c.table[:, :width].contiguous()
+    for kw in ({}, {"max_len": prefix}):
+        c.lens = torch.tensor(lens, dtype=torch.int32)
+        out = c.run(**kw)
+        c.lens = cut
+        c.check(out)
+
+
 @pytest.mark.parametrize("H,KVH,T,D,lens", [(8, 2, 4, 128, [130, 64, 7]), (16, 2, 4, 128, [193, 66, 4]),
                                             (16, 1, 4, 64, [129, 260, 5]), (4, 1, 3, 64, [128, 2, 300]),
                                             (16, 1, 16, 128, [70, 16, 5])])
