@@ -22,6 +22,7 @@
 // The call took 168 us with mma.sync, 83 with the first tcgen05 form. Merging the splits through distributed
 // shared memory before the write: 67.8 against 64.8, not kept.
 // TMEM columns: S/P buffers of the two warpgroups at 0, 64 and 128, 192, their O at 256 and 256 + D.
+#include <cfloat>
 #include <type_traits>
 
 #include "paged_attention.cuh"
@@ -332,7 +333,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) paged_prefix_kernel(const _
       }
       const float m_new = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
       if (u == 0) {
-        m_run = m_new == -INFINITY ? 0.f : m_new;
+        m_run = fmaxf(m_new, -FLT_MAX);   // -infinity everywhere: the first other score moves it (inf - inf is none)
       } else if (__any_sync(0xffffffffu, m_new > m_run + kLazy)) {
         landed = landed && mbar_wait(o_full + 8 * w, (u - 1) & 1);   // the products into O so far
         __syncwarp();

@@ -173,6 +173,26 @@ def test_attention_prefix_rising_scores():
     c.check(c.run())
 
 
+@pytest.mark.parametrize("hidden", [[0, 1, 2, 3, 8, 9, 10, 11], list(range(8)), list(range(16))])
+@pytest.mark.parametrize("scale", [1.0, -1.0])
+def test_attention_prefix_keys_without_weight_first(hidden, scale):
+    """Pages of the prefix whose scores are all -infinity -- the first step of each warpgroup, a warpgroup's whole
+    part, a split's -- ahead of keys with scores far below zero: as if they were not there."""
+    c = Case([530 + 3 * i for i in range(12)], H=8, KVH=2, D=128, prefix=512, ps=16, dtype=BF16, seed=70)
+    c.scale *= scale
+    c.q = c.q.abs()
+    c.k.copy_((0.2 * c.k.float() - 20 * scale).to(BF16))      # scores of about -180
+    gone = c.prefix_table[hidden].long()
+    c.k[gone, :, :, 0] = -float("inf") * scale
+    c.kd.copy_(c.k)
+    out = c.run(scale=c.scale)
+    n = 16 * len(hidden)
+    keep = [i for i in range(32) if i not in hidden]
+    c.prefix_table, c.prefix, c.lens, c.table = c.prefix_table[keep], 512 - n, c.lens - n, c.table[:, len(hidden):]
+    c.check(out)
+    assert (out != 0).any(-1).all()
+
+
 def test_attention_prefix_heads_of_64():
     c = Case([600 + 7 * i for i in range(24)], H=12, KVH=2, D=64, T=3, prefix=576, ps=32, dtype=BF16, seed=3)
     c.check(c.run())
