@@ -84,7 +84,7 @@ def paged_attention(kv: PagedKV, q: torch.Tensor, page_table: torch.Tensor, seql
     position ``seqlens[b] - T + 1 + t``; one that sees none gives zeros. ``prefix_table`` int32 [pages] and
     ``prefix_len``: the first ``prefix_len`` positions of every sequence lie in these pages (the entries of
     ``page_table`` for them are not read) and are computed once for the batch. ``max_len``: an upper bound of
-    ``seqlens`` known to the host, which only guides the split. ``workspace``: uint8 scratch of
+    ``seqlens`` known to the host, which only guides the split. ``workspace``: contiguous scratch of
     ``paged_attention_workspace`` bytes, 16-byte aligned, not shared by calls that may overlap; without it
     one is allocated per call."""
     r = _lib.binding().attention(kv._desc, q, page_table, seqlens, scale, prefix_table, prefix_len, max_len, out, out_dtype,

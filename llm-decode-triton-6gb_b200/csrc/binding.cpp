@@ -256,6 +256,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t na) {
     check_device(&table, "page_table", dev); check_device(&lens, "seqlens", dev); check_device(&out, "out", dev);
     check_device(prefix, "prefix_table", dev);
     const at::Tensor* ws = optional(a[10], "workspace");
+    if (ws && !ws->is_contiguous()) bad_value("workspace is contiguous, got " + show(*ws));   // its bytes are counted below
     check_device(ws, "workspace", dev);
     check_cuda(dev);
     check_pool(dev, a[12]);

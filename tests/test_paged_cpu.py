@@ -131,6 +131,14 @@ def test_outputs_that_overlap_themselves_are_refused():
                       tokens=torch.zeros(1, 4, dtype=torch.int64).expand(2, 4))
 
 
+def test_workspace_without_its_own_memory_is_refused():
+    """A workspace whose elements are one memory (expanded) or lie apart has fewer bytes than its size says."""
+    for ws in (torch.zeros(1, dtype=torch.uint8).expand(1 << 20), torch.zeros(1 << 21, dtype=torch.uint8)[::2],
+               torch.zeros(1, 64, dtype=torch.uint8).expand(1 << 14, 64)):
+        with pytest.raises(ValueError, match="workspace"):
+            paged_attention(pool(), **attn_args(), workspace=ws)
+
+
 @pytest.mark.parametrize("kw,status", [
     (dict(dtype=2), DTYPE), (dict(page_size=0), SHAPE), (dict(page_size=1025), SHAPE), (dict(KVH=0), SHAPE),
     (dict(k=P + 2), ALIGN), (dict(sv_s=60), ALIGN), (dict(k=None), ARG), (dict(num_pages=-1), ARG), (dict(D=-8), ARG),
