@@ -382,9 +382,10 @@ typedef struct {
  *   y  = x' * cos[pos] + rotate_half(x') * sin[pos]
  *   q_out[i, h, :] = y(q);  K page slot = y(k);  V page slot = v.
  * Everything between the loads and the stores is fp32 and rounded once. cos / sin: [S_max, D] tables
- * (row stride ld_cs) in the cache's dtype or F32 (cs_dtype). q_out may alias q. A token whose sequence is
- * outside [0, B) or whose position is outside [0, S_max) is padding: nothing of it is written; one whose
- * page is outside the table or the pool gets its q_out only. Two tokens of a call must not share a slot.
+ * (row stride ld_cs) in the cache's dtype or F32 (cs_dtype). q_out may be q itself; it overlaps no other input.
+ * A token whose sequence is outside [0, B) or whose position is outside [0, S_max) is padding: nothing of it is
+ * written; one whose page is outside the table or the pool gets its q_out only. Two tokens of a call must not
+ * share a slot, nor two slots of the pools their memory.
  * D % 16 == 0, D <= 256, H % KVH == 0, H < 65536; 16-byte aligned pointers (weights too), strides % 8 == 0.
  * flags: B2D_LAUNCH_PDL. */
 int b2d_paged_rope_append(const b2d_paged_kv* kv, const void* q, int64_t sq_n, int64_t sq_h,

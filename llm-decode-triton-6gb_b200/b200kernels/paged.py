@@ -63,11 +63,11 @@ def paged_rope_append(kv: PagedKV, q: torch.Tensor, k: torch.Tensor, v: torch.Te
                       eps: float = 1e-6, flags: int = 0) -> torch.Tensor:
     """q [N, H, D], k / v [N, KVH, D] (projection outputs; strided views are fine), positions int64 [N],
     page_table int32 [B, pages], cos / sin [S_max, D] in the cache's dtype or fp32 -> q_out [N, H, D] (may be
-    q itself); the rotated keys and the values are written to their pages. Token i belongs to sequence
+    q itself, overlaps no other input); the rotated keys and the values are written to their pages. Token i belongs to sequence
     ``seq_ids[i]`` (int32 [N]) or, without them, ``i // (N // B)``. ``q_weight`` / ``k_weight`` [D]: RMS norm
     of every head before the rotation. fp32 between loads and stores, one rounding. A token whose sequence is
     outside [0, B) or whose position is outside [0, S_max) is padding: nothing of it is written. Two tokens
-    of a call must not share a slot."""
+    of a call must not share a slot; pools whose pages, or whose keys and values, are one memory are refused."""
     r = _lib.binding().rope_append(kv._desc, q, k, v, positions, page_table, cos, sin, q_out, seq_ids, q_weight, k_weight,
                                    eps, flags, kv._index)
     if r.__class__ is int:

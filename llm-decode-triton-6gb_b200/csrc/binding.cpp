@@ -92,10 +92,34 @@ void check_last(const at::Tensor& t, const char* name) {
   if (t.numel() > 0 && t.size(-1) > 1 && t.stride(-1) != 1)
     bad_value(std::string("the last dimension of ") + name + " must be contiguous, got " + show(t));
 }
-// An output whose rows are one memory (an expanded tensor) would be written by several blocks at once.
+// Whether strides nest: from the smallest on, each is past all that the ones before it span, so that no two
+// indices name one element. Every slice, transpose or part of a tensor that does not overlap itself is such.
+bool nests(at::IntArrayRef sizes, at::IntArrayRef strides) {
+  int64_t order[64], span = 0;   // span: the largest offset so far
+  int n = 0;
+  for (size_t d = 0; d < sizes.size(); ++d) {
+    if (sizes[d] == 0) return true;
+    if (sizes[d] == 1) continue;
+    int at = n++;
+    for (; at > 0 && strides[order[at - 1]] > strides[d]; --at) order[at] = order[at - 1];
+    order[at] = d;
+  }
+  for (int i = 0; i < n; ++i) {
+    if (strides[order[i]] <= span) return false;
+    span += (sizes[order[i]] - 1) * strides[order[i]];
+  }
+  return true;
+}
+// An output that overlaps itself would be written by several blocks at once. (Outputs have at most 4 dimensions.)
 void check_output(const at::Tensor& t, const char* name) {
-  for (int64_t d = 0; d < t.dim(); ++d)
-    if (t.size(d) > 1 && t.stride(d) == 0 && t.numel() > 0) bad_value(std::string(name) + " overlaps itself: " + show(t));
+  if (!nests(t.sizes(), t.strides())) bad_value(std::string(name) + " overlaps itself: " + show(t));
+}
+// The same of the pools that an append writes.
+void check_written_pools(const b2d_paged_kv* kv) {
+  const int64_t sizes[4] = {kv->num_pages, kv->KVH, kv->page_size, kv->D};
+  const int64_t k[4] = {kv->sk_p, kv->sk_h, kv->sk_s, 1}, v[4] = {kv->sv_p, kv->sv_h, kv->sv_s, 1};
+  if (!nests(sizes, k) || !nests(sizes, v)) bad_value("the cache's pages overlap one another: an append would write them at once");
+  if (kv->k == kv->v && kv->num_pages > 0) bad_value("the cache's keys and values overlap: an append would write both to one memory");
 }
 void check_device(const at::Tensor* t, const char* name, const at::Device& d) {
   if (t && t->device() != d) {
@@ -195,6 +219,7 @@ PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t na) {
     if (out.sizes() != q.sizes() || out.scalar_type() != dt) bad_value("q_out has q's shape and dtype, got " + show(out));
     check_last(out, "q_out");
     check_output(out, "q_out");
+    check_written_pools(kv);
     check_device(&out, "q_out", dev);
     check_cuda(dev);
     check_pool(dev, a[14]);

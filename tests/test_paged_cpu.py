@@ -131,6 +131,43 @@ def test_outputs_that_overlap_themselves_are_refused():
                       tokens=torch.zeros(1, 4, dtype=torch.int64).expand(2, 4))
 
 
+def test_outputs_whose_rows_run_into_each_other_are_refused():
+    """Overlap without a zero stride: windows of one memory."""
+    def windows(dtype, *shape_and_strides):
+        return torch.zeros(4096, dtype=dtype).as_strided(*shape_and_strides)
+    with pytest.raises(ValueError, match="overlaps itself"):
+        paged_attention(pool(), **attn_args(), out=windows(torch.float16, (2, 1, 4, 64), (64, 64, 32, 1)))
+    with pytest.raises(ValueError, match="overlaps itself"):
+        paged_attention(pool(), **attn_args(), out=windows(torch.float16, (2, 1, 4, 64), (192, 64, 64, 1)))
+    with pytest.raises(ValueError, match="overlaps itself"):
+        paged_rope_append(pool(), **append_args(), q_out=windows(torch.float16, (2, 4, 64), (64, 64, 1)))
+    with pytest.raises(ValueError, match="overlaps itself"):
+        verify_drafts(torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 4, 10), torch.zeros(2, 4),
+                      tokens=windows(torch.int64, (2, 4), (3, 1)))
+    # views of larger tensors are fine: the call goes on to ask for a GPU
+    for out in (torch.zeros(1, 2, 6, 64).half().transpose(0, 1)[:, :, 1:5], torch.zeros(4, 2, 1, 64).half().permute(1, 2, 0, 3)):
+        with pytest.raises(ValueError, match="CUDA"):
+            paged_attention(pool(), **attn_args(), out=out)
+    with pytest.raises(ValueError, match="CUDA"):
+        paged_rope_append(pool(), **append_args(), q_out=torch.zeros(2, 8, 64).half()[:, ::2])
+
+
+def test_append_refuses_pools_that_overlap():
+    one = torch.zeros(1, 2, 16, 64).half()
+    both = torch.zeros(4, 2, 2, 16, 64).half()
+    for k, v in ((one.expand(4, 2, 16, 64), both[:, 0]), (both[:, 1], one.expand(4, 2, 16, 64)),
+                 (torch.zeros(9000).half().as_strided((4, 2, 16, 64), (1024, 1024, 64, 1)), both[:, 0]),
+                 (both[:, 0], both[:, 0])):
+        with pytest.raises(ValueError, match="overlap"):
+            paged_rope_append(PagedKV(k, v), **append_args())
+        with pytest.raises(ValueError, match="CUDA"):      # read only: fine
+            paged_attention(PagedKV(k, v), **attn_args())
+    nhd = torch.zeros(4, 2, 16, 2, 64).half().transpose(2, 3)   # [pages, K or V, head, slot, D]
+    for k, v in ((both[:, 0], both[:, 1]), (nhd[:, 0], nhd[:, 1]), (one, one.clone())):
+        with pytest.raises(ValueError, match="CUDA"):
+            paged_rope_append(PagedKV(k, v), **append_args())
+
+
 def test_workspace_without_its_own_memory_is_refused():
     """A workspace whose elements are one memory (expanded) or lie apart has fewer bytes than its size says."""
     for ws in (torch.zeros(1, dtype=torch.uint8).expand(1 << 20), torch.zeros(1 << 21, dtype=torch.uint8)[::2],
