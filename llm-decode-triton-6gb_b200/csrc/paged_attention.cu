@@ -425,14 +425,14 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
       ++seg;
     }
     if (ok && behind < end) {   // only a unit's lead is left: the consumers stop
-      if (seg > 0) __all_sync(0xffffffffu, mbar_wait(q_empty, (seg - 1) & 1));
-      if (lane == 0) {
+      if (seg > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait(q_empty, (seg - 1) & 1));
+      if (ok && lane == 0) {
         ahead.kind = -1;
         ahead.next = end;
         s_seg = ahead;
         mbar_arrive(q_full);
       }
-      mbar_arrive(q_full);
+      if (ok) mbar_arrive(q_full);
     }
     cp_async_wait<0>();
   } else {

@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) paged_prefix_kernel(const _
     const int ahead = pair ? 1 : 2;   // tiles of scores that run ahead of the first P V
     for (int i = 0; i < ahead && i < n; ++i) {
       load(false, i);
-      if (i == 0) mbar_wait(q_full, 0);
+      if (i == 0) ok = ok && __all_sync(0xffffffffu, mbar_wait(q_full, 0));
     }
     for (int i = 0; i < n; ++i) {
       load(true, i);
@@ -221,15 +221,19 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) paged_prefix_kernel(const _
     }
   } else if (warp >= kIssuer) {
     // ---- the products of warpgroup w, in the order that its buffers need: P V of a step, then the scores of the
-    // step after the next, which overwrite that P (the tensor core takes a thread's products in order)
+    // step after the next, which overwrite that P (the tensor core takes a thread's products in order). After a wait
+    // that ran out `done` never completes, and the softmax warps give NaN: the waits hand on the number of tries that
+    // they have left. That costs about 1.2 us of 65 in the call of the header against dropping their outcome (a flag in
+    // registers with a vote a wait: 1.8, a flag in shared memory: 4.6).
     const int w = warp - kIssuer, steps = steps_of(w);
     constexpr uint32_t ID_S = idesc<T, kSub, false>(), ID_O = idesc<T, D, true>();
     const int ahead = pair ? 1 : 2;
+    int tries = kMbarTries;
     // the producer's position of a K or V tile
     auto unit_k = [&](int tile) { return tile < ahead ? tile : 2 * tile - ahead + 1; };
     auto unit_v = [&](int tile) { return min(tile + ahead, n) + tile; };
     auto ready = [&](int unit) {
-      mbar_wait(full + 8 * (unit % kRing), (unit / kRing) & 1);
+      tries = mbar_wait_tries(full + 8 * (unit % kRing), (unit / kRing) & 1, tries);
       return static_cast<uint32_t>(unit % kRing);
     };
     auto scores = [&](int u) {   // S_w[u & 1] = Q K^T for step u
@@ -251,7 +255,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) paged_prefix_kernel(const _
     };
     auto values = [&](int u) {   // O_w += P_w V for step u
       const uint32_t slot = ready(unit_v(tile_of(w, u)));
-      mbar_wait(p_full + 16 * w + 8 * (u & 1), (u >> 1) & 1);
+      tries = mbar_wait_tries(p_full + 16 * w + 8 * (u & 1), (u >> 1) & 1, tries);
       tc_fence_after();
       const uint32_t vb = ring + slot * TILEB + (u & 1) * SUBB;
       if (elect_one()) {
@@ -267,14 +271,14 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) paged_prefix_kernel(const _
       __syncwarp();
     };
     if (n > 0) {
-      mbar_wait(q_full, 0);
+      tries = mbar_wait_tries(q_full, 0, tries);
       tc_fence_after();
       for (int u = 0; u < 2 && u < steps; ++u) scores(u);
       for (int u = 0; u < steps; ++u) {
         values(u);
         if (u + 2 < steps) scores(u + 2);
       }
-      if (elect_one()) mma_commit(done);
+      if (__all_sync(0xffffffffu, tries > 0) && elect_one()) mma_commit(done);
     }
     __syncwarp();
   } else {

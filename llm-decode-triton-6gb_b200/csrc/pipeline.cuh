@@ -30,10 +30,17 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
 }
 // Bounded wait: false if the phase never completed (only a fault elsewhere could cause it), so that every
 // launch ends; the callers then give NaN.
+constexpr int kMbarTries = 1 << 22;
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
-  for (int i = 0; i < (1 << 22); ++i)
+  for (int i = 0; i < kMbarTries; ++i)
     if (mbar_try_wait(bar, parity)) return true;
   return false;
+}
+// The same with a number of tries that a row of waits hands on: 0 once one of them has run out.
+__device__ __forceinline__ int mbar_wait_tries(uint32_t bar, uint32_t parity, int tries) {
+  for (int i = 0; i < tries; ++i)
+    if (mbar_try_wait(bar, parity)) return tries;
+  return 0;
 }
 __device__ __forceinline__ void fence_mbar_init() { asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory"); }
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }

@@ -1,5 +1,7 @@
 """CPU: refusals of the paged-cache and draft-verification calls (Python and C ABI), and their oracle."""
 import ctypes as C
+import re
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -225,6 +227,21 @@ def test_c_verify_checks():
     assert call(K=32, ldo=33) == SHAPE and call(V=0) == SHAPE and call(V=2 ** 30 + 1) == SHAPE and call(ldo=4) == SHAPE and call(dt=5) == DTYPE
     assert call(draft=None) == ARG and call(tp=None) == ARG and call(u=None) == ARG and call(out=None) == ARG
     assert call(B=-1) == ARG and call(draft=P + 4) == ALIGN and call(tp=P + 2) == ALIGN
+
+
+# ---- the kernels' sources
+def test_every_bounded_wait_of_the_paged_kernels_is_looked_at():
+    """A wait on an mbarrier that runs out has to reach the result (as NaN): each one's outcome goes into a flag, or
+    into the number of tries that the next waits have."""
+    csrc = Path(__file__).resolve().parent.parent / "llm-decode-triton-6gb_b200" / "csrc"
+    found = 0
+    for name in ("paged_attention.cu", "paged_prefix.cu"):
+        for line in (csrc / name).read_text().splitlines():
+            code = line.split("//")[0]
+            if re.search(r"mbar_wait(_tries)?\(", code):
+                found += 1
+                assert re.search(r"\b(ok|landed) (=|&&) .*mbar_wait\(|\btries = mbar_wait_tries\(.*, tries\);", code), f"{name}: {line.strip()}"
+    assert found >= 15
 
 
 # ---- the oracle draws from the target's own distribution
