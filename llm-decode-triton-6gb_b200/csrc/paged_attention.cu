@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
 
   if (warp == kWarps) {
     // ---- producer
-    int it = 0, seg = 0;   // stages and segments so far
+    int it = 0, seg = 0, sent = 0;   // stages, segments and slots filled so far
     bool ok = true;
     // lane -> (K or V, 64-element column, page of the stage): 32 lanes are enough from boxes of 8 rows on
     const int bp = a.box_rows, boxes = bp ? KEYS / bp : 1, per = HALVES * boxes;
@@ -384,6 +384,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
             __syncwarp();
             if (lane == 0) mbar_expect_tx(full + 8 * slot, bytes);
             __syncwarp();
+            sent = u + 1;
             if (copy) tma_load_4d(dst, x ? &maps.v : &maps.k, 64 * col, a.div.slot(tok, a.div.page(tok)), g.kvh, page, full + 8 * slot);
           }
           if (i == 0) send_q();
@@ -435,6 +436,10 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
       if (ok) mbar_arrive(q_full);
     }
     cp_async_wait<0>();
+    // Nothing is under way into this block's memory when it ends (the consumers wait for every copy as well, unless one
+    // of their waits ran out)
+    bool landed = true;
+    for (int u = max(sent - kSlots, 0); u < sent; ++u) landed = landed && mbar_wait(full + 8 * (u % kSlots), (u / kSlots) & 1);
   } else {
     // ---- consumers: keys are the products' M axis (16 of a warp's keys), rows their N axis (8 per tile)
     const int g8 = lane >> 2, tq = lane & 3, mi = lane >> 3, ri = lane & 7;
