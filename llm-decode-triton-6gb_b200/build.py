@@ -1,9 +1,11 @@
 """Build libb200decode.so (all CUDA kernels + the C ABI) in-tree for sm_100a.
 
-    python llm-decode-triton-6gb_b200/build.py [--verbose]
+    python llm-decode-triton-6gb_b200/build.py [--verbose] [--force] [--no-binding]
 
 The shared library lands next to the Python package (``b200kernels/libb200decode.so``) so it
-travels with the source tree; nothing is installed into site-packages.
+travels with the source tree; nothing is installed into site-packages. The CPython module of the paged-cache and
+draft-verification calls (``b200kernels/_binding.so``) is built beside it where torch is installed; hosts that use the
+C ABI alone need neither it nor torch (``--no-binding``).
 """
 from __future__ import annotations
 
@@ -31,12 +33,28 @@ def nvcc_path() -> str:
     return cand
 
 
+def _older(path: Path, deps) -> bool:
+    return not path.exists() or any(p.stat().st_mtime > path.stat().st_mtime for p in deps if p.exists())
+
+
+def needs_library() -> bool:
+    return _older(LIB_PATH, [CSRC / s for s in SOURCES] + list(CSRC.glob("*.cuh")) + [INCLUDE / "b200decode.h", Path(__file__)])
+
+
+def _has_torch() -> bool:
+    try:
+        import torch  # noqa: F401
+    except ImportError:
+        return False
+    return True
+
+
+def needs_binding() -> bool:
+    return _has_torch() and _older(BINDING_PATH, [CSRC / "binding.cpp", INCLUDE / "b200decode.h", Path(__file__)])
+
+
 def needs_build() -> bool:
-    if not LIB_PATH.exists() or not BINDING_PATH.exists():
-        return True
-    t = min(LIB_PATH.stat().st_mtime, BINDING_PATH.stat().st_mtime)
-    deps = [CSRC / s for s in SOURCES] + [CSRC / "binding.cpp"] + list(CSRC.glob("*.cuh")) + [INCLUDE / "b200decode.h", Path(__file__)]
-    return any(p.stat().st_mtime > t for p in deps if p.exists())
+    return needs_library() or needs_binding()
 
 
 def _compile(src: Path, obj: Path, verbose: bool) -> subprocess.CompletedProcess:
@@ -66,39 +84,51 @@ def _build_binding(out: Path, verbose: bool) -> subprocess.CompletedProcess:
     return subprocess.run(cmd, capture_output=True, text=True)
 
 
-def build(verbose: bool = False, force: bool = False) -> Path:
+def _report(res: subprocess.CompletedProcess, verbose: bool) -> bool:
+    if verbose or res.returncode != 0:
+        sys.stdout.write(res.stdout)
+        sys.stderr.write(res.stderr)
+    return res.returncode == 0
+
+
+def _build_library(tmp: Path, verbose: bool) -> None:
+    from concurrent.futures import ThreadPoolExecutor
+    objs = [tmp / (Path(s).stem + ".o") for s in SOURCES]
+    with ThreadPoolExecutor(max_workers=min(len(SOURCES), os.cpu_count() or 1)) as ex:
+        results = list(ex.map(lambda so: _compile(CSRC / so[0], so[1], verbose), zip(SOURCES, objs)))
+    if not all([_report(res, verbose) for res in results]):
+        raise RuntimeError("the compiler failed")
+    cmd = [nvcc_path(), "-shared", *ARCH, "-cudart", "shared", "-o", str(LIB_PATH) + ".tmp", *map(str, objs)]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if not _report(res, verbose):
+        raise RuntimeError(f"nvcc link failed with exit code {res.returncode}")
+    os.replace(str(LIB_PATH) + ".tmp", LIB_PATH)
+
+
+def build(verbose: bool = False, force: bool = False, binding: bool = True) -> Path:
     """Compiles every source to an object file in parallel (one nvcc per source), then links the
-    shared library; objects live in a temporary directory next to the library."""
-    if not force and not needs_build():
-        return LIB_PATH
+    shared library; objects live in a temporary directory next to the library. The binding is compiled at the same
+    time (not without torch, or with ``binding=False``); if it fails, that is raised once the library is in place."""
     import tempfile
     from concurrent.futures import ThreadPoolExecutor
-    with tempfile.TemporaryDirectory(dir=LIB_PATH.parent) as tmp:
-        objs = [Path(tmp) / (Path(s).stem + ".o") for s in SOURCES]
-        with ThreadPoolExecutor(max_workers=min(len(SOURCES) + 1, os.cpu_count() or 1)) as ex:
-            binding = ex.submit(_build_binding, Path(tmp) / BINDING_PATH.name, verbose)
-            results = list(ex.map(lambda so: _compile(CSRC / so[0], so[1], verbose), zip(SOURCES, objs)))
-            results.append(binding.result())
-        failed = False
-        for res in results:
-            if verbose or res.returncode != 0:
-                sys.stdout.write(res.stdout)
-                sys.stderr.write(res.stderr)
-            failed |= res.returncode != 0
-        if failed:
-            raise RuntimeError("the compiler failed")
-        cmd = [nvcc_path(), "-shared", *ARCH, "-cudart", "shared", "-o", str(LIB_PATH) + ".tmp", *map(str, objs)]
-        res = subprocess.run(cmd, capture_output=True, text=True)
-        if verbose or res.returncode != 0:
-            sys.stdout.write(res.stdout)
-            sys.stderr.write(res.stderr)
-        if res.returncode != 0:
-            raise RuntimeError(f"nvcc link failed with exit code {res.returncode}")
-        os.replace(Path(tmp) / BINDING_PATH.name, BINDING_PATH)
-    os.replace(str(LIB_PATH) + ".tmp", LIB_PATH)
+    library = force or needs_library()
+    with tempfile.TemporaryDirectory(dir=LIB_PATH.parent) as tmp, ThreadPoolExecutor(max_workers=1) as ex:
+        made = None
+        if binding and (_has_torch() if force else needs_binding()):
+            made = ex.submit(_build_binding, Path(tmp) / BINDING_PATH.name, verbose)
+        if library:
+            _build_library(Path(tmp), verbose)
+        if made is not None:
+            try:
+                ok = _report(made.result(), verbose)
+            except OSError as e:   # no compiler
+                raise RuntimeError(f"{BINDING_PATH.name}, the Python binding, could not be built: {e}") from e
+            if not ok:
+                raise RuntimeError(f"{BINDING_PATH.name}, the Python binding, does not compile")
+            os.replace(Path(tmp) / BINDING_PATH.name, BINDING_PATH)
     return LIB_PATH
 
 
 if __name__ == "__main__":
-    build(verbose="--verbose" in sys.argv, force="--force" in sys.argv)
+    build(verbose="--verbose" in sys.argv, force="--force" in sys.argv, binding="--no-binding" not in sys.argv)
     print(LIB_PATH)
