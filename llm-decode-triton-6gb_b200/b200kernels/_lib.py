@@ -160,18 +160,29 @@ _binding = None
 
 def binding():
     """The CPython module of csrc/binding.cpp (the checks and calls of the paged-cache and draft-verification
-    entry points), bound to the library's functions; raises if it has not been built."""
+    entry points), bound to the library's functions; raises if it has not been built, or for another torch."""
     global _binding
     if _binding is None:
         import importlib.machinery
         import importlib.util
+        import sys
+
+        import torch
         path = LIB_PATH.parent / "_binding.so"
+        build = "build it with `python llm-decode-triton-6gb_b200/build.py`"
         if not path.exists():
-            raise RuntimeError(f"{path} is missing: build it with `python llm-decode-triton-6gb_b200/build.py`")
+            raise RuntimeError(f"{path} is missing: {build}")
         lib = load()
         loader = importlib.machinery.ExtensionFileLoader("_binding", str(path))
-        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_binding", loader))
-        loader.exec_module(module)
+        try:
+            module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_binding", loader))
+            loader.exec_module(module)
+        except ImportError as e:   # it needs symbols that this torch does not have
+            raise RuntimeError(f"{path} does not load: {build}") from e
+        host = f"torch {torch.__version__} {sys.implementation.cache_tag}"
+        built_for = module.built_for() if hasattr(module, "built_for") else "of unknown origin"
+        if built_for != f"b2d built for {host}":
+            raise RuntimeError(f"{path} is {built_for}, not for {host}: {build}")
         module.bind(*(C.cast(getattr(lib, f), C.c_void_p).value for f in (
             "b2d_paged_rope_append", "b2d_paged_attention_workspace_bytes", "b2d_paged_attention", "b2d_verify_drafts")))
         _binding = module

@@ -49,8 +49,17 @@ def _has_torch() -> bool:
     return True
 
 
+def host_tag() -> str:
+    """What the binding depends on (``b200kernels/_lib.py`` compares the same text when it loads the module)."""
+    import torch
+    return f"torch {torch.__version__} {sys.implementation.cache_tag}"
+
+
 def needs_binding() -> bool:
-    return _has_torch() and _older(BINDING_PATH, [CSRC / "binding.cpp", INCLUDE / "b200decode.h", Path(__file__)])
+    if not _has_torch():
+        return False
+    return (_older(BINDING_PATH, [CSRC / "binding.cpp", INCLUDE / "b200decode.h", Path(__file__)])
+            or f"b2d built for {host_tag()}\0".encode() not in BINDING_PATH.read_bytes())
 
 
 def needs_build() -> bool:
@@ -74,8 +83,8 @@ def _build_binding(out: Path, verbose: bool) -> subprocess.CompletedProcess:
     root = Path(torch.__file__).resolve().parent
     cuda = Path(nvcc_path()).resolve().parent.parent
     cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}",
-           f"-I{root / 'include'}", f"-I{root / 'include/torch/csrc/api/include'}", f"-I{cuda / 'include'}",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DB2D_HOST_TAG="{host_tag()}"',
+           f"-I{INCLUDE}", f"-I{root / 'include'}", f"-I{root / 'include/torch/csrc/api/include'}", f"-I{cuda / 'include'}",
            f"-I{sysconfig.get_paths()['include']}", "-o", str(out), str(CSRC / "binding.cpp"),
            f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python",
            f"-Wl,-rpath,{root / 'lib'}"]

@@ -380,6 +380,10 @@ PyObject* verify(PyObject*, PyObject* const* a, Py_ssize_t na) {
   });
 }
 
+// build.py looks for this text in the module, b200kernels/_lib.py asks for it before the first call.
+const char kBuiltFor[] = "b2d built for " B2D_HOST_TAG;
+PyObject* built_for(PyObject*, PyObject* const*, Py_ssize_t) { return PyUnicode_FromString(kBuiltFor); }
+
 // the addresses of the four entry points, in the order of the globals above
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t na) {
   return guarded([&]() -> PyObject* {
@@ -396,7 +400,7 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t na) {
 #define FAST(name) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr
 PyMethodDef kMethods[] = {{"rope_append", FAST(rope_append)}, {"attention", FAST(attention)},
                           {"attention_workspace", FAST(attention_workspace)}, {"verify", FAST(verify)},
-                          {"bind", FAST(bind)}, {nullptr, nullptr, 0, nullptr}};
+                          {"bind", FAST(bind)}, {"built_for", FAST(built_for)}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

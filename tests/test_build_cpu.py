@@ -60,3 +60,27 @@ def test_kernels_that_do_not_compile_fail_the_build(builder, monkeypatch):
     with pytest.raises(RuntimeError, match="compiler"):
         builder.build(binding=False)
     assert not builder.LIB_PATH.exists()
+
+
+def test_a_binding_of_another_torch_is_rebuilt(builder):
+    """The module calls torch's C++ ABI: one that was built against another torch or Python is out of date, however new
+    the file is."""
+    builder.LIB_PATH.write_bytes(b"")
+    for built_for, needed in ((b"b2d built for " + builder.host_tag().encode() + b"\0", False), (b"b2d built for torch 1.0.0 cpython-312\0", True),
+                              (b"", True)):
+        builder.BINDING_PATH.write_bytes(b"\x7fELF" + built_for)
+        assert builder.needs_build() is needed
+    real = ROOT / "llm-decode-triton-6gb_b200" / "b200kernels" / "_binding.so"
+    assert b"b2d built for " + builder.host_tag().encode() + b"\0" in real.read_bytes()
+
+
+def test_a_binding_of_another_torch_is_not_used(monkeypatch):
+    import torch
+    from b200kernels import _lib
+    monkeypatch.setattr(_lib, "_binding", None)
+    assert _lib.binding() is not None
+    monkeypatch.setattr(_lib, "_binding", None)
+    monkeypatch.setattr(torch, "__version__", "1.0.0")
+    with pytest.raises(RuntimeError, match="built for torch .* not for torch 1.0.0"):
+        _lib.binding()
+    assert _lib._binding is None
