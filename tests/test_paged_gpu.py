@@ -205,6 +205,43 @@ def test_attention_long_ragged():
     c.check(c.run(max_len=1))          # a wrong hint costs time only
 
 
+@pytest.mark.parametrize("lens,H,KVH,T,D,prefix,ps", [
+    ([5000, 1, 2777, 4096, 0, 63, 64, 65, 129], 8, 2, 1, 128, 0, 16),      # shares of a ragged batch
+    ([3001, 517, 2, 128, 1500], 12, 2, 3, 64, 0, 64), ([700, 1300], 16, 1, 4, 128, 0, 32),
+    ([9001], 1, 1, 1, 128, 0, 16), ([8200], 4, 1, 1, 64, 0, 64),           # a unit in many parts
+    ([260, 77, 1001], 8, 2, 2, 128, 0, 5),                                 # pages that tensor copies do not fit
+    ([1100, 1000, 1001, 400, 1530], 8, 2, 1, 128, 1000, 8),                # a prefix on the streaming kernel
+    ([3000 + 37 * i for i in range(9)], 4, 4, 1, 64, 2944, 64),
+    ([2100 + 19 * i for i in range(20)], 8, 2, 2, 128, 2048, 16),          # and on the tensor cores
+    ([2000 + 7 * i for i in range(17)], 4, 1, 2, 64, 1984, 16), ([330 + i for i in range(40)], 8, 2, 4, 128, 320, 32)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_attention_counts_every_key_once(lens, H, KVH, T, D, prefix, ps, dtype):
+    """Queries of zeros weigh all keys alike, and values that mark a key's position modulo D / 2 and its run of 64 then
+    give counts over the number of keys: a key that is lost or taken twice at a border of stages, shares or splits
+    changes a count by a whole. Weights are 1 (2^0 is exact) and all sums whole numbers below 2^24, so five roundings are
+    left at most: the reciprocal of the sum, the product with it, and the sum of four warps' quotients; 5 x 2^-24."""
+    c = Case(lens, H=H, KVH=KVH, T=T, D=D, ps=ps, prefix=prefix, dtype=dtype, seed=D + ps)
+    half = D // 2
+    mark = lambda pos: torch.cat([torch.nn.functional.one_hot(pos % half, half), torch.nn.functional.one_hot(pos // 64 % half, half)], -1).to(dtype)
+    top = -(-max(max(lens), prefix) // ps) * ps
+    marks = mark(torch.arange(top)).view(-1, 1, ps, D)   # [page, 1, slot, D]
+    if prefix:
+        c.v[c.prefix_table.long()] = torch.where(c.v[c.prefix_table.long()].isnan(), NAN, marks[:c.prefix_table.numel()])
+    for b in range(len(lens)):
+        at = (c.table[b] >= 0).nonzero()[:, 0]
+        pages = c.table[b, at].long()
+        c.v[pages] = torch.where(c.v[pages].isnan(), NAN, marks[at])
+    c.vd.copy_(c.v)
+    c.q.zero_()
+    got = f64(c.run(out_dtype=F32))
+    running = np.cumsum(f64(mark(torch.arange(top))), 0)
+    for b, n_b in enumerate(lens):
+        for t in range(T):
+            n = n_b - T + 1 + t
+            want = running[n - 1] / n if n > 0 else np.zeros(D)
+            assert (np.abs(got[b, t] - want) <= 5 * 2.0 ** -24 * want).all(), (b, t, np.abs(got[b, t] - want).max() * max(n, 1))
+
+
 def test_attention_large_scores():
     """Scores of several hundred: the running maximum matters, one key takes nearly all the weight."""
     for dtype in (F16, BF16):
@@ -471,6 +508,50 @@ def test_append(N, B, H, KVH, D, ps, dtype, table_dtype, norm):
     untouched = torch.ones(B * per + 2, ps, dtype=torch.bool)
     untouched[page, slot] = False
     assert (kp.cpu().transpose(1, 2)[untouched] == 5).all() and (vp.cpu().transpose(1, 2)[untouched] == 6).all()
+
+
+@pytest.mark.parametrize("N,norm", [(3000, "q"), (3000, "both"), (300, "q"), (5, "q"), (5000, "none")])
+def test_append_mixed_batch(N, norm):
+    """Tokens of a mixed batch in any order (``seq_ids``), padding among them, through the staged and the direct kernel;
+    a norm of the queries alone."""
+    B, H, KVH, D, ps = 7, 32, 8, 128, 16
+    g = torch.Generator().manual_seed(N)
+    per = -(-N // ps) + 1
+    table = torch.randperm(B * per + 3, generator=g)[:B * per].int().view(B, per)
+    seq = torch.randint(-1, B + 1, (N,), generator=g).int()            # -1 and B: padding
+    positions = torch.zeros(N, dtype=torch.int64)
+    for b in range(-1, B + 1):
+        at = (seq == b).nonzero()[:, 0]
+        positions[at] = torch.arange(at.numel()) + (b + 1)
+    order = torch.randperm(N, generator=g)
+    seq, positions = seq[order], positions[order]
+    S = int(positions.max()) + 1
+    q, k, v = (torch.randn(N, h, D, generator=g).to(BF16) for h in (H, KVH, KVH))
+    ang = torch.randn(S, D, generator=g) * 3
+    cos, sin = ang.cos(), ang.sin()
+    w = (1 + 0.3 * torch.randn(D, generator=g)).to(BF16)
+    qw, kw = w if norm != "none" else None, w if norm == "both" else None
+    kp, vp = (torch.full((B * per + 3, KVH, ps, D), 5.0, dtype=BF16, device=DEV) for _ in range(2))
+    q_out = torch.full((N, H, D), 9.0, dtype=BF16, device=DEV)
+    paged_rope_append(PagedKV(kp, vp), q.to(DEV), k.to(DEV), v.to(DEV), positions.to(DEV), table.to(DEV), cos.to(DEV), sin.to(DEV),
+                      q_out=q_out, seq_ids=seq.to(DEV), q_weight=None if qw is None else qw.to(DEV),
+                      k_weight=None if kw is None else kw.to(DEV), eps=1e-5)
+    live = (seq >= 0) & (seq < B)
+    c, s = f64(cos)[positions.numpy()], f64(sin)[positions.numpy()]
+
+    def check(got, x, weight):
+        ref, size = rope_ref(f64(x), c, s, None if weight is None else f64(weight), 1e-5)
+        err = np.abs(f64(got) - ref[live.numpy()])
+        assert (err <= half_step(BF16) * np.abs(ref[live.numpy()]) + 2.0 ** -19 * size[live.numpy()] + 2.0 ** -25).all(), err.max()
+
+    check(q_out.cpu()[live], q, qw)
+    assert (q_out.cpu()[~live] == 9).all()
+    page, slot = table[seq[live].long(), positions[live] // ps].long(), positions[live] % ps
+    check(kp.cpu()[page, :, slot], k, kw)
+    assert torch.equal(vp.cpu()[page, :, slot], v[live])
+    untouched = torch.ones(B * per + 3, ps, dtype=torch.bool)
+    untouched[page, slot] = False
+    assert (kp.cpu().transpose(1, 2)[untouched] == 5).all() and (vp.cpu().transpose(1, 2)[untouched] == 5).all()
 
 
 def test_append_padding_and_bad_pages_write_nothing():
