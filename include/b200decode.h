@@ -403,7 +403,9 @@ int b2d_paged_rope_append(const b2d_paged_kv* kv, const void* q, int64_t sq_n, i
  * empty sequence) gives zeros. seqlens beyond the page table are cut to it, or to prefix_len where that is longer.
  * prefix_table / prefix_len: the positions [0, prefix_len) of EVERY sequence are those of the pages
  * prefix_table[0 .. ceil(prefix_len / page_size)) (int32, device) -- a shared system prompt, read and
- * multiplied once for the whole batch; page_table's entries for them are not read. prefix_len 0: none.
+ * multiplied once for the whole batch; page_table's entries for them are not read. prefix_len 0: none. Pages of 8, 16,
+ * 32 or a multiple of 64 positions with prefix_len a multiple of the page (of 64 for larger pages) are the fast
+ * form: others are right, but all keys of the call take smaller copies and the prefix no tcgen05 products.
  * max_len: an upper bound of seqlens known to the host (0: the page table's reach); it only guides the
  * split over the SMs, longer sequences stay right.
  * D 64 or 128; H / KVH in 1..16; T in 1..16; 16-byte aligned q, strides % 8 == 0; the page table reaches less

@@ -6,7 +6,8 @@
     from b200kernels.paged import PagedKV, paged_rope_append, paged_attention   # paged cache, shared prefix
     from b200kernels.speculative import verify_drafts           # speculative sampling
 
-Every op runs in ``libb200decode.so`` (C ABI in ``include/b200decode.h``) through ctypes.
+Every op runs in ``libb200decode.so`` (C ABI in ``include/b200decode.h``), called through ctypes; ``paged`` and
+``speculative`` call it through a small CPython module (``_binding.so``).
 """
 from ._lib import LIB_PATH, load  # noqa: F401
 

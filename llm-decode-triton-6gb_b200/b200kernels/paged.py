@@ -81,9 +81,12 @@ def paged_attention(kv: PagedKV, q: torch.Tensor, page_table: torch.Tensor, seql
                     workspace: torch.Tensor | None = None, flags: int = 0) -> torch.Tensor:
     """q [B, T, H, D], page_table int32 [B, pages], seqlens int32 [B] (cached keys, the T new tokens included)
     -> [B, T, H, D] in ``out_dtype`` (q's dtype or torch.float32). Query t of sequence b sees the keys before
-    position ``seqlens[b] - T + 1 + t``; one that sees none gives zeros. ``prefix_table`` int32 [pages] and
+    position ``seqlens[b] - T + 1 + t``; one that sees none gives zeros. Lengths past the table's pages (and the prefix)
+    are cut to them. ``prefix_table`` int32 [pages] and
     ``prefix_len``: the first ``prefix_len`` positions of every sequence lie in these pages (the entries of
-    ``page_table`` for them are not read) and are computed once for the batch. ``max_len``: an upper bound of
+    ``page_table`` for them are not read, and need not be there) and are computed once for the batch -- fast where
+    pages hold 8, 16, 32 or a multiple of 64 positions and ``prefix_len`` is a multiple of the page (of 64 for larger
+    pages); other sizes are right, but take slower copies for the whole call. ``max_len``: an upper bound of
     ``seqlens`` known to the host, which only guides the split. ``workspace``: contiguous scratch of
     ``paged_attention_workspace`` bytes, 16-byte aligned, not shared by calls that may overlap; without it
     one is allocated per call."""

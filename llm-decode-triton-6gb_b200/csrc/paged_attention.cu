@@ -119,8 +119,9 @@ __device__ __forceinline__ Span span_of(const PagedAttnArgs& a, int len) {
 template <int D, int NT>
 struct Line {
   static constexpr int KEYS = stage_keys<D>(), ROWS = 8 * NT;
-  // from time stamps in the kernel (which lengthen it): a unit's start and end cost 1.3 us with one row tile
-  // and 4 us with more, a stage 1 us (1.6 with three row tiles)
+  // from time stamps in the kernel, which lengthen what they measure: a unit's start and end cost 1.3 us with one row
+  // tile and 4 us with more, a stage 1 us (1.6 with three row tiles). Four row tiles have the value of three, without a
+  // measurement of their own.
   static constexpr int LEAD = NT == 1 ? 2 : NT == 2 ? 4 : 3;
   int tiles, units, tiles_p, cost_p, base, ctas, quota, extra;
   __device__ __forceinline__ Line(const PagedAttnArgs& a) {
@@ -884,7 +885,9 @@ bool encode_pool(CUtensorMap* m, const b2d_paged_kv& kv, void* base, int64_t sp,
 }
 
 // Key rows of a tensor copy: a page, or 64 rows of a larger one; every copy starts on a multiple of 8 rows
-// and ends inside its page, and the prefix ends between two copies. 0: the pages do not allow it.
+// and ends inside its page, and the prefix ends between two copies. 0: the pages do not allow it, and the whole call
+// takes cp.async and keeps its prefix on the streaming kernel (64 sequences on 4096 shared keys, pages of 16, bf16: 37 us;
+// on 4100: 137).
 int box_rows(const b2d_paged_kv& kv, int prefix_len) {
   const int ps = kv.page_size;
   if (kv.num_pages < 1 || ps < 8 || (64 % ps != 0 && ps % 64 != 0)) return 0;

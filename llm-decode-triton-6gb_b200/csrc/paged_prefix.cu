@@ -1,8 +1,9 @@
 // Attention over a prefix that the whole batch shares, on the 5th-generation tensor cores (sm_100a): the
 // queries of all sequences that read one KV head form one row axis, so the prefix is read once for up to 256
-// rows and the two products are 128 x 128 x 128 matrix products. Used from more than 32 rows on (below, the
-// mma.sync kernel of csrc/paged_attention.cu is bound by the same bytes); leaves (O, m, l) per row and split
-// of the keys, which that file's per-sequence kernel takes in.
+// rows and its products are matrix products of 128 rows: 128 x 64 x D for the scores, 128 x D x 64 for the values. Used
+// from more than 32 rows on (below, the mma.sync kernel of csrc/paged_attention.cu is bound by the same bytes);
+// leaves (O, m, l) per row and split of the keys. The combine launch of that file merges them with the sequences' own
+// parts: it waits for the streaming launch, which runs beside this one and waits for it at its end.
 //
 // A CTA owns (256 rows as two tiles of 128, KV head, split). Per 64 keys and row tile:
 //   S = Q K^T     tcgen05.mma kind::f16, M = 128, N = 64, both operands K-major in shared memory, S in TMEM
@@ -16,8 +17,8 @@
 // fp32 and in both 16-bit types), so O in TMEM is rarely rescaled. K and V come as 128-byte-swizzled tensor
 // copies, page by page, through a ring of four 128-key tiles.
 // Measured on B200 (32 sequences x 4 drafts, 32 / 8 heads of 128, 16384 shared keys, bf16; 34.4 GFLOP): the call
-// takes 65 us by graph replay; with cold caches this kernel is 43.9 us of it, the sequences' own keys 28.3, the
-// combine 14.7. One product of 64 keys and 256 rows after another took about 1.1 us with time stamps in the
+// takes 65 to 66 us by graph replay; with cold caches this kernel is 44.5 us of it, the sequences' own keys 28.9, the
+// combine 12.9. One product of 64 keys and 256 rows after another took about 1.1 us with time stamps in the
 // kernel, which lengthen it; their shared-memory reads alone are estimated at 0.7 and the exponentials at 0.55.
 // The call took 168 us with mma.sync, 83 with the first tcgen05 form. Merging the splits through distributed
 // shared memory before the write: 67.8 against 64.8, not kept.
