@@ -44,6 +44,8 @@ class PagedKV:
             raise ValueError("the last dimension of the pages must be contiguous")
         if not 1 <= k_pages.shape[2] <= MAX_PAGE_SIZE or k_pages.shape[1] == 0:
             raise ValueError(f"pages hold 1..{MAX_PAGE_SIZE} positions of at least one head, got {tuple(k_pages.shape)}")
+        if max(k_pages.shape) >= 2 ** 31:
+            raise ValueError(f"too many pages, heads or elements (2^31 or more): {tuple(k_pages.shape)}")
         if v_pages.device != k_pages.device:
             raise ValueError(f"k/v pages are on {k_pages.device} and {v_pages.device}")
         self.k_pages, self.v_pages = k_pages, v_pages

@@ -33,6 +33,14 @@ def test_pool_refusals(k, v, err):
         PagedKV(k, v)
 
 
+def test_pool_of_too_many_pages_or_heads_is_refused():
+    """The kernels count pages and heads in 32 bits; a number past them must not wrap."""
+    one = torch.zeros(1, 1, 1, 16).half()
+    for shape in ((2 ** 31, 1, 1, 16), (2 ** 32 + 4, 1, 1, 16), (4, 2 ** 32 + 2, 1, 16)):
+        with pytest.raises(ValueError, match="too many"):
+            PagedKV(one.expand(shape), one.expand(shape))
+
+
 def append_args(N=2, H=4, kvh=2, D=64, B=2):
     return dict(q=torch.zeros(N, H, D).half(), k=torch.zeros(N, kvh, D).half(), v=torch.zeros(N, kvh, D).half(),
                 positions=torch.zeros(N, dtype=torch.int64), page_table=torch.zeros(B, 3, dtype=torch.int32),
