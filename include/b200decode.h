@@ -420,6 +420,82 @@ int b2d_paged_attention(const b2d_paged_kv* kv, const void* q, int64_t sq_b, int
                         void* out, int64_t so_b, int64_t so_t, int64_t so_h, int out_dtype,
                         void* workspace, size_t workspace_bytes, int flags, void* stream);
 
+/* ================================================================ page tables of a step
+ * Which page each new token of a step goes to, worked out on the device from the requests' lengths (no counterpart in
+ * the reference). State, owned by the caller: page_table [B, pages_per_seq] (row stride ld_table), held [B] = pages that
+ * each sequence holds (the entries before it), free_pages [num_pages] = a ring of the pages that nobody holds, ring =
+ * {index of the first, count}; all int32. cached / new_tokens [B] (int32, negative counts as 0): tokens that are cached,
+ * and those that the step adds. With want = cached + new, target = ceil(want / page_size), in the order of the sequences:
+ *   a sequence is refused where target > pages_per_seq, where its pages do not fit what the ring has left behind those of
+ *   the sequences before it (refused ones counted), or where its tokens do not fit max_tokens in the same way; it keeps
+ *   its state, and granted[b] = -1. Sequences that ask for no page (no token) are not refused for it.
+ *   the others take target - held pages from the ring's front, or put held - target back behind its end (the entries become
+ *   -1; they can be taken from the next call on). granted[b] = new.
+ * Tokens lie one behind another in the order of the sequences: token n of the starts[b + 1] - starts[b] granted ones of b has
+ * positions[n] = cached + its index, seq_ids[n] = b, slots[n] = page * page_size + positions[n] % page_size (-1 where the table's
+ * entry is outside [0, num_pages)); behind the last token up to max_tokens all three are -1, which the appends take for
+ * padding. seqlens[b] = want (cached, where refused); starts [B + 1]. positions and slots are int64, the rest is int32.
+ * B <= 8192; page_size 1..1024; num_pages, max_tokens and pages_per_seq * page_size < 2^31 - 1024. Entries are written only
+ * inside the arrays, whatever the state holds; page ids are handed on as they are. One launch; calls that share state
+ * must not overlap. flags: B2D_LAUNCH_PDL. */
+int b2d_page_plan(int32_t* page_table, int64_t ld_table, int pages_per_seq, int32_t* held, int32_t* free_pages,
+                  int num_pages, int32_t* ring, const int32_t* cached, const int32_t* new_tokens, int B, int page_size,
+                  int max_tokens, int64_t* positions, int32_t* seq_ids, int64_t* slots, int32_t* seqlens,
+                  int32_t* starts, int32_t* granted, int flags, void* stream);
+
+/* ================================================================ paged KV cache in 4 bits
+ * The paged cache above with keys and values in 4 bits (no counterpart in the reference). Per position, head and run of
+ * `group` elements x (fp32):
+ *   m = round16(min x), s = round16(max((max x - m) / 15, 0)), c = clamp(rint((x - m) / s), 0, 15) (0 where s = 0),
+ * round16 to dtype (F16 or BF16), the rest IEEE fp32; the entry stands for m + s c. A run with an infinity or a NaN (or whose
+ * m or s overflow) stands for NaN. A pool is num_pages x KVH blocks of b2d_int4_page_bytes bytes, block (page, head) at
+ * pages + page * sp_p + head * sp_h (bytes); inside it lie tiles of 16 positions in the order of the kernels' matrix
+ * fragments: 8 D bytes of key codes, 8 D of value codes, then per position and run {s, m} of the keys, then of the values.
+ * The order inside a tile is the library's own: b2d_int4_append writes it, b2d_int4_read gives the values back.
+ * D 64 or 128; group 32 or 64; page_size a multiple of 16 up to 1024; pages 16-byte aligned, strides multiples of 16.
+ * Page ids outside [0, num_pages) are never followed: nothing is written there, and reads give zeros.
+ * ================================================================================== */
+typedef struct {
+  uint8_t* pages;
+  int64_t sp_p, sp_h;
+  int num_pages, page_size, KVH, D, group, dtype;
+} b2d_int4_kv;
+
+/* Bytes of one (page, head) block; 0 for sizes that are not supported. */
+size_t b2d_int4_page_bytes(int page_size, int D, int group);
+
+/* b2d_paged_rope_append into a 4-bit cache, for more forms of the rotation. q [N, H, D] may be NULL (keys and values alone;
+ * q_out is then not used, H not read), and so may cos and sin (no rotation: keys that are rotated already). cos / sin [S_max, R / 2] (row stride
+ * ld_cs, cs_dtype F32 or the cache's): the first R elements of a head turn, R = rotary_dim, a multiple of 16 up to D, as the
+ * pairs (d, d + R / 2), or (2 d, 2 d + 1) where interleaved != 0; the others stay. Scaling for long contexts lies in the tables.
+ *   x' = x * r * weight, r = 1 / sqrt(mean(x^2) + eps);   (a, b) -> (a cos - b sin, b cos + a sin)
+ * Keys: r from 64-bit sums and every product and sum rounded to fp32 in this order, so that their codes are the formula's;
+ * they and the raw values are quantised from there. q: fp32, one rounding at the end. positions, seq_ids,
+ * page_table, weights, padding, aliasing of q_out: as b2d_paged_rope_append. 16-byte aligned pointers, strides % 8 == 0 (ld_cs: rows
+ * aligned to 16 bytes). */
+int b2d_int4_append(const b2d_int4_kv* kv, const void* q, int64_t sq_n, int64_t sq_h, const void* k, int64_t sk_n,
+                    int64_t sk_h, const void* v, int64_t sv_n, int64_t sv_h, const int64_t* positions,
+                    const int32_t* seq_ids, const int32_t* page_table, int64_t ld_table, int pages_per_seq, int B,
+                    const void* cos, const void* sin, int64_t ld_cs, int S_max, int cs_dtype, int rotary_dim,
+                    int interleaved, const void* q_weight, const void* k_weight, float eps, void* q_out, int64_t sqo_n,
+                    int64_t sqo_h, int N, int H, int flags, void* stream);
+
+/* The values of N cached positions, addressed as the append does: k_out / v_out [N, KVH, D] (strides in elements, % 8 == 0,
+ * 16-byte aligned; either may be NULL) = m + s c in out_dtype (the cache's, or F32). Padding (a sequence outside [0, B), a
+ * position outside the page table) is left as it is. */
+int b2d_int4_read(const b2d_int4_kv* kv, const int64_t* positions, const int32_t* seq_ids, const int32_t* page_table,
+                  int64_t ld_table, int pages_per_seq, int B, void* k_out, int64_t sk_n, int64_t sk_h, void* v_out,
+                  int64_t sv_n, int64_t sv_h, int out_dtype, int N, int flags, void* stream);
+
+/* b2d_paged_attention over a 4-bit cache (no shared prefix): arguments, masks, lengths, workspace and limits as there. q has
+ * the cache's dtype. Keys and values enter the products as codes (exact); a weight times its value's s is rounded to fp16
+ * (2^-11) for the second product, everything else is fp32. */
+size_t b2d_int4_attention_workspace_bytes(const b2d_int4_kv* kv, int B, int T, int H, int pages_per_seq, int max_len);
+int b2d_int4_attention(const b2d_int4_kv* kv, const void* q, int64_t sq_b, int64_t sq_t, int64_t sq_h,
+                       const int32_t* page_table, int64_t ld_table, int pages_per_seq, const int32_t* seqlens, int max_len,
+                       int B, int T, int H, float scale, void* out, int64_t so_b, int64_t so_t, int64_t so_h,
+                       int out_dtype, void* workspace, size_t workspace_bytes, int flags, void* stream);
+
 /* ================================================================ verification of drafted tokens
  * Speculative sampling (no counterpart in the reference, which decodes greedily one token at a time).
  * draft_tokens [B, K] (int64, row stride ld_tokens) were drawn from draft_probs [B, K, V] (strides sd_b,

@@ -40,6 +40,12 @@ class PagedKvDesc(C.Structure):
                 ("num_pages", _i32), ("page_size", _i32), ("KVH", _i32), ("D", _i32), ("dtype", _i32)]
 
 
+class Int4KvDesc(C.Structure):
+    """b2d_int4_kv (include/b200decode.h)."""
+    _fields_ = [("pages", _p), ("sp_p", _i64), ("sp_h", _i64), ("num_pages", _i32), ("page_size", _i32), ("KVH", _i32),
+                ("D", _i32), ("group", _i32), ("dtype", _i32)]
+
+
 # name -> (restype, argtypes); mirrors include/b200decode.h
 SIGNATURES = {
     "b2d_strerror": (C.c_char_p, [_i32]),
@@ -97,6 +103,17 @@ SIGNATURES = {
                                    _p, _sz, _i32, _p]),
     "b2d_verify_drafts": (_i32, [_p, _i64, _p, _p, _i64, _i64, _p, _i64, _i64, _i32, _p, _i64, _p, _i64, _p,
                                  _i32, _i32, _i32, _i32, _p]),
+    "b2d_page_plan": (_i32, [_p, _i64, _i32, _p, _p, _i32, _p, _p, _p, _i32, _i32, _i32, _p, _p, _p, _p, _p, _p, _i32,
+                             _p]),
+    "b2d_int4_page_bytes": (_sz, [_i32, _i32, _i32]),
+    "b2d_int4_append": (_i32, [C.POINTER(Int4KvDesc), _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _i64,
+                               _i32, _i32, _p, _p, _i64, _i32, _i32, _i32, _i32, _p, _p, _f32, _p, _i64, _i64, _i32,
+                               _i32, _i32, _p]),
+    "b2d_int4_read": (_i32, [C.POINTER(Int4KvDesc), _p, _p, _p, _i64, _i32, _i32, _p, _i64, _i64, _p, _i64, _i64, _i32,
+                             _i32, _i32, _p]),
+    "b2d_int4_attention_workspace_bytes": (_sz, [C.POINTER(Int4KvDesc), _i32, _i32, _i32, _i32, _i32]),
+    "b2d_int4_attention": (_i32, [C.POINTER(Int4KvDesc), _p, _i64, _i64, _i64, _p, _i64, _i32, _p, _i32, _i32, _i32,
+                                  _i32, _f32, _p, _i64, _i64, _i64, _i32, _p, _sz, _i32, _p]),
 }
 
 _lib = None
@@ -159,8 +176,8 @@ _binding = None
 
 
 def binding():
-    """The CPython module of csrc/binding.cpp (the checks and calls of the paged-cache and draft-verification
-    entry points), bound to the library's functions; raises if it has not been built, or for another torch."""
+    """The CPython module of csrc/binding.cpp (the checks and calls of the paged caches', page planning and draft
+    verification's entry points), bound to the library's functions; raises if it has not been built, or for another torch."""
     global _binding
     if _binding is None:
         import importlib.machinery
@@ -184,6 +201,8 @@ def binding():
         if built_for != f"b2d built for {host}":
             raise RuntimeError(f"{path} is {built_for}, not for {host}: {build}")
         module.bind(*(C.cast(getattr(lib, f), C.c_void_p).value for f in (
-            "b2d_paged_rope_append", "b2d_paged_attention_workspace_bytes", "b2d_paged_attention", "b2d_verify_drafts")))
+            "b2d_paged_rope_append", "b2d_paged_attention_workspace_bytes", "b2d_paged_attention", "b2d_verify_drafts",
+            "b2d_int4_append", "b2d_int4_read", "b2d_int4_attention_workspace_bytes", "b2d_int4_attention",
+            "b2d_page_plan")))
         _binding = module
     return _binding

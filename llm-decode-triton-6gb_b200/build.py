@@ -22,7 +22,8 @@ INCLUDE = REPO_ROOT / "include"
 LIB_PATH = PKG_ROOT / "b200kernels" / "libb200decode.so"
 BINDING_PATH = PKG_ROOT / "b200kernels" / "_binding.so"   # CPython module of csrc/binding.cpp
 SOURCES = ["capi.cu", "nf4_gemm.cu", "nf4_gemm_tma.cu", "nf4_tc5.cu", "nf4_format.cu", "gqa_decode.cu", "decode_glue.cu", "tp_allreduce.cu", "lm_head.cu",
-           "paged_append.cu", "paged_attention.cu", "paged_prefix.cu", "verify_drafts.cu"]
+           "paged_append.cu", "paged_attention.cu", "paged_prefix.cu", "verify_drafts.cu",
+           "int4_append.cu", "int4_attention.cu", "page_plan.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

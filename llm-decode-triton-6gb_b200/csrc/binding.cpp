@@ -1,4 +1,4 @@
-// CPython binding of the paged-cache and draft-verification calls: checks the tensors and calls the C ABI
+// CPython binding of the paged-cache (16 and 4 bits), page-planning and draft-verification calls: checks the tensors and calls the C ABI
 // (include/b200decode.h) through the function addresses that b200kernels/_lib.py took from libb200decode.so.
 //
 // These calls take few microseconds on the GPU, where the same checks in Python and the ctypes conversion of
@@ -26,6 +26,11 @@ decltype(&b2d_paged_rope_append) g_append = nullptr;
 decltype(&b2d_paged_attention_workspace_bytes) g_workspace = nullptr;
 decltype(&b2d_paged_attention) g_attention = nullptr;
 decltype(&b2d_verify_drafts) g_verify = nullptr;
+decltype(&b2d_int4_append) g_int4_append = nullptr;
+decltype(&b2d_int4_read) g_int4_read = nullptr;
+decltype(&b2d_int4_attention_workspace_bytes) g_int4_workspace = nullptr;
+decltype(&b2d_int4_attention) g_int4_attention = nullptr;
+decltype(&b2d_page_plan) g_plan = nullptr;
 
 struct TypeErr : std::runtime_error { using std::runtime_error::runtime_error; };
 struct ValueErr : std::runtime_error { using std::runtime_error::runtime_error; };
@@ -380,18 +385,286 @@ PyObject* verify(PyObject*, PyObject* const* a, Py_ssize_t na) {
   });
 }
 
+// ---- the cache in 4 bits
+const b2d_int4_kv* pool4(PyObject* o) { return static_cast<const b2d_int4_kv*>(PyLong_AsVoidPtr(o)); }
+at::ScalarType pool4_dtype(const b2d_int4_kv* kv) { return kv->dtype == B2D_F16 ? at::kHalf : at::kBFloat16; }
+// The pool that an append writes: no two blocks are one memory.
+void check_written_pool4(const b2d_int4_kv* kv, int64_t block) {
+  const int64_t sizes[3] = {kv->num_pages, kv->KVH, block}, strides[3] = {kv->sp_p, kv->sp_h, 1};
+  if (!nests(sizes, strides)) bad_value("the cache's pages overlap one another: an append would write them at once");
+}
+// positions, seq_ids and page_table of N tokens; returns the table's sequences
+int64_t check_addresses(const at::Tensor& positions, const at::Tensor* seq, const at::Tensor& table, int64_t N) {
+  check_vector(positions, "positions", at::kLong, N);
+  check_table(table, "page_table", 2);
+  const int64_t B = table.size(0);
+  if (seq) check_vector(*seq, "seq_ids", at::kInt, N);
+  else if (N > 0 && (B == 0 || N % B != 0))
+    bad_value(std::to_string(N) + " tokens do not divide over " + std::to_string(B) + " sequences: pass seq_ids");
+  return B;
+}
+
+// (desc, q, k, v, positions, page_table, cos, sin, interleaved, q_out, seq_ids, q_weight, k_weight, eps, flags, device index,
+// bytes of a block)
+PyObject* int4_append(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  return guarded([&]() -> PyObject* {
+    check_count(na, 17);
+    const b2d_int4_kv* kv = pool4(a[0]);
+    const at::Tensor *q = optional(a[1], "q"), *cos = optional(a[6], "cos"), *sin = optional(a[7], "sin");
+    const at::Tensor &k = tensor(a[2], "k"), &v = tensor(a[3], "v"), &positions = tensor(a[4], "positions"),
+                     &table = tensor(a[5], "page_table");
+    const at::Tensor *seq = optional(a[10], "seq_ids"), *qw = optional(a[11], "q_weight"), *kw = optional(a[12], "k_weight");
+    const at::ScalarType dt = pool4_dtype(kv);
+    const int interleaved = PyObject_IsTrue(a[8]);
+    if (interleaved < 0) throw PyErr();
+    if (k.dim() != 3) bad_value("k is [N, KVH, D], got " + show(k));
+    const int64_t N = k.size(0), D = kv->D;
+    check_shape(k, "k", {N, kv->KVH, D});
+    check_shape(v, "v", {N, kv->KVH, D});
+    if (q && (q->dim() != 3 || q->size(0) != N || q->size(2) != D || q->size(1) % kv->KVH != 0))
+      bad_value("q does not fit " + std::to_string(N) + " tokens of a cache of " + std::to_string(kv->KVH) + " heads of " +
+                std::to_string(D) + ": " + show(*q));
+    if ((q && q->scalar_type() != dt) || k.scalar_type() != dt || v.scalar_type() != dt)
+      throw TypeErr("q, k and v have the cache's dtype, got " + (q ? show(*q) + ", " : std::string()) + show(k) + ", " + show(v));
+    const int64_t B = check_addresses(positions, seq, table, N);
+    if (!cos != !sin) bad_value("cos and sin come together");
+    int64_t R = 0;
+    if (cos) {
+      R = cos->dim() == 2 ? 2 * cos->size(1) : 0;
+      if (R < 16 || R % 16 != 0 || R > D || cos->sizes() != sin->sizes() || cos->strides() != sin->strides())
+        bad_value("cos and sin are [S_max, R / 2] of one layout, R a multiple of 16 up to " + std::to_string(D) + "; got " + show(*cos) +
+                  ", " + show(*sin));
+      check_last(*cos, "cos and sin");
+      if (cos->scalar_type() != sin->scalar_type() || (cos->scalar_type() != dt && cos->scalar_type() != at::kFloat))
+        throw TypeErr("cos and sin are fp32 or have the cache's dtype, got " + show(*cos) + ", " + show(*sin));
+    }
+    for (const at::Tensor* w : {qw, kw})
+      if (w) check_vector(*w, "q_weight / k_weight", dt, D);
+    if (q) check_last(*q, "q");
+    check_last(k, "k");
+    check_last(v, "v");
+    const at::Device dev = k.device();
+    check_device(q, "q", dev); check_device(&v, "v", dev); check_device(&positions, "positions", dev);
+    check_device(&table, "page_table", dev); check_device(cos, "cos", dev); check_device(sin, "sin", dev);
+    check_device(seq, "seq_ids", dev); check_device(qw, "q_weight", dev); check_device(kw, "k_weight", dev);
+    if (!q && a[9] != Py_None) bad_value("q_out without q");
+    at::Tensor made;
+    if (q && a[9] == Py_None) made = at::empty(q->sizes(), q->options());
+    const at::Tensor* out = !q ? nullptr : a[9] == Py_None ? &made : &tensor(a[9], "q_out");
+    if (out) {
+      if (out->sizes() != q->sizes() || out->scalar_type() != dt) bad_value("q_out has q's shape and dtype, got " + show(*out));
+      check_last(*out, "q_out");
+      check_output(*out, "q_out");
+      check_device(out, "q_out", dev);
+    }
+    check_written_pool4(kv, integer(a[16]));
+    check_cuda(dev);
+    check_pool(dev, a[15]);
+    const OnDevice on(dev);
+    const int st = g_int4_append(
+        kv, ptr(q), q ? q->stride(0) : 0, q ? q->stride(1) : 0, k.const_data_ptr(), k.stride(0), k.stride(1), v.const_data_ptr(),
+        v.stride(0), v.stride(1), static_cast<const int64_t*>(positions.const_data_ptr()), static_cast<const int32_t*>(ptr(seq)),
+        static_cast<const int32_t*>(table.const_data_ptr()), table.stride(0), narrow(table.size(1), "page_table"),
+        narrow(B, "page_table"), ptr(cos), ptr(sin), cos ? cos->stride(0) : 0, cos ? narrow(cos->size(0), "cos") : 0,
+        cos ? code(cos->scalar_type()) : B2D_F32, static_cast<int>(R), interleaved, ptr(qw), ptr(kw), static_cast<float>(number(a[13])),
+        out ? out->mutable_data_ptr() : nullptr, out ? out->stride(0) : 0, out ? out->stride(1) : 0, narrow(N, "k"),
+        q ? narrow(q->size(1), "q") : 0, integer32(a[14], "flags"), on.stream);
+    if (st != B2D_OK) return PyLong_FromLong(st);
+    if (!q) Py_RETURN_NONE;
+    return a[9] == Py_None ? THPVariable_Wrap(made) : given(a[9]);
+  });
+}
+
+// (desc, positions, page_table, seq_ids, k_out, v_out, out_dtype, flags, device index); k_out, v_out: tensors, None to make
+// one, False to leave it out
+PyObject* int4_read(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  return guarded([&]() -> PyObject* {
+    check_count(na, 9);
+    const b2d_int4_kv* kv = pool4(a[0]);
+    const at::Tensor &positions = tensor(a[1], "positions"), &table = tensor(a[2], "page_table");
+    const at::Tensor* seq = optional(a[3], "seq_ids");
+    if (positions.dim() != 1) bad_value("positions is int64 [N], got " + show(positions));
+    const int64_t N = positions.size(0), B = check_addresses(positions, seq, table, N);
+    const at::Device dev = positions.device();
+    const at::ScalarType dt = pool4_dtype(kv);
+    at::ScalarType ot = out_type(a[6], dt);
+    if (a[6] == Py_None)   // that of a given output
+      for (int i : {4, 5})
+        if (a[i] != Py_None && a[i] != Py_False) ot = tensor(a[i], "k_out / v_out").scalar_type();
+    if (ot != dt && ot != at::kFloat) throw TypeErr("keys and values are read in fp32 or in the cache's dtype");
+    at::Tensor made[2];
+    const at::Tensor* out[2] = {nullptr, nullptr};
+    const char* const name[2] = {"k_out", "v_out"};
+    for (int i = 0; i < 2; ++i) {
+      if (a[4 + i] == Py_False) continue;
+      if (a[4 + i] == Py_None) {
+        made[i] = at::empty({N, kv->KVH, kv->D}, positions.options().dtype(ot));
+        out[i] = &made[i];
+      } else {
+        out[i] = &tensor(a[4 + i], name[i]);
+        check_shape(*out[i], name[i], {N, kv->KVH, kv->D});
+        if (out[i]->scalar_type() != ot) throw TypeErr(std::string(name[i]) + " has the dtype asked for, and that of the other; got " + show(*out[i]));
+        check_last(*out[i], name[i]);
+        check_output(*out[i], name[i]);
+        check_device(out[i], name[i], dev);
+      }
+    }
+    if (out[0] && out[1] && N > 0 && out[0]->const_data_ptr() == out[1]->const_data_ptr()) bad_value("k_out and v_out are one memory");
+    check_device(&table, "page_table", dev); check_device(seq, "seq_ids", dev);
+    check_cuda(dev);
+    check_pool(dev, a[8]);
+    const OnDevice on(dev);
+    const int st = g_int4_read(
+        kv, static_cast<const int64_t*>(positions.const_data_ptr()), static_cast<const int32_t*>(ptr(seq)),
+        static_cast<const int32_t*>(table.const_data_ptr()), table.stride(0), narrow(table.size(1), "page_table"),
+        narrow(B, "page_table"), out[0] ? out[0]->mutable_data_ptr() : nullptr, out[0] ? out[0]->stride(0) : 0,
+        out[0] ? out[0]->stride(1) : 0, out[1] ? out[1]->mutable_data_ptr() : nullptr, out[1] ? out[1]->stride(0) : 0,
+        out[1] ? out[1]->stride(1) : 0, code(ot), narrow(N, "positions"), integer32(a[7], "flags"), on.stream);
+    if (st != B2D_OK) return PyLong_FromLong(st);
+    PyObject* r[2];
+    for (int i = 0; i < 2; ++i) r[i] = a[4 + i] == Py_None ? THPVariable_Wrap(made[i]) : given(a[4 + i] == Py_False ? Py_None : a[4 + i]);
+    PyObject* both = PyTuple_Pack(2, r[0], r[1]);
+    Py_DECREF(r[0]);
+    Py_DECREF(r[1]);
+    return both;
+  });
+}
+
+// (desc, q, page_table, seqlens, scale, max_len, out, out_dtype, workspace, flags, device index)
+PyObject* int4_attention(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  return guarded([&]() -> PyObject* {
+    check_count(na, 11);
+    const b2d_int4_kv* kv = pool4(a[0]);
+    const at::Tensor &q = tensor(a[1], "q"), &table = tensor(a[2], "page_table"), &lens = tensor(a[3], "seqlens");
+    const at::ScalarType dt = pool4_dtype(kv);
+    if (q.dim() != 4) bad_value("q is [B, T, H, D], got " + show(q));
+    const int64_t B = q.size(0), T = q.size(1), H = q.size(2), D = q.size(3);
+    if (D != kv->D || H % kv->KVH != 0)
+      bad_value("q does not fit a cache of " + std::to_string(kv->KVH) + " heads of " + std::to_string(kv->D) + ": " + show(q));
+    if (q.scalar_type() != dt) throw TypeErr("q has the cache's dtype, got " + show(q));
+    check_table(table, "page_table", 2);
+    if (table.size(0) != B) bad_value("page_table has a row per sequence, got " + show(table) + " for " + show(q));
+    check_vector(lens, "seqlens", at::kInt, B);
+    const int max_len = integer32(a[5], "max_len");
+    const at::Device dev = q.device();
+    const at::ScalarType ot = out_type(a[7], dt);
+    at::Tensor made;
+    if (a[6] == Py_None) made = at::empty({B, T, H, D}, q.options().dtype(ot));
+    const at::Tensor& out = a[6] == Py_None ? made : tensor(a[6], "out");
+    if (out.sizes() != q.sizes() || (a[7] != Py_None && out.scalar_type() != ot) ||
+        (out.scalar_type() != dt && out.scalar_type() != at::kFloat))
+      bad_value("out has q's shape and is fp32 or of the cache's dtype (and of out_dtype), got " + show(out));
+    check_last(q, "q");
+    check_last(out, "out");
+    check_output(out, "out");
+    check_device(&table, "page_table", dev); check_device(&lens, "seqlens", dev); check_device(&out, "out", dev);
+    const at::Tensor* ws = optional(a[8], "workspace");
+    if (ws && !ws->is_contiguous()) bad_value("workspace is contiguous, got " + show(*ws));   // its bytes are counted below
+    check_device(ws, "workspace", dev);
+    check_cuda(dev);
+    check_pool(dev, a[10]);
+    const OnDevice on(dev);
+    const int per_seq = narrow(table.size(1), "page_table"), b = narrow(B, "q"), tn = narrow(T, "q"), h = narrow(H, "q");
+    at::Tensor scratch;
+    if (!ws) {
+      const size_t n = g_int4_workspace(kv, b, tn, h, per_seq, max_len);
+      if (n > 0) scratch = at::empty({static_cast<int64_t>(n)}, q.options().dtype(at::kByte));
+      ws = &scratch;
+    }
+    const bool has = ws->defined() && ws->numel() > 0;
+    const double scale = a[4] == Py_None ? 1.0 / std::sqrt(static_cast<double>(D)) : number(a[4]);
+    const int st = g_int4_attention(
+        kv, q.const_data_ptr(), q.stride(0), q.stride(1), q.stride(2), static_cast<const int32_t*>(table.const_data_ptr()),
+        table.stride(0), per_seq, static_cast<const int32_t*>(lens.const_data_ptr()), max_len, b, tn, h, static_cast<float>(scale),
+        out.mutable_data_ptr(), out.stride(0), out.stride(1), out.stride(2), code(out.scalar_type()),
+        has ? ws->mutable_data_ptr() : nullptr, has ? static_cast<size_t>(ws->nbytes()) : 0, integer32(a[9], "flags"), on.stream);
+    if (st != B2D_OK) return PyLong_FromLong(st);
+    return a[6] == Py_None ? THPVariable_Wrap(made) : given(a[6]);
+  });
+}
+
+// (desc, q, page_table, max_len) -> scratch for `int4_attention`
+PyObject* int4_workspace(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  return guarded([&]() -> PyObject* {
+    check_count(na, 4);
+    const at::Tensor &q = tensor(a[1], "q"), &table = tensor(a[2], "page_table");
+    if (q.dim() != 4) bad_value("q is [B, T, H, D], got " + show(q));
+    check_table(table, "page_table", 2);
+    check_cuda(q.device());
+    const OnDevice on(q.device());
+    const size_t n = g_int4_workspace(pool4(a[0]), narrow(q.size(0), "q"), narrow(q.size(1), "q"), narrow(q.size(2), "q"),
+                                      narrow(table.size(1), "page_table"), integer32(a[3], "max_len"));
+    return THPVariable_Wrap(at::empty({static_cast<int64_t>(n)}, q.options().dtype(at::kByte)));
+  });
+}
+
+// (page_table, held, free, ring, page_size, cached, new, positions, seq_ids, slots, seqlens, starts, granted, flags)
+PyObject* page_plan(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  return guarded([&]() -> PyObject* {
+    check_count(na, 14);
+    const at::Tensor &table = tensor(a[0], "page_table"), &held = tensor(a[1], "held"), &free = tensor(a[2], "free"),
+                     &ring = tensor(a[3], "ring"), &cached = tensor(a[5], "cached"), &fresh = tensor(a[6], "new"),
+                     &positions = tensor(a[7], "positions"), &seq = tensor(a[8], "seq_ids"), &slots = tensor(a[9], "slots"),
+                     &lens = tensor(a[10], "seqlens"), &starts = tensor(a[11], "starts"), &granted = tensor(a[12], "granted");
+    check_table(table, "page_table", 2);
+    check_output(table, "page_table");
+    const int64_t B = table.size(0);
+    if (positions.dim() != 1 || free.dim() != 1) bad_value("positions and free are vectors, got " + show(positions) + ", " + show(free));
+    const int64_t N = positions.size(0);
+    check_vector(held, "held", at::kInt, B);
+    check_vector(free, "free", at::kInt, free.size(0));
+    check_vector(ring, "ring", at::kInt, 2);
+    check_vector(cached, "cached", at::kInt, B);
+    check_vector(fresh, "new", at::kInt, B);
+    check_vector(positions, "positions", at::kLong, N);
+    check_vector(seq, "seq_ids", at::kInt, N);
+    check_vector(slots, "slots", at::kLong, N);
+    check_vector(lens, "seqlens", at::kInt, B);
+    check_vector(starts, "starts", at::kInt, B + 1);
+    check_vector(granted, "granted", at::kInt, B);
+    const at::Device dev = table.device();
+    const at::Tensor* const written[] = {&table, &held, &free, &ring, &positions, &seq, &slots, &lens, &starts, &granted};
+    const char* const names[] = {"page_table", "held", "free", "ring", "positions", "seq_ids", "slots", "seqlens", "starts", "granted"};
+    for (int i = 0; i < 10; ++i) {
+      check_device(written[i], names[i], dev);
+      for (int j = 0; j < i; ++j)
+        if (written[i]->numel() > 0 && written[j]->numel() > 0 && written[i]->const_data_ptr() == written[j]->const_data_ptr())
+          bad_value(std::string(names[i]) + " and " + names[j] + " are one memory");
+      for (const at::Tensor* in : {&cached, &fresh})
+        if (written[i]->numel() > 0 && in->numel() > 0 && written[i]->const_data_ptr() == in->const_data_ptr())
+          bad_value(std::string(names[i]) + " is written while the lengths are read: they are one memory");
+    }
+    check_device(&cached, "cached", dev); check_device(&fresh, "new", dev);
+    check_cuda(dev);
+    const OnDevice on(dev);
+    auto i32 = [](const at::Tensor& t) { return static_cast<int32_t*>(t.mutable_data_ptr()); };
+    auto i64 = [](const at::Tensor& t) { return static_cast<int64_t*>(t.mutable_data_ptr()); };
+    const int st = g_plan(i32(table), B > 1 ? table.stride(0) : table.size(1), narrow(table.size(1), "page_table"), i32(held), i32(free),
+                          narrow(free.size(0), "free"), i32(ring), static_cast<const int32_t*>(cached.const_data_ptr()),
+                          static_cast<const int32_t*>(fresh.const_data_ptr()), narrow(B, "page_table"), integer32(a[4], "page_size"),
+                          narrow(N, "positions"), i64(positions), i32(seq), i64(slots), i32(lens), i32(starts), i32(granted),
+                          integer32(a[13], "flags"), on.stream);
+    return PyLong_FromLong(st);
+  });
+}
+
 // build.py looks for this text in the module, b200kernels/_lib.py asks for it before the first call.
 const char kBuiltFor[] = "b2d built for " B2D_HOST_TAG;
 PyObject* built_for(PyObject*, PyObject* const*, Py_ssize_t) { return PyUnicode_FromString(kBuiltFor); }
 
-// the addresses of the four entry points, in the order of the globals above
+// the addresses of the entry points, in the order of the globals above
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t na) {
   return guarded([&]() -> PyObject* {
-    check_count(na, 4);
+    check_count(na, 9);
     g_append = reinterpret_cast<decltype(g_append)>(PyLong_AsVoidPtr(a[0]));
     g_workspace = reinterpret_cast<decltype(g_workspace)>(PyLong_AsVoidPtr(a[1]));
     g_attention = reinterpret_cast<decltype(g_attention)>(PyLong_AsVoidPtr(a[2]));
     g_verify = reinterpret_cast<decltype(g_verify)>(PyLong_AsVoidPtr(a[3]));
+    g_int4_append = reinterpret_cast<decltype(g_int4_append)>(PyLong_AsVoidPtr(a[4]));
+    g_int4_read = reinterpret_cast<decltype(g_int4_read)>(PyLong_AsVoidPtr(a[5]));
+    g_int4_workspace = reinterpret_cast<decltype(g_int4_workspace)>(PyLong_AsVoidPtr(a[6]));
+    g_int4_attention = reinterpret_cast<decltype(g_int4_attention)>(PyLong_AsVoidPtr(a[7]));
+    g_plan = reinterpret_cast<decltype(g_plan)>(PyLong_AsVoidPtr(a[8]));
     if (PyErr_Occurred()) throw PyErr();
     Py_RETURN_NONE;
   });
@@ -400,6 +673,9 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t na) {
 #define FAST(name) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr
 PyMethodDef kMethods[] = {{"rope_append", FAST(rope_append)}, {"attention", FAST(attention)},
                           {"attention_workspace", FAST(attention_workspace)}, {"verify", FAST(verify)},
+                          {"int4_append", FAST(int4_append)}, {"int4_read", FAST(int4_read)},
+                          {"int4_attention", FAST(int4_attention)}, {"int4_workspace", FAST(int4_workspace)},
+                          {"page_plan", FAST(page_plan)},
                           {"bind", FAST(bind)}, {"built_for", FAST(built_for)}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1,0 +1,823 @@
+// Attention of the newest tokens of every sequence over the paged cache in 4 bits, causal among themselves (sm_100a). The
+// layout is in int4_kv.cuh, the 16-bit counterpart in paged_attention.cu.
+//
+//   k = m + s c, so q.k = sum over runs (s sum q c + m sum q): the products are with the codes, and a key's two factors per run
+//   enter its score in fp32 behind them. o = sum_j p_j v_j = sum_j (p_j s_j) c_j + sum_j p_j m_j: a value's s goes into its
+//   weight (per run of elements), the second sum is fp32 and has one term per key, row and run.
+//
+// Codes become operands by masks (fp16 subnormals, see int4_kv.cuh): 5 instructions for 8 elements. Products are transposed as
+// in the 16-bit kernel: keys (elements) as M, rows as N tiles of 8, where a row is one of the T x G query vectors that read a
+// KV head.
+//  * A query row is scaled by a power of two into [2^14, 2^15) so that it and its part for the high nibbles (2^-4) are as
+//    exact in fp16 as in its own type.
+//  * A weight p_j s_j is rounded to fp16 (2^-11) around the largest s that the warp has seen: 2^(7 - E) p s lies below 2^15
+//    with p <= 2^8 and s <= 2^E, and down to 2^-21 of the largest it keeps all 11 bits. E and the running maximum move rarely
+//    (a maximum only when a score exceeds it by 2^8), on one vote.
+//  * Every warp is on its own: it copies its tiles of 16 keys (2.3 KB, keys, values and factors in one asynchronous bulk copy)
+//    through a private ring of shared memory, waits on its own mbarriers, and meets the block's other warps only at the end
+//    of a unit. Codes are finite whatever a page holds; factors of keys that a row does not see are taken out by selection.
+//
+// Units of work are (sequence, KV head, tile of up to 32 rows). As in the 16-bit kernel the units' stages (64 keys, a
+// tile a warp) form one line of which every block takes an equal share, found from the lengths on the device; parts of a unit
+// that several blocks share meet in a combine launch. No atomics: results are the same bits every run.
+#include "int4_kv.cuh"
+#include "pipeline.cuh"
+
+namespace b2d {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kStage = kWarps * kTileKeys;      // keys of a position of the line
+constexpr int kMaxT = 16, kMaxG = 16;
+constexpr int kMaxBatch = 256;                  // sequences of a launch (larger batches take several)
+constexpr int kMaxCtas = 640;
+constexpr float kLazy = 8.f;                    // log2 of the largest weight before the running maximum moves
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Blocks of an SM, by registers (accumulators: 32 a row tile), and tiles of a warp's ring, by shared memory.
+template <int NT>
+constexpr int kBlocks = NT == 1 ? 4 : NT == 2 ? 3 : 2;
+template <int D, int RUNS, int NT>
+struct Smem {
+  static constexpr int TILE = int4_tile_bytes(D, RUNS);
+  static constexpr int MERGE = kWarps * 8 * (D + 4) * 4;
+  static constexpr int Q = NT * (D / 16) * 32 * 8;              // prepared fragments
+  static constexpr int FIXED = MERGE + Q + 2048;                // and the static arrays
+  static constexpr int ROOM = 224 * 1024 / kBlocks<NT> - FIXED;
+  static constexpr int SLOTS = ROOM / (kWarps * TILE) < 8 ? ROOM / (kWarps * TILE) : 8;
+  static constexpr int RING = kWarps * SLOTS * TILE;
+  static constexpr int BYTES = RING + MERGE + Q;
+};
+
+struct Int4AttnArgs {
+  const void* q; int64_t sq_b, sq_t, sq_h;
+  const int32_t* table; int64_t ld_table;
+  const int32_t* seqlens;
+  void* out; int64_t so_b, so_t, so_h;
+  b2d_int4_kv kv;
+  PageDiv div;
+  int pages_per_seq, B, T, H, G, rows;   // rows = T G: query vectors of a sequence and KV head
+  int inv_g;        // 2^16 / G, rounded up
+  float scale_log2;
+  int ctas, whole, out_f32, out_vec;
+  // Workspace: [ctas][2][row tile] entries of D unnormalised fp32 sums, and (m in the log2 domain, l)
+  float* acc;
+  float* ml;
+};
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(dst), "l"(src),
+               "r"(bytes), "r"(bar) : "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ void store_out(const Int4AttnArgs& a, int64_t off, float v) {
+  if (a.out_f32) static_cast<float*>(a.out)[off] = v;
+  else static_cast<T*>(a.out)[off] = Dt<T>::from_f32(v);
+}
+// two neighbouring outputs; `out_vec`: every row starts on a boundary of their size
+template <typename T>
+__device__ __forceinline__ void store_out2(const Int4AttnArgs& a, int64_t off, float x, float y) {
+  if (!a.out_vec) {
+    store_out<T>(a, off, x);
+    store_out<T>(a, off + 1, y);
+  } else if (a.out_f32) {
+    *reinterpret_cast<float2*>(static_cast<float*>(a.out) + off) = make_float2(x, y);
+  } else {
+    *reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + off) = Dt<T>::pack2(x, y);
+  }
+}
+
+// The line of all units' work: the sequences in order, KV head by KV head and row tile by row tile. A unit takes LEAD
+// positions, what its start and end cost in stages, and one for each stage; one without keys takes none. CTA c takes the
+// positions [share(c), share(c + 1)); the host has checked that they fit 31 bits. In whole mode a unit is one position.
+template <int NT>
+struct Line {
+  static constexpr int ROWS = 8 * NT, LEAD = 3;
+  int tiles, units, ctas, quota, extra;
+  __device__ __forceinline__ Line(const Int4AttnArgs& a) {
+    tiles = (a.rows + ROWS - 1) / ROWS;
+    units = a.kv.KVH * tiles;
+  }
+  static __device__ __forceinline__ int cost_of(const Int4AttnArgs& a, int len) {
+    return a.whole ? 1 : len > 0 ? (len + kStage - 1) / kStage + LEAD : 0;
+  }
+  __device__ __forceinline__ void close(const Int4AttnArgs& a, int cost) {   // of all sequences
+    const int total = cost * units;
+    ctas = min(total, a.ctas);   // the CTAs with a share, none of them empty
+    quota = ctas > 0 ? total / ctas : 0;
+    extra = total - quota * ctas;   // so many CTAs take one position more
+  }
+  __device__ __forceinline__ int share(int c) const { return c < ctas ? c * quota + min(c, extra) : ctas * quota + extra; }
+  __device__ __forceinline__ int owner(int x) const {
+    const int cut = extra * (quota + 1);
+    return x < cut ? x / (quota + 1) : extra + (x - cut) / quota;
+  }
+};
+
+// The sequences' lengths, cut to the page table, into s_len and the exclusive running sums of their units' cost into
+// s_sum[0 .. B] (all THREADS of the block take part).
+template <int NT, int THREADS>
+__device__ __forceinline__ void scan_costs(const Int4AttnArgs& a, int* s_sum, int* s_len, int* s_warp) {
+  constexpr int W = THREADS / 32;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int reach = a.pages_per_seq * a.kv.page_size;
+  int run = 0;
+  for (int b0 = 0; b0 < a.B; b0 += THREADS) {
+    const int b = b0 + tid;
+    const int len = b < a.B ? min(max(a.seqlens[b], 0), reach) : 0;
+    const int own = b < a.B ? Line<NT>::cost_of(a, len) : 0;
+    int v = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += up;
+    }
+    if (lane == 31) s_warp[warp] = v;
+    __syncthreads();
+    int before = run;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      if (w < warp) before += s_warp[w];
+      run += s_warp[w];
+    }
+    if (b < a.B) {
+      s_sum[b] = before + v - own;
+      s_len[b] = len;
+    }
+    __syncthreads();
+  }
+  if (tid == 0) s_sum[a.B] = run;
+  __syncthreads();
+}
+
+// A CTA's stretch of one unit: keys [t_begin, t_end).
+struct Segment {
+  int b, kvh, row0, nrows;
+  int t_begin, t_end, limit;     // query t sees the keys before limit + t
+  int kind;                      // 0: the whole unit, 1 / 2: the end (or middle) / the start of a shared one, < 0: none
+  int next;                      // position behind it
+};
+// The segment at position pos of a share that ends at `end`; none where only a unit's lead lies in the share.
+template <int NT>
+__device__ __forceinline__ Segment segment_at(const Int4AttnArgs& a, const Line<NT>& line, const int* s_sum,
+                                              const int* s_len, int pos, int end) {
+  constexpr int ROWS = 8 * NT, LEAD = Line<NT>::LEAD;
+  Segment g;
+  int lo = 0, hi = a.B - 1;   // the last sequence that starts at or before pos
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (s_sum[mid] * line.units <= pos) lo = mid;
+    else hi = mid - 1;
+  }
+  g.b = lo;
+  const int len = s_len[lo], cost = s_sum[lo + 1] - s_sum[lo];
+  int start = s_sum[lo] * line.units;
+  const int u = (pos - start) / cost;
+  start += u * cost;
+  g.limit = len - a.T + 1;
+  g.kvh = line.tiles == 1 ? u : u / line.tiles;
+  g.row0 = (u - g.kvh * line.tiles) * ROWS;
+  g.nrows = min(a.rows - g.row0, ROWS);
+  g.next = min(end, start + cost);
+  if (a.whole) {
+    g.t_begin = 0;
+    g.t_end = len;
+    g.kind = 0;
+  } else {
+    const int s0 = max(pos - start - LEAD, 0), s1 = g.next - start - LEAD;
+    g.t_begin = s0 * kStage;
+    g.t_end = min(len, s1 * kStage);
+    g.kind = s1 <= s0 ? -1 : s0 > 0 ? 1 : s1 < cost - LEAD ? 2 : 0;
+  }
+  return g;
+}
+
+__device__ __forceinline__ int div_g(const Int4AttnArgs& a, int r) { return r * a.inv_g >> 16; }   // r < 256, G <= 16: exact
+
+template <typename T, int D, int RUNS, int NT>
+__global__ void __launch_bounds__(kThreads, kBlocks<NT>) int4_attention_kernel(const __grid_constant__ Int4AttnArgs a) {
+  using S = Smem<D, RUNS, NT>;
+  constexpr int ROWS = 8 * NT, STEPS = D / 16, RSTEPS = STEPS / RUNS;   // products of a tile, and of a run of elements
+  constexpr int TILE = S::TILE, SLOTS = S::SLOTS, KW = D / 32;          // KW: key words of a lane and key
+  static_assert(SLOTS >= 2, "a ring of at least two tiles");
+  constexpr bool Q_REGS = NT <= 2;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float s_m[kWarps][ROWS], s_l[kWarps][ROWS];
+  __shared__ float s_rowf[ROWS], s_qs[RUNS][ROWS];
+  __shared__ __align__(8) uint64_t s_bar[kWarps * SLOTS];
+  __shared__ int s_sum[kMaxBatch + 1], s_len[kMaxBatch], s_warp[kWarps];
+  __shared__ int64_t s_at[ROWS];        // per row: offset in the output, or workspace entry
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g8 = lane >> 2, tq = lane & 3;
+  uint8_t* const ring = smem + warp * (SLOTS * TILE);
+  float* const s_o = reinterpret_cast<float*>(smem + S::RING);
+  uint2* const s_q = reinterpret_cast<uint2*>(smem + S::RING + S::MERGE);   // [row tile][step][lane]
+  const uint32_t ring_s = smem_u32(ring), full = smem_u32(s_bar + warp * SLOTS);
+  if (lane < SLOTS) mbar_init(full + 8 * lane, 1);
+  fence_mbar_init();
+  pdl_wait();
+  pdl_launch_dependents();
+  const Line<NT> line = [&] {
+    Line<NT> l(a);
+    scan_costs<NT, kThreads>(a, s_sum, s_len, s_warp);
+    l.close(a, s_sum[a.B]);
+    return l;
+  }();
+  const int first = line.share(blockIdx.x), end = line.share(blockIdx.x + 1);
+
+  // ---- the warp's copies, ahead of its products: tile `ft` of `fg` next, of the warp's `fn` there
+  int fpos = first, ft = 0, fn = 0, sent = 0, page = 0;
+  Segment fg;
+  fg.next = first;
+  // page of the warp's tile ft0 + lane
+  auto lookup = [&](int ft0) {
+    const int key = fg.t_begin + ((ft0 + lane) * kWarps + warp) * kTileKeys;
+    return key < fg.t_end ? __ldg(a.table + fg.b * a.ld_table + a.div.page(key)) : -1;
+  };
+  auto fetch = [&]() {   // the next tile, if any; its slot is free
+    while (ft >= fn) {
+      if (fpos >= end) return;
+      fg = segment_at<NT>(a, line, s_sum, s_len, fpos, end);
+      fpos = fg.next;
+      ft = 0;
+      const int tiles = fg.kind < 0 ? 0 : (fg.t_end - fg.t_begin + kTileKeys - 1) / kTileKeys;
+      fn = tiles > warp ? (tiles - warp + kWarps - 1) / kWarps : 0;
+      if (fn > 0) page = lookup(0);
+    }
+    if (ft > 0 && (ft & 31) == 0) page = lookup(ft);
+    const int p = __shfl_sync(0xffffffffu, page, ft & 31), slot = sent % SLOTS;
+    if (p >= 0 && p < a.kv.num_pages) {
+      if (lane == 0) {
+        const int key = fg.t_begin + (ft * kWarps + warp) * kTileKeys;
+        const int in_page = a.div.slot(key, a.div.page(key)) / kTileKeys;
+        mbar_expect_tx(full + 8 * slot, TILE);
+        bulk_load(ring_s + slot * TILE, a.kv.pages + p * a.kv.sp_p + fg.kvh * a.kv.sp_h + static_cast<int64_t>(in_page) * TILE,
+                  TILE, full + 8 * slot);
+      }
+    } else {   // a page id outside the pool: keys and values of zeros
+      for (int i = lane; i < TILE / 16; i += 32) *reinterpret_cast<uint4*>(ring + slot * TILE + 16 * i) = make_uint4(0, 0, 0, 0);
+      fence_proxy_async();   // the slot's next copy comes after these writes
+      __syncwarp();
+      if (lane == 0) mbar_arrive(full + 8 * slot);
+    }
+    ++ft;
+    ++sent;
+  };
+#pragma unroll 1
+  for (int i = 0; i < SLOTS; ++i) fetch();
+
+  int it = 0;            // the warp's tiles so far
+  bool landed = true;
+  for (int pos = first; pos < end;) {
+    const Segment g = segment_at<NT>(a, line, s_sum, s_len, pos, end);
+    pos = g.next;
+    if (g.kind < 0) continue;
+    // ---- Q: warp n prepares row tile n (every thread is behind the last unit's barriers)
+    for (int n = warp; n < NT; n += kWarps) {
+      const int r = 8 * n + g8, rr = g.row0 + r, t = div_g(a, rr);
+      const bool on = r < g.nrows;
+      const T* src = static_cast<const T*>(a.q) + g.b * a.sq_b + t * a.sq_t + static_cast<int64_t>(g.kvh * a.G + rr - t * a.G) * a.sq_h + 4 * tq;
+      uint2 raw[STEPS];
+#pragma unroll
+      for (int j = 0; j < STEPS; ++j) raw[j] = on ? __ldg(reinterpret_cast<const uint2*>(src + 16 * j)) : make_uint2(0, 0);
+      float big = 0.f;
+      auto value = [&](int j, int e) { return Dt<T>::to_f32(reinterpret_cast<const T*>(&raw[j])[e]); };
+#pragma unroll
+      for (int j = 0; j < STEPS; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) big = fmaxf(big, fabsf(value(j, e)));
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+      // up = 2^x with 2^x big in [2^14, 2^15); |x| <= 100
+      const int ex = static_cast<int>(__float_as_uint(big) >> 23);
+      const int x = big > 0.f && ex < 255 ? min(max(14 + 127 - ex, -100), 100) : 0;
+      const float up = __uint_as_float((127 + x) << 23), down = __uint_as_float((127 - x) << 23);
+      float qs[RUNS];
+#pragma unroll
+      for (int u = 0; u < RUNS; ++u) qs[u] = 0.f;
+#pragma unroll
+      for (int j = 0; j < STEPS; ++j) {
+        const float q0 = value(j, 0) * up, q1 = value(j, 1) * up, q2 = value(j, 2) * up, q3 = value(j, 3) * up;
+        const __half2 lo = __floats2half2_rn(q0, q1), hi = __floats2half2_rn(q2, q3);
+        qs[j / RSTEPS] += (__low2float(lo) + __high2float(lo)) + (__low2float(hi) + __high2float(hi));
+        s_q[(n * STEPS + j) * 32 + lane] = make_uint2(Dt<__half>::pack2(q0, q1), Dt<__half>::pack2(q2 * 0.0625f, q3 * 0.0625f));
+      }
+#pragma unroll
+      for (int u = 0; u < RUNS; ++u) {
+        qs[u] += __shfl_xor_sync(0xffffffffu, qs[u], 1);
+        qs[u] += __shfl_xor_sync(0xffffffffu, qs[u], 2);
+        if (tq == 0) s_qs[u][r] = qs[u] * 0x1p-24f;
+      }
+      if (tq == 0) s_rowf[r] = down * 0x1p24f * a.scale_log2;
+    }
+    if (tid < g.nrows) {
+      const int rr = g.row0 + tid, t = div_g(a, rr), head = g.kvh * a.G + rr - t * a.G;
+      s_at[tid] = g.kind == 0 ? g.b * a.so_b + t * a.so_t + head * a.so_h
+                              : (static_cast<int64_t>(blockIdx.x) * 2 + (g.kind - 1)) * ROWS + tid;
+    }
+    __syncthreads();
+    uint2 qb[Q_REGS ? NT : 1][STEPS];   // row 8 n + g8, elements 16 j + 4 tq ..
+    if constexpr (Q_REGS) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < STEPS; ++j) qb[n][j] = s_q[(n * STEPS + j) * 32 + lane];
+    }
+    float rowf[NT][2], qs[RUNS][NT][2];   // of rows 8 n + 2 tq (+ 1)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        rowf[n][e] = s_rowf[8 * n + 2 * tq + e];
+#pragma unroll
+        for (int u = 0; u < RUNS; ++u) qs[u][n][e] = s_qs[u][8 * n + 2 * tq + e];
+      }
+    // keys that this thread's rows see; below lim_min no row is masked
+    const bool causal = a.T > 1;
+    const int lim_min = causal ? g.limit + div_g(a, g.row0) : g.limit;
+    auto lim = [&](int n, int e) { return causal ? g.limit + div_g(a, g.row0 + min(8 * n + 2 * tq + e, g.nrows - 1)) : g.limit; };
+
+    float o[STEPS][NT][4];   // element 16 m + g8 (+ 8), row 8 n + 2 tq (+ 1), in units of 2^(E - 7 - 24) (2^(E - 7 - 20))
+    float om[RUNS][NT][2];   // sum of p m over this thread's keys
+    float m_run[NT][2], l_run[NT][2];   // log2 domain; the sum over this thread's keys only
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int m = 0; m < STEPS; ++m) o[m][n][0] = o[m][n][1] = o[m][n][2] = o[m][n][3] = 0.f;
+#pragma unroll
+      for (int u = 0; u < RUNS; ++u) om[u][n][0] = om[u][n][1] = 0.f;
+      m_run[n][0] = m_run[n][1] = -INFINITY;
+      l_run[n][0] = l_run[n][1] = 0.f;
+    }
+    float v_top = 0.f, v_unit = 1.f;   // 2^E and 2^(7 - E); v_top = 0: no value yet
+
+    const int tiles = (g.t_end - g.t_begin + kTileKeys - 1) / kTileKeys;
+#pragma unroll 1
+    for (int tile = warp; tile < tiles; tile += kWarps, ++it) {
+      const int slot = it % SLOTS, key0 = g.t_begin + tile * kTileKeys;
+      landed = landed && mbar_wait(full + 8 * slot, (it / SLOTS) & 1);
+      const uint8_t* const buf = ring + slot * TILE;
+      float acc[RUNS][NT][4];   // key g8 (+ 8), row 8 n + 2 tq (+ 1)
+      {
+        uint32_t kw[2][KW];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint8_t* p = buf + (g8 + 8 * h) * (D / 2) + tq * (D / 8);
+          if constexpr (KW == 4) {
+            const uint4 x = *reinterpret_cast<const uint4*>(p);
+            kw[h][0] = x.x; kw[h][1] = x.y; kw[h][2] = x.z; kw[h][3] = x.w;
+          } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(p);
+            kw[h][0] = x.x; kw[h][1] = x.y;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < STEPS; ++j) {
+          const int sh = 8 * (j & 1), u = j / RSTEPS;
+          const uint32_t x = kw[0][j / 2] >> sh, y = kw[1][j / 2] >> sh;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const uint2 q = Q_REGS ? qb[Q_REGS ? n : 0][j] : s_q[(n * STEPS + j) * 32 + lane];
+            if (j % RSTEPS == 0) Mma<__half>::run0(acc[u][n], x & 0x000F000Fu, y & 0x000F000Fu, x & 0x00F000F0u, y & 0x00F000F0u, q.x, q.y);
+            else Mma<__half>::run(acc[u][n], x & 0x000F000Fu, y & 0x000F000Fu, x & 0x00F000F0u, y & 0x00F000F0u, q.x, q.y);
+          }
+        }
+      }
+      // scores: p holds x - m_run, then the weights
+      float p[NT][4];
+      {
+        float2 f[2][RUNS];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int u = 0; u < RUNS; ++u)
+            f[h][u] = unpack_sm<T>(*reinterpret_cast<const uint32_t*>(buf + int4_ks_off(D) + ((g8 + 8 * h) * RUNS + u) * 4));
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int h = c >> 1, e = c & 1;
+            float x = 0.f;
+#pragma unroll
+            for (int u = 0; u < RUNS; ++u) {
+              x = u == 0 ? f[h][u].x * acc[u][n][c] : fmaf(f[h][u].x, acc[u][n][c], x);
+              x = fmaf(f[h][u].y, qs[u][n][e], x);
+            }
+            p[n][c] = x * rowf[n][e];
+          }
+      }
+      float2 vf[2][RUNS];   // the values' factors of keys g8 (+ 8)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int u = 0; u < RUNS; ++u)
+          vf[h][u] = unpack_sm<T>(*reinterpret_cast<const uint32_t*>(buf + int4_vs_off(D, RUNS) + ((g8 + 8 * h) * RUNS + u) * 4));
+      const bool masked = key0 + kTileKeys > min(lim_min, g.t_end);
+      if (masked) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int key = key0 + g8 + 8 * h;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if (key >= lim(n, e) || key >= g.t_end) p[n][2 * h + e] = -INFINITY;
+          if (key >= g.t_end) {   // what lies behind the last key is not the cache's
+#pragma unroll
+            for (int u = 0; u < RUNS; ++u) vf[h][u] = make_float2(0.f, 0.f);
+          }
+        }
+      }
+      float s_top = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int u = 0; u < RUNS; ++u) s_top = fmaxf(s_top, vf[h][u].x);
+      bool move = s_top > v_top;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) move |= fmaxf(p[n][e], p[n][2 + e]) > m_run[n][e] + kLazy;
+      if (__any_sync(0xffffffffu, move)) {
+        const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(s_top));
+        float keep = 1.f;
+        if (__uint_as_float(bits) > v_top) {   // 2^E with room for twice the largest s; E in [-110, 110]
+          const int ex = min(max(static_cast<int>(bits >> 23) - 127 + 2, -110), 110);
+          const float unit = __uint_as_float((127 + 7 - ex) << 23);
+          keep = v_top > 0.f ? unit / v_unit : 1.f;
+          v_top = __uint_as_float((127 + ex) << 23);
+          v_unit = unit;
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float top = fmaxf(p[n][e], p[n][2 + e]);
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+            const bool up = top > m_run[n][e] + kLazy;
+            const float alpha = up ? exp2_fast(m_run[n][e] - top) : 1.f;   // m_run = -inf: 0
+            if (up) m_run[n][e] = top;
+            l_run[n][e] *= alpha;
+#pragma unroll
+            for (int u = 0; u < RUNS; ++u) om[u][n][e] *= alpha;
+#pragma unroll
+            for (int m = 0; m < STEPS; ++m) {
+              o[m][n][e] *= alpha * keep;
+              o[m][n][2 + e] *= alpha * keep;
+            }
+          }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float mr = m_run[n][c & 1];
+          p[n][c] = exp2_fast(p[n][c] - (mr == -INFINITY ? 0.f : mr));
+          l_run[n][c & 1] += p[n][c];
+        }
+      uint32_t pb[RUNS][NT][2];   // P s as the B operand: row 8 n + g8, keys 2 tq .. (+ 8)
+#pragma unroll
+      for (int u = 0; u < RUNS; ++u) {
+        const float s0 = vf[0][u].x * v_unit, s1 = vf[1][u].x * v_unit;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float w[4] = {p[n][0] * s0, p[n][1] * s0, p[n][2] * s1, p[n][3] * s1};
+          float b[4] = {p[n][0] * vf[0][u].y, p[n][1] * vf[0][u].y, p[n][2] * vf[1][u].y, p[n][3] * vf[1][u].y};
+          if (masked) {   // factors that are infinite or NaN reach the rows that see their key, and no other
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              if (key0 + g8 + 8 * (c >> 1) >= lim(n, c & 1)) w[c] = b[c] = 0.f;
+          }
+          om[u][n][0] += b[0] + b[2];
+          om[u][n][1] += b[1] + b[3];
+          pb[u][n][0] = transpose8(Dt<__half>::pack2(w[0], w[1]));
+          pb[u][n][1] = transpose8(Dt<__half>::pack2(w[2], w[3]));
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) {
+        const uint4 vw = *reinterpret_cast<const uint4*>(buf + int4_v_off(D) + c * 512 + lane * 16);
+        const uint32_t w4[4] = {vw.x, vw.y, vw.z, vw.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int m = 4 * c + i, u = m / RSTEPS;
+          const uint32_t x = w4[i], y = x >> 8;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+            Mma<__half>::run(o[m][n], x & 0x000F000Fu, x & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u, pb[u][n][0], pb[u][n][1]);
+        }
+      }
+      __syncwarp();   // the warp is done with the slot
+      fetch();
+    }
+
+    // ---- the unit's (or this CTA's part of it) result: the warps meet in shared memory
+    const float to_lo = 0x1p24f / v_unit, to_hi = 0x1p20f / v_unit;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) {
+          l_run[n][e] += __shfl_xor_sync(0xffffffffu, l_run[n][e], x);
+#pragma unroll
+          for (int u = 0; u < RUNS; ++u) om[u][n][e] += __shfl_xor_sync(0xffffffffu, om[u][n][e], x);
+        }
+        if (g8 == 0) {
+          s_m[warp][8 * n + 2 * tq + e] = m_run[n][e];
+          s_l[warp][8 * n + 2 * tq + e] = landed ? l_run[n][e] : NAN;
+        }
+      }
+    __syncthreads();
+    if (tid < g.nrows) {   // (m, l) of a row, and the warps' factors in the place of their maxima
+      float mx = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, s_m[w][tid]);
+      float f[kWarps];
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        f[w] = s_m[w][tid] == -INFINITY ? 0.f : exp2_fast(s_m[w][tid] - mx);
+        l += f[w] * s_l[w][tid];
+      }
+      // a row that sees no key: zeros (l is NaN, not 0, where a visible score is)
+      const float inv = g.kind == 0 ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+      if (g.kind != 0) *reinterpret_cast<float2*>(a.ml + s_at[tid] * 2) = make_float2(mx, l);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) s_m[w][tid] = f[w] * inv;
+    }
+    __syncthreads();
+    constexpr int PAD = D + 4;   // the rows 2 tq of the accumulators' columns fall into different banks
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      if (8 * n >= g.nrows) break;
+      if (n > 0) __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float factor = s_m[warp][8 * n + 2 * tq + e];
+        float* dst = s_o + (warp * 8 + 2 * tq + e) * PAD + g8;
+#pragma unroll
+        for (int m = 0; m < STEPS; ++m) {
+          const float b = om[m / RSTEPS][n][e];
+          dst[16 * m] = fmaf(o[m][n][e], to_lo, b) * factor;
+          dst[16 * m + 8] = fmaf(o[m][n][2 + e], to_hi, b) * factor;
+        }
+      }
+      __syncthreads();
+      const int live = min(g.nrows - 8 * n, 8);
+      for (int idx = tid; idx < live * (D / 4); idx += kThreads) {
+        const int row = idx / (D / 4), d = 4 * (idx % (D / 4));
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float4 x = *reinterpret_cast<const float4*>(s_o + (w * 8 + row) * PAD + d);
+          v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+        }
+        const int64_t at = s_at[8 * n + row];
+        if (g.kind == 0) {
+          store_out2<T>(a, at + d, v.x, v.y);
+          store_out2<T>(a, at + d + 2, v.z, v.w);
+        } else {
+          *reinterpret_cast<float4*>(a.acc + at * D + d) = v;
+        }
+      }
+    }
+    __syncthreads();   // s_at, s_m and s_o are free again
+  }
+  // Nothing is under way into this block's memory when it ends: unless a wait ran out, every tile has been waited for
+  if (!landed)
+    for (int u = max(sent - SLOTS, 0); u < sent; ++u) landed = mbar_wait(full + 8 * (u % SLOTS), (u / SLOTS) & 1) && landed;
+}
+
+// Merges the entries of units that several CTAs share: a block of 128 threads for 512 / D rows of a (sequence, KV head), four
+// elements a thread, with a running maximum, so that one round trip to memory follows the first kernel's end. GROUPS > 1: so
+// many groups of 128 threads share the entries of a unit that many CTAs have cut.
+template <typename T, int D, int NT, int GROUPS>
+__global__ void __launch_bounds__(128 * GROUPS) int4_combine_kernel(const __grid_constant__ Int4AttnArgs a) {
+  constexpr int ROWS = 8 * NT, QUADS = D / 4, BLOCK_ROWS = 128 / QUADS;
+  __shared__ int s_sum[kMaxBatch + 1], s_len[kMaxBatch], s_warp[4 * GROUPS];
+  __shared__ float4 s_v[GROUPS > 1 ? 128 * GROUPS : 1];   // the groups' sums and (m, l)
+  __shared__ float2 s_ml[GROUPS > 1 ? 128 * GROUPS : 1];
+  const int tid = threadIdx.x, group = tid / 128;
+  pdl_launch_dependents();
+  // the lengths are inputs of the whole call, complete before its first kernel began
+  Line<NT> line(a);
+  scan_costs<NT, 128 * GROUPS>(a, s_sum, s_len, s_warp);
+  line.close(a, s_sum[a.B]);
+  const int b = blockIdx.x / a.kv.KVH, kvh = blockIdx.x - b * a.kv.KVH, cost = s_sum[b + 1] - s_sum[b];
+  const int row = blockIdx.y * BLOCK_ROWS + tid % 128 / QUADS, d = (tid % QUADS) * 4;
+  const bool on = row < a.rows;
+  // the CTAs that share the row's unit: entry (c, started there) of each
+  int c0 = 0, c1 = -1, p0 = 0;
+  if (on && cost > 0) {
+    const int start = s_sum[b] * line.units + (kvh * line.tiles + row / ROWS) * cost;
+    p0 = start + Line<NT>::LEAD;
+    c0 = line.owner(p0);
+    c1 = line.owner(start + cost - 1);
+    if (c0 == c1) c1 = -2;   // written by the first kernel
+  }
+  pdl_wait();
+  float m = -INFINITY, l = 0.f;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int c = c0 + 8 * group; c <= c1; c += 8 * GROUPS) {   // eight entries in flight
+    float4 x[8];
+    float2 ml[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      ml[k] = make_float2(-INFINITY, 0.f);
+      x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (c + k <= c1) {
+        const int64_t at = (static_cast<int64_t>(c + k) * 2 + (line.share(c + k) <= p0 ? 1 : 0)) * ROWS + row % ROWS;
+        ml[k] = *reinterpret_cast<const float2*>(a.ml + at * 2);
+        x[k] = *reinterpret_cast<const float4*>(a.acc + at * D + d);
+      }
+    }
+    float mx = m;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) mx = fmaxf(mx, ml[k].x);
+    const float keep = m == -INFINITY ? 0.f : exp2_fast(m - mx);
+    m = mx;
+    l *= keep;
+    v.x *= keep; v.y *= keep; v.z *= keep; v.w *= keep;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float f = ml[k].x == -INFINITY ? 0.f : exp2_fast(ml[k].x - mx);
+      l = fmaf(f, ml[k].y, l);
+      v.x = fmaf(f, x[k].x, v.x); v.y = fmaf(f, x[k].y, v.y);
+      v.z = fmaf(f, x[k].z, v.z); v.w = fmaf(f, x[k].w, v.w);
+    }
+  }
+  if constexpr (GROUPS > 1) {
+    s_v[tid] = v;
+    s_ml[tid] = make_float2(m, l);
+    __syncthreads();
+    if (group > 0) return;
+    float mx = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < GROUPS; ++k) mx = fmaxf(mx, s_ml[tid + 128 * k].x);
+    l = 0.f;
+    v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < GROUPS; ++k) {
+      const float2 ml = s_ml[tid + 128 * k];
+      const float4 x = s_v[tid + 128 * k];
+      const float f = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - mx);
+      l = fmaf(f, ml.y, l);
+      v.x = fmaf(f, x.x, v.x); v.y = fmaf(f, x.y, v.y);
+      v.z = fmaf(f, x.z, v.z); v.w = fmaf(f, x.w, v.w);
+    }
+  }
+  if (!on || c1 == -2) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;   // a row that sees no key, or a sequence without keys: zeros
+  const int t = div_g(a, row), head = kvh * a.G + row - t * a.G;
+  const int64_t at = b * a.so_b + t * a.so_t + static_cast<int64_t>(head) * a.so_h + d;
+  store_out2<T>(a, at, v.x * inv, v.y * inv);
+  store_out2<T>(a, at + 2, v.z * inv, v.w * inv);
+}
+
+// ------------------------------------------------------------------ host
+// Row tiles of 8 in a unit, at most 4: as few units as possible, of equal size (40 rows: two of 24)
+int row_tiles(int rows) {
+  const int units = (rows + 31) / 32, per = (rows + units - 1) / units;
+  return (per + 7) / 8;
+}
+
+struct Plan {
+  int nt, ctas, whole, many, fits;
+  int64_t entries;
+  size_t bytes;
+};
+
+Plan make_plan(const b2d_int4_kv* kv, int B, int T, int H, int pages_per_seq, int max_len, int sm) {
+  Plan p{};
+  const int64_t reach = static_cast<int64_t>(pages_per_seq) * kv->page_size;
+  const int rows = T * (H / kv->KVH);
+  p.nt = row_tiles(rows);
+  const int tile = 8 * p.nt;
+  const int64_t keys = max_len > 0 && max_len < reach ? max_len : reach;
+  const int64_t units = static_cast<int64_t>(B) * kv->KVH * ((rows + tile - 1) / tile);
+  p.fits = units * ((reach + kStage - 1) / kStage + 4) < (int64_t(1) << 31);
+  p.whole = keys <= kStage;
+  int64_t ctas = p.whole ? units : units * ((keys + kStage - 1) / kStage + 4);
+  const int per_sm = p.nt == 1 ? kBlocks<1> : p.nt == 2 ? kBlocks<2> : kBlocks<3>;
+  if (ctas > static_cast<int64_t>(per_sm) * sm) ctas = per_sm * sm;
+  if (ctas > kMaxCtas) ctas = kMaxCtas;
+  p.ctas = static_cast<int>(ctas < 1 ? 1 : ctas);
+  p.many = p.ctas > 16 * units;
+  if (!p.whole) {
+    p.entries = static_cast<int64_t>(p.ctas) * 2 * tile;
+    p.bytes = static_cast<size_t>(p.entries) * (kv->D + 2) * 4;
+  }
+  return p;
+}
+
+template <typename T, int D, int RUNS, int NT>
+int launch_attention(const Int4AttnArgs& a, bool many, bool pdl, cudaStream_t s) {
+  auto kern = int4_attention_kernel<T, D, RUNS, NT>;
+  constexpr int bytes = Smem<D, RUNS, NT>::BYTES;
+  static bool configured[64] = {};   // per device; setting it twice is harmless
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) {
+      set_cuda_error(e);
+      return B2D_ERR_LAUNCH;
+    }
+    if (dev >= 0 && dev < 64) configured[dev] = true;
+  }
+  const int st = launch_kernel(kern, dim3(a.ctas), dim3(kThreads), bytes, s, pdl, a);
+  if (st != B2D_OK || a.whole) return st;
+  const dim3 grid(a.B * a.kv.KVH, (a.rows + 512 / D - 1) / (512 / D));
+  if (many) return launch_kernel(int4_combine_kernel<T, D, NT, 4>, grid, dim3(512), 0, s, true, a);
+  return launch_kernel(int4_combine_kernel<T, D, NT, 1>, grid, dim3(128), 0, s, true, a);
+}
+
+template <typename T, int D, int RUNS>
+int run(const Int4AttnArgs& a, const Plan& p, bool pdl, cudaStream_t s) {
+  switch (p.nt) {
+    case 1: return launch_attention<T, D, RUNS, 1>(a, p.many, pdl, s);
+    case 2: return launch_attention<T, D, RUNS, 2>(a, p.many, pdl, s);
+    case 3: return launch_attention<T, D, RUNS, 3>(a, p.many, pdl, s);
+    default: return launch_attention<T, D, RUNS, 4>(a, p.many, pdl, s);
+  }
+}
+template <typename T>
+int run(const Int4AttnArgs& a, const Plan& p, bool pdl, cudaStream_t s) {
+  if (a.kv.D == 64) return a.kv.group == 64 ? run<T, 64, 1>(a, p, pdl, s) : run<T, 64, 2>(a, p, pdl, s);
+  return a.kv.group == 64 ? run<T, 128, 2>(a, p, pdl, s) : run<T, 128, 4>(a, p, pdl, s);
+}
+
+int check_shapes(const b2d_int4_kv* kv, int B, int T, int H, int pages_per_seq, int max_len) {
+  const int st = check_int4_kv(kv);
+  if (st != B2D_OK) return st;
+  if (B < 0 || T < 0 || H < 0 || pages_per_seq < 0 || max_len < 0) return B2D_ERR_ARG;
+  if (H % kv->KVH != 0 || H / kv->KVH > kMaxG || T > kMaxT) return B2D_ERR_SHAPE;
+  // positions and their sums with a stage's keys fit 31 bits
+  if (static_cast<int64_t>(pages_per_seq) * kv->page_size > (int64_t(1) << 31) - 1024) return B2D_ERR_SHAPE;
+  return B2D_OK;
+}
+
+}  // namespace
+}  // namespace b2d
+
+using namespace b2d;
+
+extern "C" size_t b2d_int4_attention_workspace_bytes(const b2d_int4_kv* kv, int B, int T, int H, int pages_per_seq,
+                                                     int max_len) {
+  if (check_shapes(kv, B, T, H, pages_per_seq, max_len) != B2D_OK || B == 0 || T == 0 || H == 0) return 0;
+  DeviceInfo di;
+  if (device_info(&di) != B2D_OK) return 0;
+  // the launches of a large batch: full ones and a rest
+  const size_t full = B >= kMaxBatch ? make_plan(kv, kMaxBatch, T, H, pages_per_seq, max_len, di.sm_count).bytes : 0;
+  const size_t rest = B % kMaxBatch ? make_plan(kv, B % kMaxBatch, T, H, pages_per_seq, max_len, di.sm_count).bytes : 0;
+  return full > rest ? full : rest;
+}
+
+extern "C" int b2d_int4_attention(const b2d_int4_kv* kv, const void* q, int64_t sq_b, int64_t sq_t, int64_t sq_h,
+                                  const int32_t* page_table, int64_t ld_table, int pages_per_seq, const int32_t* seqlens,
+                                  int max_len, int B, int T, int H, float scale, void* out, int64_t so_b, int64_t so_t,
+                                  int64_t so_h, int out_dtype, void* workspace, size_t workspace_bytes, int flags,
+                                  void* stream) {
+  int st;
+  if ((st = check_shapes(kv, B, T, H, pages_per_seq, max_len)) != B2D_OK) return st;
+  if (out_dtype != kv->dtype && out_dtype != B2D_F32) return B2D_ERR_DTYPE;
+  if (B == 0 || T == 0 || H == 0) return B2D_OK;
+  if (ld_table < 0) return B2D_ERR_SHAPE;
+  if (!q || !seqlens || !out || (!page_table && pages_per_seq > 0)) return B2D_ERR_ARG;
+  if (!aligned(q, 16) || (sq_b | sq_t | sq_h) % 8 || !aligned(page_table, 4) || !aligned(seqlens, 4) ||
+      !aligned(out, out_dtype == B2D_F32 ? 4 : 2) || !aligned(workspace, 16))
+    return B2D_ERR_ALIGN;
+  DeviceInfo di;
+  if ((st = device_info(&di)) != B2D_OK) return st;
+  const int size = out_dtype == B2D_F32 ? 4 : 2;
+  for (int b0 = 0; b0 < B; b0 += kMaxBatch) {
+    const int n = B - b0 < kMaxBatch ? B - b0 : kMaxBatch;
+    const Plan p = make_plan(kv, n, T, H, pages_per_seq, max_len, di.sm_count);
+    if (!p.fits) return B2D_ERR_SHAPE;
+    if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes)) return B2D_ERR_WORKSPACE;
+    Int4AttnArgs a{};
+    a.q = static_cast<const uint8_t*>(q) + b0 * sq_b * 2;
+    a.sq_b = sq_b; a.sq_t = sq_t; a.sq_h = sq_h;
+    a.table = page_table ? page_table + b0 * ld_table : nullptr;
+    a.ld_table = ld_table; a.seqlens = seqlens + b0;
+    a.out = static_cast<uint8_t*>(out) + b0 * so_b * size;
+    a.so_b = so_b; a.so_t = so_t; a.so_h = so_h;
+    a.kv = *kv; a.div = page_div(kv->page_size);
+    a.pages_per_seq = pages_per_seq;
+    a.B = n; a.T = T; a.H = H; a.G = H / kv->KVH; a.rows = T * a.G; a.inv_g = (65536 + a.G - 1) / a.G;
+    a.scale_log2 = scale * kLog2e;
+    a.ctas = p.ctas; a.whole = p.whole;
+    a.out_f32 = out_dtype == B2D_F32;
+    a.out_vec = aligned(a.out, 2 * size) && (so_b | so_t | so_h) % 2 == 0;
+    a.acc = static_cast<float*>(workspace);
+    a.ml = a.acc ? a.acc + p.entries * kv->D : nullptr;
+    const bool pdl = (flags & B2D_LAUNCH_PDL) != 0;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    st = kv->dtype == B2D_F16 ? run<__half>(a, p, pdl, s) : run<__nv_bfloat16>(a, p, pdl, s);
+    if (st != B2D_OK) return st;
+  }
+  return B2D_OK;
+}
