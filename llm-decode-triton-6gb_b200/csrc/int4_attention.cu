@@ -20,6 +20,8 @@
 // Units of work are (sequence, KV head, tile of up to 32 rows). As in the 16-bit kernel the units' stages (64 keys, a
 // tile a warp) form one line of which every block takes an equal share, found from the lengths on the device; parts of a unit
 // that several blocks share meet in a combine launch. No atomics: results are the same bits every run.
+#include <type_traits>
+
 #include "int4_kv.cuh"
 #include "pipeline.cuh"
 
@@ -33,6 +35,7 @@ constexpr int kMaxT = 16, kMaxG = 16;
 constexpr int kMaxBatch = 256;                  // sequences of a launch (larger batches take several)
 constexpr int kMaxCtas = 640;
 constexpr float kLazy = 8.f;                    // log2 of the largest weight before the running maximum moves
+constexpr float kNone = -1.7e38f;               // running maximum before the first score
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Blocks of an SM, by registers (accumulators: 32 a row tile), and tiles of a warp's ring, by shared memory.
@@ -69,6 +72,31 @@ struct Int4AttnArgs {
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(dst), "l"(src),
                "r"(bytes), "r"(bar) : "memory");
+}
+
+__device__ __align__(16) uint8_t g_zero_tile[int4_tile_bytes(128, 4)];   // never written
+
+// N neighbouring words of shared memory, aligned to their size
+template <int N>
+__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
+  if constexpr (N == 4) {
+    const uint4 x = *reinterpret_cast<const uint4*>(p);
+    w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+  } else if constexpr (N == 2) {
+    const uint2 x = *reinterpret_cast<const uint2*>(p);
+    w[0] = x.x; w[1] = x.y;
+  } else {
+    static_assert(N == 1, "1, 2 or 4 words");
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+}
+
+// codes at 2^(-20 - SHIFT) -> themselves less 8
+template <int SHIFT>
+__device__ __forceinline__ uint32_t minus_8(uint32_t x) {
+  const uint32_t eight = 0x00800080u >> SHIFT;
+  const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&eight));
+  return *reinterpret_cast<const uint32_t*>(&y);
 }
 
 template <typename T>
@@ -203,6 +231,10 @@ __global__ void __launch_bounds__(kThreads, kBlocks<NT>) int4_attention_kernel(c
   constexpr int TILE = S::TILE, SLOTS = S::SLOTS, KW = D / 32;          // KW: key words of a lane and key
   static_assert(SLOTS >= 2, "a ring of at least two tiles");
   constexpr bool Q_REGS = NT <= 2;
+  // Codes enter the second product around their middle, 8: weights times codes from 0 to 15 would grow with the number of keys where
+  // their values cancel, and the tensor cores' sums cut what does not fit below. One row tile: a product with -8 throughout
+  // (8 a tile of keys); more: subtracted from the codes themselves (32, for all row tiles).
+  constexpr bool BY_PRODUCT = NT == 1;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float s_m[kWarps][ROWS], s_l[kWarps][ROWS];
   __shared__ float s_rowf[ROWS], s_qs[RUNS][ROWS];
@@ -227,49 +259,50 @@ __global__ void __launch_bounds__(kThreads, kBlocks<NT>) int4_attention_kernel(c
   }();
   const int first = line.share(blockIdx.x), end = line.share(blockIdx.x + 1);
 
-  // ---- the warp's copies, ahead of its products: tile `ft` of `fg` next, of the warp's `fn` there
-  int fpos = first, ft = 0, fn = 0, sent = 0, page = 0;
-  Segment fg;
-  fg.next = first;
-  // page of the warp's tile ft0 + lane
-  auto lookup = [&](int ft0) {
-    const int key = fg.t_begin + ((ft0 + lane) * kWarps + warp) * kTileKeys;
-    return key < fg.t_end ? __ldg(a.table + fg.b * a.ld_table + a.div.page(key)) : -1;
-  };
-  auto fetch = [&]() {   // the next tile, if any; its slot is free
-    while (ft >= fn) {
-      if (fpos >= end) return;
-      fg = segment_at<NT>(a, line, s_sum, s_len, fpos, end);
-      fpos = fg.next;
-      ft = 0;
-      const int tiles = fg.kind < 0 ? 0 : (fg.t_end - fg.t_begin + kTileKeys - 1) / kTileKeys;
-      fn = tiles > warp ? (tiles - warp + kWarps - 1) / kWarps : 0;
-      if (fn > 0) page = lookup(0);
+  // ---- the warp's copies, ahead of its products: tile `ft` of the warp's `fn` in segment `fg` next. The sources of tiles up
+  // to `fc` are at hand: lane l has that of tile l (modulo 32).
+  bool landed = true;   // until a wait runs out: no copies are sent after that
+  int fpos = first, ft = 0, fn = 0, fc = 0, fslot = 0, ahead = 0;   // ahead: copies under way
+  Segment fg{};
+  const uint8_t* src = nullptr;
+  auto lookup = [&] {
+    fc = min(fn, ft + 32);
+    const int key = fg.t_begin + ((ft + ((lane - ft) & 31)) * kWarps + warp) * kTileKeys;
+    src = g_zero_tile;   // of a page id outside the pool: keys and values of zeros
+    if (key < fg.t_end) {
+      const int pi = a.div.page(key), page = __ldg(a.table + fg.b * a.ld_table + pi);
+      if (page >= 0 && page < a.kv.num_pages)
+        src = a.kv.pages + page * a.kv.sp_p + fg.kvh * a.kv.sp_h + static_cast<int64_t>(a.div.slot(key, pi) / kTileKeys) * TILE;
     }
-    if (ft > 0 && (ft & 31) == 0) page = lookup(ft);
-    const int p = __shfl_sync(0xffffffffu, page, ft & 31), slot = sent % SLOTS;
-    if (p >= 0 && p < a.kv.num_pages) {
-      if (lane == 0) {
-        const int key = fg.t_begin + (ft * kWarps + warp) * kTileKeys;
-        const int in_page = a.div.slot(key, a.div.page(key)) / kTileKeys;
-        mbar_expect_tx(full + 8 * slot, TILE);
-        bulk_load(ring_s + slot * TILE, a.kv.pages + p * a.kv.sp_p + fg.kvh * a.kv.sp_h + static_cast<int64_t>(in_page) * TILE,
-                  TILE, full + 8 * slot);
-      }
-    } else {   // a page id outside the pool: keys and values of zeros
-      for (int i = lane; i < TILE / 16; i += 32) *reinterpret_cast<uint4*>(ring + slot * TILE + 16 * i) = make_uint4(0, 0, 0, 0);
-      fence_proxy_async();   // the slot's next copy comes after these writes
-      __syncwarp();
-      if (lane == 0) mbar_arrive(full + 8 * slot);
+  };
+  auto issue = [&] {   // the next tile into the next slot, which is free
+    if (landed && lane == (ft & 31)) {
+      mbar_expect_tx(full + 8 * fslot, TILE);
+      bulk_load(ring_s + fslot * TILE, src, TILE, full + 8 * fslot);
     }
     ++ft;
-    ++sent;
+    fslot = fslot + 1 == SLOTS ? 0 : fslot + 1;
   };
-#pragma unroll 1
-  for (int i = 0; i < SLOTS; ++i) fetch();
+  auto refill = [&] {   // every free slot, from the next segments if need be
+    while (landed && ahead < SLOTS) {
+      if (ft == fc) {
+        while (ft == fn) {
+          if (fpos >= end) return;
+          fg = segment_at<NT>(a, line, s_sum, s_len, fpos, end);
+          fpos = fg.next;
+          const int tiles = fg.kind < 0 ? 0 : (fg.t_end - fg.t_begin + kTileKeys - 1) / kTileKeys;
+          fn = tiles > warp ? (tiles - warp + kWarps - 1) / kWarps : 0;
+          ft = 0;
+        }
+        lookup();
+      }
+      issue();
+      ++ahead;
+    }
+  };
+  refill();
 
-  int it = 0;            // the warp's tiles so far
-  bool landed = true;
+  int slot = 0, parity = 0;   // of the warp's next tile
   for (int pos = first; pos < end;) {
     const Segment g = segment_at<NT>(a, line, s_sum, s_len, pos, end);
     pos = g.next;
@@ -340,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks<NT>) int4_attention_kernel(c
     auto lim = [&](int n, int e) { return causal ? g.limit + div_g(a, g.row0 + min(8 * n + 2 * tq + e, g.nrows - 1)) : g.limit; };
 
     float o[STEPS][NT][4];   // element 16 m + g8 (+ 8), row 8 n + 2 tq (+ 1), in units of 2^(E - 7 - 24) (2^(E - 7 - 20))
-    float om[RUNS][NT][2];   // sum of p m over this thread's keys
+    float om[RUNS][NT][2];   // sum of p (m + 8 s) over this thread's keys
     float m_run[NT][2], l_run[NT][2];   // log2 domain; the sum over this thread's keys only
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -348,31 +381,21 @@ __global__ void __launch_bounds__(kThreads, kBlocks<NT>) int4_attention_kernel(c
       for (int m = 0; m < STEPS; ++m) o[m][n][0] = o[m][n][1] = o[m][n][2] = o[m][n][3] = 0.f;
 #pragma unroll
       for (int u = 0; u < RUNS; ++u) om[u][n][0] = om[u][n][1] = 0.f;
-      m_run[n][0] = m_run[n][1] = -INFINITY;
+      m_run[n][0] = m_run[n][1] = kNone;
       l_run[n][0] = l_run[n][1] = 0.f;
     }
     float v_top = 0.f, v_unit = 1.f;   // 2^E and 2^(7 - E); v_top = 0: no value yet
 
-    const int tiles = (g.t_end - g.t_begin + kTileKeys - 1) / kTileKeys;
-#pragma unroll 1
-    for (int tile = warp; tile < tiles; tile += kWarps, ++it) {
-      const int slot = it % SLOTS, key0 = g.t_begin + tile * kTileKeys;
-      landed = landed && mbar_wait(full + 8 * slot, (it / SLOTS) & 1);
+    // One tile: its scores, its weights, its part of o. MASKED: some row does not see some key of it.
+    auto tile = [&](auto masked_, int key0) {
+      constexpr bool MASKED = decltype(masked_)::value;
+      landed = landed && mbar_wait(full + 8 * slot, parity);
       const uint8_t* const buf = ring + slot * TILE;
       float acc[RUNS][NT][4];   // key g8 (+ 8), row 8 n + 2 tq (+ 1)
       {
         uint32_t kw[2][KW];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint8_t* p = buf + (g8 + 8 * h) * (D / 2) + tq * (D / 8);
-          if constexpr (KW == 4) {
-            const uint4 x = *reinterpret_cast<const uint4*>(p);
-            kw[h][0] = x.x; kw[h][1] = x.y; kw[h][2] = x.z; kw[h][3] = x.w;
-          } else {
-            const uint2 x = *reinterpret_cast<const uint2*>(p);
-            kw[h][0] = x.x; kw[h][1] = x.y;
-          }
-        }
+        for (int h = 0; h < 2; ++h) load_words(buf + (g8 + 8 * h) * (D / 2) + tq * (D / 8), kw[h]);
 #pragma unroll
         for (int j = 0; j < STEPS; ++j) {
           const int sh = 8 * (j & 1), u = j / RSTEPS;
@@ -385,37 +408,38 @@ __global__ void __launch_bounds__(kThreads, kBlocks<NT>) int4_attention_kernel(c
           }
         }
       }
-      // scores: p holds x - m_run, then the weights
-      float p[NT][4];
-      {
-        float2 f[2][RUNS];
+      // scores: acc[0] becomes them over rowf, d what they are past the running maximum
+      float d[NT][4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h) {
+        uint32_t f[RUNS];
+        load_words(buf + int4_ks_off(D) + (g8 + 8 * h) * (4 * RUNS), f);
 #pragma unroll
-          for (int u = 0; u < RUNS; ++u)
-            f[h][u] = unpack_sm<T>(*reinterpret_cast<const uint32_t*>(buf + int4_ks_off(D) + ((g8 + 8 * h) * RUNS + u) * 4));
+        for (int u = 0; u < RUNS; ++u) {
+          const float2 sm = unpack_sm<T>(f[u]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float x = acc[u][n][2 * h + e];
+              acc[0][n][2 * h + e] = fmaf(sm.y, qs[u][n][e], u == 0 ? sm.x * x : fmaf(sm.x, x, acc[0][n][2 * h + e]));
+            }
+        }
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int h = c >> 1, e = c & 1;
-            float x = 0.f;
-#pragma unroll
-            for (int u = 0; u < RUNS; ++u) {
-              x = u == 0 ? f[h][u].x * acc[u][n][c] : fmaf(f[h][u].x, acc[u][n][c], x);
-              x = fmaf(f[h][u].y, qs[u][n][e], x);
-            }
-            p[n][c] = x * rowf[n][e];
-          }
+          for (int e = 0; e < 2; ++e) d[n][2 * h + e] = fmaf(acc[0][n][2 * h + e], rowf[n][e], -m_run[n][e]);
       }
       float2 vf[2][RUNS];   // the values' factors of keys g8 (+ 8)
+      float s_top = 0.f, d_top = -INFINITY;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h) {
+        uint32_t f[RUNS];
+        load_words(buf + int4_vs_off(D, RUNS) + (g8 + 8 * h) * (4 * RUNS), f);
 #pragma unroll
-        for (int u = 0; u < RUNS; ++u)
-          vf[h][u] = unpack_sm<T>(*reinterpret_cast<const uint32_t*>(buf + int4_vs_off(D, RUNS) + ((g8 + 8 * h) * RUNS + u) * 4));
-      const bool masked = key0 + kTileKeys > min(lim_min, g.t_end);
-      if (masked) {
+        for (int u = 0; u < RUNS; ++u) vf[h][u] = unpack_sm<T>(f[u]);
+      }
+      if constexpr (MASKED) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int key = key0 + g8 + 8 * h;
@@ -423,24 +447,21 @@ __global__ void __launch_bounds__(kThreads, kBlocks<NT>) int4_attention_kernel(c
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e)
-              if (key >= lim(n, e) || key >= g.t_end) p[n][2 * h + e] = -INFINITY;
+              if (key >= lim(n, e) || key >= g.t_end) d[n][2 * h + e] = -INFINITY;
           if (key >= g.t_end) {   // what lies behind the last key is not the cache's
 #pragma unroll
             for (int u = 0; u < RUNS; ++u) vf[h][u] = make_float2(0.f, 0.f);
           }
         }
       }
-      float s_top = 0.f;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h) {
 #pragma unroll
         for (int u = 0; u < RUNS; ++u) s_top = fmaxf(s_top, vf[h][u].x);
-      bool move = s_top > v_top;
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) move |= fmaxf(p[n][e], p[n][2 + e]) > m_run[n][e] + kLazy;
-      if (__any_sync(0xffffffffu, move)) {
+        for (int n = 0; n < NT; ++n) d_top = fmaxf(d_top, fmaxf(d[n][2 * h], d[n][2 * h + 1]));
+      }
+      if (__any_sync(0xffffffffu, s_top > v_top || d_top > kLazy)) {
         const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(s_top));
         float keep = 1.f;
         if (__uint_as_float(bits) > v_top) {   // 2^E with room for twice the largest s; E in [-110, 110]
@@ -454,19 +475,27 @@ __global__ void __launch_bounds__(kThreads, kBlocks<NT>) int4_attention_kernel(c
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float top = fmaxf(p[n][e], p[n][2 + e]);
+            float x[2], top = -INFINITY;
 #pragma unroll
-            for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+            for (int h = 0; h < 2; ++h) {
+              x[h] = d[n][2 * h + e] == -INFINITY ? -INFINITY : acc[0][n][2 * h + e] * rowf[n][e];
+              top = fmaxf(top, x[h]);
+            }
+#pragma unroll
+            for (int i = 4; i < 32; i <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
             const bool up = top > m_run[n][e] + kLazy;
-            const float alpha = up ? exp2_fast(m_run[n][e] - top) : 1.f;   // m_run = -inf: 0
+            const float alpha = up ? exp2_fast(m_run[n][e] - top) : 1.f;   // m_run = kNone: 0
             if (up) m_run[n][e] = top;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) d[n][2 * h + e] = x[h] - m_run[n][e];
             l_run[n][e] *= alpha;
+            const float ak = alpha * keep;
 #pragma unroll
             for (int u = 0; u < RUNS; ++u) om[u][n][e] *= alpha;
 #pragma unroll
             for (int m = 0; m < STEPS; ++m) {
-              o[m][n][e] *= alpha * keep;
-              o[m][n][2 + e] *= alpha * keep;
+              o[m][n][e] *= ak;
+              o[m][n][2 + e] *= ak;
             }
           }
       }
@@ -474,44 +503,88 @@ __global__ void __launch_bounds__(kThreads, kBlocks<NT>) int4_attention_kernel(c
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const float mr = m_run[n][c & 1];
-          p[n][c] = exp2_fast(p[n][c] - (mr == -INFINITY ? 0.f : mr));
-          l_run[n][c & 1] += p[n][c];
+          d[n][c] = exp2_fast(d[n][c]);   // the weights
+          l_run[n][c & 1] += d[n][c];
         }
       uint32_t pb[RUNS][NT][2];   // P s as the B operand: row 8 n + g8, keys 2 tq .. (+ 8)
 #pragma unroll
       for (int u = 0; u < RUNS; ++u) {
-        const float s0 = vf[0][u].x * v_unit, s1 = vf[1][u].x * v_unit;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float w[4] = {p[n][0] * s0, p[n][1] * s0, p[n][2] * s1, p[n][3] * s1};
-          float b[4] = {p[n][0] * vf[0][u].y, p[n][1] * vf[0][u].y, p[n][2] * vf[1][u].y, p[n][3] * vf[1][u].y};
-          if (masked) {   // factors that are infinite or NaN reach the rows that see their key, and no other
+        for (int h = 0; h < 2; ++h) {
+          const float su = vf[h][u].x * v_unit, center = fmaf(8.f, vf[h][u].x, vf[h][u].y);
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-              if (key0 + g8 + 8 * (c >> 1) >= lim(n, c & 1)) w[c] = b[c] = 0.f;
+          for (int n = 0; n < NT; ++n) {
+            float w0 = d[n][2 * h] * su, w1 = d[n][2 * h + 1] * su;
+            if constexpr (MASKED) {   // factors that are infinite or NaN reach the rows that see their key, and no other
+              const int key = key0 + g8 + 8 * h;
+              if (key < lim(n, 0)) om[u][n][0] = fmaf(d[n][2 * h], center, om[u][n][0]);
+              else w0 = 0.f;
+              if (key < lim(n, 1)) om[u][n][1] = fmaf(d[n][2 * h + 1], center, om[u][n][1]);
+              else w1 = 0.f;
+            } else {
+              om[u][n][0] = fmaf(d[n][2 * h], center, om[u][n][0]);
+              om[u][n][1] = fmaf(d[n][2 * h + 1], center, om[u][n][1]);
+            }
+            pb[u][n][h] = transpose8(Dt<__half>::pack2(w0, w1));
           }
-          om[u][n][0] += b[0] + b[2];
-          om[u][n][1] += b[1] + b[3];
-          pb[u][n][0] = transpose8(Dt<__half>::pack2(w[0], w[1]));
-          pb[u][n][1] = transpose8(Dt<__half>::pack2(w[2], w[3]));
         }
       }
 #pragma unroll
       for (int c = 0; c < D / 64; ++c) {
-        const uint4 vw = *reinterpret_cast<const uint4*>(buf + int4_v_off(D) + c * 512 + lane * 16);
-        const uint32_t w4[4] = {vw.x, vw.y, vw.z, vw.w};
+        uint32_t vw[4];
+        load_words(buf + int4_v_off(D) + c * 512 + lane * 16, vw);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int m = 4 * c + i, u = m / RSTEPS;
-          const uint32_t x = w4[i], y = x >> 8;
+          uint32_t a0, a1 = vw[i] & 0x00F000F0u, a2, a3;
+          if constexpr (BY_PRODUCT) {
+            // whole bytes for element g8: 16 times element g8 + 8, which the other half has, is taken off at the end
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
-            Mma<__half>::run(o[m][n], x & 0x000F000Fu, x & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u, pb[u][n][0], pb[u][n][1]);
+            for (int n = 0; n < NT; ++n)   // -(8 + 128) and -128
+              Mma<__half>::run(o[m][n], 0x80888088u, 0x80808080u, 0x80888088u, 0x80808080u, pb[u][n][0], pb[u][n][1]);
+            a0 = vw[i] & 0x00FF00FFu;
+            a2 = __byte_perm(vw[i], 0u, 0x4341);
+            a3 = a2 & 0x00F000F0u;
+          } else {
+            const uint32_t y = vw[i] >> 8;
+            a0 = minus_8<4>(vw[i] & 0x000F000Fu);
+            a1 = minus_8<0>(a1);
+            a2 = minus_8<4>(y & 0x000F000Fu);
+            a3 = minus_8<0>(y & 0x00F000F0u);
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) Mma<__half>::run(o[m][n], a0, a1, a2, a3, pb[u][n][0], pb[u][n][1]);
         }
       }
       __syncwarp();   // the warp is done with the slot
-      fetch();
+      slot += landed;
+      if (slot == SLOTS) {
+        slot = 0;
+        parity ^= 1;
+      }
+    };
+    const int tiles = (g.t_end - g.t_begin + kTileKeys - 1) / kTileKeys, seen = min(lim_min, g.t_end) / kTileKeys - g.t_begin / kTileKeys;
+    int left = tiles > warp ? (tiles - warp + kWarps - 1) / kWarps : 0;     // the warp's tiles
+    int clear = seen > warp ? (seen - warp + kWarps - 1) / kWarps : 0;      // of which the first are seen whole by all rows
+    int key0 = g.t_begin + warp * kTileKeys;
+    // While the segment has further tiles to fetch: one follows each tile into its slot. Nothing but this in the loop: the
+    // search for pages and segments, or the masks, would cost every tile 50 to 80 register moves and tests.
+    while (clear > 0 && fg.next == g.next && ft < fn) {
+      if (ft == fc) lookup();
+      const int n = min(clear, fc - ft);
+#pragma unroll 1
+      for (int i = 0; i < n; ++i, key0 += kStage) {
+        tile(std::false_type{}, key0);
+        issue();
+      }
+      clear -= n;
+      left -= n;
+    }
+#pragma unroll 1
+    for (; left > 0; --left, key0 += kStage) {
+      tile(std::true_type{}, key0);
+      ahead -= landed;
+      refill();
     }
 
     // ---- the unit's (or this CTA's part of it) result: the warps meet in shared memory
@@ -539,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks<NT>) int4_attention_kernel(c
       float f[kWarps];
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        f[w] = s_m[w][tid] == -INFINITY ? 0.f : exp2_fast(s_m[w][tid] - mx);
+        f[w] = exp2_fast(s_m[w][tid] - mx);   // (without a key: no weights, and their factor is of no account)
         l += f[w] * s_l[w][tid];
       }
       // a row that sees no key: zeros (l is NaN, not 0, where a visible score is)
@@ -561,8 +634,9 @@ __global__ void __launch_bounds__(kThreads, kBlocks<NT>) int4_attention_kernel(c
 #pragma unroll
         for (int m = 0; m < STEPS; ++m) {
           const float b = om[m / RSTEPS][n][e];
-          dst[16 * m] = fmaf(o[m][n][e], to_lo, b) * factor;
-          dst[16 * m + 8] = fmaf(o[m][n][2 + e], to_hi, b) * factor;
+          const float hi = o[m][n][2 + e], lo = BY_PRODUCT ? o[m][n][e] - hi : o[m][n][e];
+          dst[16 * m] = fmaf(lo, to_lo, b) * factor;
+          dst[16 * m + 8] = fmaf(hi, to_hi, b) * factor;
         }
       }
       __syncthreads();
@@ -586,9 +660,16 @@ __global__ void __launch_bounds__(kThreads, kBlocks<NT>) int4_attention_kernel(c
     }
     __syncthreads();   // s_at, s_m and s_o are free again
   }
-  // Nothing is under way into this block's memory when it ends: unless a wait ran out, every tile has been waited for
-  if (!landed)
-    for (int u = max(sent - SLOTS, 0); u < sent; ++u) landed = mbar_wait(full + 8 * (u % SLOTS), (u / SLOTS) & 1) && landed;
+  // Nothing is under way into this block's memory when it ends: every tile that was sent has been waited for, unless a wait ran out
+  if (!landed) {
+    for (; ahead > 0; --ahead) {
+      landed = mbar_wait(full + 8 * slot, parity);
+      if (++slot == SLOTS) {
+        slot = 0;
+        parity ^= 1;
+      }
+    }
+  }
 }
 
 // Merges the entries of units that several CTAs share: a block of 128 threads for 512 / D rows of a (sequence, KV head), four
@@ -755,8 +836,8 @@ int check_shapes(const b2d_int4_kv* kv, int B, int T, int H, int pages_per_seq, 
   if (st != B2D_OK) return st;
   if (B < 0 || T < 0 || H < 0 || pages_per_seq < 0 || max_len < 0) return B2D_ERR_ARG;
   if (H % kv->KVH != 0 || H / kv->KVH > kMaxG || T > kMaxT) return B2D_ERR_SHAPE;
-  // positions and their sums with a stage's keys fit 31 bits
-  if (static_cast<int64_t>(pages_per_seq) * kv->page_size > (int64_t(1) << 31) - 1024) return B2D_ERR_SHAPE;
+  // positions fit 31 bits, and so do those up to 32 stages past the end
+  if (static_cast<int64_t>(pages_per_seq) * kv->page_size > (int64_t(1) << 31) - 4096) return B2D_ERR_SHAPE;
   return B2D_OK;
 }
 
