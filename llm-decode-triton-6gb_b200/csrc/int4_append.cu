@@ -29,11 +29,19 @@ struct Int4AppendArgs {
   void* q_out; int64_t sqo_n, sqo_h;
   b2d_int4_kv kv;
   PageDiv div;
-  int N, H, B, per_seq, pages_per_seq, rotary, interleaved, parts;
+  int N, H, B, per_seq, pages_per_seq, rotary, q_parts;
+  uint32_t per_inv;
   int64_t limit;   // positions from here on are padding
 };
 
 constexpr int kWarps = 4;
+
+// Sequence of token n where every one has `per` tokens; inv = 2^32 / per, rounded down: the quotient or one less
+__device__ __forceinline__ int sequence_of(int n, int per, uint32_t inv) {
+  const int q = static_cast<int>(__umulhi(static_cast<uint32_t>(n), inv));
+  return n - q * per >= per ? q + 1 : q;
+}
+uint32_t inverse_of(int per) { return per < 2 ? 0xFFFFFFFFu : static_cast<uint32_t>((uint64_t(1) << 32) / per); }
 
 template <typename T>
 __device__ __forceinline__ void unpack8(const uint4& u, float* f) {
@@ -60,183 +68,313 @@ struct Chunks {
   uint4 a, b;
 };
 
-// A token's rotation factors of a lane's eight pairs.
-struct Turn {
-  float c[8], s[8];
+// Two fp32 operations an instruction (the kernels are bound by issued instructions, not by arithmetic).
+struct F2 {
+  uint64_t v;
 };
-
-// (a, b) -> (a c - b s, b c + a s) for a lane's pairs; EXACT: every product and sum rounded by itself
-template <bool EXACT>
-__device__ __forceinline__ void turn_pair(float& a, float& b, float c, float s) {
-  const float a0 = a, b0 = b;
-  if constexpr (EXACT) {
-    a = __fsub_rn(__fmul_rn(a0, c), __fmul_rn(b0, s));
-    b = __fadd_rn(__fmul_rn(b0, c), __fmul_rn(a0, s));
-  } else {
-    a = fmaf(a0, c, -b0 * s);
-    b = fmaf(b0, c, a0 * s);
-  }
+__device__ __forceinline__ F2 pack(float x, float y) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(r.v) : "f"(x), "f"(y));
+  return r;
 }
-template <bool EXACT>
-__device__ __forceinline__ void turn(float (&x)[16], const Turn& t, bool interleaved) {
-  if (interleaved) {
+__device__ __forceinline__ void unpack(const F2& a, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;\n" : "=f"(x), "=f"(y) : "l"(a.v)); }
+__device__ __forceinline__ F2 add2(const F2& a, const F2& b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(const F2& a, const F2& b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(const F2& a, const F2& b, const F2& c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+// 8 values as four pairs of neighbours
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4& u, F2 (&f)[4]) {
+  float x[8];
+  unpack8<T>(u, x);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) turn_pair<EXACT>(x[2 * e], x[2 * e + 1], t.c[e], t.s[e]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) turn_pair<EXACT>(x[e], x[8 + e], t.c[e], t.s[e]);
-  }
+  for (int i = 0; i < 4; ++i) f[i] = pack(x[2 * i], x[2 * i + 1]);
 }
 
-// 16 neighbouring elements of a run's lanes -> {s, m} and the codes
+__device__ __forceinline__ float max_nan(float a, float b) {   // NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float r;
+  asm("min.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// The smallest normal number of the 16-bit types
+template <typename T> __device__ constexpr float kNormal = 0x1p-14f;
+template <> constexpr float kNormal<__nv_bfloat16> = 0x1p-126f;
+
+// 16 neighbouring elements of a run's lanes -> {s, m} and the codes, each in the low bits of a word whose others are
+// 0x4B400000.
+// The quotients (x - m) / s share their divisor: each is the product with 1 / s corrected by its exact remainder, which rounds as
+// the division does (P. Markstein, Computation of elementary functions on the IBM RISC System/6000, 1990), and a sum with
+// 2^23 + 2^22 rounds it to a whole number, ties to even. They lie in 0..15 by themselves where s is a normal number (its rounding
+// moves 15 by less than a half) and m, where it was rounded up past elements, passed them by less than half a step; other
+// runs, and divisors whose reciprocal could overflow, take the division and the clamps.
 template <typename T>
 __device__ __forceinline__ uint32_t quantise(const float (&x)[16], int run_lanes, uint32_t (&code)[16]) {
-  float lo = x[0], hi = x[0], odd = 0.f;
+  float lo = min3(x[0], x[1], x[2]), hi = max3_nan(x[0], x[1], x[2]);
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    lo = fminf(lo, x[e]);
-    hi = fmaxf(hi, x[e]);
-    odd = fmaf(x[e], 0.f, odd);   // NaN once an element is infinite or NaN
+  for (int e = 3; e < 15; e += 2) {
+    lo = min3(lo, x[e], x[e + 1]);
+    hi = max3_nan(hi, x[e], x[e + 1]);
   }
+  lo = fminf(lo, x[15]);
+  hi = max_nan(hi, x[15]);
   for (int o = 1; o < run_lanes; o <<= 1) {
     lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    odd += __shfl_xor_sync(0xffffffffu, odd, o);
+    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
   }
-  const T mt = Dt<T>::from_f32(lo);
-  const float m = Dt<T>::to_f32(mt);
-  const T st = Dt<T>::from_f32(fmaxf(__fdiv_rn(__fsub_rn(hi, m), 15.f), 0.f));
-  const float s = Dt<T>::to_f32(st);
-  const bool sound = odd == 0.f && fabsf(m) < INFINITY && s < INFINITY;
+  const float m = Dt<T>::to_f32(Dt<T>::from_f32(lo));
+  const float s = Dt<T>::to_f32(Dt<T>::from_f32(fmaxf(__fdiv_rn(__fsub_rn(hi, m), 15.f), 0.f)));
+  const bool sound = fabsf(hi) < INFINITY && fabsf(m) < INFINITY && s < INFINITY;
+  constexpr float kEven = 12582912.f;   // 2^23 + 2^22
+  if (sound && s >= kNormal<T> && s >= 0x1p-100f && fabsf(m) < 256.f * s) {
+    const float r = __fdiv_rn(1.f, s);
+    const F2 r2 = pack(r, r), s2 = pack(-s, -s), m2 = pack(-m, -m), even2 = pack(kEven, kEven);
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    const float c = s > 0.f ? rintf(__fdiv_rn(__fsub_rn(x[e], m), s)) : 0.f;
-    code[e] = sound ? static_cast<uint32_t>(fminf(fmaxf(c, 0.f), 15.f)) : 0u;
+    for (int e = 0; e < 16; e += 2) {
+      const F2 d = add2(pack(x[e], x[e + 1]), m2), q = mul2(d, r2);
+      float c0, c1;
+      unpack(add2(fma2(fma2(q, s2, d), r2, q), even2), c0, c1);
+      code[e] = __float_as_uint(c0);
+      code[e + 1] = __float_as_uint(c1);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float c = sound && s > 0.f ? rintf(__fdiv_rn(__fsub_rn(x[e], m), s)) : 0.f;
+      code[e] = __float_as_uint(fminf(fmaxf(c, 0.f), 15.f) + kEven);
+    }
   }
-  if (!sound) return Dt<T>::pack2(NAN, NAN);
-  return Dt<T>::pack2(s, m);
+  return sound ? Dt<T>::pack2(s, m) : Dt<T>::pack2(NAN, NAN);
 }
 
-// T: cache and activation dtype, C: the tables' type
-template <typename T, typename C, int D>
-__global__ void __launch_bounds__(kWarps * 32) int4_append_kernel(const __grid_constant__ Int4AppendArgs a) {
-  constexpr int LANES = D / 16, HPW = 32 / LANES;   // lanes of a head, heads of a warp
-  __shared__ __align__(16) float s_row[kWarps][HPW][D];
-  pdl_launch_dependents();
-  pdl_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = lane % LANES, sub = lane / LANES;
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
-  const int64_t n = unit / a.parts;
-  const int part = static_cast<int>(unit - n * a.parts);
-  if (n >= a.N) return;
-  const int64_t pos = a.positions[n];
-  const int seq = a.seq_ids ? a.seq_ids[n] : static_cast<int>(n) / a.per_seq;
-  if (seq < 0 || seq >= a.B || pos < 0 || pos >= a.limit) return;   // padding
-  const int KVH = a.kv.KVH, run_lanes = a.kv.group / 16, runs = D / a.kv.group;
-  const int q_items = a.q ? (a.H + HPW - 1) / HPW : 0, kv_items = (KVH + HPW - 1) / HPW, items = q_items + 2 * kv_items;
-  // the lane's chunks: of the turning elements, of the rest
-  const bool turns = a.cos && 16 * j < a.rotary, halves = turns && !a.interleaved;
-  const int o1 = halves ? 8 * j : 16 * j, o2 = halves ? a.rotary / 2 + 8 * j : 16 * j + 8;
+// What both parts of the append know of a lane: head `sub` of its warp's, elements [o1, o1 + 8) and [o2, o2 + 8) of it.
+template <int D>
+struct Place {
+  static constexpr int LANES = D / 16, HPW = 32 / LANES;   // lanes of a head, heads of a warp
+  int j, sub, o1, o2;
+  bool turns;
+  __device__ __forceinline__ Place(int rotary, bool near) {
+    const int lane = threadIdx.x & 31;
+    j = lane % LANES;
+    sub = lane / LANES;
+    turns = 16 * j < rotary;
+    o1 = turns && !near ? 8 * j : 16 * j;
+    o2 = turns && !near ? rotary / 2 + 8 * j : 16 * j + 8;
+  }
+};
 
+// The query heads of token n: items part, part + parts, ... of HPW heads each; the next one is under way behind the present one.
+template <typename T, typename C, int D, bool NEAR>
+__device__ __forceinline__ void append_queries(const Int4AppendArgs& a, int64_t n, int64_t pos, int part, int parts) {
+  const Place<D> at(a.rotary, NEAR);
+  constexpr int LANES = Place<D>::LANES, HPW = Place<D>::HPW;
+  const int64_t q_step = static_cast<int64_t>(parts) * HPW * a.sq_h, o_step = static_cast<int64_t>(parts) * HPW * a.sqo_h;
+  const T* q1 = static_cast<const T*>(a.q) + n * a.sq_n + (part * HPW + at.sub) * a.sq_h + at.o1;
+  const T* q2 = q1 + (at.o2 - at.o1);
+  int qh = part * HPW + at.sub, h = qh;   // the head that is loaded next, and the one that is stored next
+  auto load = [&](Chunks& x) {
+    if (qh < a.H) {
+      x.a = *reinterpret_cast<const uint4*>(q1);
+      x.b = *reinterpret_cast<const uint4*>(q2);
+    }
+    q1 += q_step;
+    q2 += q_step;
+    qh += parts * HPW;
+  };
+  Chunks c0{}, c1{};
+  load(c0);
+  // y1 = r (x1 f11 + x2 f12), y2 = r (x2 f22 + x1 f21), r the norm's factor: the weights' products with cos and sin. Pairs
+  // 2 i and 2 i + 1 share an instruction (neighbours: the two chunks' i-th pairs).
+  F2 f11[4], f12[4], f22[4], f21[4];
+  {
+    float c[8], sn[8], w[16];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      c[e] = 1.f;
+      sn[e] = 0.f;
+      w[e] = w[8 + e] = 1.f;
+    }
+    if (at.turns) {
+      load8(static_cast<const C*>(a.cos) + pos * a.ld_cs + 8 * at.j, c);
+      load8(static_cast<const C*>(a.sin) + pos * a.ld_cs + 8 * at.j, sn);
+    }
+    if (a.q_weight) {
+      load8(static_cast<const T*>(a.q_weight) + at.o1, w);
+      load8(static_cast<const T*>(a.q_weight) + at.o2, w + 8);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int e0 = NEAR ? i : 2 * i, e1 = NEAR ? i + 4 : 2 * i + 1;   // the pairs
+      const float u0 = w[NEAR ? 2 * e0 : e0], v0 = w[NEAR ? 2 * e0 + 1 : 8 + e0], u1 = w[NEAR ? 2 * e1 : e1], v1 = w[NEAR ? 2 * e1 + 1 : 8 + e1];
+      f11[i] = pack(c[e0] * u0, c[e1] * u1);
+      f12[i] = pack(-sn[e0] * v0, -sn[e1] * v1);
+      f22[i] = pack(c[e0] * v0, c[e1] * v1);
+      f21[i] = pack(sn[e0] * u0, sn[e1] * u1);
+    }
+  }
+  T* p1 = static_cast<T*>(a.q_out) + n * a.sqo_n + h * a.sqo_h + at.o1;
+  T* p2 = p1 + (at.o2 - at.o1);
+  auto step = [&](const Chunks& now) {
+    F2 x1[4], x2[4];
+    if constexpr (NEAR) {
+      float xa[8], xb[8];
+      unpack8<T>(now.a, xa);
+      unpack8<T>(now.b, xb);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x1[i] = pack(xa[2 * i], xb[2 * i]);
+        x2[i] = pack(xa[2 * i + 1], xb[2 * i + 1]);
+      }
+    } else {
+      unpack8<T>(now.a, x1);
+      unpack8<T>(now.b, x2);
+    }
+    float r = 1.f;
+    if (a.q_weight) {
+      F2 s1 = mul2(x1[0], x1[0]), s2 = mul2(x2[0], x2[0]);
+#pragma unroll
+      for (int i = 1; i < 4; ++i) {
+        s1 = fma2(x1[i], x1[i], s1);
+        s2 = fma2(x2[i], x2[i], s2);
+      }
+      float ss, st;
+      unpack(add2(s1, s2), ss, st);
+      ss += st;
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      r = rsqrtf(fmaf(ss, 1.f / D, a.eps));
+    }
+    const F2 r2 = pack(r, r);
+    float y[16];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      F2 y1 = mul2(x1[i], f11[i]), y2 = mul2(x2[i], f22[i]);
+      if (at.turns) {   // (else f12 and f21 are zeros, which an infinity would make NaN)
+        y1 = fma2(x2[i], f12[i], y1);
+        y2 = fma2(x1[i], f21[i], y2);
+      }
+      y1 = mul2(y1, r2);
+      y2 = mul2(y2, r2);
+      if constexpr (NEAR) {
+        unpack(y1, y[2 * i], y[8 + 2 * i]);
+        unpack(y2, y[2 * i + 1], y[8 + 2 * i + 1]);
+      } else {
+        unpack(y1, y[2 * i], y[2 * i + 1]);
+        unpack(y2, y[8 + 2 * i], y[8 + 2 * i + 1]);
+      }
+    }
+    if (h < a.H) {
+      *reinterpret_cast<uint4*>(p1) = pack8<T>(y);
+      *reinterpret_cast<uint4*>(p2) = pack8<T>(y + 8);
+    }
+    p1 += o_step;
+    p2 += o_step;
+    h += parts * HPW;
+  };
+  int left = ((a.H + HPW - 1) / HPW - part + parts - 1) / parts;
+  while (left > 0) {   // two buffers in turn, neither of them moved
+    load(c1);
+    step(c0);
+    if (--left == 0) break;
+    load(c0);
+    step(c1);
+    --left;
+  }
+}
+
+// The key and value heads of token n: items part, part + parts, ... of the keys', then the values'.
+template <typename T, typename C, int D, bool NEAR>
+__device__ __forceinline__ void append_keys_values(const Int4AppendArgs& a, int64_t n, int64_t pos, int seq, int part, int parts,
+                                                   float (*s_row)[D]) {
+  const Place<D> at(a.rotary, NEAR);
+  constexpr int LANES = Place<D>::LANES, HPW = Place<D>::HPW;
+  const int KVH = a.kv.KVH, run_lanes = a.kv.group / 16, runs = D / a.kv.group, items = (KVH + HPW - 1) / HPW, j = at.j;
   auto load = [&](int item) {
     Chunks x{make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-    if (item < q_items) {
-      const int h = item * HPW + sub;
-      if (h < a.H) {
-        const T* p = static_cast<const T*>(a.q) + n * a.sq_n + h * a.sq_h;
-        x.a = *reinterpret_cast<const uint4*>(p + o1);
-        x.b = *reinterpret_cast<const uint4*>(p + o2);
-      }
-    } else if (item < items) {
-      const bool key = item < q_items + kv_items;
-      const int h = (item - q_items - (key ? 0 : kv_items)) * HPW + sub;
-      if (h < KVH) {
-        const T* p = key ? static_cast<const T*>(a.k) + n * a.sk_n + h * a.sk_h : static_cast<const T*>(a.v) + n * a.sv_n + h * a.sv_h;
-        x.a = __ldg(reinterpret_cast<const uint4*>(p + (key ? o1 : 16 * j)));
-        x.b = __ldg(reinterpret_cast<const uint4*>(p + (key ? o2 : 16 * j + 8)));
-      }
+    const bool key = item < items;
+    const int h = (key ? item : item - items) * HPW + at.sub;
+    if (item < 2 * items && h < KVH) {
+      const T* p = key ? static_cast<const T*>(a.k) + n * a.sk_n + h * a.sk_h : static_cast<const T*>(a.v) + n * a.sv_n + h * a.sv_h;
+      x.a = __ldg(reinterpret_cast<const uint4*>(p + (key ? at.o1 : 16 * j)));
+      x.b = __ldg(reinterpret_cast<const uint4*>(p + (key ? at.o2 : 16 * j + 8)));
     }
     return x;
   };
   Chunks next = load(part);
-  // where the token's entries go
-  int page = -1, tile_row = 0;
-  const uint8_t* head0 = nullptr;
-  if (pos < static_cast<int64_t>(a.pages_per_seq) * a.kv.page_size) {
-    const int p = static_cast<int>(pos), pi = a.div.page(p);
-    page = a.table[static_cast<int64_t>(seq) * a.ld_table + pi];
-    if (page >= a.kv.num_pages) page = -1;
-    if (page >= 0) {
-      const int slot = a.div.slot(p, pi);
-      tile_row = slot % kTileKeys;
-      head0 = a.kv.pages + page * a.kv.sp_p + static_cast<int64_t>(slot / kTileKeys) * int4_tile_bytes(D, runs);
-    }
-  }
-  Turn t;
-  if (turns) {
-    load8(static_cast<const C*>(a.cos) + pos * a.ld_cs + 8 * j, t.c);
-    load8(static_cast<const C*>(a.sin) + pos * a.ld_cs + 8 * j, t.s);
-  }
-  float w[16];
-  const void* loaded = nullptr;   // the weights in w
-  for (int item = part; item < items; item += a.parts) {
+  if (pos >= static_cast<int64_t>(a.pages_per_seq) * a.kv.page_size) return;
+  const int p = static_cast<int>(pos), pi = a.div.page(p), slot = a.div.slot(p, pi), tile_row = slot % kTileKeys;
+  const int page = a.table[static_cast<int64_t>(seq) * a.ld_table + pi];
+  if (page < 0 || page >= a.kv.num_pages) return;   // the whole warp
+  uint8_t* const head0 = a.kv.pages + page * a.kv.sp_p + static_cast<int64_t>(slot / kTileKeys) * int4_tile_bytes(D, runs) + at.sub * a.kv.sp_h;
+#pragma unroll 1
+  for (int item = part; item < 2 * items; item += parts) {
     const Chunks now = next;
-    next = load(item + a.parts);
+    next = load(item + parts);
+    const bool key = item < items;
+    const int h0 = (key ? item : item - items) * HPW;
+    const bool on = h0 + at.sub < KVH;
+    uint8_t* const tile = head0 + h0 * a.kv.sp_h;
     float x[16];
+    uint32_t code[16];
     unpack8<T>(now.a, x);
     unpack8<T>(now.b, x + 8);
-    if (item < q_items + kv_items) {   // norm and rotation
-      const bool key = item >= q_items;
-      const void* weight = key ? a.k_weight : a.q_weight;
-      if (weight) {
-        if (weight != loaded) {
-          load8(static_cast<const T*>(weight) + o1, w);
-          load8(static_cast<const T*>(weight) + o2, w + 8);
-          loaded = weight;
+    if (key) {
+      if (a.k_weight) {
+        float w[16];
+        load8(static_cast<const T*>(a.k_weight) + at.o1, w);
+        load8(static_cast<const T*>(a.k_weight) + at.o2, w + 8);
+        double ss = 0.0, st = 0.0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          ss = fma(static_cast<double>(x[e]), static_cast<double>(x[e]), ss);
+          st = fma(static_cast<double>(x[8 + e]), static_cast<double>(x[8 + e]), st);
         }
-        float r;
-        if (key) {
-          double ss = 0.0;
+        ss += st;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) ss = fma(static_cast<double>(x[e]), static_cast<double>(x[e]), ss);
-#pragma unroll
-          for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-          r = static_cast<float>(rsqrt(ss / D + static_cast<double>(a.eps)));
-        } else {
-          float ss = 0.f;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) ss = fmaf(x[e], x[e], ss);
-#pragma unroll
-          for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-          r = rsqrtf(fmaf(ss, 1.f / D, a.eps));
-        }
+        for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float r = static_cast<float>(rsqrt(ss / D + static_cast<double>(a.eps)));
 #pragma unroll
         for (int e = 0; e < 16; ++e) x[e] = __fmul_rn(__fmul_rn(x[e], r), w[e]);
       }
-      if (!key) {
-        if (turns) turn<false>(x, t, a.interleaved);
-        const int h = item * HPW + sub;
-        if (h < a.H) {
-          T* p = static_cast<T*>(a.q_out) + n * a.sqo_n + h * a.sqo_h;
-          *reinterpret_cast<uint4*>(p + o1) = pack8<T>(x);
-          *reinterpret_cast<uint4*>(p + o2) = pack8<T>(x + 8);
+      if (at.turns) {
+        float c[8], s[8];
+        load8(static_cast<const C*>(a.cos) + pos * a.ld_cs + 8 * j, c);
+        load8(static_cast<const C*>(a.sin) + pos * a.ld_cs + 8 * j, s);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {   // (a, b) -> (a c - b s, b c + a s), every product and sum rounded by itself
+          float &x1 = x[NEAR ? 2 * e : e], &x2 = x[NEAR ? 2 * e + 1 : 8 + e];
+          const float y1 = __fsub_rn(__fmul_rn(x1, c[e]), __fmul_rn(x2, s[e]));
+          x2 = __fadd_rn(__fmul_rn(x2, c[e]), __fmul_rn(x1, s[e]));
+          x1 = y1;
         }
-        continue;
       }
-      if (turns) turn<true>(x, t, a.interleaved);
-    }
-    if (page < 0) continue;   // the whole warp
-    const bool key = item < q_items + kv_items;
-    const int h = (item - q_items - (key ? 0 : kv_items)) * HPW + sub;
-    uint8_t* const tile = const_cast<uint8_t*>(head0) + h * a.kv.sp_h;
-    uint32_t code[16];
-    if (key) {
-      if (a.cos && !a.interleaved) {   // into neighbouring elements
-        float* row = s_row[warp][sub];
+      if (!NEAR && a.rotary > 0) {   // into neighbouring elements
+        float* row = s_row[at.sub];
 #pragma unroll
         for (int e = 0; e < 8; e += 4) {
-          *reinterpret_cast<float4*>(row + o1 + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
-          *reinterpret_cast<float4*>(row + o2 + e) = make_float4(x[8 + e], x[9 + e], x[10 + e], x[11 + e]);
+          *reinterpret_cast<float4*>(row + at.o1 + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+          *reinterpret_cast<float4*>(row + at.o2 + e) = make_float4(x[8 + e], x[9 + e], x[10 + e], x[11 + e]);
         }
         __syncwarp();
 #pragma unroll
@@ -246,33 +384,50 @@ __global__ void __launch_bounds__(kWarps * 32) int4_append_kernel(const __grid_c
         }
         __syncwarp();
       }
-      const uint32_t sm = quantise<T>(x, run_lanes, code);
+    }
+    const uint32_t sm = quantise<T>(x, run_lanes, code);
+    if (key) {
       // lane j has step j: one byte of each half of the words (t', j / 2), t' = 0..3; the pair of lanes joins them
       uint32_t v[4];
+      constexpr uint32_t kAbove = 0x4B400000u * (1u + (1u << 4) + (1u << 16) + (1u << 20));   // what lies above the codes
 #pragma unroll
       for (int u = 0; u < 4; ++u)
-        v[u] = code[4 * u] | code[4 * u + 2] << 4 | code[4 * u + 1] << 16 | code[4 * u + 3] << 20;
+        v[u] = code[4 * u] + (code[4 * u + 2] << 4) + (code[4 * u + 1] << 16) + (code[4 * u + 3] << 20) - kAbove;
       const bool upper = j & 1;
       const uint32_t r0 = __shfl_xor_sync(0xffffffffu, upper ? v[0] : v[2], 1);
       const uint32_t r1 = __shfl_xor_sync(0xffffffffu, upper ? v[1] : v[3], 1);
-      if (h < KVH) {
+      if (on) {
         uint8_t* row = tile + tile_row * (D / 2) + (upper ? 2 : 0) * (D / 8) + 4 * (j / 2);
         *reinterpret_cast<uint32_t*>(row) = upper ? r0 | v[2] << 8 : v[0] | r0 << 8;
         *reinterpret_cast<uint32_t*>(row + D / 8) = upper ? r1 | v[3] << 8 : v[1] | r1 << 8;
         if (j % run_lanes == 0)
           *reinterpret_cast<uint32_t*>(tile + int4_ks_off(D) + (tile_row * runs + j / run_lanes) * 4) = sm;
       }
-    } else {
-      const uint32_t sm = quantise<T>(x, run_lanes, code);
-      if (h < KVH) {
-        uint8_t* p = tile + int4_v_off(D) + (j / 4) * 512 + ((tile_row % 8) / 2) * 16 + (j % 4) * 4 + (tile_row & 1) * 2 + tile_row / 8;
+    } else if (on) {
+      uint8_t* b = tile + int4_v_off(D) + (j / 4) * 512 + ((tile_row % 8) / 2) * 16 + (j % 4) * 4 + (tile_row & 1) * 2 + tile_row / 8;
 #pragma unroll
-        for (int g = 0; g < 8; ++g) p[g * 64] = static_cast<uint8_t>(code[g] | code[g + 8] << 4);
-        if (j % run_lanes == 0)
-          *reinterpret_cast<uint32_t*>(tile + int4_vs_off(D, runs) + (tile_row * runs + j / run_lanes) * 4) = sm;
-      }
+      for (int g = 0; g < 8; ++g) b[g * 64] = static_cast<uint8_t>(code[g] + (code[g + 8] << 4));
+      if (j % run_lanes == 0)
+        *reinterpret_cast<uint32_t*>(tile + int4_vs_off(D, runs) + (tile_row * runs + j / run_lanes) * 4) = sm;
     }
   }
+}
+
+// T: cache and activation dtype, C: the tables' type, NEAR: pairs of neighbouring elements. Of a token's gridDim.y warps (in
+// blocks of their own) the first q_parts take the queries.
+template <typename T, typename C, int D, bool NEAR>
+__global__ void __launch_bounds__(kWarps * 32, 6) int4_append_kernel(const __grid_constant__ Int4AppendArgs a) {
+  __shared__ __align__(16) float s_row[kWarps][Place<D>::HPW][D];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, part = blockIdx.y;
+  const int64_t n = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
+  if (n >= a.N) return;
+  const int64_t pos = a.positions[n];
+  const int seq = a.seq_ids ? a.seq_ids[n] : sequence_of(static_cast<int>(n), a.per_seq, a.per_inv);
+  if (seq < 0 || seq >= a.B || pos < 0 || pos >= a.limit) return;   // padding
+  if (part < a.q_parts) append_queries<T, C, D, NEAR>(a, n, pos, part, a.q_parts);
+  else append_keys_values<T, C, D, NEAR>(a, n, pos, seq, part - a.q_parts, gridDim.y - a.q_parts, s_row[warp]);
 }
 
 struct Int4ReadArgs {
@@ -283,7 +438,8 @@ struct Int4ReadArgs {
   void* v; int64_t sv_n, sv_h;
   b2d_int4_kv kv;
   PageDiv div;
-  int N, B, per_seq, pages_per_seq, parts;
+  int N, B, per_seq, pages_per_seq;
+  uint32_t per_inv;
 };
 
 // The inverse, lane for lane: 16 neighbouring elements of a head from the step's bytes. O: output type.
@@ -293,87 +449,101 @@ __global__ void __launch_bounds__(kWarps * 32) int4_read_kernel(const __grid_con
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = lane % LANES, sub = lane / LANES;
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
-  const int64_t n = unit / a.parts;
-  const int part = static_cast<int>(unit - n * a.parts);
+  const int64_t n = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
   if (n >= a.N) return;
   const int64_t pos = a.positions[n];
-  const int seq = a.seq_ids ? a.seq_ids[n] : static_cast<int>(n) / a.per_seq;
+  const int seq = a.seq_ids ? a.seq_ids[n] : sequence_of(static_cast<int>(n), a.per_seq, a.per_inv);
   if (seq < 0 || seq >= a.B || pos < 0 || pos >= static_cast<int64_t>(a.pages_per_seq) * a.kv.page_size) return;
   const int KVH = a.kv.KVH, run_lanes = a.kv.group / 16, runs = D / a.kv.group;
-  const int k_items = a.k ? (KVH + HPW - 1) / HPW : 0, items = k_items + (a.v ? (KVH + HPW - 1) / HPW : 0);
+  const int items = (KVH + HPW - 1) / HPW;
   const int p = static_cast<int>(pos), pi = a.div.page(p), slot = a.div.slot(p, pi), row = slot % kTileKeys;
   const int page = a.table[static_cast<int64_t>(seq) * a.ld_table + pi];
   const bool there = page >= 0 && page < a.kv.num_pages;
-  const uint8_t* head0 = a.kv.pages + (there ? page * a.kv.sp_p + static_cast<int64_t>(slot / kTileKeys) * int4_tile_bytes(D, runs) : 0);
-  for (int item = part; item < items; item += a.parts) {
-    const bool key = item < k_items;
-    const int h = (item - (key ? 0 : k_items)) * HPW + sub;
-    if (h >= KVH) continue;
-    float x[16];
-    if (there) {
-      const uint8_t* tile = head0 + h * a.kv.sp_h;
-      uint32_t code[16];
-      const uint32_t sm = __ldg(reinterpret_cast<const uint32_t*>(tile + (key ? int4_ks_off(D) : int4_vs_off(D, runs)) + (row * runs + j / run_lanes) * 4));
-      if (key) {
+  const uint8_t* tile = a.kv.pages + (there ? page * a.kv.sp_p + static_cast<int64_t>(slot / kTileKeys) * int4_tile_bytes(D, runs) : 0) +
+                        (blockIdx.y * HPW + sub) * a.kv.sp_h;
+  O* ko = static_cast<O*>(a.k) + n * a.sk_n + (blockIdx.y * HPW + sub) * a.sk_h + 16 * j;
+  O* vo = static_cast<O*>(a.v) + n * a.sv_n + (blockIdx.y * HPW + sub) * a.sv_h + 16 * j;
+  const int64_t heads = static_cast<int64_t>(gridDim.y) * HPW;
+  for (int item = blockIdx.y; item < items; item += gridDim.y, tile += heads * a.kv.sp_h, ko += heads * a.sk_h, vo += heads * a.sv_h) {
+    if (item * HPW + sub >= KVH) continue;
+    uint32_t kw[4], vw[8], ksm = 0, vsm = 0;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(tile + row * (D / 2) + u * (D / 8) + 4 * (j / 2))) >> 8 * (j & 1);
-          code[4 * u] = w & 15;
-          code[4 * u + 1] = w >> 16 & 15;
-          code[4 * u + 2] = w >> 4 & 15;
-          code[4 * u + 3] = w >> 20 & 15;
-        }
-      } else {
+    for (int u = 0; u < 4; ++u) kw[u] = vw[u] = vw[4 + u] = 0;
+    if (there) {   // every load under way before the first is used
+      if (a.k) {
+        ksm = __ldg(reinterpret_cast<const uint32_t*>(tile + int4_ks_off(D) + (row * runs + j / run_lanes) * 4));
+        const uint8_t* b = tile + row * (D / 2) + 4 * (j / 2);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) kw[u] = __ldg(reinterpret_cast<const uint32_t*>(b + u * (D / 8)));
+      }
+      if (a.v) {
+        vsm = __ldg(reinterpret_cast<const uint32_t*>(tile + int4_vs_off(D, runs) + (row * runs + j / run_lanes) * 4));
         const uint8_t* b = tile + int4_v_off(D) + (j / 4) * 512 + ((row % 8) / 2) * 16 + (j % 4) * 4 + (row & 1) * 2 + row / 8;
 #pragma unroll
-        for (int g = 0; g < 8; ++g) {
-          const uint32_t w = __ldg(b + g * 64);
-          code[g] = w & 15;
-          code[g + 8] = w >> 4;
-        }
+        for (int g = 0; g < 8; ++g) vw[g] = __ldg(b + g * 64);
       }
-      const float2 f = unpack_sm<T>(sm);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) x[e] = fmaf(f.x, static_cast<float>(code[e]), f.y);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) x[e] = 0.f;
     }
-    O* o = static_cast<O*>(key ? a.k : a.v) + n * (key ? a.sk_n : a.sv_n) + h * (key ? a.sk_h : a.sv_h) + 16 * j;
-    if constexpr (sizeof(O) == 4) {
+    auto put = [&](O* o, uint32_t sm, const uint32_t (&code)[16]) {   // codes in the words' low bits
+      const float2 f = unpack_sm<T>(sm);
+      const F2 s2 = pack(f.x, f.x), m2 = pack(f.y, f.y), base2 = pack(-8388608.f, -8388608.f);
+      float x[16];
 #pragma unroll
-      for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4*>(o + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
-    } else {
-      *reinterpret_cast<uint4*>(o) = pack8<O>(x);
-      *reinterpret_cast<uint4*>(o + 8) = pack8<O>(x + 8);
+      for (int e = 0; e < 16; e += 2) {   // a code behind 2^23 in a float's bits
+        const F2 c = pack(__uint_as_float((code[e] & 15u) | 0x4B000000u), __uint_as_float((code[e + 1] & 15u) | 0x4B000000u));
+        unpack(fma2(s2, add2(c, base2), m2), x[e], x[e + 1]);
+      }
+      if constexpr (sizeof(O) == 4) {
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4*>(o + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+      } else {
+        *reinterpret_cast<uint4*>(o) = pack8<O>(x);
+        *reinterpret_cast<uint4*>(o + 8) = pack8<O>(x + 8);
+      }
+    };
+    uint32_t code[16];
+    if (a.k) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const uint32_t w = kw[u] >> 8 * (j & 1);
+        code[4 * u] = w;
+        code[4 * u + 1] = w >> 16;
+        code[4 * u + 2] = w >> 4;
+        code[4 * u + 3] = w >> 20;
+      }
+      put(ko, ksm, code);
+    }
+    if (a.v) {
+#pragma unroll
+      for (int g = 0; g < 8; ++g) {
+        code[g] = vw[g];
+        code[g + 8] = vw[g] >> 4;
+      }
+      put(vo, vsm, code);
     }
   }
 }
 
-// Warps a token: enough for a few per scheduler, at most one per item.
+// Warps a token of a share of the work, at most one per item: enough of them to fill the SMs several times over.
 int warps_per_token(int64_t N, int items, int sm) {
-  int parts = 1;
-  while (parts < items && N * parts < static_cast<int64_t>(sm) * 128) parts *= 2;
-  return parts < items ? parts : items;
+  const int64_t parts = (static_cast<int64_t>(sm) * 24 + N - 1) / N;
+  return static_cast<int>(parts < items ? parts : items);
 }
 
 template <typename T, typename C, int D>
-int launch_append(Int4AppendArgs& a, int sm, bool pdl, cudaStream_t s) {
-  constexpr int HPW = 512 / D;
-  const int items = (a.q ? (a.H + HPW - 1) / HPW : 0) + 2 * ((a.kv.KVH + HPW - 1) / HPW);
-  a.parts = warps_per_token(a.N, items, sm);
-  const int64_t blocks = (static_cast<int64_t>(a.N) * a.parts + kWarps - 1) / kWarps;
-  if (blocks > INT32_MAX) return B2D_ERR_SHAPE;
-  return launch_kernel(int4_append_kernel<T, C, D>, dim3(static_cast<unsigned>(blocks)), dim3(kWarps * 32), 0, s, pdl, a);
+int launch_append(Int4AppendArgs& a, bool near, int sm, bool pdl, cudaStream_t s) {
+  constexpr int HPW = Place<D>::HPW;
+  a.q_parts = a.q && a.H > 0 ? warps_per_token(a.N, (a.H + HPW - 1) / HPW, sm) : 0;
+  const dim3 grid((a.N + kWarps - 1) / kWarps, a.q_parts + warps_per_token(a.N, 2 * ((a.kv.KVH + HPW - 1) / HPW), sm));
+  if (grid.y > 65535) return B2D_ERR_SHAPE;
+  if (near) return launch_kernel(int4_append_kernel<T, C, D, true>, grid, dim3(kWarps * 32), 0, s, pdl, a);
+  return launch_kernel(int4_append_kernel<T, C, D, false>, grid, dim3(kWarps * 32), 0, s, pdl, a);
 }
 template <typename T, typename O, int D>
-int launch_read(Int4ReadArgs& a, int sm, bool pdl, cudaStream_t s) {
+int launch_read(const Int4ReadArgs& a, int sm, bool pdl, cudaStream_t s) {
   constexpr int HPW = 512 / D;
-  a.parts = warps_per_token(a.N, ((a.k ? 1 : 0) + (a.v ? 1 : 0)) * ((a.kv.KVH + HPW - 1) / HPW), sm);
-  const int64_t blocks = (static_cast<int64_t>(a.N) * a.parts + kWarps - 1) / kWarps;
-  if (blocks > INT32_MAX) return B2D_ERR_SHAPE;
-  return launch_kernel(int4_read_kernel<T, O, D>, dim3(static_cast<unsigned>(blocks)), dim3(kWarps * 32), 0, s, pdl, a);
+  const int items = (a.kv.KVH + HPW - 1) / HPW;
+  const dim3 grid((a.N + kWarps - 1) / kWarps, warps_per_token(a.N, items, sm));
+  return launch_kernel(int4_read_kernel<T, O, D>, grid, dim3(kWarps * 32), 0, s, pdl, a);
 }
 
 int check_tokens(const b2d_int4_kv* kv, const int32_t* seq_ids, int N, int B, int64_t ld_table, int pages_per_seq) {
@@ -415,17 +585,18 @@ extern "C" int b2d_int4_append(const b2d_int4_kv* kv, const void* q, int64_t sq_
   if ((st = device_info(&di)) != B2D_OK) return st;
   Int4AppendArgs a{q, sq_n, sq_h, k, sk_n, sk_h, v, sv_n, sv_h, positions, seq_ids, page_table, ld_table, cos, sin, ld_cs,
                    q_weight, k_weight, eps, q_out, sqo_n, sqo_h, *kv, page_div(kv->page_size), N, H, B, seq_ids ? 1 : N / B,
-                   pages_per_seq, cos ? rotary_dim : 0, interleaved != 0, 1, cos ? S_max : INT64_MAX};
+                   pages_per_seq, cos ? rotary_dim : 0, 0, inverse_of(seq_ids ? 1 : N / B), cos ? S_max : INT64_MAX};
   const bool pdl = (flags & B2D_LAUNCH_PDL) != 0, f32 = cos && cs_dtype == B2D_F32;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int sm = di.sm_count;
+  const bool near = cos && interleaved;
   if (kv->dtype == B2D_F16) {
-    if (kv->D == 64) return f32 ? launch_append<__half, float, 64>(a, sm, pdl, s) : launch_append<__half, __half, 64>(a, sm, pdl, s);
-    return f32 ? launch_append<__half, float, 128>(a, sm, pdl, s) : launch_append<__half, __half, 128>(a, sm, pdl, s);
+    if (kv->D == 64) return f32 ? launch_append<__half, float, 64>(a, near, sm, pdl, s) : launch_append<__half, __half, 64>(a, near, sm, pdl, s);
+    return f32 ? launch_append<__half, float, 128>(a, near, sm, pdl, s) : launch_append<__half, __half, 128>(a, near, sm, pdl, s);
   }
   if (kv->D == 64)
-    return f32 ? launch_append<__nv_bfloat16, float, 64>(a, sm, pdl, s) : launch_append<__nv_bfloat16, __nv_bfloat16, 64>(a, sm, pdl, s);
-  return f32 ? launch_append<__nv_bfloat16, float, 128>(a, sm, pdl, s) : launch_append<__nv_bfloat16, __nv_bfloat16, 128>(a, sm, pdl, s);
+    return f32 ? launch_append<__nv_bfloat16, float, 64>(a, near, sm, pdl, s) : launch_append<__nv_bfloat16, __nv_bfloat16, 64>(a, near, sm, pdl, s);
+  return f32 ? launch_append<__nv_bfloat16, float, 128>(a, near, sm, pdl, s) : launch_append<__nv_bfloat16, __nv_bfloat16, 128>(a, near, sm, pdl, s);
 }
 
 extern "C" int b2d_int4_read(const b2d_int4_kv* kv, const int64_t* positions, const int32_t* seq_ids, const int32_t* page_table,
@@ -444,7 +615,7 @@ extern "C" int b2d_int4_read(const b2d_int4_kv* kv, const int64_t* positions, co
   DeviceInfo di;
   if ((st = device_info(&di)) != B2D_OK) return st;
   Int4ReadArgs a{positions, seq_ids, page_table, ld_table, k_out, sk_n, sk_h, v_out, sv_n, sv_h, *kv,
-                 page_div(kv->page_size), N, B, seq_ids ? 1 : N / B, pages_per_seq, 1};
+                 page_div(kv->page_size), N, B, seq_ids ? 1 : N / B, pages_per_seq, inverse_of(seq_ids ? 1 : N / B)};
   const bool pdl = (flags & B2D_LAUNCH_PDL) != 0, f32 = out_dtype == B2D_F32;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int sm = di.sm_count;
