@@ -488,7 +488,7 @@ int b2d_int4_read(const b2d_int4_kv* kv, const int64_t* positions, const int32_t
                   int64_t sv_n, int64_t sv_h, int out_dtype, int N, int flags, void* stream);
 
 /* b2d_paged_attention over a 4-bit cache (no shared prefix): arguments, masks, lengths, workspace and limits as there (the
- * page table reaches less than 2^31 - 4096 positions). q has the cache's dtype. Keys and values enter the products as codes
+ * page table reaches at most 2^31 - 32768 positions). q has the cache's dtype. Keys and values enter the products as codes
  * (exact); a weight times its value's s is rounded to fp16 (2^-11) for the second product, everything else is fp32. */
 size_t b2d_int4_attention_workspace_bytes(const b2d_int4_kv* kv, int B, int T, int H, int pages_per_seq, int max_len);
 int b2d_int4_attention(const b2d_int4_kv* kv, const void* q, int64_t sq_b, int64_t sq_t, int64_t sq_h,

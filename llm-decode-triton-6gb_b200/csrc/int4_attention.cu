@@ -34,6 +34,9 @@ constexpr int kStage = kWarps * kTileKeys;      // keys of a position of the lin
 constexpr int kMaxT = 16, kMaxG = 16;
 constexpr int kMaxBatch = 256;                  // sequences of a launch (larger batches take several)
 constexpr int kMaxCtas = 640;
+// Up to so many keys a unit is one CTA's, and there is no combine launch (8 sequences of up to 256 keys, 8 KV heads: 8.2 -> 7.5 us; of
+// 300: 7.4 -> 7.9); with two units an SM or more up to twice as many (64 sequences of up to 512 keys: 16.5 -> 13.7 us).
+constexpr int kWholeKeys = 256;
 constexpr float kLazy = 8.f;                    // log2 of the largest weight before the running maximum moves
 constexpr float kNone = -1.7e38f;               // running maximum before the first score
 constexpr float kLog2e = 1.4426950408889634f;
@@ -122,7 +125,7 @@ __device__ __forceinline__ void store_out2(const Int4AttnArgs& a, int64_t off, f
 // positions [share(c), share(c + 1)); the host has checked that they fit 31 bits. In whole mode a unit is one position.
 template <int NT>
 struct Line {
-  static constexpr int ROWS = 8 * NT, LEAD = 3;
+  static constexpr int ROWS = 8 * NT, LEAD = 5;
   int tiles, units, ctas, quota, extra;
   __device__ __forceinline__ Line(const Int4AttnArgs& a) {
     tiles = (a.rows + ROWS - 1) / ROWS;
@@ -230,11 +233,6 @@ __global__ void __launch_bounds__(kThreads, kBlocks<NT>) int4_attention_kernel(c
   constexpr int ROWS = 8 * NT, STEPS = D / 16, RSTEPS = STEPS / RUNS;   // products of a tile, and of a run of elements
   constexpr int TILE = S::TILE, SLOTS = S::SLOTS, KW = D / 32;          // KW: key words of a lane and key
   static_assert(SLOTS >= 2, "a ring of at least two tiles");
-  constexpr bool Q_REGS = NT <= 2;
-  // Codes enter the second product around their middle, 8: weights times codes from 0 to 15 would grow with the number of keys where
-  // their values cancel, and the tensor cores' sums cut what does not fit below. One row tile: a product with -8 throughout
-  // (8 a tile of keys); more: subtracted from the codes themselves (32, for all row tiles).
-  constexpr bool BY_PRODUCT = NT == 1;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float s_m[kWarps][ROWS], s_l[kWarps][ROWS];
   __shared__ float s_rowf[ROWS], s_qs[RUNS][ROWS];
@@ -307,43 +305,47 @@ __global__ void __launch_bounds__(kThreads, kBlocks<NT>) int4_attention_kernel(c
     const Segment g = segment_at<NT>(a, line, s_sum, s_len, pos, end);
     pos = g.next;
     if (g.kind < 0) continue;
-    // ---- Q: warp n prepares row tile n (every thread is behind the last unit's barriers)
-    for (int n = warp; n < NT; n += kWarps) {
-      const int r = 8 * n + g8, rr = g.row0 + r, t = div_g(a, rr);
-      const bool on = r < g.nrows;
-      const T* src = static_cast<const T*>(a.q) + g.b * a.sq_b + t * a.sq_t + static_cast<int64_t>(g.kvh * a.G + rr - t * a.G) * a.sq_h + 4 * tq;
-      uint2 raw[STEPS];
+    // ---- Q: D / 8 threads a row, 8 elements each (every thread is behind the last unit's barriers)
+    constexpr int QL = D / 8, QROWS = kThreads / QL, QN = (ROWS + QROWS - 1) / QROWS;   // threads a row, rows at a time, times
+    uint4 q_raw[QN];
 #pragma unroll
-      for (int j = 0; j < STEPS; ++j) raw[j] = on ? __ldg(reinterpret_cast<const uint2*>(src + 16 * j)) : make_uint2(0, 0);
-      float big = 0.f;
-      auto value = [&](int j, int e) { return Dt<T>::to_f32(reinterpret_cast<const T*>(&raw[j])[e]); };
+    for (int i = 0; i < QN; ++i) {
+      const int r = i * QROWS + tid / QL, rr = g.row0 + r, t = div_g(a, rr);
+      q_raw[i] = make_uint4(0, 0, 0, 0);
+      if (r < g.nrows)
+        q_raw[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + g.b * a.sq_b + t * a.sq_t +
+                                                        static_cast<int64_t>(g.kvh * a.G + rr - t * a.G) * a.sq_h + 8 * (tid % QL)));
+    }
 #pragma unroll
-      for (int j = 0; j < STEPS; ++j)
+    for (int i = 0; i < QN; ++i) {
+      const int r = i * QROWS + tid / QL, l = tid % QL;
+      const T* raw = reinterpret_cast<const T*>(&q_raw[i]);
+      float q[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) big = fmaxf(big, fabsf(value(j, e)));
-      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+      for (int e = 0; e < 8; ++e) q[e] = Dt<T>::to_f32(raw[e]);
+      float big = fmaxf(fmaxf(fmaxf(fabsf(q[0]), fabsf(q[1])), fmaxf(fabsf(q[2]), fabsf(q[3]))),
+                        fmaxf(fmaxf(fabsf(q[4]), fabsf(q[5])), fmaxf(fabsf(q[6]), fabsf(q[7]))));
+#pragma unroll
+      for (int x = 1; x < QL; x <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, x));
       // up = 2^x with 2^x big in [2^14, 2^15); |x| <= 100
       const int ex = static_cast<int>(__float_as_uint(big) >> 23);
       const int x = big > 0.f && ex < 255 ? min(max(14 + 127 - ex, -100), 100) : 0;
       const float up = __uint_as_float((127 + x) << 23), down = __uint_as_float((127 - x) << 23);
-      float qs[RUNS];
+      const bool on = ROWS % QROWS == 0 || r < ROWS;
+      float sum = 0.f;
 #pragma unroll
-      for (int u = 0; u < RUNS; ++u) qs[u] = 0.f;
-#pragma unroll
-      for (int j = 0; j < STEPS; ++j) {
-        const float q0 = value(j, 0) * up, q1 = value(j, 1) * up, q2 = value(j, 2) * up, q3 = value(j, 3) * up;
+      for (int h = 0; h < 2; ++h) {   // elements 16 (l / 2) + 8 (l & 1) + 4 h ..: step l / 2, lane 4 (r & 7) + 2 (l & 1) + h
+        const float q0 = q[4 * h] * up, q1 = q[4 * h + 1] * up, q2 = q[4 * h + 2] * up, q3 = q[4 * h + 3] * up;
         const __half2 lo = __floats2half2_rn(q0, q1), hi = __floats2half2_rn(q2, q3);
-        qs[j / RSTEPS] += (__low2float(lo) + __high2float(lo)) + (__low2float(hi) + __high2float(hi));
-        s_q[(n * STEPS + j) * 32 + lane] = make_uint2(Dt<__half>::pack2(q0, q1), Dt<__half>::pack2(q2 * 0.0625f, q3 * 0.0625f));
+        sum += (__low2float(lo) + __high2float(lo)) + (__low2float(hi) + __high2float(hi));
+        if (on)
+          s_q[((r >> 3) * STEPS + l / 2) * 32 + 4 * (r & 7) + 2 * (l & 1) + h] =
+              make_uint2(Dt<__half>::pack2(q0, q1), Dt<__half>::pack2(q2 * 0.0625f, q3 * 0.0625f));
       }
 #pragma unroll
-      for (int u = 0; u < RUNS; ++u) {
-        qs[u] += __shfl_xor_sync(0xffffffffu, qs[u], 1);
-        qs[u] += __shfl_xor_sync(0xffffffffu, qs[u], 2);
-        if (tq == 0) s_qs[u][r] = qs[u] * 0x1p-24f;
-      }
-      if (tq == 0) s_rowf[r] = down * 0x1p24f * a.scale_log2;
+      for (int x = 1; x < QL / RUNS; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      if (on && l % (QL / RUNS) == 0) s_qs[l / (QL / RUNS)][r] = sum * 0x1p-24f;
+      if (on && l == 0) s_rowf[r] = down * 0x1p24f * a.scale_log2;
     }
     if (tid < g.nrows) {
       const int rr = g.row0 + tid, t = div_g(a, rr), head = g.kvh * a.G + rr - t * a.G;
@@ -351,13 +353,6 @@ __global__ void __launch_bounds__(kThreads, kBlocks<NT>) int4_attention_kernel(c
                               : (static_cast<int64_t>(blockIdx.x) * 2 + (g.kind - 1)) * ROWS + tid;
     }
     __syncthreads();
-    uint2 qb[Q_REGS ? NT : 1][STEPS];   // row 8 n + g8, elements 16 j + 4 tq ..
-    if constexpr (Q_REGS) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int j = 0; j < STEPS; ++j) qb[n][j] = s_q[(n * STEPS + j) * 32 + lane];
-    }
     float rowf[NT][2], qs[RUNS][NT][2];   // of rows 8 n + 2 tq (+ 1)
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -402,7 +397,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks<NT>) int4_attention_kernel(c
           const uint32_t x = kw[0][j / 2] >> sh, y = kw[1][j / 2] >> sh;
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const uint2 q = Q_REGS ? qb[Q_REGS ? n : 0][j] : s_q[(n * STEPS + j) * 32 + lane];
+            const uint2 q = s_q[(n * STEPS + j) * 32 + lane];
             if (j % RSTEPS == 0) Mma<__half>::run0(acc[u][n], x & 0x000F000Fu, y & 0x000F000Fu, x & 0x00F000F0u, y & 0x00F000F0u, q.x, q.y);
             else Mma<__half>::run(acc[u][n], x & 0x000F000Fu, y & 0x000F000Fu, x & 0x00F000F0u, y & 0x00F000F0u, q.x, q.y);
           }
@@ -536,22 +531,11 @@ __global__ void __launch_bounds__(kThreads, kBlocks<NT>) int4_attention_kernel(c
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int m = 4 * c + i, u = m / RSTEPS;
-          uint32_t a0, a1 = vw[i] & 0x00F000F0u, a2, a3;
-          if constexpr (BY_PRODUCT) {
-            // whole bytes for element g8: 16 times element g8 + 8, which the other half has, is taken off at the end
-#pragma unroll
-            for (int n = 0; n < NT; ++n)   // -(8 + 128) and -128
-              Mma<__half>::run(o[m][n], 0x80888088u, 0x80808080u, 0x80888088u, 0x80808080u, pb[u][n][0], pb[u][n][1]);
-            a0 = vw[i] & 0x00FF00FFu;
-            a2 = __byte_perm(vw[i], 0u, 0x4341);
-            a3 = a2 & 0x00F000F0u;
-          } else {
-            const uint32_t y = vw[i] >> 8;
-            a0 = minus_8<4>(vw[i] & 0x000F000Fu);
-            a1 = minus_8<0>(a1);
-            a2 = minus_8<4>(y & 0x000F000Fu);
-            a3 = minus_8<0>(y & 0x00F000F0u);
-          }
+          const uint32_t y = vw[i] >> 8;
+          // around their middle: weights times codes from 0 to 15 would grow with the number of keys where their values cancel, and
+          // the tensor cores' sums cut what does not fit below
+          const uint32_t a0 = minus_8<4>(vw[i] & 0x000F000Fu), a1 = minus_8<0>(vw[i] & 0x00F000F0u);
+          const uint32_t a2 = minus_8<4>(y & 0x000F000Fu), a3 = minus_8<0>(y & 0x00F000F0u);
 #pragma unroll
           for (int n = 0; n < NT; ++n) Mma<__half>::run(o[m][n], a0, a1, a2, a3, pb[u][n][0], pb[u][n][1]);
         }
@@ -634,9 +618,8 @@ __global__ void __launch_bounds__(kThreads, kBlocks<NT>) int4_attention_kernel(c
 #pragma unroll
         for (int m = 0; m < STEPS; ++m) {
           const float b = om[m / RSTEPS][n][e];
-          const float hi = o[m][n][2 + e], lo = BY_PRODUCT ? o[m][n][e] - hi : o[m][n][e];
-          dst[16 * m] = fmaf(lo, to_lo, b) * factor;
-          dst[16 * m + 8] = fmaf(hi, to_hi, b) * factor;
+          dst[16 * m] = fmaf(o[m][n][e], to_lo, b) * factor;
+          dst[16 * m + 8] = fmaf(o[m][n][2 + e], to_hi, b) * factor;
         }
       }
       __syncthreads();
@@ -779,9 +762,9 @@ Plan make_plan(const b2d_int4_kv* kv, int B, int T, int H, int pages_per_seq, in
   const int tile = 8 * p.nt;
   const int64_t keys = max_len > 0 && max_len < reach ? max_len : reach;
   const int64_t units = static_cast<int64_t>(B) * kv->KVH * ((rows + tile - 1) / tile);
-  p.fits = units * ((reach + kStage - 1) / kStage + 4) < (int64_t(1) << 31);
-  p.whole = keys <= kStage;
-  int64_t ctas = p.whole ? units : units * ((keys + kStage - 1) / kStage + 4);
+  p.fits = units * ((reach + kStage - 1) / kStage + Line<1>::LEAD) < (int64_t(1) << 31);
+  p.whole = keys <= kWholeKeys || (keys <= 2 * kWholeKeys && units >= 2 * sm);
+  int64_t ctas = p.whole ? units : units * ((keys + kStage - 1) / kStage + Line<1>::LEAD);
   const int per_sm = p.nt == 1 ? kBlocks<1> : p.nt == 2 ? kBlocks<2> : kBlocks<3>;
   if (ctas > static_cast<int64_t>(per_sm) * sm) ctas = per_sm * sm;
   if (ctas > kMaxCtas) ctas = kMaxCtas;
