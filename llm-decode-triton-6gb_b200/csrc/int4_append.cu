@@ -442,7 +442,51 @@ struct Int4ReadArgs {
   uint32_t per_inv;
 };
 
-// The inverse, lane for lane: 16 neighbouring elements of a head from the step's bytes. O: output type.
+// The inverse, lane for lane: 16 neighbouring elements of a head from the step's bytes. O: output type. A warp has a token. A value
+// word holds four positions' bytes; where the 16 tokens of a tile lie together in the call (their 16 warps see that alike),
+// each of these warps takes four positions of the keys or of the values, and a quarter of the loads is left.
+template <typename T, typename O>
+__device__ __forceinline__ void put_values(O* o, uint32_t sm, const uint32_t (&code)[16]) {   // codes in the words' low bits
+  const float2 f = unpack_sm<T>(sm);
+  const F2 s2 = pack(f.x, f.x), m2 = pack(f.y, f.y), base2 = pack(-8388608.f, -8388608.f);
+  float x[16];
+#pragma unroll
+  for (int e = 0; e < 16; e += 2) {   // a code behind 2^23 in a float's bits
+    const F2 c = pack(__uint_as_float((code[e] & 15u) | 0x4B000000u), __uint_as_float((code[e + 1] & 15u) | 0x4B000000u));
+    unpack(fma2(s2, add2(c, base2), m2), x[e], x[e + 1]);
+  }
+  if constexpr (sizeof(O) == 4) {
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4*>(o + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+  } else {
+    *reinterpret_cast<uint4*>(o) = pack8<O>(x);
+    *reinterpret_cast<uint4*>(o + 8) = pack8<O>(x + 8);
+  }
+}
+template <typename T, typename O>
+__device__ __forceinline__ void put_key(O* o, uint32_t sm, const uint32_t (&w)[4], int j) {
+  uint32_t code[16];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const uint32_t x = w[u] >> 8 * (j & 1);
+    code[4 * u] = x;
+    code[4 * u + 1] = x >> 16;
+    code[4 * u + 2] = x >> 4;
+    code[4 * u + 3] = x >> 20;
+  }
+  put_values<T, O>(o, sm, code);
+}
+template <typename T, typename O>
+__device__ __forceinline__ void put_value(O* o, uint32_t sm, const uint32_t (&w)[8], int shift) {
+  uint32_t code[16];
+#pragma unroll
+  for (int g = 0; g < 8; ++g) {
+    code[g] = w[g] >> shift;
+    code[g + 8] = w[g] >> (shift + 4);
+  }
+  put_values<T, O>(o, sm, code);
+}
+
 template <typename T, typename O, int D>
 __global__ void __launch_bounds__(kWarps * 32) int4_read_kernel(const __grid_constant__ Int4ReadArgs a) {
   constexpr int LANES = D / 16, HPW = 32 / LANES;
@@ -459,13 +503,64 @@ __global__ void __launch_bounds__(kWarps * 32) int4_read_kernel(const __grid_con
   const int p = static_cast<int>(pos), pi = a.div.page(p), slot = a.div.slot(p, pi), row = slot % kTileKeys;
   const int page = a.table[static_cast<int64_t>(seq) * a.ld_table + pi];
   const bool there = page >= 0 && page < a.kv.num_pages;
-  const uint8_t* tile = a.kv.pages + (there ? page * a.kv.sp_p + static_cast<int64_t>(slot / kTileKeys) * int4_tile_bytes(D, runs) : 0) +
-                        (blockIdx.y * HPW + sub) * a.kv.sp_h;
-  O* ko = static_cast<O*>(a.k) + n * a.sk_n + (blockIdx.y * HPW + sub) * a.sk_h + 16 * j;
-  O* vo = static_cast<O*>(a.v) + n * a.sv_n + (blockIdx.y * HPW + sub) * a.sv_h + 16 * j;
-  const int64_t heads = static_cast<int64_t>(gridDim.y) * HPW;
-  for (int item = blockIdx.y; item < items; item += gridDim.y, tile += heads * a.kv.sp_h, ko += heads * a.sk_h, vo += heads * a.sv_h) {
-    if (item * HPW + sub >= KVH) continue;
+  const uint8_t* const tile0 = a.kv.pages + (there ? page * a.kv.sp_p + static_cast<int64_t>(slot / kTileKeys) * int4_tile_bytes(D, runs) : 0);
+  bool whole = gridDim.y == 1 && n >= row && n - row + kTileKeys <= a.N;
+  if (whole) {
+    const int64_t other = n - row + (lane & 15);
+    whole = a.positions[other] == pos - row + (lane & 15) &&
+            (a.seq_ids ? a.seq_ids[other] : sequence_of(static_cast<int>(other), a.per_seq, a.per_inv)) == seq;
+    whole = __all_sync(0xffffffffu, whole);
+  }
+  if (whole) {
+    const bool values = row & 4;
+    const int quarter = row & 3;
+    if (!(values ? a.v : a.k)) return;
+    const int64_t sn = values ? a.sv_n : a.sk_n, sh = values ? a.sv_h : a.sk_h;
+    O* const out0 = static_cast<O*>(values ? a.v : a.k) + (n - row) * sn + 16 * j;
+    for (int item = row >> 3; item < items; item += 2) {
+      const int h = item * HPW + sub;
+      if (h >= KVH) continue;
+      const uint8_t* const tile = tile0 + h * a.kv.sp_h;
+      O* const out = out0 + h * sh;
+      uint32_t sm[4] = {0, 0, 0, 0};
+      if (values) {   // the bytes of a word: rows 2 t, 2 t + 8, 2 t + 1, 2 t + 9
+        uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        const int row0 = 2 * quarter;
+        if (there) {
+#pragma unroll
+          for (int g = 0; g < 8; ++g)
+            w[g] = __ldg(reinterpret_cast<const uint32_t*>(tile + int4_v_off(D) + (j / 4) * 512 + (g * 4 + quarter) * 16 + (j % 4) * 4));
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            sm[i] = __ldg(reinterpret_cast<const uint32_t*>(tile + int4_vs_off(D, runs) + ((row0 + (i >> 1) + 8 * (i & 1)) * runs + j / run_lanes) * 4));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) put_value<T, O>(out + (row0 + (i >> 1) + 8 * (i & 1)) * sn, sm[i], w, 8 * i);
+      } else {
+        uint32_t w[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) w[i][u] = 0;
+        if (there) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            sm[i] = __ldg(reinterpret_cast<const uint32_t*>(tile + int4_ks_off(D) + ((4 * quarter + i) * runs + j / run_lanes) * 4));
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              w[i][u] = __ldg(reinterpret_cast<const uint32_t*>(tile + (4 * quarter + i) * (D / 2) + 4 * (j / 2) + u * (D / 8)));
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) put_key<T, O>(out + (4 * quarter + i) * sn, sm[i], w[i], j);
+      }
+    }
+    return;
+  }
+  for (int item = blockIdx.y; item < items; item += gridDim.y) {
+    const int h = item * HPW + sub;
+    if (h >= KVH) continue;
+    const uint8_t* const tile = tile0 + h * a.kv.sp_h;
     uint32_t kw[4], vw[8], ksm = 0, vsm = 0;
 #pragma unroll
     for (int u = 0; u < 4; ++u) kw[u] = vw[u] = vw[4 + u] = 0;
@@ -483,43 +578,8 @@ __global__ void __launch_bounds__(kWarps * 32) int4_read_kernel(const __grid_con
         for (int g = 0; g < 8; ++g) vw[g] = __ldg(b + g * 64);
       }
     }
-    auto put = [&](O* o, uint32_t sm, const uint32_t (&code)[16]) {   // codes in the words' low bits
-      const float2 f = unpack_sm<T>(sm);
-      const F2 s2 = pack(f.x, f.x), m2 = pack(f.y, f.y), base2 = pack(-8388608.f, -8388608.f);
-      float x[16];
-#pragma unroll
-      for (int e = 0; e < 16; e += 2) {   // a code behind 2^23 in a float's bits
-        const F2 c = pack(__uint_as_float((code[e] & 15u) | 0x4B000000u), __uint_as_float((code[e + 1] & 15u) | 0x4B000000u));
-        unpack(fma2(s2, add2(c, base2), m2), x[e], x[e + 1]);
-      }
-      if constexpr (sizeof(O) == 4) {
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4*>(o + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
-      } else {
-        *reinterpret_cast<uint4*>(o) = pack8<O>(x);
-        *reinterpret_cast<uint4*>(o + 8) = pack8<O>(x + 8);
-      }
-    };
-    uint32_t code[16];
-    if (a.k) {
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const uint32_t w = kw[u] >> 8 * (j & 1);
-        code[4 * u] = w;
-        code[4 * u + 1] = w >> 16;
-        code[4 * u + 2] = w >> 4;
-        code[4 * u + 3] = w >> 20;
-      }
-      put(ko, ksm, code);
-    }
-    if (a.v) {
-#pragma unroll
-      for (int g = 0; g < 8; ++g) {
-        code[g] = vw[g];
-        code[g + 8] = vw[g] >> 4;
-      }
-      put(vo, vsm, code);
-    }
+    if (a.k) put_key<T, O>(static_cast<O*>(a.k) + n * a.sk_n + h * a.sk_h + 16 * j, ksm, kw, j);
+    if (a.v) put_value<T, O>(static_cast<O*>(a.v) + n * a.sv_n + h * a.sv_h + 16 * j, vsm, vw, 0);
   }
 }
 

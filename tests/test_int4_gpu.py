@@ -222,6 +222,37 @@ def test_append_in_place_strides_and_views():
     assert (ko[:, KVH] == 7).all() and (ko[:, :, D:] == 7).all()
 
 
+@pytest.mark.parametrize("D,KVH", [(128, 8), (128, 9), (64, 17), (64, 8), (128, 1)])
+@pytest.mark.parametrize("out", ["both", "keys", "values"])
+def test_read_of_whole_tiles_and_their_borders(D, KVH, out):
+    """Whole sequences of odd lengths, whose tiles lie anywhere in the call, among tokens in another order, padding and pages
+    outside the pool: each row as it is read alone."""
+    g = torch.Generator().manual_seed(D + KVH)
+    lens, ps = [3333, 16, 1, 47, 1600, 15, 640], 32
+    per = -(-max(lens) // ps)
+    table = torch.randperm(len(lens) * per, generator=g).int().view(len(lens), per)
+    seq = torch.repeat_interleave(torch.arange(len(lens)), torch.tensor(lens)).int()
+    pos = torch.cat([torch.arange(n) for n in lens])
+    N = pos.numel()
+    k, v = (torch.randn(N, KVH, D, generator=g).half() for _ in range(2))
+    kv = empty_pool(table.numel(), KVH, ps, D, F16)
+    paged_int4_append(kv, None, k.to(DEV), v.to(DEV), pos.to(DEV), table.to(DEV), seq_ids=seq.to(DEV))
+    table[0, 5], table[4, 3] = -1, 10 ** 6
+    order = torch.cat([torch.arange(1000), 1000 + torch.randperm(500, generator=g), torch.arange(1500, N)])
+    seq, pos, k, v = seq[order], pos[order], k[order], v[order]
+    seq[2000:2003], pos[40] = -1, -7                     # padding inside of tiles
+    keep = torch.ones(N, dtype=torch.bool)
+    keep[2000:2003] = keep[40] = False
+    gone = keep & (((seq == 0) & (pos // ps == 5)) | ((seq == 4) & (pos // ps == 3)))
+    outs = [torch.full((N, KVH, D), 9.0, device=DEV) if out != skip else False for skip in ("values", "keys")]
+    got = paged_int4_read(kv, pos.to(DEV), table.to(DEV), seq_ids=seq.to(DEV), k_out=outs[0], v_out=outs[1])
+    for x, y in zip(got, (k, v)):
+        if x is None:
+            continue
+        assert (x[~keep] == 9).all() and (x[gone] == 0).all()
+        check_values(x.cpu()[keep & ~gone], y[keep & ~gone].float().numpy(), 64, F16)
+
+
 # ------------------------------------------------------------------ attention
 class Case:
     """Random sequences whose unused slots and pages hold NaN factors and whose unused table entries point nowhere."""
