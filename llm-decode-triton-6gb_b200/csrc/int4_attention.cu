@@ -20,6 +20,16 @@
 // Units of work are (sequence, KV head, tile of up to 32 rows). As in the 16-bit kernel the units' stages (64 keys, a
 // tile a warp) form one line of which every block takes an equal share, found from the lengths on the device; parts of a unit
 // that several blocks share meet in a combine launch. No atomics: results are the same bits every run.
+//
+// Measured on B200 (GPU time of a call, graph replays over rotated inputs; each key and value once at the copy rate of 6.55 TB/s
+// in brackets): 8 sequences of 16001..32768 keys, 32 / 8 heads of 128, fp16: 52 us (34); 64 of 100..4609, groups of 32: 54 us (30);
+// 8 of 512..2048: 12.0 us (1.8); 16 x 5 drafts, up to 4099 keys: 31 us (6.0); one of 300 keys: 7.0 us. The 16-bit kernel takes 13.8,
+// 38 and 7.5 us for the last three. Long: the loop reads at 5.8 TB/s (about 270 instructions a tile, 63 % of the slots issue, the logic
+// pipe 50 % busy); 6 us pass before the first tiles land and 3 go to the combine. Short: dependent steps of one warp -- lengths 0.7,
+// segment and pages 1.4, queries 0.4, a tile 1.0, merge 0.9, combine 1.7 us. More row tiles: eight warps an SM (their
+// accumulators take the registers) issue in 41 % of the slots. Not kept: a producer warp for one block of 15 consumers an SM (a
+// lane's bulk copies serialise, all warps meet at a unit's end: 56 and 94 us for the first two); clusters in place of the combine (7.2
+// us for 300 keys); five blocks an SM (63 us for the first); whole bytes as operands (fewer masks, more products: the same).
 #include <type_traits>
 
 #include "int4_kv.cuh"
@@ -34,9 +44,9 @@ constexpr int kStage = kWarps * kTileKeys;      // keys of a position of the lin
 constexpr int kMaxT = 16, kMaxG = 16;
 constexpr int kMaxBatch = 256;                  // sequences of a launch (larger batches take several)
 constexpr int kMaxCtas = 640;
-// Up to so many keys a unit is one CTA's, and there is no combine launch (8 sequences of up to 256 keys, 8 KV heads: 8.2 -> 7.5 us; of
-// 300: 7.4 -> 7.9); with two units an SM or more up to twice as many (64 sequences of up to 512 keys: 16.5 -> 13.7 us).
-constexpr int kWholeKeys = 256;
+// Up to so many keys a unit is one CTA's, and there is no combine launch (8 sequences of up to 256 keys, 8 KV heads: 8.2 -> 7.5 us in a
+// graph; one of 300: 7.2 -> 7.7); with two units an SM or more up to 512 keys (64 sequences: 16.5 -> 13.7 us).
+constexpr int kWholeKeys = 256, kWholeKeysMany = 512;
 constexpr float kLazy = 8.f;                    // log2 of the largest weight before the running maximum moves
 constexpr float kNone = -1.7e38f;               // running maximum before the first score
 constexpr float kLog2e = 1.4426950408889634f;
@@ -763,7 +773,7 @@ Plan make_plan(const b2d_int4_kv* kv, int B, int T, int H, int pages_per_seq, in
   const int64_t keys = max_len > 0 && max_len < reach ? max_len : reach;
   const int64_t units = static_cast<int64_t>(B) * kv->KVH * ((rows + tile - 1) / tile);
   p.fits = units * ((reach + kStage - 1) / kStage + Line<1>::LEAD) < (int64_t(1) << 31);
-  p.whole = keys <= kWholeKeys || (keys <= 2 * kWholeKeys && units >= 2 * sm);
+  p.whole = keys <= kWholeKeys || (keys <= kWholeKeysMany && units >= 2 * sm);
   int64_t ctas = p.whole ? units : units * ((keys + kStage - 1) / kStage + Line<1>::LEAD);
   const int per_sm = p.nt == 1 ? kBlocks<1> : p.nt == 2 ? kBlocks<2> : kBlocks<3>;
   if (ctas > static_cast<int64_t>(per_sm) * sm) ctas = per_sm * sm;

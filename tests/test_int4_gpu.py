@@ -508,6 +508,33 @@ def test_attention_workspaces_graphs_and_streams():
         paged_int4_attention(*args[0], workspace=short)
 
 
+def test_programmatic_launches_see_what_the_kernel_before_wrote():
+    """Chains of dependent launches: a read writes what an append takes, whose keys and queries an attention takes."""
+    a = Case([700, 900, 333], H=8, KVH=2, dtype=BF16, seed=21)
+    pos, seq, table, lens = a.pos.to(DEV), a.seq.to(DEV), a.table.to(DEV), a.lens.to(DEV)
+    N, w = pos.numel(), torch.rand(128, device=DEV).bfloat16()
+    cos, sin = (t.to(DEV) for t in rotary_tables(1000, 128))
+    k, v, q = (torch.zeros(N, h, 128, dtype=BF16, device=DEV) for h in (2, 2, 8))
+    last = (lens.cumsum(0) - 1).long()
+
+    def chain(flags):
+        kv = empty_pool(a.kv.num_pages, 2, a.ps, 128, BF16)
+        out = []
+        for _ in range(8):
+            k.zero_(), v.zero_(), q.zero_()
+            paged_int4_read(a.kv, pos, table, seq_ids=seq, k_out=k, v_out=v, flags=flags)
+            q.copy_(k.repeat_interleave(4, 1))
+            q_rot = paged_int4_append(kv, q, k, v, pos, table, cos, sin,
+                                      q_weight=w, k_weight=w, seq_ids=seq, flags=flags)
+            paged_int4_read(a.kv, pos, table, seq_ids=seq, k_out=k, v_out=v, flags=flags)
+            paged_int4_append(kv, None, k, v, pos, table, cos, sin, seq_ids=seq, flags=flags)
+            out.append(paged_int4_attention(kv, q_rot[last][:, None], table, lens, flags=flags))
+        return out
+
+    plain, early = chain(0), chain(_lib.LAUNCH_PDL)
+    assert all(torch.equal(x, y) for x, y in zip(plain, early)) and torch.isfinite(plain[0]).all()
+
+
 def test_pool_past_four_gigabytes():
     """Pages further apart than 32 bits of bytes."""
     D, ps, KVH = 128, 16, 2
