@@ -3,7 +3,7 @@
     python llm-decode-triton-6gb_b200/build.py [--verbose] [--force] [--no-binding]
 
 The shared library lands next to the Python package (``b200kernels/libb200decode.so``) so it
-travels with the source tree; nothing is installed into site-packages. The CPython module of the paged-cache and
+travels with the source tree; nothing is installed into site-packages. The CPython module of the paged-cache, page-planning and
 draft-verification calls (``b200kernels/_binding.so``) is built beside it where torch is installed; hosts that use the
 C ABI alone need neither it nor torch (``--no-binding``).
 """
