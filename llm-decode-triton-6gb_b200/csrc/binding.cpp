@@ -598,6 +598,18 @@ PyObject* int4_workspace(PyObject*, PyObject* const* a, Py_ssize_t na) {
   });
 }
 
+// Whether the memory that two tensors span has bytes in common.
+bool overlap(const at::Tensor& x, const at::Tensor& y) {
+  if (x.numel() == 0 || y.numel() == 0) return false;
+  auto span = [](const at::Tensor& t) {
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+    return (last + 1) * static_cast<int64_t>(t.element_size());
+  };
+  const auto a = reinterpret_cast<uintptr_t>(x.const_data_ptr()), b = reinterpret_cast<uintptr_t>(y.const_data_ptr());
+  return a < b + span(y) && b < a + span(x);
+}
+
 // (page_table, held, free, ring, page_size, cached, new, positions, seq_ids, slots, seqlens, starts, granted, flags)
 PyObject* page_plan(PyObject*, PyObject* const* a, Py_ssize_t na) {
   return guarded([&]() -> PyObject* {
@@ -628,11 +640,9 @@ PyObject* page_plan(PyObject*, PyObject* const* a, Py_ssize_t na) {
     for (int i = 0; i < 10; ++i) {
       check_device(written[i], names[i], dev);
       for (int j = 0; j < i; ++j)
-        if (written[i]->numel() > 0 && written[j]->numel() > 0 && written[i]->const_data_ptr() == written[j]->const_data_ptr())
-          bad_value(std::string(names[i]) + " and " + names[j] + " are one memory");
+        if (overlap(*written[i], *written[j])) bad_value(std::string(names[i]) + " and " + names[j] + " are one memory, or parts of it");
       for (const at::Tensor* in : {&cached, &fresh})
-        if (written[i]->numel() > 0 && in->numel() > 0 && written[i]->const_data_ptr() == in->const_data_ptr())
-          bad_value(std::string(names[i]) + " is written while the lengths are read: they are one memory");
+        if (overlap(*written[i], *in)) bad_value(std::string(names[i]) + " is written while the lengths are read: they are one memory, or parts of it");
     }
     check_device(&cached, "cached", dev); check_device(&fresh, "new", dev);
     check_cuda(dev);

@@ -12,8 +12,8 @@
 //  * v: loaded in that order at once. A position's codes lie in single bytes (the other bytes of a word are other
 //    positions'), so that no store reads what another token writes.
 //
-// Measured on B200: 8168 tokens of 32 + 8 + 8 heads of 128 with norms, bf16: 48 us, 2.95 TB/s of the bytes that it cannot do
-// without (143 MB; copy rate 6.55); 320 tokens 4.9 us; one token 2.6 us (launch and a chain of three loads). Bound by issued
+// Measured on B200: 8168 tokens of 32 + 8 + 8 heads of 128 with norms, bf16: 48 us, 3.6 TB/s of the bytes that it cannot do
+// without (177 MB; copy rate 6.55); 320 tokens 4.9 us; one token 2.6 us (launch and a chain of three loads). Bound by issued
 // instructions and latency: 3200 warp instructions a token, 53 % of the slots, 21 warps per SM. Earlier forms: one warp for all heads of
 // a token with a division per code 87 us; packed fp32 instructions and corrected quotients 50; queries apart from keys 48. Reading
 // 8 x 4001 tokens: 38 us, 4.5 TB/s (a warp a token without the shared words 44).

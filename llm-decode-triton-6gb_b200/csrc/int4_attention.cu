@@ -22,11 +22,11 @@
 // that several blocks share meet in a combine launch. No atomics: results are the same bits every run.
 //
 // Measured on B200 (GPU time of a call, graph replays over rotated inputs; each key and value once at the copy rate of 6.55 TB/s
-// in brackets): 8 sequences of 16001..32768 keys, 32 / 8 heads of 128, fp16: 52 us (34); 64 of 100..4609, groups of 32: 54 us (30);
-// 8 of 512..2048: 12.0 us (1.8); 16 x 5 drafts, up to 4099 keys: 31 us (6.0); one of 300 keys: 7.0 us. The 16-bit kernel takes 13.8,
+// in brackets): 8 sequences of 16001..32768 keys, 32 / 8 heads of 128, fp16: 51 us (34); 64 of 100..4609, groups of 32: 55 us (30);
+// 8 of 512..2048: 10.8 us (1.8); 16 x 5 drafts, up to 4099 keys: 31 us (6.0); one of 300 keys: 6.7 us. The 16-bit kernel takes 13.8,
 // 38 and 7.5 us for the last three. Long: the loop reads at 5.8 TB/s (about 270 instructions a tile, 63 % of the slots issue, the logic
-// pipe 50 % busy); 6 us pass before the first tiles land and 3 go to the combine. Short: dependent steps of one warp -- lengths 0.7,
-// segment and pages 1.4, queries 0.4, a tile 1.0, merge 0.9, combine 1.7 us. More row tiles: eight warps an SM (their
+// pipe 50 % busy); 6 us pass before the first tiles land and 2 go to the combine. Short: dependent steps of one warp -- lengths 0.7,
+// segment and pages 1.4, queries 0.4, a tile 1.0, merge 0.9, combine 1.4 us. More row tiles: eight warps an SM (their
 // accumulators take the registers) issue in 41 % of the slots. Not kept: a producer warp for one block of 15 consumers an SM (a
 // lane's bulk copies serialise, all warps meet at a unit's end: 56 and 94 us for the first two); clusters in place of the combine (7.2
 // us for 300 keys); five blocks an SM (63 us for the first); whole bytes as operands (fewer masks, more products: the same).
@@ -759,7 +759,7 @@ int row_tiles(int rows) {
 }
 
 struct Plan {
-  int nt, ctas, whole, many, fits;
+  int nt, ctas, whole, groups, fits;
   int64_t entries;
   size_t bytes;
 };
@@ -779,7 +779,9 @@ Plan make_plan(const b2d_int4_kv* kv, int B, int T, int H, int pages_per_seq, in
   if (ctas > static_cast<int64_t>(per_sm) * sm) ctas = per_sm * sm;
   if (ctas > kMaxCtas) ctas = kMaxCtas;
   p.ctas = static_cast<int>(ctas < 1 ? 1 : ctas);
-  p.many = p.ctas > 16 * units;
+  // a unit's parts, eight in flight a group of the combine's threads: 9 of them take 10.8 us a call in two groups (8 x 512..2048 keys)
+  // against 12.0 in one; 74 of them (one sequence of 30000 keys, 8 KV heads) 18.7 in four against 20.6 in eight
+  p.groups = p.ctas > 16 * units ? 4 : p.ctas > 4 * units ? 2 : 1;
   if (!p.whole) {
     p.entries = static_cast<int64_t>(p.ctas) * 2 * tile;
     p.bytes = static_cast<size_t>(p.entries) * (kv->D + 2) * 4;
@@ -788,7 +790,7 @@ Plan make_plan(const b2d_int4_kv* kv, int B, int T, int H, int pages_per_seq, in
 }
 
 template <typename T, int D, int RUNS, int NT>
-int launch_attention(const Int4AttnArgs& a, bool many, bool pdl, cudaStream_t s) {
+int launch_attention(const Int4AttnArgs& a, int groups, bool pdl, cudaStream_t s) {
   auto kern = int4_attention_kernel<T, D, RUNS, NT>;
   constexpr int bytes = Smem<D, RUNS, NT>::BYTES;
   static bool configured[64] = {};   // per device; setting it twice is harmless
@@ -805,17 +807,18 @@ int launch_attention(const Int4AttnArgs& a, bool many, bool pdl, cudaStream_t s)
   const int st = launch_kernel(kern, dim3(a.ctas), dim3(kThreads), bytes, s, pdl, a);
   if (st != B2D_OK || a.whole) return st;
   const dim3 grid(a.B * a.kv.KVH, (a.rows + 512 / D - 1) / (512 / D));
-  if (many) return launch_kernel(int4_combine_kernel<T, D, NT, 4>, grid, dim3(512), 0, s, true, a);
+  if (groups == 4) return launch_kernel(int4_combine_kernel<T, D, NT, 4>, grid, dim3(512), 0, s, true, a);
+  if (groups == 2) return launch_kernel(int4_combine_kernel<T, D, NT, 2>, grid, dim3(256), 0, s, true, a);
   return launch_kernel(int4_combine_kernel<T, D, NT, 1>, grid, dim3(128), 0, s, true, a);
 }
 
 template <typename T, int D, int RUNS>
 int run(const Int4AttnArgs& a, const Plan& p, bool pdl, cudaStream_t s) {
   switch (p.nt) {
-    case 1: return launch_attention<T, D, RUNS, 1>(a, p.many, pdl, s);
-    case 2: return launch_attention<T, D, RUNS, 2>(a, p.many, pdl, s);
-    case 3: return launch_attention<T, D, RUNS, 3>(a, p.many, pdl, s);
-    default: return launch_attention<T, D, RUNS, 4>(a, p.many, pdl, s);
+    case 1: return launch_attention<T, D, RUNS, 1>(a, p.groups, pdl, s);
+    case 2: return launch_attention<T, D, RUNS, 2>(a, p.groups, pdl, s);
+    case 3: return launch_attention<T, D, RUNS, 3>(a, p.groups, pdl, s);
+    default: return launch_attention<T, D, RUNS, 4>(a, p.groups, pdl, s);
   }
 }
 template <typename T>

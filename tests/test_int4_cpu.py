@@ -162,6 +162,10 @@ def test_plan_refusals():
     refused(lambda: tables.step(i32(3), i32(3), out=good._replace(seq_ids=i32(4))), "seq_ids")
     new = i32(3)
     refused(lambda: tables.step(i32(3), new, out=good._replace(granted=new)), "one memory")
+    run = torch.zeros(9, dtype=torch.int64)               # windows of one memory that share an element
+    refused(lambda: tables.step(i32(3), i32(3), out=good._replace(positions=run[:5], slots=run[4:])), "one memory")
+    refused(lambda: tables.step(i32(3), i32(3), out=good._replace(positions=run[:4], slots=run[4:8], seq_ids=i32(4))), "CUDA")
+    refused(lambda: tables.step(tables.free[2:5], i32(3), out=good), "one memory")
     for field, bad in (("held", i32(4)), ("free", i32(2, 4)), ("ring", i32(3)), ("page_table", i32(1, 4).expand(3, 4)), ("page_table", i32(4, 3).t())):
         t = PageTables.empty(8, 16, 3, 4, "cpu")
         setattr(t, field, bad)
