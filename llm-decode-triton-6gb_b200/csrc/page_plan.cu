@@ -5,9 +5,8 @@
 // that saturate; the state is read by all and written behind a cluster barrier) and keeps what the rest needs of a sequence
 // in shared memory. Tokens and moved pages are then shared out by their number: a thread finds the sequence of its first one
 // by bisection. A token's page comes from the ring itself where the step took it, so nothing waits for the table's new entries.
-// Bound by latency: dependent rounds of loads and the scans between them. Measured on B200: 3.6 us for 8 requests of one token; 1024
-// requests with 65 thousand tokens 18 us, 9 us for the step that takes their pages back (one block in both: 40 us for the two). Small steps
-// take a block of 128 threads (8 requests: 3.6 us against 5.7 with 1024), large ones a cluster of eight blocks.
+// Bound by latency: dependent rounds of loads and the scans between them. Measured on B200, a step that takes pages and one that
+// gives them back by turns: 4.0 us for 8 requests of one token, 4.8 for 8 x 256 tokens, 10.1 for 1024 x 64 (one block alone: 61).
 #include "common.cuh"
 #include "paged.cuh"
 
@@ -15,7 +14,7 @@ namespace b2d {
 namespace {
 
 constexpr int kMaxSeqs = 8192;
-constexpr int kClusterSize = 8;
+constexpr int kClusterSize = 16;   // 1024 x 64 tokens: 10.1 us, with 8 blocks 12.9
 
 struct PlanArgs {
   int32_t* table; int64_t ld_table;
@@ -223,7 +222,8 @@ int launch_plan(const PlanArgs& a, bool pdl, cudaStream_t s) {
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !configured[dev]) {
     constexpr int most = (5 * kMaxSeqs + 3) * 4;
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    if (CLUSTER > 8 && e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) {
       set_cuda_error(e);
       return B2D_ERR_LAUNCH;
@@ -281,8 +281,11 @@ extern "C" int b2d_page_plan(int32_t* page_table, int64_t ld_table, int pages_pe
                    aligned(positions, 16) && aligned(seq_ids, 16) && aligned(slots, 16)};
   const bool pdl = (flags & B2D_LAUNCH_PDL) != 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  // (a block's scan spans its threads; a thread writes four tokens)
-  if (B <= 128 && max_tokens <= 1024) return launch_plan<1, 128>(a, pdl, s);
-  if (B <= 1024 && max_tokens <= 4096) return launch_plan<1, 1024>(a, pdl, s);
-  return launch_plan<kClusterSize, 1024>(a, pdl, s);
+  // us a step, half of the steps taking pages and half giving them back: a thread writes four tokens, and up to 1024 of them one
+  // block is faster than a cluster, which starts and ends later (8 x 1 tokens 4.0 against 4.1; 512 x 1: 4.8 against 5.8; 8 x 256: 5.5
+  // against 4.8); the scans go over the sequences in rounds of a block, where more threads cost more in each (256 or 512
+  // threads for 8 x 1: 4.0 or 4.3, 512 x 1: 5.5 or 4.8; in a cluster 8 x 256: 4.8 or 5.9, 1024 x 64: 12.4 or 10.1)
+  const bool few = B <= 256;
+  if (max_tokens <= 1024) return few ? launch_plan<1, 256>(a, pdl, s) : launch_plan<1, 512>(a, pdl, s);
+  return few ? launch_plan<kClusterSize, 256>(a, pdl, s) : launch_plan<kClusterSize, 512>(a, pdl, s);
 }
