@@ -13,7 +13,7 @@
 //    positions'), so that no store reads what another token writes.
 //
 // Measured on B200: 8168 tokens of 32 + 8 + 8 heads of 128 with norms, bf16: 48 us, 3.6 TB/s of the bytes that it cannot do
-// without (177 MB; copy rate 6.55); 320 tokens 4.9 us; one token 2.6 us (launch and a chain of three loads). Bound by issued
+// without (177 MB; copy rate 6.55); 320 tokens 4.2 us; one token 2.6 us (launch and a chain of three loads). Bound by issued
 // instructions and latency: 3200 warp instructions a token, 53 % of the slots, 21 warps per SM. Earlier forms: one warp for all heads of
 // a token with a division per code 87 us; packed fp32 instructions and corrected quotients 50; queries apart from keys 48. Reading
 // 8 x 4001 tokens: 38 us, 4.5 TB/s (a warp a token without the shared words 44).
@@ -590,9 +590,10 @@ __global__ void __launch_bounds__(kWarps * 32) int4_read_kernel(const __grid_con
   }
 }
 
-// Warps a token of a share of the work, at most one per item: enough of them to fill the SMs several times over.
+// Warps a token of a share of the work, at most one per item, so that eight of an SM have some: 64 x 5 tokens 4.2 us (one warp a token
+// 5.6, 24 an SM 5.2), 8 x 100 7.0 (8.2, 7.9), one token 2.7 (4.6, 2.6), 8 x 1021 48.9 (49.0, 48.9); reading 300 tokens 2.7 (3.3, 2.7).
 int warps_per_token(int64_t N, int items, int sm) {
-  const int64_t parts = (static_cast<int64_t>(sm) * 24 + N - 1) / N;
+  const int64_t parts = (static_cast<int64_t>(sm) * 8 + N - 1) / N;
   return static_cast<int>(parts < items ? parts : items);
 }
 

@@ -6,7 +6,7 @@
 // in shared memory. Tokens and moved pages are then shared out by their number: a thread finds the sequence of its first one
 // by bisection. A token's page comes from the ring itself where the step took it, so nothing waits for the table's new entries.
 // Bound by latency: dependent rounds of loads and the scans between them. Measured on B200, a step that takes pages and one that
-// gives them back by turns: 4.0 us for 8 requests of one token, 4.8 for 8 x 256 tokens, 10.1 for 1024 x 64 (one block alone: 61).
+// gives them back by turns: 3.9 us for 8 requests of one token, 4.8 for 8 x 256 tokens, 9.8 for 1024 x 64 (one block alone: 61).
 #include "common.cuh"
 #include "paged.cuh"
 
@@ -14,7 +14,7 @@ namespace b2d {
 namespace {
 
 constexpr int kMaxSeqs = 8192;
-constexpr int kClusterSize = 16;   // 1024 x 64 tokens: 10.1 us, with 8 blocks 12.9
+constexpr int kClusterSize = 16;   // 1024 x 64 tokens: 9.8 us, with 8 blocks 12.9
 
 struct PlanArgs {
   int32_t* table; int64_t ld_table;
@@ -281,10 +281,11 @@ extern "C" int b2d_page_plan(int32_t* page_table, int64_t ld_table, int pages_pe
                    aligned(positions, 16) && aligned(seq_ids, 16) && aligned(slots, 16)};
   const bool pdl = (flags & B2D_LAUNCH_PDL) != 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  // us a step, half of the steps taking pages and half giving them back: a thread writes four tokens, and up to 1024 of them one
-  // block is faster than a cluster, which starts and ends later (8 x 1 tokens 4.0 against 4.1; 512 x 1: 4.8 against 5.8; 8 x 256: 5.5
-  // against 4.8); the scans go over the sequences in rounds of a block, where more threads cost more in each (256 or 512
-  // threads for 8 x 1: 4.0 or 4.3, 512 x 1: 5.5 or 4.8; in a cluster 8 x 256: 4.8 or 5.9, 1024 x 64: 12.4 or 10.1)
+  // us a step, half of the steps taking pages and half giving them back. A thread writes four tokens, and up to 1024 of them one block
+  // is faster than a cluster, which starts and ends later (8 x 128 tokens 4.5 against 5.0, 512 x 2 4.8 against 5.8; but 512 x 4
+  // 5.5 against 6.2 and 8 x 256 5.5 against 4.8). The scans go over the sequences in rounds of a block, where more warps cost
+  // more in each: 256 threads and 512 take 3.9 and 4.1 for 8 x 1, 5.6 and 4.9 for 512 x 1; in a cluster 4.8 and 5.9 for
+  // 8 x 256, 12.4 and 9.8 for 1024 x 64.
   const bool few = B <= 256;
   if (max_tokens <= 1024) return few ? launch_plan<1, 256>(a, pdl, s) : launch_plan<1, 512>(a, pdl, s);
   return few ? launch_plan<kClusterSize, 256>(a, pdl, s) : launch_plan<kClusterSize, 512>(a, pdl, s);
