@@ -481,7 +481,7 @@ int b2d_int4_append(const b2d_int4_kv* kv, const void* q, int64_t sq_n, int64_t 
                     int64_t sqo_h, int N, int H, int flags, void* stream);
 
 /* The values of N cached positions, addressed as the append does: k_out / v_out [N, KVH, D] (strides in elements, % 8 == 0,
- * 16-byte aligned; either may be NULL) = m + s c in out_dtype (the cache's, or F32). Padding (a sequence outside [0, B), a
+ * 16-byte aligned, no element in common; either may be NULL) = m + s c in out_dtype (the cache's, or F32). Padding (a sequence outside [0, B), a
  * position outside the page table) is left as it is. */
 int b2d_int4_read(const b2d_int4_kv* kv, const int64_t* positions, const int32_t* seq_ids, const int32_t* page_table,
                   int64_t ld_table, int pages_per_seq, int B, void* k_out, int64_t sk_n, int64_t sk_h, void* v_out,
@@ -489,7 +489,9 @@ int b2d_int4_read(const b2d_int4_kv* kv, const int64_t* positions, const int32_t
 
 /* b2d_paged_attention over a 4-bit cache (no shared prefix): arguments, masks, lengths, workspace and limits as there (the
  * page table reaches at most 2^31 - 32768 positions). q has the cache's dtype. Keys and values enter the products as codes
- * (exact); a weight times its value's s is rounded to fp16 (2^-11) for the second product, everything else is fp32. */
+ * (exact); a weight times its value's s is rounded to fp16 (2^-11) for the second product, everything else is fp32. out may be q
+ * itself (of its dtype and strides) and overlaps no other input. bf16: values whose s is 2^111 or more and queries of 2^114 or more
+ * may give infinities or NaN where the exact result is finite. */
 size_t b2d_int4_attention_workspace_bytes(const b2d_int4_kv* kv, int B, int T, int H, int pages_per_seq, int max_len);
 int b2d_int4_attention(const b2d_int4_kv* kv, const void* q, int64_t sq_b, int64_t sq_t, int64_t sq_h,
                        const int32_t* page_table, int64_t ld_table, int pages_per_seq, const int32_t* seqlens, int max_len,

@@ -146,8 +146,8 @@ def paged_int4_read(kv: PagedKVInt4, positions: torch.Tensor, page_table: torch.
                     k_out: torch.Tensor | bool | None = None, v_out: torch.Tensor | bool | None = None,
                     out_dtype: torch.dtype | None = None, flags: int = 0) -> tuple[torch.Tensor | None, torch.Tensor | None]:
     """What the cache holds at N positions, addressed as by ``paged_int4_append`` -> (k, v) [N, KVH, D] in ``out_dtype`` (the
-    cache's dtype or torch.float32; that of given outputs). ``k_out`` / ``v_out``: where to write, False: leave it out. Rows of
-    padding (a sequence outside [0, B), a position outside the page table) are left as they were; a page id outside the pool
+    cache's dtype or torch.float32; that of given outputs). ``k_out`` / ``v_out``: where to write (they share no
+    element), False: leave it out. Rows of padding (a sequence outside [0, B), a position outside the page table) are left as they were; a page id outside the pool
     gives zeros."""
     r = _lib.binding().int4_read(kv._desc, positions, page_table, seq_ids, k_out, v_out, out_dtype, flags, kv._index)
     if r.__class__ is int:
@@ -162,9 +162,10 @@ def paged_int4_attention(kv: PagedKVInt4, q: torch.Tensor, page_table: torch.Ten
     """q [B, T, H, D], page_table int32 [B, pages], seqlens int32 [B] (cached keys, the T new tokens included) ->
     [B, T, H, D] in ``out_dtype`` (q's dtype or torch.float32). Query t of sequence b sees the keys before position
     ``seqlens[b] - T + 1 + t``; one that sees none gives zeros. Lengths past the table's pages are cut to them. T and H / KVH up to 16.
-    ``max_len``: an upper bound of ``seqlens`` known to the host, which only guides the split. ``workspace``: contiguous
-    scratch of ``paged_int4_attention_workspace`` bytes, 16-byte aligned, not shared by calls that may overlap; without
-    it one is allocated per call."""
+    ``max_len``: an upper bound of ``seqlens`` known to the host, which only guides the split. ``out`` may be q itself and
+    overlaps no other input. ``workspace``: contiguous scratch of ``paged_int4_attention_workspace`` bytes, 16-byte
+    aligned, not shared by calls that may overlap; without it one is allocated per call. bf16 only: values whose
+    s is 2^111 or more, and queries of 2^114 or more, may give infinities or NaN though the exact result is finite."""
     r = _lib.binding().int4_attention(kv._desc, q, page_table, seqlens, scale, max_len, out, out_dtype, workspace, flags,
                                       kv._index)
     if r.__class__ is int:

@@ -393,6 +393,18 @@ void check_written_pool4(const b2d_int4_kv* kv, int64_t block) {
   const int64_t sizes[3] = {kv->num_pages, kv->KVH, block}, strides[3] = {kv->sp_p, kv->sp_h, 1};
   if (!nests(sizes, strides)) bad_value("the cache's pages overlap one another: an append would write them at once");
 }
+// Whether the memory that two tensors span has bytes in common.
+bool overlap(const at::Tensor& x, const at::Tensor& y) {
+  if (x.numel() == 0 || y.numel() == 0) return false;
+  auto span = [](const at::Tensor& t) {
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+    return (last + 1) * static_cast<int64_t>(t.element_size());
+  };
+  const auto a = reinterpret_cast<uintptr_t>(x.const_data_ptr()), b = reinterpret_cast<uintptr_t>(y.const_data_ptr());
+  return a < b + span(y) && b < a + span(x);
+}
+
 // positions, seq_ids and page_table of N tokens; returns the table's sequences
 int64_t check_addresses(const at::Tensor& positions, const at::Tensor* seq, const at::Tensor& table, int64_t N) {
   check_vector(positions, "positions", at::kLong, N);
@@ -509,7 +521,10 @@ PyObject* int4_read(PyObject*, PyObject* const* a, Py_ssize_t na) {
         check_device(out[i], name[i], dev);
       }
     }
-    if (out[0] && out[1] && N > 0 && out[0]->const_data_ptr() == out[1]->const_data_ptr()) bad_value("k_out and v_out are one memory");
+    // (strided ones may lie between one another's elements)
+    if (out[0] && out[1] && overlap(*out[0], *out[1]) &&
+        (out[0]->const_data_ptr() == out[1]->const_data_ptr() || (out[0]->is_contiguous() && out[1]->is_contiguous())))
+      bad_value("k_out and v_out are one memory, or parts of it");
     check_device(&table, "page_table", dev); check_device(seq, "seq_ids", dev);
     check_cuda(dev);
     check_pool(dev, a[8]);
@@ -557,9 +572,12 @@ PyObject* int4_attention(PyObject*, PyObject* const* a, Py_ssize_t na) {
     check_last(q, "q");
     check_last(out, "out");
     check_output(out, "out");
+    const bool in_place = out.const_data_ptr() == q.const_data_ptr() && out.scalar_type() == dt && out.strides() == q.strides();
+    if (!in_place && out.is_contiguous() && q.is_contiguous() && overlap(out, q)) bad_value("out overlaps q and is not q itself");
     check_device(&table, "page_table", dev); check_device(&lens, "seqlens", dev); check_device(&out, "out", dev);
     const at::Tensor* ws = optional(a[8], "workspace");
     if (ws && !ws->is_contiguous()) bad_value("workspace is contiguous, got " + show(*ws));   // its bytes are counted below
+    if (ws && out.is_contiguous() && overlap(*ws, out)) bad_value("out and workspace are one memory, or parts of it");
     check_device(ws, "workspace", dev);
     check_cuda(dev);
     check_pool(dev, a[10]);
@@ -596,18 +614,6 @@ PyObject* int4_workspace(PyObject*, PyObject* const* a, Py_ssize_t na) {
                                       narrow(table.size(1), "page_table"), integer32(a[3], "max_len"));
     return THPVariable_Wrap(at::empty({static_cast<int64_t>(n)}, q.options().dtype(at::kByte)));
   });
-}
-
-// Whether the memory that two tensors span has bytes in common.
-bool overlap(const at::Tensor& x, const at::Tensor& y) {
-  if (x.numel() == 0 || y.numel() == 0) return false;
-  auto span = [](const at::Tensor& t) {
-    int64_t last = 0;
-    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
-    return (last + 1) * static_cast<int64_t>(t.element_size());
-  };
-  const auto a = reinterpret_cast<uintptr_t>(x.const_data_ptr()), b = reinterpret_cast<uintptr_t>(y.const_data_ptr());
-  return a < b + span(y) && b < a + span(x);
 }
 
 // (page_table, held, free, ring, page_size, cached, new, positions, seq_ids, slots, seqlens, starts, granted, flags)

@@ -123,6 +123,23 @@ def attn_args(B=2, T=1, H=4, D=64):
                 seqlens=torch.ones(B, dtype=torch.int32))
 
 
+def test_outputs_that_overlap_are_refused():
+    pos, table = torch.zeros(4, dtype=torch.int64), torch.zeros(2, 3, dtype=torch.int32)
+    memory = torch.zeros(3 * 4 * 2 * 64).half()
+    first, shifted, behind = (memory[n:n + 512].view(4, 2, 64) for n in (0, 256, 512))
+    refused(lambda: paged_int4_read(pool(), pos, table, k_out=first, v_out=shifted), "one memory")
+    refused(lambda: paged_int4_read(pool(), pos, table, k_out=first, v_out=behind), "CUDA")
+    both = memory[:1024].view(4, 4, 64)                       # rows of keys and values by turns
+    refused(lambda: paged_int4_read(pool(), pos, table, k_out=both[:, :2], v_out=both[:, 2:]), "CUDA")
+    q, shifted, behind = (memory[n:n + 512].view(2, 1, 4, 64) for n in (0, 8, 512))
+    args = {**attn_args(), "q": q}
+    refused(lambda: paged_int4_attention(pool(), **args, out=shifted), "overlaps q")
+    refused(lambda: paged_int4_attention(pool(), **args, out=memory.view(torch.float32)[:512].view(2, 1, 4, 64)), "overlaps q")
+    refused(lambda: paged_int4_attention(pool(), **args, out=behind, workspace=memory[1016:].view(U8)), "workspace")
+    refused(lambda: paged_int4_attention(pool(), **args, out=q), "CUDA")
+    refused(lambda: paged_int4_attention(pool(), **args, out=behind), "CUDA")
+
+
 @pytest.mark.parametrize("change,err", [
     (dict(q=torch.zeros(2, 1, 4, 128).half()), ValueError),
     (dict(q=torch.zeros(2, 1, 5, 64).half()), ValueError),

@@ -478,6 +478,20 @@ def test_attention_nonfinite_queries_stay_alone():
     assert torch.equal(got, clean)
 
 
+@pytest.mark.parametrize("lens,H,T", [([200, 90, 5], 8, 1), ([5000, 1700, 33], 8, 1), ([900, 4000], 16, 8), ([120, 30], 16, 8)])
+def test_attention_in_place(lens, H, T):
+    """The queries' memory as the output: units whole, cut over blocks, and of several row tiles."""
+    c = Case(lens, H=H, KVH=2, T=T, dtype=BF16, seed=H + T)
+    want = c.run()
+    q = c.q.to(DEV)
+    for max_len in (0, max(lens)):
+        mine = q.clone()
+        got = paged_int4_attention(c.kv, mine, c.table.to(DEV), c.lens.to(DEV), max_len=max_len, out=mine)
+        clean = paged_int4_attention(c.kv, q, c.table.to(DEV), c.lens.to(DEV), max_len=max_len)
+        assert got.data_ptr() == mine.data_ptr() and torch.equal(mine, clean)
+    assert torch.isfinite(want).all()
+
+
 def test_attention_workspaces_graphs_and_streams():
     """Two captured graphs and an eager call, each with scratch of its own, on several streams at once; the launch flag."""
     a, b = Case([9000, 1700, 900], seed=1), Case([800, 9500], T=4, H=16, seed=2)     # parts that meet in scratch
