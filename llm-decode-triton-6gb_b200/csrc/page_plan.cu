@@ -283,10 +283,11 @@ extern "C" int b2d_page_plan(int32_t* page_table, int64_t ld_table, int pages_pe
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   // us a step, half of the steps taking pages and half giving them back. A thread writes four tokens, and up to 1024 of them one block
   // is faster than a cluster, which starts and ends later (8 x 128 tokens 4.5 against 5.0, 512 x 2 4.8 against 5.8; but 512 x 4
-  // 5.5 against 6.2 and 8 x 256 5.5 against 4.8). The scans go over the sequences in rounds of a block, where more warps cost
+  // 5.5 against 6.2 and 8 x 256 5.5 against 4.8), unless many sequences move pages (512 move four each: 6.6 against 5.3, 1024 11.3
+  // against 7.1; 1024 x 1 token 6.8 against 7.1). The scans go over the sequences in rounds of a block, where more warps cost
   // more in each: 256 threads and 512 take 3.9 and 4.1 for 8 x 1, 5.6 and 4.9 for 512 x 1; in a cluster 4.8 and 5.9 for
   // 8 x 256, 12.4 and 9.8 for 1024 x 64.
   const bool few = B <= 256;
-  if (max_tokens <= 1024) return few ? launch_plan<1, 256>(a, pdl, s) : launch_plan<1, 512>(a, pdl, s);
+  if (max_tokens <= 1024 && B <= 512) return few ? launch_plan<1, 256>(a, pdl, s) : launch_plan<1, 512>(a, pdl, s);
   return few ? launch_plan<kClusterSize, 256>(a, pdl, s) : launch_plan<kClusterSize, 512>(a, pdl, s);
 }
