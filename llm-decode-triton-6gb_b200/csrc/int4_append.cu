@@ -16,7 +16,8 @@
 // without (177 MB; copy rate 6.55); 320 tokens 4.2 us; one token 2.6 us (launch and a chain of three loads). Bound by issued
 // instructions and latency: 3200 warp instructions a token, 53 % of the slots, 21 warps per SM. Earlier forms: one warp for all heads of
 // a token with a division per code 87 us; packed fp32 instructions and corrected quotients 50; queries apart from keys 48. Reading
-// 8 x 4001 tokens: 38 us, 4.5 TB/s (a warp a token without the shared words 44).
+// 8 x 4001 tokens: 35.7 us, 4.8 TB/s, with 16-byte stores 38.5; 8 x 1021 tokens 12.0 and 14.6 (a warp a token without the
+// shared words and with stores of 16 bytes: 44).
 #include "int4_kv.cuh"
 
 namespace b2d {
@@ -449,10 +450,10 @@ struct Int4ReadArgs {
   uint32_t per_inv;
 };
 
-// The inverse, lane for lane: 16 neighbouring elements of a head from the step's bytes. O: output type. A warp has a token. A value
+// The inverse, lane for lane: 16 neighbouring elements of a head from the step's bytes. O: output type, WIDE: stores of 32 bytes. A warp has a token. A value
 // word holds four positions' bytes; where the 16 tokens of a tile lie together in the call (their 16 warps see that alike),
 // each of these warps takes four positions of the keys or of the values, and a quarter of the loads is left.
-template <typename T, typename O>
+template <typename T, typename O, bool WIDE>
 __device__ __forceinline__ void put_values(O* o, uint32_t sm, const uint32_t (&code)[16]) {   // codes in the words' low bits
   const float2 f = unpack_sm<T>(sm);
   const F2 s2 = pack(f.x, f.x), m2 = pack(f.y, f.y), base2 = pack(-8388608.f, -8388608.f);
@@ -462,15 +463,27 @@ __device__ __forceinline__ void put_values(O* o, uint32_t sm, const uint32_t (&c
     const F2 c = pack(__uint_as_float((code[e] & 15u) | 0x4B000000u), __uint_as_float((code[e + 1] & 15u) | 0x4B000000u));
     unpack(fma2(s2, add2(c, base2), m2), x[e], x[e + 1]);
   }
+  uint32_t w[sizeof(O) * 4];
   if constexpr (sizeof(O) == 4) {
 #pragma unroll
-    for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4*>(o + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+    for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(x[e]);
   } else {
-    *reinterpret_cast<uint4*>(o) = pack8<O>(x);
-    *reinterpret_cast<uint4*>(o + 8) = pack8<O>(x + 8);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = Dt<O>::pack2(x[2 * i], x[2 * i + 1]);
+  }
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(O)) * 4; i += 8) {
+    uint32_t* const to = reinterpret_cast<uint32_t*>(o) + i;
+    if constexpr (WIDE) {
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(to), "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]),
+                   "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7]) : "memory");
+    } else {
+      reinterpret_cast<uint4*>(to)[0] = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+      reinterpret_cast<uint4*>(to)[1] = make_uint4(w[i + 4], w[i + 5], w[i + 6], w[i + 7]);
+    }
   }
 }
-template <typename T, typename O>
+template <typename T, typename O, bool WIDE>
 __device__ __forceinline__ void put_key(O* o, uint32_t sm, const uint32_t (&w)[4], int j) {
   uint32_t code[16];
 #pragma unroll
@@ -481,9 +494,9 @@ __device__ __forceinline__ void put_key(O* o, uint32_t sm, const uint32_t (&w)[4
     code[4 * u + 2] = x >> 4;
     code[4 * u + 3] = x >> 20;
   }
-  put_values<T, O>(o, sm, code);
+  put_values<T, O, WIDE>(o, sm, code);
 }
-template <typename T, typename O>
+template <typename T, typename O, bool WIDE>
 __device__ __forceinline__ void put_value(O* o, uint32_t sm, const uint32_t (&w)[8], int shift) {
   uint32_t code[16];
 #pragma unroll
@@ -491,10 +504,10 @@ __device__ __forceinline__ void put_value(O* o, uint32_t sm, const uint32_t (&w)
     code[g] = w[g] >> shift;
     code[g + 8] = w[g] >> (shift + 4);
   }
-  put_values<T, O>(o, sm, code);
+  put_values<T, O, WIDE>(o, sm, code);
 }
 
-template <typename T, typename O, int D>
+template <typename T, typename O, int D, bool WIDE>
 __global__ void __launch_bounds__(kWarps * 32) int4_read_kernel(const __grid_constant__ Int4ReadArgs a) {
   constexpr int LANES = D / 16, HPW = 32 / LANES;
   pdl_launch_dependents();
@@ -542,7 +555,7 @@ __global__ void __launch_bounds__(kWarps * 32) int4_read_kernel(const __grid_con
             sm[i] = __ldg(reinterpret_cast<const uint32_t*>(tile + int4_vs_off(D, runs) + ((row0 + (i >> 1) + 8 * (i & 1)) * runs + j / run_lanes) * 4));
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) put_value<T, O>(out + (row0 + (i >> 1) + 8 * (i & 1)) * sn, sm[i], w, 8 * i);
+        for (int i = 0; i < 4; ++i) put_value<T, O, WIDE>(out + (row0 + (i >> 1) + 8 * (i & 1)) * sn, sm[i], w, 8 * i);
       } else {
         uint32_t w[4][4];
 #pragma unroll
@@ -559,7 +572,7 @@ __global__ void __launch_bounds__(kWarps * 32) int4_read_kernel(const __grid_con
           }
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) put_key<T, O>(out + (4 * quarter + i) * sn, sm[i], w[i], j);
+        for (int i = 0; i < 4; ++i) put_key<T, O, WIDE>(out + (4 * quarter + i) * sn, sm[i], w[i], j);
       }
     }
     return;
@@ -585,8 +598,8 @@ __global__ void __launch_bounds__(kWarps * 32) int4_read_kernel(const __grid_con
         for (int g = 0; g < 8; ++g) vw[g] = __ldg(b + g * 64);
       }
     }
-    if (a.k) put_key<T, O>(static_cast<O*>(a.k) + n * a.sk_n + h * a.sk_h + 16 * j, ksm, kw, j);
-    if (a.v) put_value<T, O>(static_cast<O*>(a.v) + n * a.sv_n + h * a.sv_h + 16 * j, vsm, vw, 0);
+    if (a.k) put_key<T, O, WIDE>(static_cast<O*>(a.k) + n * a.sk_n + h * a.sk_h + 16 * j, ksm, kw, j);
+    if (a.v) put_value<T, O, WIDE>(static_cast<O*>(a.v) + n * a.sv_n + h * a.sv_h + 16 * j, vsm, vw, 0);
   }
 }
 
@@ -611,7 +624,10 @@ int launch_read(const Int4ReadArgs& a, int sm, bool pdl, cudaStream_t s) {
   constexpr int HPW = 512 / D;
   const int items = (a.kv.KVH + HPW - 1) / HPW;
   const dim3 grid((a.N + kWarps - 1) / kWarps, warps_per_token(a.N, items, sm));
-  return launch_kernel(int4_read_kernel<T, O, D>, grid, dim3(kWarps * 32), 0, s, pdl, a);
+  // 32 bytes a store where all rows begin at multiples of 32 (8 x 4001 tokens 35.7 us, in halves 38.5)
+  const bool wide = aligned(a.k, 32) && aligned(a.v, 32) && (a.sk_n | a.sk_h | a.sv_n | a.sv_h) * sizeof(O) % 32 == 0;
+  if (wide) return launch_kernel(int4_read_kernel<T, O, D, true>, grid, dim3(kWarps * 32), 0, s, pdl, a);
+  return launch_kernel(int4_read_kernel<T, O, D, false>, grid, dim3(kWarps * 32), 0, s, pdl, a);
 }
 
 int check_tokens(const b2d_int4_kv* kv, const int32_t* seq_ids, int N, int B, int64_t ld_table, int pages_per_seq) {

@@ -569,6 +569,25 @@ def test_pool_past_four_gigabytes():
     assert all(torch.equal(x, y) for x, y in zip(*out)) and torch.isfinite(out[0][2]).all()
 
 
+@pytest.mark.parametrize("D,dtype,out_dtype", [(64, F16, F16), (128, BF16, BF16), (128, F16, F32), (64, BF16, F32)])
+def test_read_into_rows_of_any_allowed_alignment(D, dtype, out_dtype):
+    """Outputs that begin, or whose rows lie, at multiples of 16 bytes but not of 32, whole tiles and single tokens; what lies
+    beside them stays."""
+    c = Case([40, 21], KVH=3, H=3, D=D, dtype=dtype, seed=D)
+    N, item = c.pos.numel(), 8                               # rows apart by multiples of 8 elements
+    want = paged_int4_read(c.kv, c.pos.to(DEV), c.table.to(DEV), seq_ids=c.seq.to(DEV), out_dtype=out_dtype)
+    shuffle = torch.randperm(N, generator=torch.Generator().manual_seed(1))
+    for order in (torch.arange(N), shuffle):
+        for start, pad in ((0, 0), (4 if out_dtype == F32 else 8, 0), (0, item), (item, item)):
+            row = 3 * D + pad
+            memory = torch.full((2, N * row + 64), 7.0, dtype=out_dtype, device=DEV)
+            k, v = (m[start:start + N * row].view(N, row)[:, :3 * D].view(N, 3, D) for m in memory)
+            paged_int4_read(c.kv, c.pos[order].to(DEV), c.table.to(DEV), seq_ids=c.seq[order].to(DEV), k_out=k, v_out=v)
+            assert torch.equal(k, want[0][order.to(DEV)]) and torch.equal(v, want[1][order.to(DEV)])
+            k.fill_(7), v.fill_(7)
+            assert (memory == 7).all()
+
+
 # ------------------------------------------------------------------ page planning
 STATE = ("page_table", "held", "free", "ring")
 
