@@ -489,9 +489,10 @@ int b2d_int4_read(const b2d_int4_kv* kv, const int64_t* positions, const int32_t
 
 /* b2d_paged_attention over a 4-bit cache (no shared prefix): arguments, masks, lengths, workspace and limits as there (the
  * page table reaches at most 2^31 - 32768 positions). q has the cache's dtype. Keys and values enter the products as codes
- * (exact); a weight times its value's s is rounded to fp16 (2^-11) for the second product, everything else is fp32. out may be q
- * itself (of its dtype and strides) and overlaps no other input. bf16: values whose s is 2^111 or more and queries of 2^114 or more
- * may give infinities or NaN where the exact result is finite. */
+ * (exact); a weight p times its value's s is rounded to fp16 for the second product: by 2^-11 where p s is 2^-19 or more of the
+ * largest p s of its row (a query and head, all runs; what the row does not see does not count), by 2^-30 of that where it is
+ * less. Everything else is fp32. out may be q itself (of its dtype and strides) and overlaps no other input. bf16: values whose s is
+ * 2^111 or more, queries of 2^114 or more and scores of 2^126 or more may give infinities, NaN or zeros where the exact result is finite. */
 size_t b2d_int4_attention_workspace_bytes(const b2d_int4_kv* kv, int B, int T, int H, int pages_per_seq, int max_len);
 int b2d_int4_attention(const b2d_int4_kv* kv, const void* q, int64_t sq_b, int64_t sq_t, int64_t sq_h,
                        const int32_t* page_table, int64_t ld_table, int pages_per_seq, const int32_t* seqlens, int max_len,

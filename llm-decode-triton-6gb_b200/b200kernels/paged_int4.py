@@ -164,8 +164,9 @@ def paged_int4_attention(kv: PagedKVInt4, q: torch.Tensor, page_table: torch.Ten
     ``seqlens[b] - T + 1 + t``; one that sees none gives zeros. Lengths past the table's pages are cut to them. T and H / KVH up to 16.
     ``max_len``: an upper bound of ``seqlens`` known to the host, which only guides the split. ``out`` may be q itself and
     overlaps no other input. ``workspace``: contiguous scratch of ``paged_int4_attention_workspace`` bytes, 16-byte
-    aligned, not shared by calls that may overlap; without it one is allocated per call. bf16 only: values whose
-    s is 2^111 or more, and queries of 2^114 or more, may give infinities or NaN though the exact result is finite."""
+    aligned, not shared by calls that may overlap; without it one is allocated per call. A weight times its value's s is
+    rounded to fp16: by 2^-11, or by 2^-30 of the row's largest such term where it is below 2^-19 of that. bf16 only: values whose s is
+    2^111 or more, queries of 2^114 or more and scores of 2^126 or more may give infinities, NaN or zeros though the exact result is finite."""
     r = _lib.binding().int4_attention(kv._desc, q, page_table, seqlens, scale, max_len, out, out_dtype, workspace, flags,
                                       kv._index)
     if r.__class__ is int:

@@ -10,9 +10,10 @@
 // KV head.
 //  * A query row is scaled by a power of two into [2^14, 2^15) so that it and its part for the high nibbles (2^-4) are as
 //    exact in fp16 as in its own type.
-//  * A weight p_j s_j is rounded to fp16 (2^-11) around the largest s that the warp has seen: 2^(7 - E) p s lies below 2^15
-//    with p <= 2^8 and s <= 2^E, and down to 2^-21 of the largest it keeps all 11 bits. E and the running maximum move rarely
-//    (a maximum only when a score exceeds it by 2^8), on one vote.
+//  * A weight p_j s_j is rounded to fp16 (2^-11) in a unit of its row: unit p s lies below 2^15, and was above 2^5 for the largest
+//    p s that the row has met, so that all 11 bits are kept down to 2^-19 of that. What counts is what a key adds to the row: one with a
+//    huge s and next to no weight, or one that the row does not see, takes nothing from the others. The unit and the running
+//    maximum move rarely (a maximum only when a score exceeds it by 2^8), on one vote, and each row's by its own scores alone.
 //  * Every warp is on its own: it copies its tiles of 16 keys (2.3 KB, keys, values and factors in one asynchronous bulk copy)
 //    through a private ring of shared memory, waits on its own mbarriers, and meets the block's other warps only at the end
 //    of a unit. Codes are finite whatever a page holds; factors of keys that a row does not see are taken out by selection.
@@ -49,6 +50,8 @@ constexpr int kMaxCtas = 640;
 constexpr int kWholeKeys = 256, kWholeKeysMany = 512;
 constexpr float kLazy = 8.f;                    // log2 of the largest weight before the running maximum moves
 constexpr float kNone = -1.7e38f;               // running maximum before the first score
+constexpr float kMost = 0x1p15f;                // largest weight times s in its row's unit (fp16 ends at 65504)
+constexpr float kUnitMost = 0x1p115f;           // largest unit, and that before the first p s
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Blocks of an SM, by registers (accumulators: 32 a row tile), and tiles of a warp's ring, by shared memory.
@@ -245,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks<NT>) int4_attention_kernel(c
   static_assert(SLOTS >= 2, "a ring of at least two tiles");
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float s_m[kWarps][ROWS], s_l[kWarps][ROWS];
-  __shared__ float s_rowf[ROWS], s_qs[RUNS][ROWS];
+  __shared__ __align__(8) float s_rowf[ROWS], s_qs[RUNS][ROWS];
   __shared__ __align__(8) uint64_t s_bar[kWarps * SLOTS];
   __shared__ int s_sum[kMaxBatch + 1], s_len[kMaxBatch], s_warp[kWarps];
   __shared__ int64_t s_at[ROWS];        // per row: offset in the output, or workspace entry
@@ -363,23 +366,32 @@ __global__ void __launch_bounds__(kThreads, kBlocks<NT>) int4_attention_kernel(c
                               : (static_cast<int64_t>(blockIdx.x) * 2 + (g.kind - 1)) * ROWS + tid;
     }
     __syncthreads();
-    float rowf[NT][2], qs[RUNS][NT][2];   // of rows 8 n + 2 tq (+ 1)
+    // The rows' factors, of rows 8 n + 2 tq (+ 1): in registers for a unit, but in each tile from shared memory where they would
+    // spill (16 x 8 drafts, groups of 64: 52 us against 67; 16 x 3, groups of 32: 34.1, 39.4; but 16 x 5, groups of 64: 37.0, 35.7)
+    constexpr bool FAR = D == 128 && NT * RUNS >= 8;
+    float rowf[NT][2], qs[RUNS][NT][2];
+    auto pair = [&](float (&to)[2], const float* row, int n) {
+      const float2 x = *reinterpret_cast<const float2*>(row + 8 * n + 2 * tq);
+      to[0] = x.x;
+      to[1] = x.y;
+    };
+    if constexpr (!FAR) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n) {
+        pair(rowf[n], s_rowf, n);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        rowf[n][e] = s_rowf[8 * n + 2 * tq + e];
-#pragma unroll
-        for (int u = 0; u < RUNS; ++u) qs[u][n][e] = s_qs[u][8 * n + 2 * tq + e];
+        for (int u = 0; u < RUNS; ++u) pair(qs[u][n], s_qs[u], n);
       }
+    }
     // keys that this thread's rows see; below lim_min no row is masked
     const bool causal = a.T > 1;
     const int lim_min = causal ? g.limit + div_g(a, g.row0) : g.limit;
     auto lim = [&](int n, int e) { return causal ? g.limit + div_g(a, g.row0 + min(8 * n + 2 * tq + e, g.nrows - 1)) : g.limit; };
 
-    float o[STEPS][NT][4];   // element 16 m + g8 (+ 8), row 8 n + 2 tq (+ 1), in units of 2^(E - 7 - 24) (2^(E - 7 - 20))
+    float o[STEPS][NT][4];   // element 16 m + g8 (+ 8), row 8 n + 2 tq (+ 1), times the row's unit and 2^-24 (2^-20)
     float om[RUNS][NT][2];   // sum of p (m + 8 s) over this thread's keys
     float m_run[NT][2], l_run[NT][2];   // log2 domain; the sum over this thread's keys only
+    float unit[NT][2];       // a weight enters the second product as p s unit
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -388,8 +400,8 @@ __global__ void __launch_bounds__(kThreads, kBlocks<NT>) int4_attention_kernel(c
       for (int u = 0; u < RUNS; ++u) om[u][n][0] = om[u][n][1] = 0.f;
       m_run[n][0] = m_run[n][1] = kNone;
       l_run[n][0] = l_run[n][1] = 0.f;
+      unit[n][0] = unit[n][1] = kUnitMost;
     }
-    float v_top = 0.f, v_unit = 1.f;   // 2^E and 2^(7 - E); v_top = 0: no value yet
 
     // One tile: its scores, its weights, its part of o. MASKED: some row does not see some key of it.
     auto tile = [&](auto masked_, int key0) {
@@ -423,20 +435,24 @@ __global__ void __launch_bounds__(kThreads, kBlocks<NT>) int4_attention_kernel(c
         for (int u = 0; u < RUNS; ++u) {
           const float2 sm = unpack_sm<T>(f[u]);
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+          for (int n = 0; n < NT; ++n) {
+            if constexpr (FAR) pair(qs[u][n], s_qs[u], n);
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const float x = acc[u][n][2 * h + e];
               acc[0][n][2 * h + e] = fmaf(sm.y, qs[u][n][e], u == 0 ? sm.x * x : fmaf(sm.x, x, acc[0][n][2 * h + e]));
             }
+          }
         }
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n) {
+          if constexpr (FAR) pair(rowf[n], s_rowf, n);
 #pragma unroll
           for (int e = 0; e < 2; ++e) d[n][2 * h + e] = fmaf(acc[0][n][2 * h + e], rowf[n][e], -m_run[n][e]);
+        }
       }
       float2 vf[2][RUNS];   // the values' factors of keys g8 (+ 8)
-      float s_top = 0.f, d_top = -INFINITY;
+      float s_top[2] = {0.f, 0.f}, d_top = -INFINITY;   // the largest s of keys g8 (+ 8)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t f[RUNS];
@@ -444,6 +460,10 @@ __global__ void __launch_bounds__(kThreads, kBlocks<NT>) int4_attention_kernel(c
 #pragma unroll
         for (int u = 0; u < RUNS; ++u) vf[h][u] = unpack_sm<T>(f[u]);
       }
+      auto hidden = [&](int n, int h, int e) {
+        const int key = key0 + g8 + 8 * h;
+        return MASKED && (key >= lim(n, e) || key >= g.t_end);
+      };
       if constexpr (MASKED) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -452,74 +472,85 @@ __global__ void __launch_bounds__(kThreads, kBlocks<NT>) int4_attention_kernel(c
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e)
-              if (key >= lim(n, e) || key >= g.t_end) d[n][2 * h + e] = -INFINITY;
+              if (hidden(n, h, e)) d[n][2 * h + e] = -INFINITY;
           if (key >= g.t_end) {   // what lies behind the last key is not the cache's
 #pragma unroll
             for (int u = 0; u < RUNS; ++u) vf[h][u] = make_float2(0.f, 0.f);
           }
         }
       }
+      float w[NT][4], w_top[2] = {0.f, 0.f};   // the weights in their rows' units
+      auto weigh = [&](int n, int c) {
+        d[n][c] = exp2_fast(d[n][c]);
+        w[n][c] = d[n][c] * unit[n][c & 1];
+      };
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int u = 0; u < RUNS; ++u) s_top = fmaxf(s_top, vf[h][u].x);
+        for (int u = 0; u < RUNS; ++u) s_top[h] = fmaxf(s_top[h], vf[h][u].x);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) d_top = fmaxf(d_top, fmaxf(d[n][2 * h], d[n][2 * h + 1]));
-      }
-      if (__any_sync(0xffffffffu, s_top > v_top || d_top > kLazy)) {
-        const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(s_top));
-        float keep = 1.f;
-        if (__uint_as_float(bits) > v_top) {   // 2^E with room for twice the largest s; E in [-110, 110]
-          const int ex = min(max(static_cast<int>(bits >> 23) - 127 + 2, -110), 110);
-          const float unit = __uint_as_float((127 + 7 - ex) << 23);
-          keep = v_top > 0.f ? unit / v_unit : 1.f;
-          v_top = __uint_as_float((127 + ex) << 23);
-          v_unit = unit;
+        for (int n = 0; n < NT; ++n) {
+          d_top = fmaxf(d_top, fmaxf(d[n][2 * h], d[n][2 * h + 1]));
+          weigh(n, 2 * h);
+          weigh(n, 2 * h + 1);
+          w_top[h] = fmaxf(w_top[h], fmaxf(w[n][2 * h], w[n][2 * h + 1]));
         }
+      }
+      if (__any_sync(0xffffffffu, fmaxf(w_top[0] * s_top[0], w_top[1] * s_top[1]) > kMost || d_top > kLazy)) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n) {
+          if constexpr (FAR) pair(rowf[n], s_rowf, n);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float x[2], top = -INFINITY;
+            float top = -INFINITY, most = 0.f;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              x[h] = d[n][2 * h + e] == -INFINITY ? -INFINITY : acc[0][n][2 * h + e] * rowf[n][e];
-              top = fmaxf(top, x[h]);
-            }
+            for (int h = 0; h < 2; ++h) top = fmaxf(top, hidden(n, h, e) ? -INFINITY : acc[0][n][2 * h + e] * rowf[n][e]);
 #pragma unroll
             for (int i = 4; i < 32; i <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
             const bool up = top > m_run[n][e] + kLazy;
             const float alpha = up ? exp2_fast(m_run[n][e] - top) : 1.f;   // m_run = kNone: 0
             if (up) m_run[n][e] = top;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) d[n][2 * h + e] = x[h] - m_run[n][e];
+            for (int h = 0; h < 2; ++h) {
+              d[n][2 * h + e] = hidden(n, h, e) ? -INFINITY : fmaf(acc[0][n][2 * h + e], rowf[n][e], -m_run[n][e]);
+              most = fmaxf(most, exp2_fast(d[n][2 * h + e]) * s_top[h]);
+            }
+#pragma unroll
+            for (int i = 4; i < 32; i <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, i));
+            // what alpha takes from the sums the unit may give back; then the tile's largest p s goes to [2^5, 2^6)
+            float now = up ? fminf(__fdividef(unit[n][e], alpha), kUnitMost) : unit[n][e];
+            if (most * now > kMost) {
+              const int ex = min(static_cast<int>(__float_as_uint(most) >> 23) - 127, 108);
+              now = __uint_as_float((127 + 5 - ex) << 23);
+            }
+            const float keep = __fdividef(alpha * now, unit[n][e]);
+            unit[n][e] = now;
             l_run[n][e] *= alpha;
-            const float ak = alpha * keep;
 #pragma unroll
             for (int u = 0; u < RUNS; ++u) om[u][n][e] *= alpha;
 #pragma unroll
             for (int m = 0; m < STEPS; ++m) {
-              o[m][n][e] *= ak;
-              o[m][n][2 + e] *= ak;
+              o[m][n][e] *= keep;
+              o[m][n][2 + e] *= keep;
             }
+            weigh(n, e);
+            weigh(n, 2 + e);
           }
+        }
       }
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          d[n][c] = exp2_fast(d[n][c]);   // the weights
-          l_run[n][c & 1] += d[n][c];
-        }
+        for (int c = 0; c < 4; ++c) l_run[n][c & 1] += d[n][c];
       uint32_t pb[RUNS][NT][2];   // P s as the B operand: row 8 n + g8, keys 2 tq .. (+ 8)
 #pragma unroll
       for (int u = 0; u < RUNS; ++u) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float su = vf[h][u].x * v_unit, center = fmaf(8.f, vf[h][u].x, vf[h][u].y);
+          const float su = vf[h][u].x, center = fmaf(8.f, su, vf[h][u].y);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            float w0 = d[n][2 * h] * su, w1 = d[n][2 * h + 1] * su;
+            float w0 = w[n][2 * h] * su, w1 = w[n][2 * h + 1] * su;
             if constexpr (MASKED) {   // factors that are infinite or NaN reach the rows that see their key, and no other
               const int key = key0 + g8 + 8 * h;
               if (key < lim(n, 0)) om[u][n][0] = fmaf(d[n][2 * h], center, om[u][n][0]);
@@ -582,7 +613,6 @@ __global__ void __launch_bounds__(kThreads, kBlocks<NT>) int4_attention_kernel(c
     }
 
     // ---- the unit's (or this CTA's part of it) result: the warps meet in shared memory
-    const float to_lo = 0x1p24f / v_unit, to_hi = 0x1p20f / v_unit;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -623,7 +653,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks<NT>) int4_attention_kernel(c
       if (n > 0) __syncthreads();
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float factor = s_m[warp][8 * n + 2 * tq + e];
+        const float factor = s_m[warp][8 * n + 2 * tq + e], to_lo = 0x1p24f / unit[n][e], to_hi = 0.0625f * to_lo;
         float* dst = s_o + (warp * 8 + 2 * tq + e) * PAD + g8;
 #pragma unroll
         for (int m = 0; m < STEPS; ++m) {

@@ -409,6 +409,69 @@ def test_attention_sizes_of_queries_and_values(size):
     c.check(c.run())
 
 
+def check_by_row(c, out):
+    """Each row against what its own keys add to it. A weight p s keeps its 11 bits down to 2^-19 of the largest p s that the row
+    has met and is rounded by 2^-30 of that below (2^-25 steps of a unit in which the largest was 2^5 or more), times a centred
+    code up to 8: 2^-27 of it a key; its size is at most a fifteenth of the row's largest mass = sum p (|m| + 15 s). Scores and sums as
+    in the bounds above, of this mass (codes are centred, so that sums are as large as the run's range)."""
+    (k, _), (v, _) = c.pools(values_ref)
+    (ksize, _), (wide, _) = c.pools(lambda codes, s, m, D: size_ref(np.full_like(codes, 15), s, m, D))
+    ksize = c.pools(size_ref)[0][0]
+    args = (c.table.numpy(), c.lens.numpy(), c.scale)
+    ref, _, _ = paged_attention_ref(f64(c.q), k, v, *args)
+    mass, _, _ = paged_attention_ref(f64(c.q), k, wide, *args)
+    _, _, reach = paged_attention_ref(f64(c.q), ksize, v, *args)
+    n, D = int(c.lens.max()), c.q.shape[-1]
+    bound = (2.0 ** -11 + 8 * D * 2.0 ** -23 * reach[..., None] + n * 2.0 ** -23) * mass + n * 2.0 ** -27 / 15 * mass.max(-1, keepdims=True)
+    bound = bound + half_step(out.dtype) * (np.abs(ref) + bound) + 2.0 ** -25 * (out.dtype == F16)
+    err = np.abs(f64(out) - ref)
+    assert (err <= bound).all(), f"worst error / bound {(err / bound).max():.2e}"
+
+
+@pytest.mark.parametrize("H,T", [(8, 2), (16, 2), (16, 3), (16, 4)])   # 8 to 32 rows of a KV head
+@pytest.mark.parametrize("D,group,dtype", [(64, 64, BF16), (128, 32, BF16), (128, 64, F16), (64, 32, F16)])
+@pytest.mark.parametrize("where", ["hidden", "first", "middle", "last", "many"])
+def test_attention_huge_values_of_little_weight(H, T, D, group, dtype, where):
+    """Values 2^40 (fp16: 2^25) times the others' that a row does not see, or gives next to no weight, wherever they lie: the first keys
+    that a warp meets, before a running maximum that rises by 60, or behind it."""
+    g = torch.Generator().manual_seed(D + T)
+    lens = [700, 300 + T]
+    direction = torch.randn(D, generator=g).sign()
+    small, huge = (1.0, 2.0 ** 40) if dtype == BF16 else (2.0 ** -10, 2.0 ** 15 - 2.0 ** 5)
+
+    def chosen(seq, pos):
+        n = torch.tensor(lens)[seq.long()]
+        return {"hidden": pos == n - 1, "first": pos == 0, "middle": pos == 150, "last": pos == n - T - 1, "many": pos < 200}[where]
+
+    def values(seq, pos):
+        return torch.randn(pos.numel(), 2, D, generator=g).clamp(-2, 2) * torch.where(chosen(seq, pos), huge / 2, small)[:, None, None]
+
+    def keys(seq, pos):   # little weight: scores of -60 log2 units against a few
+        low = torch.where(chosen(seq, pos) & (where != "hidden"), -42.0 * D ** -0.5, 0.0)[:, None, None]
+        return 0.3 * torch.randn(pos.numel(), 2, D, generator=g) + low * direction
+
+    c = Case(lens, H=H, KVH=2, T=T, D=D, group=group, dtype=dtype, seed=H + T, keys=keys, values=values)
+    c.q = (0.2 * torch.randn(c.q.shape, generator=g) + direction).to(dtype)
+    check_by_row(c, c.run(out_dtype=F32))
+    check_by_row(c, c.run(max_len=200, out_dtype=F32))    # a unit a block
+
+
+def test_attention_rows_do_not_depend_on_one_another():
+    """Bits of a row with and without others that move their own maximum or unit in the same tiles."""
+    g = torch.Generator().manual_seed(4)
+    grow = lambda seq, pos: torch.randn(pos.numel(), 1, 64, generator=torch.Generator().manual_seed(8)) * 2.0 ** (pos % 23)[:, None, None]  # noqa: E731
+    c = Case([900], H=4, KVH=1, T=1, D=64, dtype=BF16, seed=3, values=grow)
+    c.q = torch.randn(1, 1, 4, 64, generator=g).bfloat16()
+    want = c.run()
+    check_by_row(c, want)
+    for row in range(4):
+        other = c.q.clone()
+        c.q = (torch.randn(1, 1, 4, 64, generator=g) * 20).bfloat16()
+        c.q[:, :, row] = other[:, :, row]
+        assert torch.equal(c.run()[:, :, row], want[:, :, row])
+        c.q = other
+
+
 def test_attention_layouts_and_strides():
     c = Case([100, 33, 257], dtype=BF16, T=2, seed=5)
     ref = c.run()
