@@ -18,6 +18,8 @@
 // a token with a division per code 87 us; packed fp32 instructions and corrected quotients 50; queries apart from keys 48. Reading
 // 8 x 4001 tokens: 35.7 us, 4.8 TB/s, with 16-byte stores 38.5; 8 x 1021 tokens 12.0 and 14.6 (a warp a token without the
 // shared words and with stores of 16 bytes: 44).
+#include <type_traits>
+
 #include "int4_kv.cuh"
 
 namespace b2d {
@@ -260,18 +262,35 @@ __device__ __forceinline__ void append_queries(const Int4AppendArgs& a, int64_t 
     }
     float r = 1.f;
     if (a.q_weight) {
-      F2 s1 = mul2(x1[0], x1[0]), s2 = mul2(x2[0], x2[0]);
+      auto squares = [&] {
+        F2 s1 = mul2(x1[0], x1[0]), s2 = mul2(x2[0], x2[0]);
 #pragma unroll
-      for (int i = 1; i < 4; ++i) {
-        s1 = fma2(x1[i], x1[i], s1);
-        s2 = fma2(x2[i], x2[i], s2);
+        for (int i = 1; i < 4; ++i) {
+          s1 = fma2(x1[i], x1[i], s1);
+          s2 = fma2(x2[i], x2[i], s2);
+        }
+        float ss, st;
+        unpack(add2(s1, s2), ss, st);
+        ss += st;
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        return ss;
+      };
+      float ss = squares(), eps = a.eps;
+      if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+        // squares that leave fp32 (elements of 2^60 and more, or none above 2^-40 and no eps to speak of): the head times 2^-70 or 2^80
+        const float f = h >= a.H ? 1.f : ss > 0x1p120f ? 0x1p-70f : ss < 0x1p-80f && eps < 0x1p-60f ? 0x1p80f : 1.f;
+        if (__any_sync(0xffffffffu, f != 1.f)) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            x1[i] = mul2(x1[i], pack(f, f));
+            x2[i] = mul2(x2[i], pack(f, f));
+          }
+          ss = squares();
+          eps = eps * f * f;
+        }
       }
-      float ss, st;
-      unpack(add2(s1, s2), ss, st);
-      ss += st;
-#pragma unroll
-      for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      r = rsqrtf(fmaf(ss, 1.f / D, a.eps));
+      r = rsqrtf(fmaf(ss, 1.f / D, eps));
     }
     const F2 r2 = pack(r, r);
     float y[16];

@@ -142,6 +142,39 @@ def test_append_weights_alone_of_either():
         check_values(gk, turn_ref(k.float().numpy(), None, None, False, None if kw is None else f64(kw), 1e-5, exact32=True), 64, F16)
 
 
+@pytest.mark.parametrize("D,R,interleaved", [(128, 128, False), (128, 64, True), (64, 64, False), (64, 16, True)])
+@pytest.mark.parametrize("size", [1e38, 1e30, 1e19, 2.0 ** 60, 1e-13, 1e-25, 1e-37])
+def test_append_norms_of_any_size(D, R, interleaved, size):
+    """Heads whose squares leave fp32's range, next to ordinary ones (whose bits stay) and one of zeros; queries and keys alike."""
+    N, B, H, KVH = 24, 3, 10, 5
+    q, k, v, pos, table = append_case(N, B, H, KVH, D, BF16, seed=D)
+    cos, sin = rotary_tables(512, R, 1e4)
+    w = (1 + 0.3 * torch.randn(D, generator=torch.Generator().manual_seed(6))).bfloat16()
+    kv = empty_pool(table.numel(), KVH, 16, D, BF16)
+
+    def run(q, k):
+        return paged_int4_append(kv, q.to(DEV), k.to(DEV), v.to(DEV), pos.to(DEV), table.to(DEV), cos.to(DEV), sin.to(DEV),
+                                 interleaved=interleaved, q_weight=w.to(DEV), k_weight=w.to(DEV), eps=0.0)
+
+    usual = run(q, k)
+    q, k = q.clamp(-3, 3), k.clamp(-3, 3)
+    q[:, 1::3], k[:, 1::3] = (q[:, 1::3].float() * size).bfloat16(), (k[:, 1::3].float() * size).bfloat16()
+    q[:, 5] = 0
+    out = run(q, k)
+    gk, _ = paged_int4_read(kv, pos.to(DEV), table.to(DEV), out_dtype=F32)
+    c, s = f64(cos)[pos.numpy()], f64(sin)[pos.numpy()]
+    check_values(gk, turn_ref(k.float().numpy(), c, s, interleaved, f64(w), 0.0, exact32=True), 64, BF16)
+    keep = [0, 2, 3, 6, 8, 9]
+    same = (q[:, keep].abs() < 3).all(-1)
+    assert torch.equal(out.cpu()[:, keep][same], usual.cpu()[:, keep][same]) and same.any()
+    live = [h for h in range(H) if h != 5]
+    ref = turn_ref(f64(q)[:, live], c, s, interleaved, f64(w), 0.0)
+    normed = turn_ref(f64(q)[:, live], None, None, interleaved, f64(w), 0.0)
+    bound = np.abs(turn_ref(np.abs(normed), np.abs(c), -np.abs(s), interleaved)) + np.abs(turn_ref(np.abs(normed), np.abs(c), np.abs(s), interleaved))
+    err = np.abs(f64(out)[:, live] - ref)
+    assert (err <= half_step(BF16) * np.abs(ref) + 2.0 ** -19 * bound + 2.0 ** -25).all(), err.max()
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_append_odd_values(dtype):
     """Equal elements, tiny and huge ranges, ties of the rounding, signed zeros, infinities and NaN."""
