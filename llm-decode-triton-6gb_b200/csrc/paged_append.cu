@@ -10,11 +10,13 @@
 // heads are always under way: every thread copies its own chunks through two private stages of shared memory
 // (16-byte cp.async), so no thread waits for another. The products w * cos and w * sin are formed once per
 // thread and token and serve all of its heads.
-// Measured on B200: 8168 tokens of 32 + 8 + 8 heads of 128 with norms, bf16: 45.0 us, 4.5 TB/s of read and written
-// bytes (copy rate 6.52); 320 tokens 4.9 us; one token 2.4 us (launch and latency). Bound by bytes in the limit,
+// Measured on B200: 8168 tokens of 32 + 8 + 8 heads of 128 with norms, bf16: 46.3 us, 4.35 TB/s of read and written
+// bytes (copy rate 6.55; without the look at the sums of squares 45.1); 320 tokens 4.9 us; one token 2.4 us (launch and latency). Bound by bytes in the limit,
 // 2 (H + 2 KVH) D elements a token. What is left at 8168 tokens is latency: 16.7 warps per SM are active (shared
 // memory allows 9 blocks) and issue in half of the slots. One head per thread took 49 us, three stages 51, four-element
 // halves 58 to 63 with 80 % of the slots issuing.
+#include <type_traits>
+
 #include "paged.cuh"
 
 namespace b2d {
@@ -109,11 +111,29 @@ __device__ __forceinline__ Pair turn_pair(const Pair& p, const Turn& t, bool nor
   unpack8<T>(p.lo, x1);
   unpack8<T>(p.hi, x2);
   if (norm) {
-    float ss = 0.f;
+    auto squares = [&] {
+      float ss = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) ss = fmaf(x1[e], x1[e], fmaf(x2[e], x2[e], ss));
+      for (int e = 0; e < 8; ++e) ss = fmaf(x1[e], x1[e], fmaf(x2[e], x2[e], ss));
 #pragma unroll
-    for (int o = GROUP / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      for (int o = GROUP / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      return ss;
+    };
+    float ss = squares();
+    if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+      // squares that leave fp32 (elements of 2^60 and more, or none above 2^-40 and no eps to speak of): the head times 2^-70 or 2^80
+      const float least = eps < 0x1p-60f ? 0x1p-80f : 0.f;
+      if (__any_sync(0xffffffffu, !(ss >= least && ss <= 0x1p120f))) {
+        const float f = ss > 0x1p120f ? 0x1p-70f : ss < least ? 0x1p80f : 1.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x1[e] *= f;
+          x2[e] *= f;
+        }
+        ss = squares();
+        eps = eps * f * f;
+      }
+    }
     r = rsqrtf(fmaf(ss, inv_d, eps));
   }
   float y1[8], y2[8];

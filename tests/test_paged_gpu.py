@@ -554,6 +554,36 @@ def test_append_mixed_batch(N, norm):
     assert (kp.cpu().transpose(1, 2)[untouched] == 5).all() and (vp.cpu().transpose(1, 2)[untouched] == 5).all()
 
 
+@pytest.mark.parametrize("N,H,KVH,D", [(6, 10, 5, 128), (6, 7, 7, 80), (4000, 32, 8, 128)])   # direct, with idle lanes, staged
+@pytest.mark.parametrize("size", [1e38, 1e19, 2.0 ** 60, 1e-13, 1e-25, 1e-37])
+def test_append_norms_of_any_size(N, H, KVH, D, size):
+    """Heads whose squares leave fp32's range, next to ordinary ones whose bits stay."""
+    g = torch.Generator().manual_seed(N + D)
+    per = N // 2 // 16 + 1
+    table = torch.randperm(2 * per, generator=g).int().view(2, per)
+    positions = torch.arange(N // 2).repeat(2)
+    q, k, v = (torch.randn(N, h, D, generator=g).clamp(-3, 3).to(BF16) for h in (H, KVH, KVH))
+    ang = torch.randn(N, D, generator=g) * 3
+    cos, sin = ang.cos(), ang.sin()
+    w = (1 + 0.3 * torch.randn(D, generator=g)).to(BF16)
+    kp, vp = (torch.zeros(2 * per, KVH, 16, D, dtype=BF16, device=DEV) for _ in range(2))
+    page, slot = table[torch.arange(N) // (N // 2), positions // 16].long(), positions % 16
+
+    def run(q, k):
+        out = paged_rope_append(PagedKV(kp, vp), q.to(DEV), k.to(DEV), v.to(DEV), positions.to(DEV), table.to(DEV), cos.to(DEV),
+                                sin.to(DEV), q_weight=w.to(DEV), k_weight=w.to(DEV), eps=0.0)
+        return out.cpu(), kp.cpu()[page, :, slot]
+
+    usual = run(q, k)
+    q[:, 1::3], k[:, 1::3] = (q[:, 1::3].float() * size).to(BF16), (k[:, 1::3].float() * size).to(BF16)
+    for got, x, was in zip(run(q, k), (q, k), usual):
+        keep = [h for h in range(x.shape[1]) if h % 3 != 1]
+        assert torch.equal(got[:, keep], was[:, keep])
+        ref, bound = rope_ref(f64(x), f64(cos)[positions.numpy()], f64(sin)[positions.numpy()], f64(w), 0.0)
+        err = np.abs(f64(got) - ref)
+        assert (err <= half_step(BF16) * np.abs(ref) + 2.0 ** -19 * bound + 2.0 ** -25).all(), err.max()
+
+
 def test_append_padding_and_bad_pages_write_nothing():
     N, H, KVH, D, ps, S = 8, 4, 2, 64, 16, 40
     g = torch.Generator().manual_seed(1)
