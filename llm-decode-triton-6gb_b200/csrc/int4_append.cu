@@ -469,6 +469,10 @@ struct Int4ReadArgs {
   uint32_t per_inv;
 };
 
+// Ordinary loads for what an earlier kernel of the stream may have written: this one may be resident, behind other dependent
+// launches, before that kernel begins, and the read-only path does not promise to see what is written meanwhile.
+__device__ __forceinline__ uint32_t load32(const uint8_t* p) { return *reinterpret_cast<const uint32_t*>(p); }
+
 // The inverse, lane for lane: 16 neighbouring elements of a head from the step's bytes. O: output type, WIDE: stores of 32 bytes. A warp has a token. A value
 // word holds four positions' bytes; where the 16 tokens of a tile lie together in the call (their 16 warps see that alike),
 // each of these warps takes four positions of the keys or of the values, and a quarter of the loads is left.
@@ -568,10 +572,10 @@ __global__ void __launch_bounds__(kWarps * 32) int4_read_kernel(const __grid_con
         if (there) {
 #pragma unroll
           for (int g = 0; g < 8; ++g)
-            w[g] = __ldg(reinterpret_cast<const uint32_t*>(tile + int4_v_off(D) + (j / 4) * 512 + (g * 4 + quarter) * 16 + (j % 4) * 4));
+            w[g] = load32(tile + int4_v_off(D) + (j / 4) * 512 + (g * 4 + quarter) * 16 + (j % 4) * 4);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            sm[i] = __ldg(reinterpret_cast<const uint32_t*>(tile + int4_vs_off(D, runs) + ((row0 + (i >> 1) + 8 * (i & 1)) * runs + j / run_lanes) * 4));
+            sm[i] = load32(tile + int4_vs_off(D, runs) + ((row0 + (i >> 1) + 8 * (i & 1)) * runs + j / run_lanes) * 4);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) put_value<T, O, WIDE>(out + (row0 + (i >> 1) + 8 * (i & 1)) * sn, sm[i], w, 8 * i);
@@ -584,10 +588,10 @@ __global__ void __launch_bounds__(kWarps * 32) int4_read_kernel(const __grid_con
         if (there) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            sm[i] = __ldg(reinterpret_cast<const uint32_t*>(tile + int4_ks_off(D) + ((4 * quarter + i) * runs + j / run_lanes) * 4));
+            sm[i] = load32(tile + int4_ks_off(D) + ((4 * quarter + i) * runs + j / run_lanes) * 4);
 #pragma unroll
             for (int u = 0; u < 4; ++u)
-              w[i][u] = __ldg(reinterpret_cast<const uint32_t*>(tile + (4 * quarter + i) * (D / 2) + 4 * (j / 2) + u * (D / 8)));
+              w[i][u] = load32(tile + (4 * quarter + i) * (D / 2) + 4 * (j / 2) + u * (D / 8));
           }
         }
 #pragma unroll
@@ -605,16 +609,16 @@ __global__ void __launch_bounds__(kWarps * 32) int4_read_kernel(const __grid_con
     for (int u = 0; u < 4; ++u) kw[u] = vw[u] = vw[4 + u] = 0;
     if (there) {   // every load under way before the first is used
       if (a.k) {
-        ksm = __ldg(reinterpret_cast<const uint32_t*>(tile + int4_ks_off(D) + (row * runs + j / run_lanes) * 4));
+        ksm = load32(tile + int4_ks_off(D) + (row * runs + j / run_lanes) * 4);
         const uint8_t* b = tile + row * (D / 2) + 4 * (j / 2);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) kw[u] = __ldg(reinterpret_cast<const uint32_t*>(b + u * (D / 8)));
+        for (int u = 0; u < 4; ++u) kw[u] = load32(b + u * (D / 8));
       }
       if (a.v) {
-        vsm = __ldg(reinterpret_cast<const uint32_t*>(tile + int4_vs_off(D, runs) + (row * runs + j / run_lanes) * 4));
+        vsm = load32(tile + int4_vs_off(D, runs) + (row * runs + j / run_lanes) * 4);
         const uint8_t* b = tile + int4_v_off(D) + (j / 4) * 512 + ((row % 8) / 2) * 16 + (j % 4) * 4 + (row & 1) * 2 + row / 8;
 #pragma unroll
-        for (int g = 0; g < 8; ++g) vw[g] = __ldg(b + g * 64);
+        for (int g = 0; g < 8; ++g) vw[g] = b[g * 64];
       }
     }
     if (a.k) put_key<T, O, WIDE>(static_cast<O*>(a.k) + n * a.sk_n + h * a.sk_h + 16 * j, ksm, kw, j);

@@ -160,8 +160,15 @@ struct Line {
   }
 };
 
+// An int32 from L2, in its place among the waits
+__device__ __forceinline__ int load_l2(const int32_t* p) {
+  int v;
+  asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];\n" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+
 // The sequences' lengths, cut to the page table, into s_len and the exclusive running sums of their units' cost into
-// s_sum[0 .. B] (all THREADS of the block take part).
+// s_sum[0 .. B] (all THREADS of the block take part). The lengths come from L2: the combine reads them ahead of its wait.
 template <int NT, int THREADS>
 __device__ __forceinline__ void scan_costs(const Int4AttnArgs& a, int* s_sum, int* s_len, int* s_warp) {
   constexpr int W = THREADS / 32;
@@ -170,7 +177,7 @@ __device__ __forceinline__ void scan_costs(const Int4AttnArgs& a, int* s_sum, in
   int run = 0;
   for (int b0 = 0; b0 < a.B; b0 += THREADS) {
     const int b = b0 + tid;
-    const int len = b < a.B ? min(max(a.seqlens[b], 0), reach) : 0;
+    const int len = b < a.B ? min(max(load_l2(a.seqlens + b), 0), reach) : 0;
     const int own = b < a.B ? Line<NT>::cost_of(a, len) : 0;
     int v = own;
 #pragma unroll
@@ -281,7 +288,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks<NT>) int4_attention_kernel(c
     const int key = fg.t_begin + ((ft + ((lane - ft) & 31)) * kWarps + warp) * kTileKeys;
     src = g_zero_tile;   // of a page id outside the pool: keys and values of zeros
     if (key < fg.t_end) {
-      const int pi = a.div.page(key), page = __ldg(a.table + fg.b * a.ld_table + pi);
+      const int pi = a.div.page(key), page = a.table[fg.b * a.ld_table + pi];   // (not the read-only path: see int4_append.cu)
       if (page >= 0 && page < a.kv.num_pages)
         src = a.kv.pages + page * a.kv.sp_p + fg.kvh * a.kv.sp_h + static_cast<int64_t>(a.div.slot(key, pi) / kTileKeys) * TILE;
     }
@@ -326,8 +333,8 @@ __global__ void __launch_bounds__(kThreads, kBlocks<NT>) int4_attention_kernel(c
       const int r = i * QROWS + tid / QL, rr = g.row0 + r, t = div_g(a, rr);
       q_raw[i] = make_uint4(0, 0, 0, 0);
       if (r < g.nrows)
-        q_raw[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + g.b * a.sq_b + t * a.sq_t +
-                                                        static_cast<int64_t>(g.kvh * a.G + rr - t * a.G) * a.sq_h + 8 * (tid % QL)));
+        q_raw[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + g.b * a.sq_b + t * a.sq_t +
+                                                   static_cast<int64_t>(g.kvh * a.G + rr - t * a.G) * a.sq_h + 8 * (tid % QL));
     }
 #pragma unroll
     for (int i = 0; i < QN; ++i) {

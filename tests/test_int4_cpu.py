@@ -272,6 +272,15 @@ def test_every_bounded_wait_is_looked_at():
         assert re.search(r"landed = (landed && )?mbar_wait\(", line), line
 
 
+def test_nothing_that_kernels_write_takes_the_read_only_path():
+    """With programmatic launches a kernel may be resident while earlier ones still write what it reads behind its wait: no
+    load of these kernels may be one that promises data constant for the kernel's lifetime."""
+    folder = Path(__file__).resolve().parent.parent / "llm-decode-triton-6gb_b200" / "csrc"
+    for name in ("int4_append.cu", "int4_attention.cu", "int4_kv.cuh", "page_plan.cu"):
+        code = "\n".join(line.split("//")[0] for line in (folder / name).read_text().splitlines())
+        assert not re.search(r"__ldg\(|ldg_\w+\(|\.nc\b|__restrict__", code), name
+
+
 # ---- rotary tables
 def angles(cos, sin):
     return torch.atan2(sin.double(), cos.double())

@@ -645,6 +645,84 @@ def test_programmatic_launches_see_what_the_kernel_before_wrote():
     assert all(torch.equal(x, y) for x, y in zip(plain, early)) and torch.isfinite(plain[0]).all()
 
 
+def test_programmatic_read_append_read_of_one_pool():
+    """Each read sees the append before it, all of them dependent launches on the same positions: no kernel between them."""
+    N, KVH, D, ps = 4096, 4, 128, 16
+    g = torch.Generator().manual_seed(5)
+    table = torch.randperm(N // ps, generator=g).int().view(4, -1).to(DEV)
+    pos = torch.arange(N // 4).repeat(4).to(DEV)
+    rounds = [[torch.randn(N, KVH, D, generator=g).half().to(DEV) for _ in range(2)] for _ in range(6)]
+
+    def chain(flags):
+        kv = PagedKVInt4.empty(N // ps, KVH, ps, D, F16, DEV)
+        outs = [[torch.empty(N, KVH, D, dtype=F16, device=DEV) for _ in range(2)] for _ in rounds]
+        torch.cuda.synchronize()
+        for (k, v), (ko, vo) in zip(rounds, outs):
+            paged_int4_read(kv, pos, table, k_out=ko, v_out=vo, flags=flags)      # the round's before
+            paged_int4_append(kv, None, k, v, pos, table, flags=flags)
+            paged_int4_read(kv, pos, table, k_out=ko, v_out=vo, flags=flags)
+        return outs
+
+    for plain, early in zip(chain(0), chain(_lib.LAUNCH_PDL)):
+        assert all(torch.equal(x, y) for x, y in zip(plain, early))
+    for (k, _), (ko, _) in zip(rounds, chain(_lib.LAUNCH_PDL)):
+        step = (k.unflatten(-1, (-1, 64)).float().amax(-1) - k.unflatten(-1, (-1, 64)).float().amin(-1)).max() / 15
+        assert (ko.float() - k.float()).abs().max() <= 0.51 * step
+
+
+@pytest.mark.parametrize("T,base", [(1, 900), (4, 300), (3, 2500)])
+def test_programmatic_serving_steps(T, base):
+    """Plan, append, attention, plan, ... as dependent launches with no other kernel among them: the attention's queries are the append's
+    output as it lies, its lengths and tables the plan's, and the next plan takes and gives back pages that the attention has read."""
+    B, H, KVH, D, ps, W = 24, 8, 2, 128, 16, 200
+    g = torch.Generator().manual_seed(T)
+    cos, sin = (t.to(DEV) for t in rotary_tables(W * ps, D))
+    start = torch.randint(base // 2, base, (B,), generator=g).int()
+    steps = []
+    for i in range(8):   # grow by T, and by turns fall back by some pages
+        cached = (start + T * i if i % 3 else (start * 0.7).int()).to(DEV)
+        q, k, v = (torch.randn(B * T, h, D, generator=g).half().to(DEV) for h in (H, KVH, KVH))
+        steps.append((cached, q, k, v))
+    new = torch.full((B,), T, dtype=torch.int32, device=DEV)
+    fill = [torch.randn(B * W * ps, KVH, D, generator=g).half().to(DEV) for _ in range(2)]
+
+    def chain(flags):
+        tables = PageTables.empty(B * W, ps, B, W, DEV)
+        kv = PagedKVInt4.empty(B * W, KVH, ps, D, F16, DEV)
+        every = torch.arange(B * W, dtype=torch.int32, device=DEV).view(B, W)
+        paged_int4_append(kv, None, *fill, torch.arange(W * ps, device=DEV).repeat(B), every)   # (every page holds something)
+        plans = [StepPlan.empty(B, B * T, DEV) for _ in steps]
+        q_rots, outs = ([torch.empty(B * T, H, D, dtype=F16, device=DEV) for _ in steps] for _ in range(2))
+        ws = paged_int4_attention_workspace(kv, outs[0].view(B, T, H, D), tables.page_table)
+        torch.cuda.synchronize()
+        for (cached, q, k, v), plan, q_rot, out in zip(steps, plans, q_rots, outs):
+            tables.step(cached, new, out=plan, flags=flags)
+            paged_int4_append(kv, q, k, v, plan.positions, tables.page_table, cos, sin, seq_ids=plan.seq_ids, q_out=q_rot, flags=flags)
+            paged_int4_attention(kv, q_rot.view(B, T, H, D), tables.page_table, plan.seqlens, out=out.view(B, T, H, D),
+                                 workspace=ws, flags=flags)
+        return [*outs, *q_rots, *(t for p in plans for t in p), tables.page_table, tables.held, tables.free, tables.ring, kv.pages]
+
+    plain, early = chain(0), chain(_lib.LAUNCH_PDL)
+    assert all(torch.equal(x, y) for x, y in zip(plain, early)) and all(torch.isfinite(x).all() and x.any() for x in plain[:16])
+    graph_pool = []   # and as one graph of dependent launches
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, capture_error_mode="thread_local"):
+        kv = PagedKVInt4.empty(B * W, KVH, ps, D, F16, DEV)
+        tables = PageTables(torch.full((B, W), -1, dtype=torch.int32, device=DEV), torch.zeros(B, dtype=torch.int32, device=DEV),
+                            torch.arange(B * W, dtype=torch.int32, device=DEV), torch.zeros(2, dtype=torch.int32, device=DEV), ps)
+        tables.ring[1:].fill_(B * W)
+        every = torch.arange(B * W, dtype=torch.int32, device=DEV).view(B, W)
+        paged_int4_append(kv, None, *fill, torch.arange(W * ps, device=DEV).repeat(B), every)
+        for cached, q, k, v in steps:
+            plan = tables.step(cached, new, B * T, flags=_lib.LAUNCH_PDL)
+            q_rot = paged_int4_append(kv, q, k, v, plan.positions, tables.page_table, cos, sin, seq_ids=plan.seq_ids, flags=_lib.LAUNCH_PDL)
+            graph_pool.append(paged_int4_attention(kv, q_rot.view(B, T, H, D), tables.page_table, plan.seqlens, flags=_lib.LAUNCH_PDL).view(B * T, H, D))
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(plain, graph_pool))
+
+
 def test_pool_past_four_gigabytes():
     """Pages further apart than 32 bits of bytes."""
     D, ps, KVH = 128, 16, 2
