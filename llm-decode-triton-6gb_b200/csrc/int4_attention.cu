@@ -160,13 +160,6 @@ struct Line {
   }
 };
 
-// An int32 from L2, in its place among the waits
-__device__ __forceinline__ int load_l2(const int32_t* p) {
-  int v;
-  asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];\n" : "=r"(v) : "l"(p) : "memory");
-  return v;
-}
-
 // The sequences' lengths, cut to the page table, into s_len and the exclusive running sums of their units' cost into
 // s_sum[0 .. B] (all THREADS of the block take part). The lengths come from L2: the combine reads them ahead of its wait.
 template <int NT, int THREADS>

@@ -8,6 +8,15 @@ namespace b2d {
 
 constexpr int kMaxPageSize = 1024;
 
+// An int32 from L2, in its place among the waits: lengths and page tables may be written on the device (b2d_page_plan) by a kernel
+// that had not begun when this one, behind other dependent launches, became resident, which the read-only path and lines that this
+// SM's L1 holds from before need not show.
+__device__ __forceinline__ int load_l2(const int32_t* p) {
+  int v;
+  asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];\n" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+
 // Position -> (page index, slot). Pages of a power of two take a shift; the others a division.
 struct PageDiv {
   int size, shift;   // shift < 0: not a power of two

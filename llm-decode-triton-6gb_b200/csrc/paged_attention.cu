@@ -101,7 +101,7 @@ struct Span {
 };
 __device__ __forceinline__ int length_of(const PagedAttnArgs& a, int b) {
   const int64_t reach = static_cast<int64_t>(a.pages_per_seq) * a.kv.page_size;
-  return min(max(a.seqlens[b], 0), max(static_cast<int>(reach), a.prefix_len));
+  return min(max(load_l2(a.seqlens + b), 0), max(static_cast<int>(reach), a.prefix_len));
 }
 __device__ __forceinline__ Span span_of(const PagedAttnArgs& a, int len) {
   Span s;
@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
     auto lookup = [&](const Segment& g, int i) {
       const int tok = g.t_begin + i * KEYS + pg * bp;
       if (kv > 1 || tok >= g.t_end) return -1;
-      return __ldg((g.b >= 0 && tok >= a.prefix_len ? a.table + g.b * a.ld_table : a.prefix_table) + a.div.page(tok));
+      return load_l2((g.b >= 0 && tok >= a.prefix_len ? a.table + g.b * a.ld_table : a.prefix_table) + a.div.page(tok));
     };
     // the next segment, found while this one's first copies are under way, and the pages of its first stage
     Segment ahead;
@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_stream_kernel(const __grid_
               int64_t off = -1;
               if (tok < t_end) {
                 const int pi = a.div.page(tok);
-                const int page = __ldg((tok >= split_at ? table : a.prefix_table) + pi);
+                const int page = load_l2((tok >= split_at ? table : a.prefix_table) + pi);
                 if (page >= 0 && page < a.kv.num_pages) off = page * sp + g.kvh * sh + a.div.slot(tok, pi) * ss;
               }
 #pragma unroll

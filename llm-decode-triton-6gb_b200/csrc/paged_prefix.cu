@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) paged_prefix_kernel(const _
     auto load = [&](bool is_v, int tile) {
       const int tok = (t0 + tile) * kTile + box * bp, slot = unit % kRing;
       const bool live = col < HALVES && tok < a.shared;
-      const int page = live ? __ldg(a.prefix_table + a.div.page(tok)) : -1;
+      const int page = live ? load_l2(a.prefix_table + a.div.page(tok)) : -1;
       if (unit >= kRing) ok = ok && __all_sync(0xffffffffu, mbar_wait(empty + 8 * slot, (unit / kRing - 1) & 1));
       if (!ok) return;
       const uint32_t dst = ring + slot * TILEB + col * COLB + box * bp * 128;

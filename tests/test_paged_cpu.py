@@ -238,6 +238,17 @@ def test_c_verify_checks():
 
 
 # ---- the kernels' sources
+def test_nothing_that_kernels_write_takes_the_read_only_path():
+    """With programmatic launches a kernel may be resident while earlier ones still write what it reads: no load of these kernels may
+    be one that promises data constant for the kernel's lifetime, and lengths, read ahead of a wait, come from L2. (Rotary tables and
+    weights, which no kernel writes, may take it.)"""
+    folder = Path(__file__).resolve().parent.parent / "llm-decode-triton-6gb_b200" / "csrc"
+    for name in ("paged_append.cu", "paged_attention.cu", "paged_prefix.cu", "paged.cuh", "pipeline.cuh", "verify_drafts.cu"):
+        code = "\n".join(line.split("//")[0] for line in (folder / name).read_text().splitlines())
+        code = re.sub(r"void load8\(const C\* p,.*?\n}\n", "", code, flags=re.S)
+        assert not re.search(r"__ldg\(|ldg_\w+\(|\.nc\b|__restrict__|\bseqlens\[", code), name
+
+
 def test_every_bounded_wait_of_the_paged_kernels_is_looked_at():
     """A wait on an mbarrier that runs out has to reach the result (as NaN): each one's outcome goes into a flag, or
     into the number of tries that the next waits have."""
