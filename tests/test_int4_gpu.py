@@ -618,6 +618,27 @@ def test_attention_workspaces_graphs_and_streams():
         paged_int4_attention(*args[0], workspace=short)
 
 
+def test_attention_refused_for_its_workspace_writes_nothing():
+    """300 sequences, two launches: the first runs its units whole, the second needs scratch. Without enough of it the call is refused
+    before the first, with the queries as the output too."""
+    lens = [300 + i % 200 for i in range(300)]
+    c = Case(lens, H=4, KVH=2, D=64, ps=32, seed=13, dtype=BF16)
+    table, lens = c.table.to(DEV)[:, :16].contiguous(), c.lens.to(DEV)
+    q = c.q.to(DEV)
+    need = paged_int4_attention_workspace(c.kv, q, table, max_len=512)
+    assert need.numel() > 0 and paged_int4_attention_workspace(c.kv, q[:256], table[:256], max_len=512).numel() == 0
+    for ws in (need[:0], need[:-16]):
+        mine, apart = q.clone(), torch.full_like(q, 7.0)
+        for out in (mine, apart):
+            with pytest.raises(_lib.B2DError, match="workspace"):
+                paged_int4_attention(c.kv, mine, table, lens, max_len=512, out=out, workspace=ws)
+        torch.cuda.synchronize()
+        assert torch.equal(mine, q) and (apart == 7).all()
+    got = paged_int4_attention(c.kv, mine, table, lens, max_len=512, out=mine, workspace=need)
+    c.check(got)
+    c.check(paged_int4_attention(c.kv, q, table, lens))
+
+
 def test_programmatic_launches_see_what_the_kernel_before_wrote():
     """Chains of dependent launches: a read writes what an append takes, whose keys and queries an attention takes."""
     a = Case([700, 900, 333], H=8, KVH=2, dtype=BF16, seed=21)
