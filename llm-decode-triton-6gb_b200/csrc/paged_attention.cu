@@ -1042,11 +1042,19 @@ extern "C" int b2d_paged_attention(const b2d_paged_kv* kv, const void* q, int64_
   DeviceInfo di;
   if ((st = device_info(&di)) != B2D_OK) return st;
   const int size = out_dtype == B2D_F32 ? 4 : 2;
-  for (int b0 = 0; b0 < B; b0 += kMaxBatch) {
-    const int n = B - b0 < kMaxBatch ? B - b0 : kMaxBatch;
-    const Plan p = make_plan(kv, n, T, H, pages_per_seq, prefix_len, max_len, di.sm_count);
+  // full launches of a large batch and its rest, which may need more scratch (few rows on a prefix: the streaming kernel reads it): all
+  // is checked before the first one, so that a refused call has written nothing
+  Plan plans[2] = {};
+  for (int i = 0; i < 2; ++i) {
+    const int n = i == 0 ? (B < kMaxBatch ? B : kMaxBatch) : B % kMaxBatch;
+    if (n == 0) continue;
+    const Plan p = plans[i] = make_plan(kv, n, T, H, pages_per_seq, prefix_len, max_len, di.sm_count);
     if (!p.fits) return B2D_ERR_SHAPE;
     if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes)) return B2D_ERR_WORKSPACE;
+  }
+  for (int b0 = 0; b0 < B; b0 += kMaxBatch) {
+    const int n = B - b0 < kMaxBatch ? B - b0 : kMaxBatch;
+    const Plan& p = plans[n == kMaxBatch || B < kMaxBatch ? 0 : 1];
     PagedAttnArgs a{};
     a.q = static_cast<const uint8_t*>(q) + b0 * sq_b * 2;
     a.sq_b = sq_b; a.sq_t = sq_t; a.sq_h = sq_h;

@@ -427,6 +427,23 @@ def test_attention_large_batches(B, T, prefix):
     c.check(c.run())
 
 
+def test_attention_refused_for_its_workspace_writes_nothing():
+    """288 sequences on a prefix, two launches of which the second needs more scratch: without it the call is refused before the first."""
+    g = torch.Generator().manual_seed(2)
+    c = Case((128 + torch.randint(0, 70, (288,), generator=g)).tolist(), H=1, KVH=1, D=64, prefix=128, ps=64, seed=2, dtype=BF16)
+    q, table = c.q.to(DEV), c.table.to(DEV)
+    need = paged_attention_workspace(c.cache, q, table, prefix_len=128)
+    full = paged_attention_workspace(c.cache, q[:256], table[:256], prefix_len=128).numel()
+    assert 0 < full < need.numel()
+    out = torch.full_like(q, 7.0)
+    for ws in (need[:0], need[:full], need[:-16]):
+        with pytest.raises(_lib.B2DError, match="workspace"):
+            c.run(workspace=ws, out=out)
+        torch.cuda.synchronize()
+        assert (out == 7).all()
+    c.check(c.run(workspace=need, out=out))
+
+
 def test_attention_programmatic_launches():
     """The calls as programmatic dependents of one another, in a captured chain, give the same bits."""
     for prefix, T in ((0, 1), (512, 3)):
