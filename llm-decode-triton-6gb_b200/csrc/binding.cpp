@@ -393,16 +393,46 @@ void check_written_pool4(const b2d_int4_kv* kv, int64_t block) {
   const int64_t sizes[3] = {kv->num_pages, kv->KVH, block}, strides[3] = {kv->sp_p, kv->sp_h, 1};
   if (!nests(sizes, strides)) bad_value("the cache's pages overlap one another: an append would write them at once");
 }
-// Whether the memory that two tensors span has bytes in common.
+// Whether two tensors may have bytes in common: their spans meet, and no step S between rows keeps them apart. Every byte of a tensor
+// lies a multiple of S behind the interval that its dimensions of other strides span from its start (those whose stride is a
+// multiple of S move it by whole steps); intervals that do not meet modulo S share nothing. That covers parts of a fused projection and
+// rows that take turns.
 bool overlap(const at::Tensor& x, const at::Tensor& y) {
   if (x.numel() == 0 || y.numel() == 0) return false;
-  auto span = [](const at::Tensor& t) {
-    int64_t last = 0;
-    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
-    return (last + 1) * static_cast<int64_t>(t.element_size());
+  auto extent = [](const at::Tensor& t, int64_t step) {   // step 0: of all dimensions
+    const int64_t size = t.element_size();
+    int64_t bytes = size;
+    for (int64_t d = 0; d < t.dim(); ++d)
+      if (step == 0 || t.stride(d) * size % step != 0) bytes += (t.size(d) - 1) * t.stride(d) * size;
+    return bytes;
   };
-  const auto a = reinterpret_cast<uintptr_t>(x.const_data_ptr()), b = reinterpret_cast<uintptr_t>(y.const_data_ptr());
-  return a < b + span(y) && b < a + span(x);
+  const auto a = static_cast<int64_t>(reinterpret_cast<uintptr_t>(x.const_data_ptr())),
+             b = static_cast<int64_t>(reinterpret_cast<uintptr_t>(y.const_data_ptr()));
+  if (a >= b + extent(y, 0) || b >= a + extent(x, 0)) return false;
+  for (const at::Tensor* t : {&x, &y})
+    for (int64_t d = 0; d < t->dim(); ++d) {
+      const int64_t step = t->size(d) > 1 ? t->stride(d) * static_cast<int64_t>(t->element_size()) : 0;
+      if (step == 0) continue;
+      const int64_t apart = ((b - a) % step + step) % step;
+      if (apart >= extent(x, step) && apart + extent(y, step) <= step) return false;
+    }
+  return true;
+}
+// The same elements in the same places
+bool same(const at::Tensor& x, const at::Tensor& y) {
+  if (x.const_data_ptr() != y.const_data_ptr() || x.scalar_type() != y.scalar_type() || x.sizes() != y.sizes()) return false;
+  for (int64_t d = 0; d < x.dim(); ++d)
+    if (x.size(d) > 1 && x.stride(d) != y.stride(d)) return false;
+  return true;
+}
+struct Named {
+  const at::Tensor* t;
+  const char* name;
+};
+// What a call writes while it reads the others
+void check_apart(const at::Tensor& out, const char* name, std::initializer_list<Named> others) {
+  for (const Named& o : others)
+    if (o.t && overlap(out, *o.t)) bad_value(std::string(name) + " and " + o.name + " are one memory, or parts of it");
 }
 
 // positions, seq_ids and page_table of N tokens; returns the table's sequences
@@ -469,6 +499,11 @@ PyObject* int4_append(PyObject*, PyObject* const* a, Py_ssize_t na) {
       check_output(*out, "q_out");
       check_device(out, "q_out", dev);
     }
+    if (out) {
+      if (!same(*out, *q) && overlap(*out, *q)) bad_value("q_out overlaps q and is not q itself");
+      check_apart(*out, "q_out", {{&k, "k"}, {&v, "v"}, {&positions, "positions"}, {&table, "page_table"}, {cos, "cos"}, {sin, "sin"},
+                                  {seq, "seq_ids"}, {qw, "q_weight"}, {kw, "k_weight"}});
+    }
     check_written_pool4(kv, integer(a[16]));
     check_cuda(dev);
     check_pool(dev, a[15]);
@@ -521,10 +556,9 @@ PyObject* int4_read(PyObject*, PyObject* const* a, Py_ssize_t na) {
         check_device(out[i], name[i], dev);
       }
     }
-    // (strided ones may lie between one another's elements)
-    if (out[0] && out[1] && overlap(*out[0], *out[1]) &&
-        (out[0]->const_data_ptr() == out[1]->const_data_ptr() || (out[0]->is_contiguous() && out[1]->is_contiguous())))
-      bad_value("k_out and v_out are one memory, or parts of it");
+    if (out[0] && out[1]) check_apart(*out[0], "k_out", {{out[1], "v_out"}});
+    for (int i = 0; i < 2; ++i)
+      if (out[i]) check_apart(*out[i], name[i], {{&positions, "positions"}, {&table, "page_table"}, {seq, "seq_ids"}});
     check_device(&table, "page_table", dev); check_device(seq, "seq_ids", dev);
     check_cuda(dev);
     check_pool(dev, a[8]);
@@ -572,12 +606,12 @@ PyObject* int4_attention(PyObject*, PyObject* const* a, Py_ssize_t na) {
     check_last(q, "q");
     check_last(out, "out");
     check_output(out, "out");
-    const bool in_place = out.const_data_ptr() == q.const_data_ptr() && out.scalar_type() == dt && out.strides() == q.strides();
-    if (!in_place && out.is_contiguous() && q.is_contiguous() && overlap(out, q)) bad_value("out overlaps q and is not q itself");
+    if (!same(out, q) && overlap(out, q)) bad_value("out overlaps q and is not q itself");
+    check_apart(out, "out", {{&table, "page_table"}, {&lens, "seqlens"}});
     check_device(&table, "page_table", dev); check_device(&lens, "seqlens", dev); check_device(&out, "out", dev);
     const at::Tensor* ws = optional(a[8], "workspace");
     if (ws && !ws->is_contiguous()) bad_value("workspace is contiguous, got " + show(*ws));   // its bytes are counted below
-    if (ws && out.is_contiguous() && overlap(*ws, out)) bad_value("out and workspace are one memory, or parts of it");
+    if (ws) check_apart(*ws, "workspace", {{&out, "out"}, {&q, "q"}, {&table, "page_table"}, {&lens, "seqlens"}});
     check_device(ws, "workspace", dev);
     check_cuda(dev);
     check_pool(dev, a[10]);

@@ -140,6 +140,73 @@ def test_outputs_that_overlap_are_refused():
     refused(lambda: paged_int4_attention(pool(), **args, out=behind), "CUDA")
 
 
+def test_append_outputs_that_overlap_inputs_are_refused():
+    N, H, KVH, D = 4, 4, 2, 64
+    args = append_args(N=N)
+    row = (H + 2 * KVH) * D
+    memory = torch.zeros(3 * N * row).half()
+    call = lambda **kw: lambda: paged_int4_append(pool(), **{**args, **kw})  # noqa: E731
+
+    def view(start, stride, heads=H):
+        return memory[start:].as_strided((N, heads, D), (stride, D, 1))
+
+    q = view(0, H * D)
+    for out in (view(8, H * D), view(0, row), view(0, 2 * H * D), view(N * H * D - 8, H * D), view(H * D, H * D)):   # shifted, other rows, its end
+        refused(call(q=q, q_out=out), "overlaps q and is not q")
+    refused(call(q=q, q_out=memory[:N * H * D].view(H, N, D).transpose(0, 1)), "overlaps q and is not q")   # same memory, other strides
+    refused(call(q=q, q_out=q), "CUDA")
+    refused(call(q=q, q_out=view(0, H * D)), "CUDA")
+    refused(call(q=q, q_out=view(N * H * D, H * D)), "CUDA")
+    # a fused projection: q in place, and beside one another
+    q, k, v = view(0, row), view(H * D, row, KVH), view((H + KVH) * D, row, KVH)
+    refused(call(q=q, k=k, v=v, q_out=q), "CUDA")
+    refused(call(q=args["q"], k=k, v=v, q_out=q), "CUDA")
+    refused(call(q=q, k=k, v=v, q_out=view(KVH * D, row)), "overlaps q")
+    refused(call(q=args["q"], k=k, v=v, q_out=view(KVH * D, row)), "q_out and k are one memory")
+    refused(call(q=args["q"], k=k, v=v, q_out=view(2 * KVH * D, row)), "q_out and k are one memory")
+    refused(call(q=args["q"], v=v, q_out=view((KVH + 2) * D, row)), "q_out and v are one memory")
+    refused(call(q=args["q"], k=k, v=v, q_out=view(N * row, row)), "CUDA")
+    weight = memory[70:134]
+    refused(call(q_out=view(0, H * D), q_weight=weight), "q_out and q_weight")
+    refused(call(q_out=view(0, H * D), k_weight=weight), "q_out and k_weight")
+    ids = memory[:4 * N].view(torch.int64)
+    refused(call(q_out=view(0, H * D), positions=ids), "q_out and positions")
+    tables = memory[:32 * 32].view(32, 32)
+    refused(call(q_out=view(0, H * D), cos=tables, sin=tables), "q_out and cos")
+
+
+def test_attention_outputs_that_overlap_strided_inputs_are_refused():
+    args = attn_args(B=2, T=2)
+    memory = torch.zeros(4096).half()
+    wide = memory[:2 * 2 * 8 * 64].view(2, 2, 8, 64)
+    q, beside = wide[:, :, :4], wide[:, :, 4:]                  # parts of one projection
+    call = lambda **kw: lambda: paged_int4_attention(pool(), **{**args, **kw})  # noqa: E731
+    refused(call(q=q, out=q), "CUDA")
+    refused(call(q=q, out=beside), "CUDA")
+    refused(call(q=q, out=memory[:1024].view(2, 2, 4, 64)), "overlaps q")       # the same address, other strides
+    refused(call(q=q, out=wide[:, :, 2:6]), "overlaps q")
+    refused(call(q=q, out=wide.transpose(0, 1)[:, :, :4]), "overlaps q")
+    refused(call(q=q, out=beside, workspace=memory.view(U8)[:2048]), "workspace and")
+    refused(call(q=q, out=torch.zeros(2, 2, 4, 64).half(), workspace=memory.view(U8)[:2048]), "workspace and q")
+    refused(call(seqlens=memory[:4].view(torch.int32), out=memory[:1024].view(2, 2, 4, 64)), "out and seqlens")
+    refused(call(seqlens=memory[:4].view(torch.int32), workspace=memory[:512].view(U8)), "workspace and seqlens")
+    refused(call(q=q, out=beside, workspace=memory[2048:].view(U8)), "CUDA")
+
+
+def test_read_outputs_that_overlap_are_refused():
+    pos, table = torch.zeros(4, dtype=torch.int64), torch.zeros(2, 3, dtype=torch.int32)
+    memory = torch.zeros(4096).half()
+    call = lambda k, v, **kw: lambda: paged_int4_read(pool(), pos, table, k_out=k, v_out=v, **kw)  # noqa: E731
+    turns = memory[:4 * 2 * 2 * 64].view(4, 2, 2, 64)           # a head's key and value side by side
+    refused(call(turns[:, :, 0], turns[:, :, 1]), "CUDA")
+    rows = memory[:4 * 4 * 64].view(4, 4, 64)
+    refused(call(rows[:, :2], rows[:, 1:3]), "one memory")
+    refused(call(rows[:, :2], rows[:, 2:]), "CUDA")
+    refused(call(rows[:, :2], rows[:, ::2]), "one memory")
+    refused(call(rows[:, ::2], rows[:, 1::2]), "CUDA")
+    refused(lambda: paged_int4_read(pool(), memory[:16].view(torch.int64), table, k_out=rows[:, :2]), "k_out and positions")
+
+
 @pytest.mark.parametrize("change,err", [
     (dict(q=torch.zeros(2, 1, 4, 128).half()), ValueError),
     (dict(q=torch.zeros(2, 1, 5, 64).half()), ValueError),
