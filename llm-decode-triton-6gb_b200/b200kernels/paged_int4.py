@@ -175,5 +175,9 @@ def paged_int4_attention(kv: PagedKVInt4, q: torch.Tensor, page_table: torch.Ten
 
 
 def paged_int4_attention_workspace(kv: PagedKVInt4, q: torch.Tensor, page_table: torch.Tensor, max_len: int = 0) -> torch.Tensor:
-    """Scratch for ``paged_int4_attention`` calls of these sizes (for callers that keep their buffers)."""
-    return _lib.binding().int4_workspace(kv._desc, q, page_table, max_len)
+    """Scratch for ``paged_int4_attention`` calls of these sizes (for callers that keep their buffers); empty where none is needed.
+    Sizes that the call refuses are refused here."""
+    r = _lib.binding().int4_workspace(kv._desc, q, page_table, max_len)
+    if r.__class__ is int:
+        raise _lib.B2DError("b2d_int4_attention", r)
+    return r

@@ -579,6 +579,16 @@ PyObject* int4_read(PyObject*, PyObject* const* a, Py_ssize_t na) {
   });
 }
 
+// q [B, T, H, D] and page_table of a call
+void check_queries(const b2d_int4_kv* kv, const at::Tensor& q, const at::Tensor& table) {
+  if (q.dim() != 4) bad_value("q is [B, T, H, D], got " + show(q));
+  if (q.size(3) != kv->D || q.size(2) % kv->KVH != 0)
+    bad_value("q does not fit a cache of " + std::to_string(kv->KVH) + " heads of " + std::to_string(kv->D) + ": " + show(q));
+  if (q.scalar_type() != pool4_dtype(kv)) throw TypeErr("q has the cache's dtype, got " + show(q));
+  check_table(table, "page_table", 2);
+  if (table.size(0) != q.size(0)) bad_value("page_table has a row per sequence, got " + show(table) + " for " + show(q));
+}
+
 // (desc, q, page_table, seqlens, scale, max_len, out, out_dtype, workspace, flags, device index)
 PyObject* int4_attention(PyObject*, PyObject* const* a, Py_ssize_t na) {
   return guarded([&]() -> PyObject* {
@@ -586,13 +596,8 @@ PyObject* int4_attention(PyObject*, PyObject* const* a, Py_ssize_t na) {
     const b2d_int4_kv* kv = pool4(a[0]);
     const at::Tensor &q = tensor(a[1], "q"), &table = tensor(a[2], "page_table"), &lens = tensor(a[3], "seqlens");
     const at::ScalarType dt = pool4_dtype(kv);
-    if (q.dim() != 4) bad_value("q is [B, T, H, D], got " + show(q));
+    check_queries(kv, q, table);
     const int64_t B = q.size(0), T = q.size(1), H = q.size(2), D = q.size(3);
-    if (D != kv->D || H % kv->KVH != 0)
-      bad_value("q does not fit a cache of " + std::to_string(kv->KVH) + " heads of " + std::to_string(kv->D) + ": " + show(q));
-    if (q.scalar_type() != dt) throw TypeErr("q has the cache's dtype, got " + show(q));
-    check_table(table, "page_table", 2);
-    if (table.size(0) != B) bad_value("page_table has a row per sequence, got " + show(table) + " for " + show(q));
     check_vector(lens, "seqlens", at::kInt, B);
     const int max_len = integer32(a[5], "max_len");
     const at::Device dev = q.device();
@@ -635,17 +640,23 @@ PyObject* int4_attention(PyObject*, PyObject* const* a, Py_ssize_t na) {
   });
 }
 
-// (desc, q, page_table, max_len) -> scratch for `int4_attention`
+// (desc, q, page_table, max_len) -> scratch for `int4_attention`, or the status with which it would refuse these sizes
 PyObject* int4_workspace(PyObject*, PyObject* const* a, Py_ssize_t na) {
   return guarded([&]() -> PyObject* {
     check_count(na, 4);
+    const b2d_int4_kv* kv = pool4(a[0]);
     const at::Tensor &q = tensor(a[1], "q"), &table = tensor(a[2], "page_table");
-    if (q.dim() != 4) bad_value("q is [B, T, H, D], got " + show(q));
-    check_table(table, "page_table", 2);
+    check_queries(kv, q, table);
+    const int b = narrow(q.size(0), "q"), t = narrow(q.size(1), "q"), h = narrow(q.size(2), "q"), per_seq = narrow(table.size(1), "page_table"),
+              max_len = integer32(a[3], "max_len");
+    // no sequences: the sizes are checked and nothing else is done
+    const int st = g_int4_attention(kv, nullptr, 0, 0, 0, nullptr, 0, per_seq, nullptr, max_len, 0, t, h, 1.f, nullptr, 0, 0, 0, kv->dtype,
+                                    nullptr, 0, 0, nullptr);
+    if (st != B2D_OK) return PyLong_FromLong(st);
+    check_device(&table, "page_table", q.device());
     check_cuda(q.device());
     const OnDevice on(q.device());
-    const size_t n = g_int4_workspace(pool4(a[0]), narrow(q.size(0), "q"), narrow(q.size(1), "q"), narrow(q.size(2), "q"),
-                                      narrow(table.size(1), "page_table"), integer32(a[3], "max_len"));
+    const size_t n = g_int4_workspace(kv, b, t, h, per_seq, max_len);
     return THPVariable_Wrap(at::empty({static_cast<int64_t>(n)}, q.options().dtype(at::kByte)));
   });
 }

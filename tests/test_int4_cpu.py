@@ -10,7 +10,8 @@ import torch
 
 from b200kernels import _lib
 from b200kernels.page_plan import PageTables, StepPlan
-from b200kernels.paged_int4 import PagedKVInt4, paged_int4_append, paged_int4_attention, paged_int4_read, rotary_tables
+from b200kernels.paged_int4 import (PagedKVInt4, paged_int4_append, paged_int4_attention, paged_int4_attention_workspace,
+                                    paged_int4_read, rotary_tables)
 from oracle.int4_ref import plan_ref, quantise_ref, values_ref
 
 OK, ARG, SHAPE, DTYPE, ALIGN = 0, 1, 2, 3, 4
@@ -225,6 +226,24 @@ def test_read_outputs_that_overlap_are_refused():
 def test_attention_refusals(change, err):
     with pytest.raises(err):
         paged_int4_attention(pool(), **{**attn_args(), **change})
+
+
+@pytest.mark.parametrize("q,table,err", [
+    (torch.zeros(2, 17, 4, 64).half(), torch.zeros(2, 3, dtype=torch.int32), _lib.B2DError),       # more than 16 tokens
+    (torch.zeros(2, 1, 34, 64).half(), torch.zeros(2, 3, dtype=torch.int32), _lib.B2DError),       # 17 heads of a KV head
+    (torch.zeros(2, 1, 4, 64).half(), torch.zeros(2, 1 << 27, dtype=torch.int32, device="meta"), _lib.B2DError),   # 2^31 positions
+    (torch.zeros(2, 1, 5, 64).half(), torch.zeros(2, 3, dtype=torch.int32), ValueError),
+    (torch.zeros(2, 1, 4, 128).half(), torch.zeros(2, 3, dtype=torch.int32), ValueError),
+    (torch.zeros(2, 4, 64).half(), torch.zeros(2, 3, dtype=torch.int32), ValueError),
+    (torch.zeros(2, 1, 4, 64), torch.zeros(2, 3, dtype=torch.int32), TypeError),
+    (torch.zeros(2, 1, 4, 64).half(), torch.zeros(3, 3, dtype=torch.int32), ValueError),
+    (torch.zeros(2, 1, 4, 64).half(), torch.zeros(2, 3, dtype=torch.int64), ValueError),
+    (torch.zeros(2, 1, 4, 64).half(), torch.zeros(2, 3, dtype=torch.int32), ValueError)])          # sound, but not on a GPU
+def test_workspace_refuses_what_the_attention_refuses(q, table, err):
+    with pytest.raises(err):
+        paged_int4_attention_workspace(pool(), q, table)
+    if err is _lib.B2DError:
+        refused(lambda: paged_int4_attention_workspace(pool(), q, table), "b2d_int4_attention", err)
 
 
 def test_plan_refusals():
