@@ -128,6 +128,12 @@ def test_append_rotations(D, R, interleaved, norm, dtype, table_dtype):
     assert (err <= half_step(dtype) * np.abs(ref) + 2.0 ** -19 * size + 2.0 ** -25).all(), err.max()
 
 
+@pytest.mark.parametrize("D,R", [(128, 128), (128, 96), (64, 32)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_append_rotations_with_fp16_tables(D, R, interleaved):
+    test_append_rotations(D, R, interleaved, True, F16, F16)
+
+
 def test_append_weights_alone_of_either():
     """A norm of the keys and none of the queries, and the other way round; tables of none."""
     q, k, v, pos, table = append_case(8, 2, 4, 2, 64, F16, seed=3)
@@ -818,6 +824,18 @@ def test_plan_over_many_steps(B, W, ps, P, most):
         table, held, free, ring = (getattr(tables, n).cpu() for n in STATE)
         pages = [p for b in range(B) for p in table[b, :held[b]].tolist()] + [int(free[(ring[0] + i) % P]) for i in range(int(ring[1]))]
         assert sorted(pages) == list(range(P))       # every page is held once or free
+
+
+@pytest.mark.parametrize("B,tokens", [(256, 1024), (257, 1024), (512, 1024), (512, 1025), (513, 1024), (513, 1)])
+def test_plan_on_both_sides_of_its_launch_rules(B, tokens):
+    """One block or a cluster, 256 threads or 512, with pages that come and go for nearly every sequence."""
+    g = torch.Generator().manual_seed(B)
+    tables = PageTables.empty(3 * B, 4, B, 6, DEV)
+    cached = torch.zeros(B, dtype=torch.int32)
+    for _ in range(4):
+        cached = (cached + check_step(tables, cached, torch.randint(0, 6, (B,), generator=g, dtype=torch.int32), tokens).granted.cpu().clamp(min=0))
+        cached = torch.where(torch.rand(B, generator=g) < 0.4, cached // 3, cached)
+        check_step(tables, cached, torch.zeros(B, dtype=torch.int32), 0)
 
 
 def test_plan_edges():
