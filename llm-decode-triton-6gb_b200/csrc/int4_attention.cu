@@ -504,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks<NT>) int4_attention_kernel(c
           for (int e = 0; e < 2; ++e) {
             float top = -INFINITY, most = 0.f;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) top = fmaxf(top, hidden(n, h, e) ? -INFINITY : acc[0][n][2 * h + e] * rowf[n][e]);
+            for (int h = 0; h < 2; ++h) top = fmaxf(top, hidden(n, h, e) ? -INFINITY : __fmul_rn(acc[0][n][2 * h + e], rowf[n][e]));
 #pragma unroll
             for (int i = 4; i < 32; i <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
             const bool up = top > m_run[n][e] + kLazy;
@@ -512,7 +512,10 @@ __global__ void __launch_bounds__(kThreads, kBlocks<NT>) int4_attention_kernel(c
             if (up) m_run[n][e] = top;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              d[n][2 * h + e] = hidden(n, h, e) ? -INFINITY : fmaf(acc[0][n][2 * h + e], rowf[n][e], -m_run[n][e]);
+              // behind a new maximum by the rounded scores, as it is one: at sizes whose rounding is above one its key keeps its weight
+              const float a0 = acc[0][n][2 * h + e], by_score = __fmul_rn(a0, rowf[n][e]) - m_run[n][e];
+              const float by_product = fmaf(a0, rowf[n][e], -m_run[n][e]);   // as without the vote
+              d[n][2 * h + e] = hidden(n, h, e) ? -INFINITY : up || by_product > kLazy ? by_score : by_product;
               most = fmaxf(most, exp2_fast(d[n][2 * h + e]) * s_top[h]);
             }
 #pragma unroll

@@ -428,6 +428,38 @@ def test_attention_large_scores_and_negative_scale(dtype):
     c.check(c.run(scale=c.scale))
 
 
+@pytest.mark.parametrize("size", [1e2, 1e4, 1e6, 1e9, 1e15])
+@pytest.mark.parametrize("T,H", [(1, 8), (4, 16)])
+def test_attention_scores_of_any_size(size, T, H):
+    """Scores up to 10^32, whose steps in fp32 are far above one: the key with the largest takes all the weight. (The oracle checks that no
+    other comes near it: the fp32 sums are within D 2^-23 of a score's terms, twice for a difference, and 2^-30 of weight is 30 more.)"""
+    c = Case([700, 90], H=H, KVH=2, T=T, D=64, dtype=BF16, seed=T, magnitude=1.0)
+    c = Case([700, 90], H=H, KVH=2, T=T, D=64, dtype=BF16, seed=T,
+             keys=lambda seq, pos: c.k.float() * size, values=lambda seq, pos: c.v.float())
+    c.q = (c.q.float() * size).bfloat16()
+    (k, _), (v, parts) = c.pools(values_ref)
+    ksize, wide = c.pools(size_ref)[0][0], c.pools(lambda codes, s, m, D: size_ref(np.full_like(codes, 15), s, m, D))[1][0]
+    got = f64(c.run(out_dtype=F32))
+    sure = 0
+    for b, n in enumerate(c.lens.tolist()):
+        page = c.table[b, torch.arange(n) // c.ps].long().numpy()
+        slot = np.arange(n) % c.ps
+        for t in range(T):
+            lim = n - T + 1 + t
+            for h in range(H):
+                kk, vv, ss, ww = (x[page, h * 2 // H, slot][:lim] for x in (k, v, ksize, wide))
+                q = f64(c.q[b, t, h])
+                score = kk @ q * c.scale
+                order = np.argsort(score)
+                reach = (ss @ np.abs(q)).max() * c.scale
+                if score[order[-1]] - score[order[-2]] < 4 * 64 * 2.0 ** -23 * reach + 30:
+                    continue
+                sure += 1
+                err = np.abs(got[b, t, h] - vv[order[-1]])
+                assert (err <= (2.0 ** -11 + n * 2.0 ** -23) * ww[order[-1]] + 2.0 ** -29 * np.abs(ww).max()).all(), (b, t, h, err.max())
+    assert np.isfinite(got).all() and sure > T * H
+
+
 def test_attention_rising_scores():
     """Scores that grow along the sequence: the running maximum moves again and again."""
     direction = torch.randn(64, generator=torch.Generator().manual_seed(1)).sign()
