@@ -436,7 +436,8 @@ int b2d_paged_attention(const b2d_paged_kv* kv, const void* q, int64_t sq_b, int
  * entry is outside [0, num_pages)); behind the last token up to max_tokens all three are -1, which the appends take for
  * padding. seqlens[b] = want (cached, where refused); starts [B + 1]. positions and slots are int64, the rest is int32.
  * B <= 8192; page_size 1..1024; num_pages, max_tokens and pages_per_seq * page_size < 2^31 - 1024. Entries are written only
- * inside the arrays, whatever the state holds; page ids are handed on as they are. One launch; calls that share state
+ * inside the arrays, whatever the state holds; page ids are handed on as they are. One launch (above 512 sequences or 1024 tokens
+ * a cluster of 16 blocks, which a context cut to fewer SMs than 16 of one GPC refuses: B2D_ERR_LAUNCH); calls that share state
  * must not overlap. flags: B2D_LAUNCH_PDL. */
 int b2d_page_plan(int32_t* page_table, int64_t ld_table, int pages_per_seq, int32_t* held, int32_t* free_pages,
                   int num_pages, int32_t* ring, const int32_t* cached, const int32_t* new_tokens, int B, int page_size,

@@ -9,6 +9,14 @@ out of here. Nothing goes through the host, so that a whole step -- plan, append
     q_rot = paged_rope_append(kv, q, k, v, plan.positions, tables.page_table, cos, sin, seq_ids=plan.seq_ids)
     ... paged_attention(kv, q_rot.view(B, T, H, D), tables.page_table, plan.seqlens)
 
+The last line is right where every sequence was granted T tokens. Tokens lie one sequence's behind another's: with other numbers of
+new tokens, or a sequence that is refused, the queries are gathered by ``starts``, and a refused sequence, whose ``seqlens`` stays
+``cached``, is given no keys, or it would attend with another's queries (its row of the output is then zeros):
+
+    rows = (plan.starts[:-1, None] + torch.arange(T, device="cuda")).clamp(max=max_tokens - 1).view(-1)   # [B T]
+    lens = torch.where(plan.granted > 0, plan.seqlens, 0)
+    ... paged_attention(kv, q_rot[rows].view(B, T, H, D), tables.page_table, lens)       # T new tokens, or none
+
 A request that ends, or whose drafts were refused, gives its pages back by the next step's lengths (0 and 0: all of them).
 """
 from __future__ import annotations
@@ -27,7 +35,7 @@ class StepPlan(NamedTuple):
     positions: torch.Tensor   # int64 [max_tokens]
     seq_ids: torch.Tensor     # int32 [max_tokens]
     slots: torch.Tensor       # int64 [max_tokens]: page * page_size + offset
-    seqlens: torch.Tensor     # int32 [B]: cached + new, or cached where the sequence is refused
+    seqlens: torch.Tensor     # int32 [B]: cached + new, or cached where the sequence is refused (none of the step's queries are its own)
     starts: torch.Tensor      # int32 [B + 1]: its tokens are [starts[b], starts[b + 1])
     granted: torch.Tensor     # int32 [B]: new, or -1 where refused
 

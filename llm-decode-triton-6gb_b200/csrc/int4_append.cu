@@ -12,9 +12,10 @@
 //  * v: loaded in that order at once. A position's codes lie in single bytes (the other bytes of a word are other
 //    positions'), so that no store reads what another token writes.
 //
-// Measured on B200: 8168 tokens of 32 + 8 + 8 heads of 128 with norms, bf16: 48 us, 3.6 TB/s of the bytes that it cannot do
-// without (177 MB; copy rate 6.55); 320 tokens 4.2 us; one token 2.6 us (launch and a chain of three loads). Bound by issued
-// instructions and latency: 3200 warp instructions a token, 53 % of the slots, 21 warps per SM. Earlier forms: one warp for all heads of
+// Measured on B200: 8168 tokens of 32 + 8 + 8 heads of 128 with norms, bf16: 49 us, 3.6 TB/s of the bytes that it cannot do
+// without (177 MB; copy rate 6.55); 320 tokens 4.1 us; one token 2.6 us (launch and a chain of three loads). Bound by issued
+// instructions and latency: 3400 warp instructions a token, 56 % of the slots, 21 warps per SM (six blocks; their 80 registers a
+// thread spill 32 to 48 bytes in every form). Earlier forms: one warp for all heads of
 // a token with a division per code 87 us; packed fp32 instructions and corrected quotients 50; queries apart from keys 48. Reading
 // 8 x 4001 tokens: 35.7 us, 4.8 TB/s, with 16-byte stores 38.5; 8 x 1021 tokens 12.0 and 14.6 (a warp a token without the
 // shared words and with stores of 16 bytes: 44).

@@ -23,14 +23,17 @@
 // that several blocks share meet in a combine launch. No atomics: results are the same bits every run.
 //
 // Measured on B200 (GPU time of a call, graph replays over rotated inputs; each key and value once at the copy rate of 6.55 TB/s
-// in brackets): 8 sequences of 16001..32768 keys, 32 / 8 heads of 128, fp16: 51 us (34); 64 of 100..4609, groups of 32: 55 us (30);
-// 8 of 512..2048: 10.8 us (1.8); 16 x 5 drafts, up to 4099 keys: 31 us (6.0); one of 300 keys: 6.7 us. The 16-bit kernel takes 13.8,
-// 38 and 7.5 us for the last three. Long: the loop reads at 5.8 TB/s (about 270 instructions a tile, 63 % of the slots issue, the logic
-// pipe 50 % busy); 6 us pass before the first tiles land and 2 go to the combine. Short: dependent steps of one warp -- lengths 0.7,
+// in brackets): 8 sequences of 16001..32768 keys, 32 / 8 heads of 128, fp16: 52 us (34); 64 of 100..4609, groups of 32: 55.7 us (30);
+// 8 of 512..2048: 11.3 us (1.8); 16 x 5 drafts, up to 4099 keys: 33 us (6.0); one of 300 keys: 7.0 us. The 16-bit kernel takes 13.9,
+// 38 and 7.5 us for the last three. A unit of a row's own costs 1 to 6 % of that (one for all of a warp's rows: 51.7, 54.4, 10.9, 31.0,
+// 6.7), with 32 rows of a KV head 12 % (16 x 8 drafts 53.3 and 47.8). Long: the loop reads at 5.4 TB/s, 41 us of the call (300
+// instructions a tile, 63 % of the slots issue, the logic pipe 51 % busy); 6 us pass before the first tiles land, 2 go to the
+// combine. Groups of 32: 370 instructions a tile, 4.85 TB/s, 40 us of the call. Short: dependent steps of one warp -- lengths 0.7,
 // segment and pages 1.4, queries 0.4, a tile 1.0, merge 0.9, combine 1.4 us. More row tiles: eight warps an SM (their
-// accumulators take the registers) issue in 41 % of the slots. Not kept: a producer warp for one block of 15 consumers an SM (a
-// lane's bulk copies serialise, all warps meet at a unit's end: 56 and 94 us for the first two); clusters in place of the combine (7.2
-// us for 300 keys); five blocks an SM (63 us for the first); whole bytes as operands (fewer masks, more products: the same).
+// accumulators take the registers) issue in 41 % of the slots. Spills (bytes stored, heads of 128, 1 to 4 row tiles): groups of 64 0, 12,
+// 0, 192; of 32 24, 76, 0, 752; heads of 64 none. Not kept: a producer warp for one block of 15 consumers an SM (a
+// lane's bulk copies serialise, all warps meet at a unit's end: 56 and 94 us for the first two); clusters in place of the combine (0.5 us
+// more for 300 keys); five blocks an SM (63 us for the first); whole bytes as operands (fewer masks, more products: the same).
 #include <type_traits>
 
 #include "int4_kv.cuh"
@@ -46,7 +49,7 @@ constexpr int kMaxT = 16, kMaxG = 16;
 constexpr int kMaxBatch = 256;                  // sequences of a launch (larger batches take several)
 constexpr int kMaxCtas = 640;
 // Up to so many keys a unit is one CTA's, and there is no combine launch (8 sequences of up to 256 keys, 8 KV heads: 8.2 -> 7.5 us in a
-// graph; one of 300: 7.2 -> 7.7); with two units an SM or more up to 512 keys (64 sequences: 16.5 -> 13.7 us).
+// graph when the rule was made, 7.3 now; one of 300: 7.2 -> 7.7); with two units an SM or more up to 512 keys (64 sequences: 16.5 -> 13.7).
 constexpr int kWholeKeys = 256, kWholeKeysMany = 512;
 constexpr float kLazy = 8.f;                    // log2 of the largest weight before the running maximum moves
 constexpr float kNone = -1.7e38f;               // running maximum before the first score
@@ -367,7 +370,8 @@ __global__ void __launch_bounds__(kThreads, kBlocks<NT>) int4_attention_kernel(c
     }
     __syncthreads();
     // The rows' factors, of rows 8 n + 2 tq (+ 1): in registers for a unit, but in each tile from shared memory where they would
-    // spill (16 x 8 drafts, groups of 64: 52 us against 67; 16 x 3, groups of 32: 34.1, 39.4; but 16 x 5, groups of 64: 37.0, 35.7)
+    // spill (16 x 8 drafts of up to 4000 keys, groups of 64: 53 us against 67; 16 x 3, groups of 32: 34.6, 39.4; but 16 x 5, groups of 64: 37.0,
+    // 35.9)
     constexpr bool FAR = D == 128 && NT * RUNS >= 8;
     float rowf[NT][2], qs[RUNS][NT][2];
     auto pair = [&](float (&to)[2], const float* row, int n) {

@@ -281,12 +281,14 @@ extern "C" int b2d_page_plan(int32_t* page_table, int64_t ld_table, int pages_pe
                    aligned(positions, 16) && aligned(seq_ids, 16) && aligned(slots, 16)};
   const bool pdl = (flags & B2D_LAUNCH_PDL) != 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  // us a step, half of the steps taking pages and half giving them back. A thread writes four tokens, and up to 1024 of them one block
-  // is faster than a cluster, which starts and ends later (8 x 128 tokens 4.5 against 5.0, 512 x 2 4.8 against 5.8; but 512 x 4
-  // 5.5 against 6.2 and 8 x 256 5.5 against 4.8), unless many sequences move pages (512 move four each: 6.6 against 5.3, 1024 11.3
-  // against 7.1; 1024 x 1 token 6.8 against 7.1). The scans go over the sequences in rounds of a block, where more warps cost
-  // more in each: 256 threads and 512 take 3.9 and 4.1 for 8 x 1, 5.6 and 4.9 for 512 x 1; in a cluster 4.8 and 5.9 for
-  // 8 x 256, 12.4 and 9.8 for 1024 x 64.
+  // us a step, half of the steps taking pages and half giving them back; one block against a cluster, which starts and ends
+  // later. The host knows the sequences and the most tokens, not how many pages will move. Up to 1024 tokens, four a thread, the block
+  // takes 4.5 against 5.0 for 8 x 128 and 4.8 against 5.8 for 512 x 2; above, 5.5 against 4.8 for 8 x 256. Above 512 sequences
+  // the cluster loses little without pages to move (1024 x 1 token 7.1 against 6.8) and wins much with them (1024 move four each 7.1
+  // against 11.3). The rule is on the wrong side for 512 sequences that move four pages each with few tokens (block, 6.6 against 5.3)
+  // and for 512 x 4 tokens (cluster, 6.2 against 5.5). The scans go over the sequences in rounds of a block, where more warps cost more in
+  // each: 256 threads and 512 take 3.9 and 4.1 for 8 x 1, 5.6 and 4.9 for 512 x 1; in a cluster 4.8 and 5.9 for 8 x 256,
+  // 12.4 and 9.8 for 1024 x 64.
   const bool few = B <= 256;
   if (max_tokens <= 1024 && B <= 512) return few ? launch_plan<1, 256>(a, pdl, s) : launch_plan<1, 512>(a, pdl, s);
   return few ? launch_plan<kClusterSize, 256>(a, pdl, s) : launch_plan<kClusterSize, 512>(a, pdl, s);
