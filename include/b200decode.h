@@ -447,8 +447,8 @@ int b2d_page_plan(int32_t* page_table, int64_t ld_table, int pages_per_seq, int3
 /* ================================================================ paged KV cache in 4 bits
  * The paged cache above with keys and values in 4 bits (no counterpart in the reference). Per position, head and run of
  * `group` elements x (fp32):
- *   m = round16(min x), s = round16(max((max x - m) / 15, 0)), c = clamp(rint((x - m) / s), 0, 15) (0 where s = 0),
- * round16 to dtype (F16 or BF16), the rest IEEE fp32; the entry stands for m + s c. A run with an infinity or a NaN (or whose
+ *   m = round16(min x), s = round16(max((max x - m) * (1 / 15), 0)), c = clamp(rint((x - m) / s), 0, 15) (0 where s = 0),
+ * round16 to dtype (F16 or BF16), the rest IEEE fp32 (1 / 15: the fp32 number next to it, as torch divides by 15 on a GPU); the entry stands for m + s c. A run with an infinity or a NaN (or whose
  * m or s overflow) stands for NaN. A pool is num_pages x KVH blocks of b2d_int4_page_bytes bytes, block (page, head) at
  * pages + page * sp_p + head * sp_h (bytes); inside it lie tiles of 16 positions in the order of the kernels' matrix
  * fragments: 8 D bytes of key codes, 8 D of value codes, then per position and run {s, m} of the keys, then of the values.

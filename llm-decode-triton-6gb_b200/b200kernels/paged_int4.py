@@ -4,7 +4,7 @@ No counterpart in the reference, which holds 4-bit weights but a 16-bit cache; n
 ``paged_attention`` (``paged.py``), with the same page tables (``page_plan.PageTables`` keeps them on the GPU):
 
 * ``PagedKVInt4.empty(num_pages, KVH, page_size, D, dtype, device)`` -- one layer's pool. Per position, head and run of
-  ``group_size`` elements x: m = round16(min x), s = round16((max x - m) / 15), codes rint((x - m) / s) in 0..15; the entry
+  ``group_size`` elements x: m = round16(min x), s = round16((max x - m) * (1 / 15)), codes rint((x - m) / s) in 0..15; the entry
   stands for m + s c. 4.5 (group 64) or 5 (group 32) bits an element of D = 128 against 16;
 * ``paged_int4_append`` -- (RMS norms of the query and key heads,) rotary embedding in either pair layout, of all or the
   first part of a head, keys and values quantised into their pages;

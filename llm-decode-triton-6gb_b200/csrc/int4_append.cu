@@ -155,7 +155,9 @@ __device__ __forceinline__ uint32_t quantise(const float (&x)[16], int run_lanes
     hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
   }
   const float m = Dt<T>::to_f32(Dt<T>::from_f32(lo));
-  const float s = Dt<T>::to_f32(Dt<T>::from_f32(fmaxf(__fdiv_rn(__fsub_rn(hi, m), 15.f), 0.f)));
+  // the product with the fp32 number next to 1 / 15, which is also what torch's division by 15 on a GPU does: another last bit of fp32
+  // now and then lies across a 16-bit step, and the run's codes move with its scale
+  const float s = Dt<T>::to_f32(Dt<T>::from_f32(fmaxf(__fmul_rn(__fsub_rn(hi, m), 1.f / 15.f), 0.f)));
   const bool sound = fabsf(hi) < INFINITY && fabsf(m) < INFINITY && s < INFINITY;
   constexpr float kEven = 12582912.f;   // 2^23 + 2^22
   if (sound && s >= kNormal<T> && s >= 0x1p-100f && fabsf(m) < 256.f * s) {

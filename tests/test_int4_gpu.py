@@ -81,6 +81,37 @@ def test_append_without_rotation_is_exact(D, group, dtype, N, B):
     assert torch.equal(hk, gk.to(dtype)) and torch.equal(hv, gv.to(dtype))
 
 
+@pytest.mark.parametrize("dtype,D,group", [(BF16, 128, 64), (BF16, 64, 32), (F16, 128, 64)])
+@pytest.mark.parametrize("norm", [False, True])
+def test_append_agrees_with_torch_bit_for_bit(dtype, D, group, norm):
+    """A prompt's keys and values against the same steps in elementary torch operations on the GPU: a scale that falls on the other side
+    of a 16-bit step moves codes of its run by a whole step, half the spread of the values."""
+    N, KVH, ps = 8168, 8, 64
+    for seed in range(3):
+        g = torch.Generator(device=DEV).manual_seed(seed)
+        k, v = (torch.randn(N, KVH, D, generator=g, device=DEV) for _ in range(2))
+        k = (k * torch.exp(0.3 * torch.randn(KVH, D, generator=g, device=DEV))).to(dtype)
+        v = v.to(dtype)
+        w = (1 + 0.2 * torch.randn(D, generator=g, device=DEV)).to(dtype) if norm else None
+        cos, sin = (t.to(DEV) for t in rotary_tables(N, D, 1e6))
+        kv = empty_pool(-(-N // ps), KVH, ps, D, dtype, group)
+        table, pos = torch.arange(kv.num_pages, dtype=torch.int32, device=DEV)[None], torch.arange(N, device=DEV)
+        paged_int4_append(kv, None, k, v, pos, table, cos, sin, k_weight=w, eps=1e-5)
+        got = paged_int4_read(kv, pos, table, out_dtype=F32)
+        x = k.float()
+        if norm:
+            x = x * (x.double().square().mean(-1, keepdim=True) + float(np.float32(1e-5))).rsqrt().float() * w.float()
+        a, b = x[..., :D // 2], x[..., D // 2:]
+        c, s = cos[:, None], sin[:, None]
+        for out, x in zip(got, (torch.cat((a * c - b * s, b * c + a * s), -1), v.float())):
+            x = x.unflatten(-1, (-1, group))
+            base = x.amin(-1, keepdim=True).to(dtype).float()
+            scale = ((x.amax(-1, keepdim=True) - base) / 15).clamp(min=0).to(dtype).float()
+            code = torch.where(scale > 0, ((x - base) / scale).round().clamp(0, 15), 0.0)
+            want = (base.double() + scale.double() * code.double()).float().flatten(-2)
+            assert torch.equal(out, want), int((out != want).sum())
+
+
 def test_append_touches_its_own_slots_only():
     """Every byte of the pool that is not the new entries' stays as it was, and an entry does not depend on its neighbours."""
     D, KVH, ps = 128, 2, 48
